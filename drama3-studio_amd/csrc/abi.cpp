@@ -16,6 +16,7 @@
 #include <string>
 
 #include "kernels.hpp"
+#include "kv4.hpp"
 #include "layout.hpp"
 
 namespace {
@@ -1574,6 +1575,159 @@ int dmoe_quant_moe_layer(const DmoeQuantBank* bank, const void* x, int x_dtype, 
         quant_forward_impl(bank, x, x_dtype, x_row_stride, tokens, top_k, ids_out, DMOE_I64, weights_out,
                            weights_dtype, pairs, top_k, out, out_dtype, out_row_stride, nullptr, workspace,
                            workspace_bytes, status, st, &route);
+    });
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------ 4-bit paged cache
+namespace {
+
+dmoe::Kv4Cache to_kernel(const DmoeKv4Cache* c) {
+    require(c != nullptr && c->pages != nullptr, "cache pages are required");
+    require(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "head_dim must be 64, 128 or 256");
+    require(c->page_size >= 16 && c->page_size <= 256 && (c->page_size & (c->page_size - 1)) == 0,
+            "page_size must be a power of two in [16, 256]");
+    require(c->num_pages >= 1 && c->kv_heads >= 1 && c->kv_heads <= 1024, "bad page or key/value head count");
+    require(reinterpret_cast<uintptr_t>(c->pages) % 16 == 0 && c->page_stride % 16 == 0, "pages must be 16-byte aligned");
+    require(c->page_stride >= c->kv_heads * dmoe::kv4_head_bytes(c->page_size, c->head_dim),
+            "page_stride is smaller than a page");
+    int shift = 4;
+    while (1 << shift < c->page_size) ++shift;
+    return {c->pages, c->page_stride, c->num_pages, shift, c->kv_heads, c->head_dim};
+}
+
+dmoe::Kv4Batch to_kernel(const DmoeKv4Batch* b, bool tables = true) {
+    require(b != nullptr, "batch descriptor is required");
+    require(!tables || (b->block_table && b->lengths), "block_table and lengths are required");
+    require(b->seqs >= 1 && b->seqs <= dmoe::kKv4MaxSeqs, "sequence count outside [1, 4096]");
+    require(b->rows >= 1 && b->rows <= (1 << 24), "row count outside [1, 2^24]");
+    require(b->max_rows >= 1 && b->max_rows <= b->rows, "max_rows outside [1, rows]");
+    require(b->starts || b->rows >= b->seqs, "one row a sequence needs at least as many rows as sequences");
+    require(b->table_cols >= 1 && b->table_stride >= b->table_cols, "bad block_table geometry");
+    return {b->block_table, b->table_stride, b->lengths, b->starts, b->seqs, b->table_cols, b->rows, b->max_rows};
+}
+
+dmoe::Kv4Rows to_kernel(const DmoeHeadRows* r, int rows, int heads, int dim, bool written, const char* what) {
+    const auto need = [&](bool ok, const char* why) {
+        if (!ok) throw AbiError(std::string(what) + " rows " + why);
+    };
+    need(r != nullptr && r->data != nullptr, "are required");
+    need(reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride % 8 == 0 && r->head_stride % 8 == 0,
+         "must have 16-byte aligned heads");
+    const int64_t rs = r->row_stride, hs = r->head_stride;
+    need(rs >= 0 && hs >= 0, "must have non-negative strides");
+    // bounded first, so that the products below stay in 64 bits
+    need(rs < (int64_t)1 << 38 && hs < (int64_t)1 << 38, "have a stride that is too large");
+    if (written)
+        need((rs >= (heads - 1) * hs + dim && (heads == 1 || hs >= dim)) ||
+                 (hs >= (rows - 1) * rs + dim && (rows == 1 || rs >= dim)) || (rows == 1 && heads == 1),
+             "overlap");
+    return {r->data, rs, hs};
+}
+
+dmoe::Kv4Rotary to_kernel(const DmoeRotary* r, int rows, int head_dim) {
+    if (r == nullptr) return {};
+    require(r->inv_freq != nullptr, "rotation frequencies are required");
+    require(r->dim >= 16 && r->dim % 16 == 0 && r->dim <= head_dim, "rotated channels must be a multiple of 16 up to head_dim");
+    require(r->axes >= 1, "rotation needs at least one axis");
+    require(!r->positions || is_id_dtype(r->positions_dtype), "positions must be int32 or int64");
+    require(!r->positions || r->axes == 1 || r->axis_stride >= rows, "positions axes overlap");
+    return {r->inv_freq, r->axis, r->positions, r->axis_stride, r->positions_dtype, r->axes, r->dim, r->interleaved != 0};
+}
+
+void check_half(int dtype) { require(dtype == DMOE_BF16 || dtype == DMOE_F16, "rows must be bf16 or fp16"); }
+
+int check_heads(int q_heads, int kv_heads) {
+    require(q_heads >= 1 && q_heads <= 4096 && q_heads % kv_heads == 0, "q_heads must be a multiple of the key/value heads");
+    return q_heads / kv_heads;
+}
+
+size_t attend_bytes(const dmoe::Kv4Shape& s, int dim) {
+    return (size_t)s.items * (size_t)s.tile_rows * (size_t)(dim + 2) * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" {
+
+int dmoe_kv4_append(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, const DmoeRotary* rotary,
+                    const DmoeHeadRows* q, int q_heads, const DmoeHeadRows* q_out, const DmoeHeadRows* k,
+                    const DmoeHeadRows* v, int dtype, int* status, void* stream) {
+    return checked([&] {
+        dmoe::Kv4AppendArgs a{};
+        a.cache = to_kernel(cache);
+        a.batch = to_kernel(batch);
+        check_half(dtype);
+        a.dtype = dtype;
+        a.status = status;
+        const int rows = a.batch.rows, dim = a.cache.dim;
+        a.rotary = to_kernel(rotary, rows, dim);
+        a.k = to_kernel(k, rows, a.cache.kv_heads, dim, false, "k");
+        a.v = to_kernel(v, rows, a.cache.kv_heads, dim, false, "v");
+        if (q && q->data) {
+            require(q_heads >= 1 && q_heads <= 4096, "q_heads outside [1, 4096]");
+            a.q_heads = q_heads;
+            a.q = to_kernel(q, rows, q_heads, dim, false, "q");
+            a.q_out = to_kernel(q_out, rows, q_heads, dim, true, "q_out");
+        }
+        dmoe::launch_kv4_append(a, as_stream(stream));
+    });
+}
+
+int dmoe_kv4_read(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, const DmoeHeadRows* k_out,
+                  const DmoeHeadRows* v_out, int dtype, int* status, void* stream) {
+    return checked([&] {
+        dmoe::Kv4ReadArgs a{};
+        a.cache = to_kernel(cache);
+        a.batch = to_kernel(batch);
+        check_half(dtype);
+        a.dtype = dtype;
+        a.status = status;
+        a.k = to_kernel(k_out, a.batch.rows, a.cache.kv_heads, a.cache.dim, true, "k_out");
+        a.v = to_kernel(v_out, a.batch.rows, a.cache.kv_heads, a.cache.dim, true, "v_out");
+        dmoe::launch_kv4_read(a, as_stream(stream));
+    });
+}
+
+size_t dmoe_kv4_attention_workspace_bytes(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, int q_heads) {
+    size_t bytes = 0;
+    checked([&] {
+        const dmoe::Kv4Cache c = to_kernel(cache);
+        const dmoe::Kv4Batch b = to_kernel(batch, false);
+        bytes = attend_bytes(dmoe::kv4_attend_shape(b, c.kv_heads, c.dim, check_heads(q_heads, c.kv_heads)), c.dim);
+    });
+    return bytes;
+}
+
+int dmoe_kv4_attention(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, const DmoeHeadRows* q, int q_heads,
+                       float scale, int window, const DmoeHeadRows* out, int dtype, void* workspace,
+                       size_t workspace_bytes, int* status, void* stream) {
+    return checked([&] {
+        dmoe::Kv4AttendArgs a{};
+        a.cache = to_kernel(cache);
+        a.batch = to_kernel(batch);
+        check_half(dtype);
+        a.dtype = dtype;
+        a.status = status;
+        a.q_heads = q_heads;
+        a.group = check_heads(q_heads, a.cache.kv_heads);
+        a.q = to_kernel(q, a.batch.rows, q_heads, a.cache.dim, false, "q");
+        a.out = to_kernel(out, a.batch.rows, q_heads, a.cache.dim, true, "out");
+        require(std::isfinite(scale) && scale > 0.0f, "scale must be positive and finite");
+        require(window >= 0, "window must not be negative");
+        a.scale_log2 = scale * 1.44269504f;
+        a.window = window;
+        const dmoe::Kv4Shape s = dmoe::kv4_attend_shape(a.batch, a.cache.kv_heads, a.cache.dim, a.group);
+        require(s.items <= INT32_MAX, "too many rows and heads for one call");
+        require(workspace != nullptr && workspace_bytes >= attend_bytes(s, a.cache.dim), "workspace too small");
+        require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
+        a.slots = s.slots;
+        a.min_blocks = s.min_blocks;
+        a.tile_rows = s.tile_rows;
+        a.part = static_cast<float*>(workspace);
+        a.part_ml = a.part + s.items * s.tile_rows * a.cache.dim;
+        dmoe::launch_kv4_attend(a, s, as_stream(stream));
     });
 }
 

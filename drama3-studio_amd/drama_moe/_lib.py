@@ -23,6 +23,7 @@ STATUS_BAD_EXPERT_ID = 1
 STATUS_NON_FINITE = 2
 STATUS_TOO_MANY_ROWS = 4
 STATUS_SYNC_TIMEOUT = 8
+STATUS_BAD_BATCH = 16
 
 
 def dtype_code(dtype: torch.dtype) -> int:
@@ -43,6 +44,27 @@ class Fp8Proj(ctypes.Structure):
 
 class Fp8Bank(ctypes.Structure):
     _fields_ = [("w13", Fp8Proj), ("w2", Fp8Proj), ("experts", ctypes.c_int32)]
+
+
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("num_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class Kv4Batch(ctypes.Structure):
+    _fields_ = [("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lengths", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("seqs", ctypes.c_int32), ("table_cols", ctypes.c_int32),
+                ("rows", ctypes.c_int32), ("max_rows", ctypes.c_int32)]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("axis", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("axis_stride", ctypes.c_int64), ("positions_dtype", ctypes.c_int32), ("axes", ctypes.c_int32),
+                ("dim", ctypes.c_int32), ("interleaved", ctypes.c_int32)]
+
+
+class HeadRows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
 _P = ctypes.c_void_p
@@ -89,6 +111,10 @@ _SIGNATURES = {
     "dmoe_w4a16_linear": ([_P, _I, _L, _I, _P, _L, _P, _L, _I, _I, _P, _L, _P], _I),
     "dmoe_moe_block_pre": ([_P, _L, _I, _I, _P, _L, _I, _P, _P, _L, _P, _L, _I, _P, _L, _P, _P, _L, _P], _I),
     "dmoe_moe_block_post": ([_P, _L, _I, _I, _P, _L, _I, _P, _P, _L, _P, _L, _P, _L, _P], _I),
+    "dmoe_kv4_append": ([_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P], _I),
+    "dmoe_kv4_read": ([_P, _P, _P, _P, _I, _P, _P], _I),
+    "dmoe_kv4_attention_workspace_bytes": ([_P, _P, _I], ctypes.c_size_t),
+    "dmoe_kv4_attention": ([_P, _P, _P, _I, ctypes.c_float, _I, _P, _I, _P, ctypes.c_size_t, _P, _P], _I),
     "dmoe_fp8_quantized_pairs": ([ctypes.POINTER(Fp8Bank), _P, _P, _L, _L, _I, _I, _I, _P, _I, _P,
                                   _I, _I, _I, _P, _P, ctypes.c_size_t, _P, _P], _I),
     "dmoe_combine_slots": ([_P, _L, _P, _I, _I, _I, _I, _I, _P, _I, _L, _P], _I),

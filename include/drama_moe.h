@@ -45,7 +45,8 @@ enum {
     DMOE_STATUS_BAD_EXPERT_ID = 1, /* route id outside [0, experts): that pair contributes 0 */
     DMOE_STATUS_NON_FINITE = 2,    /* non-finite value met by an FP8 quantizer */
     DMOE_STATUS_TOO_MANY_ROWS = 4,
-    DMOE_STATUS_SYNC_TIMEOUT = 8   /* the single-launch decode's grid-wide wait gave up: outputs invalid */
+    DMOE_STATUS_SYNC_TIMEOUT = 8,  /* the single-launch decode's grid-wide wait gave up: outputs invalid */
+    DMOE_STATUS_BAD_BATCH = 16     /* a batch of the 4-bit cache names rows, lengths or pages out of range: skipped */
 };
 
 /* One FP8 E4M3 projection bank: weight [E, N, K] with K contiguous (row and
@@ -469,6 +470,107 @@ DMOE_API int dmoe_moe_block_post(const void* shared_act, int64_t act_row_stride,
 DMOE_API int dmoe_combine_slots(const float* partials, int64_t partial_row_stride, const void* ids, int ids_dtype,
                                 int experts, int tokens, int top_k, int hidden, void* out, int out_dtype,
                                 int64_t out_row_stride, void* stream);
+
+/* ------------------------------------- attention over a cache held in 4 bits
+ *
+ * The attention half of a decoder layer between its projections: keys and
+ * values go into a paged cache of 4.5 bits a value, rotated by their positions
+ * on the way, and attention reads that cache.  The reference keeps its cache
+ * in bf16 inside the framework model it drives (sequence_capacity,
+ * src/drama_low_vram/backbone_graph.py:123-128); this cache has no counterpart
+ * there.
+ *
+ * Pages [num_pages] of page_size tokens (a power of two, 16..256), page_stride
+ * bytes apart (a multiple of 16, base 16-byte aligned).  A page holds for each
+ * of kv_heads heads page_size * (D + D / 8) bytes, D = head_dim in {64, 128,
+ * 256}: key codes [page_size][D/2] (channel 2j in the low half of byte j),
+ * value codes [page_size/4][D/8][4] 32-bit words (word (a, w, i): channels
+ * 8w..8w+7 of token 4a + i from the low bits up), key scales and value scales
+ * [D/32][page_size] 16-bit words.  A scale word belongs to 32 channels of one
+ * token: an fp16 scale s of at most seven significant bits whose four lowest
+ * bits hold the zero point z; a code c stands for (c - z) s, exact in fp16.
+ *
+ * Quantization of 32 values x: r = max(x, 0) - min(x, 0) in fp32, s the
+ * smallest number of seven significant bits (fp16 exponents) with 15 s >= r,
+ * z = rint(-min(x, 0) / s), c = rint(x / s) + z cut to 0..15, halves to even.
+ * Values beyond +-32640 are taken as +-32640 and NaN as 0; both raise
+ * DMOE_STATUS_NON_FINITE. */
+typedef struct DmoeKv4Cache {
+    uint8_t* pages;
+    int64_t page_stride;
+    int32_t num_pages, page_size, kv_heads, head_dim;
+} DmoeKv4Cache;
+
+/* The rows of a call.  Sequence s owns rows starts[s] .. starts[s+1] - 1
+ * (starts [seqs + 1]; NULL: row s) of the rows buffers; they are the LAST
+ * tokens of its lengths[s] tokens: with n rows, row i has place lengths[s] - n
+ * + i.  Its token p lies in page block_table[s * table_stride + p / page_size].
+ * `rows` is the row count of the buffers, max_rows the most rows of a sequence
+ * (sizes the launch).  Tables are device memory and may differ at each replay
+ * of a captured call; at most 4096 sequences.  Places below 0 (a
+ * sequence of fewer tokens than rows) hold no token.  Rows that no sequence
+ * owns are neither read nor written.  A sequence whose rows do not lie in
+ * [0, rows], that has more than max_rows rows, or whose tokens do not fit its
+ * table_cols pages is skipped, and a token whose page is outside
+ * [0, num_pages) is not stored, read as 0, and seen by no row; both raise
+ * DMOE_STATUS_BAD_BATCH. */
+typedef struct DmoeKv4Batch {
+    const int32_t* block_table;
+    int64_t table_stride;
+    const int32_t* lengths;
+    const int32_t* starts;
+    int32_t seqs, table_cols, rows, max_rows;
+} DmoeKv4Batch;
+
+/* Rotation of the first `dim` channels (a multiple of 16) of a head: pair i of
+ * them -- channels (i, i + dim/2), or (2i, 2i + 1) if interleaved -- turns by
+ * positions[axis[i]][row] * inv_freq[i], formed and reduced in fp64.
+ * positions [axes, rows] int32 or int64, axis_stride elements between axes
+ * (NULL: the row's place in its sequence, on one axis); axis [dim/2] (NULL:
+ * axis 0). */
+typedef struct DmoeRotary {
+    const float* inv_freq;
+    const uint8_t* axis;
+    const void* positions;
+    int64_t axis_stride;
+    int32_t positions_dtype, axes, dim, interleaved;
+} DmoeRotary;
+
+/* Rows [rows, heads, D] in bf16 or fp16: strides in elements, D contiguous,
+ * every head 16-byte aligned. */
+typedef struct DmoeHeadRows {
+    void* data;
+    int64_t row_stride, head_stride;
+} DmoeHeadRows;
+
+/* Appends the keys and values of the batch's rows at their places and, with q
+ * (q->data non-NULL, q_heads heads), writes the rotated queries to q_out (may
+ * be q itself).  Keys are rotated (rotary NULL: not) and rounded once to fp32
+ * before they are quantized. */
+DMOE_API int dmoe_kv4_append(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, const DmoeRotary* rotary,
+                             const DmoeHeadRows* q, int q_heads, const DmoeHeadRows* q_out, const DmoeHeadRows* k,
+                             const DmoeHeadRows* v, int dtype, int* status, void* stream);
+
+/* The keys and values that the cache holds at the places of the batch's rows,
+ * in `dtype` (exact in fp16). */
+DMOE_API int dmoe_kv4_read(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, const DmoeHeadRows* k_out,
+                           const DmoeHeadRows* v_out, int dtype, int* status, void* stream);
+
+/* Scratch bytes of dmoe_kv4_attention for this batch's seqs, rows and max_rows
+ * (0 if they are out of range).  It needs no clearing and holds nothing
+ * between calls; calls that overlap need one each. */
+DMOE_API size_t dmoe_kv4_attention_workspace_bytes(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, int q_heads);
+
+/* out row = softmax over the tokens its row sees of (scale q . k), times the
+ * values.  A row at place p sees tokens 0 .. p, with window > 0 only p -
+ * window + 1 .. p; one that sees nothing becomes 0.  q_heads a multiple of
+ * kv_heads, query head h reads key/value head h / (q_heads / kv_heads).
+ * Sums and softmax statistics are fp32; weights are rounded to fp16.  The
+ * result of a row depends on the batch it is computed in (the order of its
+ * partial sums), not on the run. */
+DMOE_API int dmoe_kv4_attention(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, const DmoeHeadRows* q,
+                                int q_heads, float scale, int window, const DmoeHeadRows* out, int dtype,
+                                void* workspace, size_t workspace_bytes, int* status, void* stream);
 
 /* ---------------------------------------------- cooperative decode: host side
  *
