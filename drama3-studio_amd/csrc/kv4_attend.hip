@@ -195,12 +195,16 @@ __global__ __launch_bounds__(kThreads) void kv4_attend_rows_kernel(Kv4AttendArgs
         }
     }
 
-    float m[MT], l[MT];
+    // Scores are held less `base`, the row's running maximum, which the first
+    // product starts from: 2^((S - base) scale) never overflows, however large
+    // the scores are.
+    float base[MT], l[MT];
+    bool seen[MT];
     v4f out[MT][kOut];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        m[t] = -__builtin_inff();
-        l[t] = 0.0f;
+        base[t] = l[t] = 0.0f;
+        seen[t] = false;
 #pragma unroll
         for (int j = 0; j < kOut; ++j) out[t][j] = v4f{0, 0, 0, 0};
     }
@@ -215,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void kv4_attend_rows_kernel(Kv4AttendArgs
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) s[t][i] = v4f{0, 0, 0, 0};
+            for (int t = 0; t < MT; ++t) s[t][i] = v4f{-base[t], -base[t], -base[t], -base[t]};
             Scales sc[kParts];
 #pragma unroll
             for (int c = 0; c < kParts; ++c) {
@@ -269,22 +273,25 @@ __global__ __launch_bounds__(kThreads) void kv4_attend_rows_kernel(Kv4AttendArgs
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) top = fmaxf(top, s[t][i][x]);
-            top = groups_max(top) * score_scale[t];
-            if (__any(top > m[t])) {
-                const float now = fmaxf(m[t], top);
-                const float fade = m[t] == now ? 1.0f : __builtin_amdgcn_exp2f(m[t] - now);
-                m[t] = now;
+            top = groups_max(top);
+            const bool up = top > 0.0f || (!seen[t] && top > -__builtin_inff());
+            if (__any(up)) {
+                const float by = up ? top : 0.0f;
+                const float fade = seen[t] ? __builtin_amdgcn_exp2f(-by * score_scale[t]) : 0.0f;
+                base[t] += by;
+                seen[t] |= up;
                 l[t] *= fade;
 #pragma unroll
                 for (int j = 0; j < kOut; ++j) out[t][j] *= fade;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][i] -= by;
             }
-            const float shift = m[t] == -__builtin_inff() ? 0.0f : kShift - m[t];
             float e[4][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    e[i][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i][x], score_scale[t], shift));
+                    e[i][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i][x], score_scale[t], kShift));
                     l[t] += e[i][x];
                 }
 #pragma unroll
@@ -333,7 +340,7 @@ __global__ __launch_bounds__(kThreads) void kv4_attend_rows_kernel(Kv4AttendArgs
     for (int t = 0; t < MT; ++t) {
         l[t] = groups_sum(l[t]);
         if (g == 0) {
-            join_m[wave][16 * t + r] = m[t];
+            join_m[wave][16 * t + r] = seen[t] ? base[t] * score_scale[t] : -__builtin_inff();
             join_l[wave][16 * t + r] = l[t];
         }
     }

@@ -1,0 +1,207 @@
+"""The 4-bit paged cache on the CPU: what its Python classes and its C entry
+points refuse before any GPU work, axis tables, and the reference that the GPU
+tests use."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import kv4_reference as ref
+from drama_moe import _lib
+from drama_moe.attention import KvCache4, PagedBatch, Rotary
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("make,message", [
+    (lambda: PagedBatch(i32(2, 3).long(), i32(2)), "block_table must be int32"),
+    (lambda: PagedBatch(i32(2, 3), i32(2).long()), "lengths must be int32"),
+    (lambda: PagedBatch(i32(3, 3), i32(2)), "one entry a sequence"),
+    (lambda: PagedBatch(i32(0, 3), i32(0)), "sequence count"),
+    (lambda: PagedBatch(i32(4097, 1), i32(4097)), "sequence count"),
+    (lambda: PagedBatch(i32(2, 0), i32(2)), "no pages"),
+    (lambda: PagedBatch(i32(3, 2).T, i32(2)), "contiguous rows"),
+    (lambda: PagedBatch(i32(2, 3), i32(2), i32(2), rows=4), r"starts must be \[sequences \+ 1\]"),
+    (lambda: PagedBatch(i32(2, 3), i32(2), i32(3)), "rows is required"),
+    (lambda: PagedBatch(i32(2, 3), i32(2), rows=1), "cover every sequence"),
+    (lambda: PagedBatch(i32(2, 3), i32(2), i32(3), rows=4, max_rows=5), "max_rows outside"),
+    (lambda: PagedBatch(i32(2, 3), i32(2), i32(3), rows=4, max_rows=0), "max_rows outside"),
+    (lambda: KvCache4(torch.zeros(4, 2, 16 * 72, dtype=torch.uint8), page_size=16, head_dim=80), "head_dim"),
+    (lambda: KvCache4(torch.zeros(4, 2, 24 * 72, dtype=torch.uint8), page_size=24, head_dim=64), "power of two"),
+    (lambda: KvCache4(torch.zeros(4, 2, 16 * 72 + 1, dtype=torch.uint8), page_size=16, head_dim=64), "pages must be"),
+    (lambda: KvCache4(torch.zeros(4, 2, 16 * 72, dtype=torch.int8), page_size=16, head_dim=64), "pages must be"),
+    (lambda: KvCache4(torch.zeros(0, 2, 16 * 72, dtype=torch.uint8), page_size=16, head_dim=64), "pages must be"),
+    (lambda: KvCache4(torch.zeros(4, 4, 16 * 72, dtype=torch.uint8)[:, ::2], page_size=16, head_dim=64), "contiguous"),
+    (lambda: KvCache4(torch.zeros(4, 2, 16 * 72 + 8, dtype=torch.uint8)[..., 8:], page_size=16, head_dim=64), "contiguous"),
+    (lambda: Rotary(torch.ones(64, dtype=torch.float64)), "inv_freq must be"),
+    (lambda: Rotary(torch.ones(12)), "multiple of 16"),
+    (lambda: Rotary(torch.ones(0)), "multiple of 16"),
+    (lambda: Rotary(torch.ones(16), axis=torch.zeros(8, dtype=torch.uint8)), "axis must be"),
+    (lambda: Rotary(torch.ones(16), axis=torch.zeros(16, dtype=torch.int64)), "axis must be"),
+    (lambda: Rotary.sections([]), "sections"),
+    (lambda: Rotary.sections([4, -1]), "sections"),
+])
+def test_python_refusals(make, message):
+    with pytest.raises(ValueError, match=message):
+        make()
+
+
+def test_there_is_no_cpu_path():
+    cache = KvCache4.allocate(4, 2, 64, page_size=16, device="cpu")
+    batch = PagedBatch(i32(1, 2), i32(1))
+    rows = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    for call in (lambda: cache.append(rows, rows, batch), lambda: cache.read(batch), lambda: cache.attend(rows, batch),
+                 cache.status):
+        with pytest.raises(RuntimeError, match="ROCm GPU"):
+            call()
+
+
+def test_axis_tables():
+    assert Rotary.sections([3, 2, 1]).tolist() == [0, 0, 0, 1, 1, 2]
+    assert Rotary.sections([3, 1, 2], cyclic=True).tolist() == [0, 1, 2, 0, 2, 0]
+    assert Rotary.sections([2, 0, 1]).tolist() == [0, 0, 2]
+    table = Rotary.sections([4, 2, 2])
+    assert table.dtype == torch.uint8
+    assert Rotary(torch.ones(8), axis=table).dim == 16
+
+
+FAKE = 0x100000
+
+
+def descriptors(cache=None, batch=None, rotary=None, rows=None):
+    c = dict(pages=FAKE, page_stride=2 * 16 * 144, num_pages=8, page_size=16, kv_heads=2, head_dim=128) | (cache or {})
+    b = dict(block_table=FAKE, table_stride=4, lengths=FAKE, starts=FAKE, seqs=2, table_cols=4, rows=6,
+             max_rows=3) | (batch or {})
+    r = dict(inv_freq=FAKE, axis=None, positions=FAKE, axis_stride=6, positions_dtype=_lib.I64, axes=2, dim=64,
+             interleaved=0) | (rotary or {})
+    h = dict(data=FAKE, row_stride=256, head_stride=128) | (rows or {})
+    return _lib.Kv4Cache(**c), _lib.Kv4Batch(**b), _lib.RotaryDesc(**r), _lib.HeadRows(**h)
+
+
+def call(entry, d, *, dtype=_lib.BF16, q_heads=4, scale=1.0, window=0, ws=FAKE, ws_bytes=1 << 40, q=None):
+    lib, by = _lib.library(), ctypes.byref
+    cache, batch, rotary, rows = d
+    q = q or _lib.HeadRows(FAKE, q_heads * 128, 128)
+    if entry == "append":
+        return lib.dmoe_kv4_append(by(cache), by(batch), by(rotary), by(q), q_heads, by(q), by(rows), by(rows), dtype,
+                                   None, None)
+    if entry == "read":
+        return lib.dmoe_kv4_read(by(cache), by(batch), by(rows), by(rows), dtype, None, None)
+    return lib.dmoe_kv4_attention(by(cache), by(batch), by(q), q_heads, scale, window, by(q), dtype, ws, ws_bytes,
+                                  None, None)
+
+
+@pytest.mark.parametrize("entry", ["append", "read", "attend"])
+@pytest.mark.parametrize("change,message", [
+    (dict(cache=dict(pages=None)), "pages are required"),
+    (dict(cache=dict(pages=FAKE + 8)), "16-byte aligned"),
+    (dict(cache=dict(page_stride=2 * 16 * 144 + 8)), "16-byte aligned"),
+    (dict(cache=dict(page_stride=16 * 144)), "smaller than a page"),
+    (dict(cache=dict(head_dim=96)), "head_dim"),
+    (dict(cache=dict(page_size=8)), "page_size"),
+    (dict(cache=dict(page_size=48)), "page_size"),
+    (dict(cache=dict(page_size=512)), "page_size"),
+    (dict(cache=dict(num_pages=0)), "head count"),
+    (dict(cache=dict(kv_heads=0)), "head count"),
+    (dict(batch=dict(block_table=None)), "block_table and lengths"),
+    (dict(batch=dict(lengths=None)), "block_table and lengths"),
+    (dict(batch=dict(seqs=0)), "sequence count"),
+    (dict(batch=dict(seqs=4097)), "sequence count"),
+    (dict(batch=dict(rows=0)), "row count"),
+    (dict(batch=dict(rows=(1 << 24) + 1)), "row count"),
+    (dict(batch=dict(max_rows=0)), "max_rows"),
+    (dict(batch=dict(max_rows=7)), "max_rows"),
+    (dict(batch=dict(starts=None, rows=1, max_rows=1)), "one row a sequence"),
+    (dict(batch=dict(table_cols=0)), "block_table geometry"),
+    (dict(batch=dict(table_stride=3)), "block_table geometry"),
+])
+def test_entry_points_refuse_bad_descriptors(entry, change, message):
+    assert call(entry, descriptors(**change)) == -1
+    assert message in _lib.library().dmoe_last_error().decode()
+
+
+@pytest.mark.parametrize("entry,change,kw,message", [
+    ("append", dict(rotary=dict(inv_freq=None)), {}, "frequencies"),
+    ("append", dict(rotary=dict(dim=24)), {}, "multiple of 16"),
+    ("append", dict(rotary=dict(dim=144)), {}, "multiple of 16"),
+    ("append", dict(rotary=dict(axes=0)), {}, "axis"),
+    ("append", dict(rotary=dict(axis_stride=5)), {}, "axes overlap"),
+    ("append", dict(rotary=dict(positions_dtype=_lib.F32)), {}, "int32 or int64"),
+    ("append", dict(), dict(dtype=_lib.F32), "bf16 or fp16"),
+    ("append", dict(rows=dict(data=None)), {}, "k rows are required"),
+    ("append", dict(rows=dict(data=FAKE + 2)), {}, "k rows must have 16-byte aligned"),
+    ("append", dict(rows=dict(row_stride=257)), {}, "16-byte aligned"),
+    ("append", dict(rows=dict(head_stride=-128)), {}, "non-negative"),
+    ("append", dict(rows=dict(row_stride=1 << 40)), {}, "too large"),
+    ("append", dict(), dict(q_heads=0), "q_heads"),
+    ("append", dict(), dict(q=_lib.HeadRows(FAKE, 128, 128)), "q_out rows overlap"),
+    ("read", dict(), dict(dtype=_lib.I32), "bf16 or fp16"),
+    ("read", dict(rows=dict(row_stride=128)), {}, "k_out rows overlap"),
+    ("attend", dict(), dict(q_heads=3), "multiple of the key/value heads"),
+    ("attend", dict(), dict(q_heads=0), "multiple of the key/value heads"),
+    ("attend", dict(), dict(scale=0.0), "scale"),
+    ("attend", dict(), dict(scale=-1.0), "scale"),
+    ("attend", dict(), dict(scale=float("nan")), "scale"),
+    ("attend", dict(), dict(scale=float("inf")), "scale"),
+    ("attend", dict(), dict(window=-1), "window"),
+    ("attend", dict(), dict(ws=None), "workspace too small"),
+    ("attend", dict(), dict(ws_bytes=64), "workspace too small"),
+    ("attend", dict(), dict(ws=FAKE + 8), "workspace must be 16-byte aligned"),
+    ("attend", dict(), dict(q=_lib.HeadRows(FAKE, 512, 0)), "out rows overlap"),
+])
+def test_entry_points_refuse_bad_arguments(entry, change, kw, message):
+    assert call(entry, descriptors(**change), **kw) == -1
+    assert message in _lib.library().dmoe_last_error().decode()
+
+
+def test_workspace_covers_more_rows_with_more_bytes():
+    lib, by = _lib.library(), ctypes.byref
+    sizes = []
+    for rows, most in ((2, 1), (600, 300), (6000, 3000)):
+        cache, batch, _, _ = descriptors(batch=dict(rows=rows, max_rows=most, block_table=None, lengths=None))
+        sizes.append(lib.dmoe_kv4_attention_workspace_bytes(by(cache), by(batch), 4))
+    assert 0 < sizes[0] <= sizes[1] <= sizes[2]
+    cache, batch, _, _ = descriptors(batch=dict(seqs=0))
+    assert lib.dmoe_kv4_attention_workspace_bytes(by(cache), by(batch), 4) == 0
+    cache, batch, _, _ = descriptors()
+    assert lib.dmoe_kv4_attention_workspace_bytes(by(cache), by(batch), 5) == 0
+
+
+# --------------------------------------------------------------- the reference
+
+def test_reference_quantizer_properties():
+    """At most half a step off inside the span, one at its ends; zero exact; s within 1/64 of the span's fifteenth."""
+    g = np.random.default_rng(1)
+    x = (g.standard_normal((400, 64)) * np.exp(g.uniform(-12, 9, (400, 1)))).astype(np.float32)
+    x[5], x[6, :32] = 0, np.abs(x[6, :32])
+    x[7, 3] = 0
+    codes, words = ref.quantize(x)
+    s = (words & 0xFFF0).view(np.float16).astype(np.float64)
+    got = ref.value(codes, words)
+    groups = x.reshape(400, 2, 32).astype(np.float64)
+    span = np.maximum(groups.max(-1), 0) - np.minimum(groups.min(-1), 0)
+    assert (15 * s >= span * (1 - 2.0 ** -23)).all()
+    assert (s <= span / 15 * (1 + 2.0 ** -6) * (1 + 2.0 ** -22) + 2.0 ** -20).all()
+    err = np.abs(got - x).reshape(400, 2, 32)
+    assert (err <= 1.0 * s[..., None] + 1e-30).all()
+    assert np.mean(err <= 0.5 * s[..., None] + 1e-30) > 0.95
+    assert got[7, 3] == 0 and not got[5].any()
+    assert (got.astype(np.float16) == got).all()
+
+
+def test_reference_pages_return_what_was_put():
+    g = np.random.default_rng(2)
+    for page, dim in ((16, 64), (32, 128), (64, 256)):
+        pages = ref.Pages(np.zeros((2, 3, page * (dim + dim // 8)), np.uint8), page, dim)
+        kv = g.standard_normal((page, 2, 3, dim))
+        for p in range(page):
+            pages.put(1, p, *kv[p].astype(np.float32))
+        for p in range(page):
+            for got, x in zip(pages.get(1, p), kv[p]):
+                assert np.array_equal(got, ref.value(*ref.quantize(x.astype(np.float32))))
+        assert not pages.raw[0].any()
