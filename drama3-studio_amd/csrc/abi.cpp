@@ -1695,7 +1695,7 @@ size_t dmoe_kv4_attention_workspace_bytes(const DmoeKv4Cache* cache, const DmoeK
     checked([&] {
         const dmoe::Kv4Cache c = to_kernel(cache);
         const dmoe::Kv4Batch b = to_kernel(batch, false);
-        bytes = attend_bytes(dmoe::kv4_attend_shape(b, c.kv_heads, c.dim, check_heads(q_heads, c.kv_heads)), c.dim);
+        bytes = attend_bytes(dmoe::kv4_attend_shape(b, 1 << c.page_shift, c.kv_heads, c.dim, check_heads(q_heads, c.kv_heads)), c.dim);
     });
     return bytes;
 }
@@ -1718,11 +1718,11 @@ int dmoe_kv4_attention(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, con
         require(window >= 0, "window must not be negative");
         a.scale_log2 = scale * 1.44269504f;
         a.window = window;
-        const dmoe::Kv4Shape s = dmoe::kv4_attend_shape(a.batch, a.cache.kv_heads, a.cache.dim, a.group);
+        const dmoe::Kv4Shape s = dmoe::kv4_attend_shape(a.batch, 1 << a.cache.page_shift, a.cache.kv_heads, a.cache.dim, a.group);
         require(s.items <= INT32_MAX, "too many rows and heads for one call");
         require(workspace != nullptr && workspace_bytes >= attend_bytes(s, a.cache.dim), "workspace too small");
         require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
-        a.slots = s.slots;
+        a.slots_log2 = s.slots_log2;
         a.min_blocks = s.min_blocks;
         a.tile_rows = s.tile_rows;
         a.part = static_cast<float*>(workspace);

@@ -25,6 +25,7 @@ namespace dmoe {
 
 constexpr int kKv4Group = 32;          // channels a scale word
 constexpr int kKv4Block = 64;          // tokens an attention step takes
+constexpr int kKv4Whole = 16;          // sequences of up to this many blocks are not cut
 constexpr int kKv4MaxSeqs = 4096;
 constexpr float kKv4Limit = 32640.0f;  // values beyond are stored as this: 15 s = 2 * 32640 is the largest span in fp16
 
@@ -84,7 +85,8 @@ struct Kv4AttendArgs {
     int dtype;
     float scale_log2;       // softmax scale * log2(e)
     int window;             // tokens a row sees, 0: all before it
-    int slots, min_blocks;  // work is cut for this many workgroups, in pieces of at least this many blocks
+    int slots_log2;         // work is cut for 2^slots_log2 workgroups,
+    int min_blocks;         // in pieces of at least this many blocks
     int tile_rows;          // packed rows (token, head of the group) of a tile
     float* part;            // [items][tile_rows][D] unnormalised sums of the pieces of a cut tile
     float* part_ml;         // [items][tile_rows][2] running maximum and sum
@@ -96,11 +98,15 @@ void launch_kv4_read(const Kv4ReadArgs& a, hipStream_t st);
 
 // Geometry of an attention call: rows of a tile, workgroups, bytes of scratch.
 struct Kv4Shape {
-    int tile_rows, slots, min_blocks;
+    int tile_rows, slots_log2, min_blocks;
     int64_t tiles;  // most tiles the batch can hold, for one key/value head
     int64_t items;  // most workgroups
 };
-Kv4Shape kv4_attend_shape(const Kv4Batch& b, int kv_heads, int dim, int group);
+Kv4Shape kv4_attend_shape(const Kv4Batch& b, int page_size, int kv_heads, int dim, int group);
+// Packed rows of a tile of launch_kv4_attend_tiles, and workgroups the work is cut for.
+int kv4_tile_rows(int64_t most_rows, int dim);
+int kv4_tile_slots_log2(int64_t most_rows, int dim);
+void launch_kv4_attend_tiles(const Kv4AttendArgs& a, const Kv4Shape& s, hipStream_t st);
 void launch_kv4_attend(const Kv4AttendArgs& a, const Kv4Shape& s, hipStream_t st);
 
 #ifdef __HIPCC__

@@ -19,6 +19,11 @@ struct Kv4Item {
     bool live;
 };
 
+// The wave's index in its workgroup and a lane's value, known to the compiler
+// to be the same in all lanes: block counters, tables and branches stay scalar.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+__device__ __forceinline__ int of_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
 __device__ __forceinline__ int64_t wave_sum_i64(int64_t v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
@@ -30,6 +35,13 @@ __device__ __forceinline__ void kv4_blocks(const Kv4Seq& q, int window, int i0, 
     const int p0 = q.len - q.n + i0, p1 = q.len - q.n + i1;
     b0 = window > 0 ? max(0, (int)max((int64_t)0, (int64_t)p0 - window + 1)) / kKv4Block : 0;
     b1 = p1 < 0 ? b0 : max(b0, p1 / kKv4Block + 1);
+}
+
+// The blocks [from, to) of a piece of a tile that sees blocks [b0, b1).
+__device__ __forceinline__ void kv4_piece(const Kv4Item& it, int b0, int b1, int& from, int& to) {
+    const uint32_t each = (uint32_t)(b1 - b0) / (uint32_t)it.splits, more = (uint32_t)(b1 - b0) - each * it.splits;
+    from = b0 + it.split * (int)each + min(it.split, (int)more);
+    to = from + (int)each + (it.split < (int)more ? 1 : 0);
 }
 
 // Workgroup `index` of a pass over pieces (kTiles = false) or over whole tiles
@@ -58,8 +70,8 @@ __device__ Kv4Item kv4_item(const Kv4AttendArgs& a, int index) {
         load(s0 + lane, q, tiles, blocks);
         work += (int64_t)tiles * blocks;
     }
-    const int64_t piece64 = (wave_sum_i64(work) * kv + a.slots - 1) / a.slots;
-    const int piece = (int)max((int64_t)a.min_blocks, piece64);
+    const int64_t share = (wave_sum_i64(work) * kv + (1 << a.slots_log2) - 1) >> a.slots_log2;
+    const int piece = __builtin_amdgcn_readfirstlane((int)max((int64_t)a.min_blocks, share));
     Kv4Item it;
     it.live = false;
     it.head = index % kv;
@@ -67,7 +79,7 @@ __device__ Kv4Item kv4_item(const Kv4AttendArgs& a, int index) {
     int before = 0, pieces_before = 0;
     for (int s0 = 0; s0 < seqs; s0 += kWave) {
         if (s0 || seqs > kWave) load(s0 + lane, q, tiles, blocks);
-        const int splits = max(1, (blocks + piece - 1) / piece);
+        const int splits = blocks <= kKv4Whole ? 1 : (blocks + piece - 1) / piece;
         const int mine = kTiles ? tiles : tiles * splits;
         int upto = mine, pieces = tiles * splits;
 #pragma unroll
@@ -79,20 +91,20 @@ __device__ Kv4Item kv4_item(const Kv4AttendArgs& a, int index) {
         if (past) {
             const int who = __ffsll(past) - 1;
             it.seq = s0 + who;
-            it.splits = __shfl(splits, who, kWave);
-            it.row0 = __shfl(q.row0, who, kWave);
-            it.n = __shfl(q.n, who, kWave);
-            it.len = __shfl(q.len, who, kWave);
-            const int at = want - (before + __shfl(upto - mine, who, kWave));
-            const int first = pieces_before + __shfl(pieces - tiles * splits, who, kWave);
+            it.splits = of_lane(splits, who);
+            it.row0 = of_lane(q.row0, who);
+            it.n = of_lane(q.n, who);
+            it.len = of_lane(q.len, who);
+            const int at = want - (before + of_lane(upto - mine, who));
+            const int first = pieces_before + of_lane(pieces - tiles * splits, who);
             it.tile = kTiles ? at : at / it.splits;
             it.split = kTiles ? 0 : at % it.splits;
             it.first = (first + it.tile * it.splits) * kv + it.head;
             it.live = true;
             return it;
         }
-        before += __shfl(upto, kWave - 1, kWave);
-        pieces_before += __shfl(pieces, kWave - 1, kWave);
+        before += of_lane(upto, kWave - 1);
+        pieces_before += of_lane(pieces, kWave - 1);
     }
     return it;
 }

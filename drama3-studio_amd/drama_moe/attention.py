@@ -35,8 +35,10 @@ def _rows(t: Tensor, name: str, rows: int, heads: int, dim: int, dtype: torch.dt
     or (for one that is only read) a copy."""
     if t.ndim != 3 or t.shape != (rows, heads, dim):
         raise ValueError(f"{name} must be [{rows}, {heads}, {dim}], got {list(t.shape)}")
-    if t.dtype not in _HALVES or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{name} must be {dtype or 'bf16 or fp16'}, got {t.dtype}")
+    if t.dtype not in _HALVES:
+        raise ValueError(f"{name} must be bf16 or fp16, got {t.dtype}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
     s0, s1, s2 = t.stride()
