@@ -1643,8 +1643,10 @@ int check_heads(int q_heads, int kv_heads) {
     return q_heads / kv_heads;
 }
 
-size_t attend_bytes(const dmoe::Kv4Shape& s, int dim) {
-    return (size_t)s.items * (size_t)s.tile_rows * (size_t)(dim + 2) * sizeof(float);
+dmoe::Kv4Shape attend_shape(const dmoe::Kv4Cache& c, const dmoe::Kv4Batch& b, int group) {
+    const dmoe::Kv4Shape s = dmoe::kv4_attend_shape(b, 1 << c.page_shift, c.kv_heads, c.dim, group);
+    require(s.groups >= 1 && s.groups <= INT32_MAX, "too many rows, heads and pages for one call");
+    return s;
 }
 
 }  // namespace
@@ -1695,7 +1697,7 @@ size_t dmoe_kv4_attention_workspace_bytes(const DmoeKv4Cache* cache, const DmoeK
     checked([&] {
         const dmoe::Kv4Cache c = to_kernel(cache);
         const dmoe::Kv4Batch b = to_kernel(batch, false);
-        bytes = attend_bytes(dmoe::kv4_attend_shape(b, 1 << c.page_shift, c.kv_heads, c.dim, check_heads(q_heads, c.kv_heads)), c.dim);
+        bytes = std::max<size_t>(attend_shape(c, b, check_heads(q_heads, c.kv_heads)).bytes(), 16);
     });
     return bytes;
 }
@@ -1718,15 +1720,15 @@ int dmoe_kv4_attention(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, con
         require(window >= 0, "window must not be negative");
         a.scale_log2 = scale * 1.44269504f;
         a.window = window;
-        const dmoe::Kv4Shape s = dmoe::kv4_attend_shape(a.batch, 1 << a.cache.page_shift, a.cache.kv_heads, a.cache.dim, a.group);
-        require(s.items <= INT32_MAX, "too many rows and heads for one call");
-        require(workspace != nullptr && workspace_bytes >= attend_bytes(s, a.cache.dim), "workspace too small");
+        const dmoe::Kv4Shape s = attend_shape(a.cache, a.batch, a.group);
+        require(workspace != nullptr && workspace_bytes >= s.bytes(), "workspace too small");
         require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
         a.slots_log2 = s.slots_log2;
         a.min_blocks = s.min_blocks;
         a.tile_rows = s.tile_rows;
         a.part = static_cast<float*>(workspace);
-        a.part_ml = a.part + s.items * s.tile_rows * a.cache.dim;
+        a.part_ml = a.part + s.part_bytes / sizeof(float);
+        a.records = s.record_bytes ? reinterpret_cast<dmoe::Kv4Record*>(a.part_ml + s.ml_bytes / sizeof(float)) : nullptr;
         dmoe::launch_kv4_attend(a, s, as_stream(stream));
     });
 }

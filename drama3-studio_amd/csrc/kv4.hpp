@@ -88,19 +88,25 @@ struct Kv4AttendArgs {
     int slots_log2;         // work is cut for 2^slots_log2 workgroups,
     int min_blocks;         // in pieces of at least this many blocks
     int tile_rows;          // packed rows (token, head of the group) of a tile
-    float* part;            // [items][tile_rows][D] unnormalised sums of the pieces of a cut tile
-    float* part_ml;         // [items][tile_rows][2] running maximum and sum
+    float* part;            // [slots][tile_rows][D] unnormalised sums of the pieces of a cut tile
+    float* part_ml;         // [slots][tile_rows][2] running maximum and sum
+    struct Kv4Record* records;  // [seqs * kv_heads] pieces of each tile, where a sequence is one (null: nothing is cut)
     int* status;
 };
 
 void launch_kv4_append(const Kv4AppendArgs& a, hipStream_t st);
 void launch_kv4_read(const Kv4ReadArgs& a, hipStream_t st);
 
-// Geometry of an attention call: rows of a tile, workgroups, bytes of scratch.
+// Geometry of an attention call: rows of a tile, workgroups, scratch.
 struct Kv4Shape {
+    bool one_tile;  // a tile holds all rows of a sequence
+    bool cut;       // tiles may be cut, and are joined by a second launch
     int tile_rows, slots_log2, min_blocks;
     int64_t tiles;  // most tiles the batch can hold, for one key/value head
-    int64_t items;  // most workgroups
+    int64_t groups; // workgroups
+    int64_t slots;  // partial sums
+    size_t part_bytes, ml_bytes, record_bytes;  // multiples of 16
+    size_t bytes() const { return part_bytes + ml_bytes + record_bytes; }
 };
 Kv4Shape kv4_attend_shape(const Kv4Batch& b, int page_size, int kv_heads, int dim, int group);
 // Packed rows of a tile of launch_kv4_attend_tiles, and workgroups the work is cut for.

@@ -3,8 +3,8 @@
 // Codes become fp16 without conversions: a nibble put into the mantissa of
 // 1024 (low) or 64 (high) is 1024 + c or 64 + c, from which 1024 + z or 64 + z
 // is taken exactly; times s it is exact again.  Queries are scaled by a power
-// of two per row into fp16 (exact), P is shifted by 2^14, which keeps weights
-// down to 2^-28 normal, and is rounded to fp16 with the sums in fp32.
+// of two per row into fp16 (exact), P is shifted by 2^8, which keeps weights
+// down to 2^-22 normal, and is rounded to fp16 with the sums in fp32.
 #pragma once
 
 #include "common.hpp"
@@ -17,7 +17,8 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
-constexpr float kKv4Shift = 14.0f;  // P is held times 2^14
+constexpr float kKv4Shift = 8.0f;  // P is held times 2^8,
+constexpr float kKv4Slack = 7.0f;  // and up to 2^7 times that: at most 2^15, half of fp16's range
 
 __device__ __forceinline__ v2h as_h2(uint32_t w) { return __builtin_bit_cast(v2h, w); }
 

@@ -134,21 +134,14 @@ __device__ __forceinline__ void store_pieces(const CodeBits& bits, const Piece (
 }
 
 template <class T>
-__global__ __launch_bounds__(T::kThreads, T::D == 256 ? 1 : 2) void kv4_attend_tiles_kernel(Kv4AttendArgs a) {
+__device__ __forceinline__ void attend_tile(const Kv4AttendArgs& a, const Kv4Segment& it, uint8_t (&lds)[2][T::kStage]) {
     constexpr int D = T::D, kSteps = D / 16, kOut = D / 32, kTiles = 2 / T::kHalves;
     static_assert(T::kHalves == 1 || T::kRows * (D + 2) * 4 <= 2 * T::kStage, "the halves are joined in the stages");
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2][T::kStage];
-    const int lane = threadIdx.x & 63, r = lane & 31, hi = lane >> 5;
+    const int lane = segment_lane(), r = lane & 31, hi = lane >> 5;
     const int wave = wave_index() % T::kGroups, half = wave_index() / T::kGroups;
-    const Kv4Item it = kv4_item<false>(a, blockIdx.x);
-    if (!it.live) return;
-    const int packed = it.n * a.group;
-    const int row_a = it.tile * T::kRows, row_b = min(row_a + T::kRows, packed);
-    const int i0 = row_a / a.group, i1 = (row_b - 1) / a.group;
-    int b0, b1, from, to;
-    kv4_blocks(Kv4Seq{it.row0, it.n, it.len}, a.window, i0, i1, b0, b1);
-    kv4_piece(it, b0, b1, from, to);
-    const int end = it.len - it.n + i1 + 1;
+    const int packed = it.n * a.group, from = it.from, to = it.to;
+    const int row_a = it.row_a, row_b = min(row_a + T::kRows, packed);
+    const int end = it.len - it.n + (row_b - 1) / a.group + 1;
     const int32_t* table = a.batch.table + (int64_t)it.seq * a.batch.table_stride;
     const CodeBits bits = code_bits();
     Piece piece[T::kMine];
@@ -172,6 +165,7 @@ __global__ __launch_bounds__(T::kThreads, T::D == 256 ? 1 : 2) void kv4_attend_t
         score_scale = scale_query(raw, most, a.dtype, a.scale_log2, query);
     }
 
+    const float slack = kKv4Slack / score_scale;
     float base = 0.0f, sum = 0.0f;  // as in the kernel of few rows: scores are held less `base`
     bool seen = false;
     v16f out[kOut];
@@ -227,7 +221,7 @@ __global__ __launch_bounds__(T::kThreads, T::D == 256 ? 1 : 2) void kv4_attend_t
 #pragma unroll
                 for (int x = 0; x < 16; ++x) top = fmaxf(top, s[i][x]);
             top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            const bool up = top > 0.0f || (!seen && top > -__builtin_inff());
+            const bool up = top > slack || (!seen && top > -__builtin_inff());
             if (__any(up)) {
                 const float by = up ? top : 0.0f;
                 const float fade = seen ? __builtin_amdgcn_exp2f(-by * score_scale) : 0.0f;
@@ -291,8 +285,8 @@ __global__ __launch_bounds__(T::kThreads, T::D == 256 ? 1 : 2) void kv4_attend_t
             for (int x = 0; x < 16; ++x) out[c][x] = f * out[c][x] + h * share[(16 * c + x) * kStride];
     }
     if (pr >= row_b) return;
-    if (it.splits > 1) {
-        const int64_t at = (int64_t)blockIdx.x * a.tile_rows + 32 * wave + r;
+    if (!it.whole) {
+        const int64_t at = it.slot * a.tile_rows + 32 * wave + r;
         float* o = a.part + at * D + 4 * hi;
 #pragma unroll
         for (int c = 0; c < kOut; ++c)
@@ -312,10 +306,26 @@ __global__ __launch_bounds__(T::kThreads, T::D == 256 ? 1 : 2) void kv4_attend_t
                                               narrow2(out[c][4 * x + 2] * inv, out[c][4 * x + 3] * inv, a.dtype)};
 }
 
+template <class T>
+__global__ __launch_bounds__(T::kThreads, T::D == 256 ? 1 : 2) void kv4_attend_tiles_kernel(Kv4AttendArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][T::kStage];
+    if constexpr (T::kHalves == 2) {
+        Kv4Shares shares(a, blockIdx.x);
+        Kv4Segment seg;
+        for (bool first = true; shares.next(seg); first = false) {
+            if (!first) __syncthreads();  // the segment before has been read
+            if (seg.n) attend_tile<T>(a, seg, lds);
+        }
+    } else {
+        Kv4Segment seg;
+        if (kv4_piece(a, seg)) attend_tile<T>(a, seg, lds);
+    }
+}
+
 template <int D>
 void launch_dim(const Kv4AttendArgs& a, const Kv4Shape& s, hipStream_t st) {
-    if (a.tile_rows == Few<D>::kRows) kv4_attend_tiles_kernel<Few<D>><<<(unsigned)s.items, Few<D>::kThreads, 0, st>>>(a);
-    else kv4_attend_tiles_kernel<Many<D>><<<(unsigned)s.items, Many<D>::kThreads, 0, st>>>(a);
+    if (a.tile_rows == Few<D>::kRows) kv4_attend_tiles_kernel<Few<D>><<<(unsigned)s.groups, Few<D>::kThreads, 0, st>>>(a);
+    else kv4_attend_tiles_kernel<Many<D>><<<(unsigned)s.groups, Many<D>::kThreads, 0, st>>>(a);
 }
 
 }  // namespace

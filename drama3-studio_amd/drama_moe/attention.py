@@ -29,20 +29,19 @@ MAX_SEQUENCES = 4096
 _HALVES = (torch.bfloat16, torch.float16)
 
 
-def _rows(t: Tensor, name: str, rows: int, heads: int, dim: int, dtype: torch.dtype | None, device, *,
-          written: bool = False) -> Tensor:
-    """t as [rows, heads, dim] with contiguous, 16-byte aligned heads: itself,
-    or (for one that is only read) a copy."""
-    if t.ndim != 3 or t.shape != (rows, heads, dim):
-        raise ValueError(f"{name} must be [{rows}, {heads}, {dim}], got {list(t.shape)}")
+def _rows(t: Tensor, name: str, shape: tuple, dtype: torch.dtype | None, device, *, written: bool = False) -> Tensor:
+    """t as rows of ``shape`` [rows, heads, dim] with contiguous, 16-byte
+    aligned heads: itself, or (for one that is only read) a copy."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     if t.dtype not in _HALVES:
         raise ValueError(f"{name} must be bf16 or fp16, got {t.dtype}")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
     s0, s1, s2 = t.stride()
-    if s2 != 1 or (s0 % 8 and rows > 1) or (s1 % 8 and heads > 1) or t.data_ptr() % 16:
+    if s2 != 1 or (s0 % 8 and shape[0] > 1) or (s1 % 8 and shape[1] > 1) or t.data_ptr() % 16:
         if written:
             raise ValueError(f"{name} must have contiguous, 16-byte aligned heads")
         return t.clone(memory_format=torch.contiguous_format)
@@ -58,8 +57,12 @@ def _head_rows(t: Tensor | None):
     return ctypes.byref(_lib.HeadRows(t.data_ptr(), s0 if rows > 1 else 0, s1 if heads > 1 else 0))
 
 
+def _heads(q: Tensor) -> int:
+    return q.shape[1] if q.ndim == 3 else 0
+
+
 def _indices(t: Tensor, name: str, ndim: int) -> Tensor:
-    if t.dtype != torch.int32 or t.ndim != ndim or (t.numel() and t.stride(-1) != 1):
+    if t.dtype is not torch.int32 or t.ndim != ndim or (t.shape[-1] > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name} must be int32 with {ndim} dimension(s) and contiguous rows")
     return t
 
@@ -84,35 +87,40 @@ class PagedBatch:
                  max_rows: int | None = None):
         _indices(block_table, "block_table", 2)
         _indices(lengths, "lengths", 1)
-        seqs = lengths.shape[0]
-        if block_table.shape[0] != seqs:
+        seqs, cols = block_table.shape
+        if lengths.shape[0] != seqs:
             raise ValueError("block_table and lengths must have one entry a sequence")
         if not 1 <= seqs <= MAX_SEQUENCES:
             raise ValueError(f"sequence count outside [1, {MAX_SEQUENCES}]")
-        if block_table.shape[1] < 1:
+        if cols < 1:
             raise ValueError("block_table has no pages")
+        device = lengths.device
+        if block_table.device != device:
+            raise ValueError("batch tables must share a device")
         if starts is not None:
             _indices(starts, "starts", 1)
             if starts.shape[0] != seqs + 1:
                 raise ValueError("starts must be [sequences + 1]")
+            if starts.device != device:
+                raise ValueError("batch tables must share a device")
             if rows is None:
                 raise ValueError("rows is required with starts")
-        rows = seqs if rows is None else int(rows)
-        if max_rows is None:
-            max_rows = 1 if starts is None else rows
-        if rows < (0 if starts is not None else seqs):
-            raise ValueError("rows must cover every sequence")
+            rows = int(rows)
+            max_rows = rows if max_rows is None else int(max_rows)
+            if rows < 0:
+                raise ValueError("rows must not be negative")
+        else:
+            rows = seqs if rows is None else int(rows)
+            max_rows = 1 if max_rows is None else int(max_rows)
+            if rows < seqs:
+                raise ValueError("rows must cover every sequence")
         if rows and not 1 <= max_rows <= rows:
             raise ValueError("max_rows outside [1, rows]")
-        self.device = lengths.device
-        if block_table.device != self.device or (starts is not None and starts.device != self.device):
-            raise ValueError("batch tables must share a device")
         self.block_table, self.lengths, self.starts = block_table, lengths, starts
-        self.rows, self.max_rows = rows, int(max_rows)
+        self.rows, self.max_rows, self.device = rows, max_rows, device
         # a table of one row may have any row stride
-        self.desc = _lib.Kv4Batch(block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]),
-                                  lengths.data_ptr(), starts.data_ptr() if starts is not None else None, seqs,
-                                  block_table.shape[1], rows, self.max_rows)
+        self.desc = _lib.Kv4Batch(block_table.data_ptr(), max(block_table.stride(0), cols), lengths.data_ptr(),
+                                  starts.data_ptr() if starts is not None else None, seqs, cols, rows, max_rows)
 
 
 class Rotary:
@@ -161,7 +169,7 @@ class KvCache4:
     kv_heads, page_size * (D + D/8)] (pages may be strided, as in a buffer
     that holds several layers')."""
 
-    __slots__ = ("pages", "page_size", "kv_heads", "head_dim", "desc", "device", "_state")
+    __slots__ = ("pages", "page_size", "kv_heads", "head_dim", "desc", "device", "_state", "_status")
 
     def __init__(self, pages: Tensor, *, page_size: int, head_dim: int):
         if head_dim not in (64, 128, 256):
@@ -178,7 +186,9 @@ class KvCache4:
         self.pages, self.page_size, self.head_dim = pages, page_size, head_dim
         self.kv_heads = pages.shape[1]
         self.device = pages.device
-        self._state = device_state(_device_of(pages)) if pages.is_cuda else None  # made here: never inside a capture
+        # the device's status word, made here and never inside a capture
+        self._state = device_state(pages.device) if pages.is_cuda else None
+        self._status = self._state.status.data_ptr() if pages.is_cuda else None
         self.desc = _lib.Kv4Cache(pages.data_ptr(), stride, pages.shape[0], page_size, self.kv_heads, head_dim)
 
     @staticmethod
@@ -217,15 +227,18 @@ class KvCache4:
         device = self._check(batch)
         rows, dim = batch.rows, self.head_dim
         dtype = k.dtype
-        k = _rows(k, "k", rows, self.kv_heads, dim, None, device)
-        v = _rows(v, "v", rows, self.kv_heads, dim, dtype, device)
+        shape = (rows, self.kv_heads, dim)
+        k = _rows(k, "k", shape, None, device)
+        v = _rows(v, "v", shape, dtype, device)
+        heads = 0
         if q is not None:
-            heads = q.shape[1] if q.ndim == 3 else 0
-            q = _rows(q, "q", rows, heads, dim, dtype, device)
+            heads = _heads(q)
+            shape = (rows, heads, dim)
+            q = _rows(q, "q", shape, dtype, device)
             if q_out is None:
-                q_out = torch.empty((rows, heads, dim), dtype=dtype, device=device)
+                q_out = torch.empty(shape, dtype=dtype, device=device)
             else:
-                _rows(q_out, "q_out", rows, heads, dim, dtype, device, written=True)
+                _rows(q_out, "q_out", shape, dtype, device, written=True)
         elif q_out is not None:
             raise ValueError("q_out needs q")
         turn = None
@@ -258,9 +271,8 @@ class KvCache4:
             return q_out
         with _on(device):
             _lib.check(_lib.library().dmoe_kv4_append(
-                ctypes.byref(self.desc), ctypes.byref(batch.desc), turn, _head_rows(q), q.shape[1] if q is not None else 0,
-                _head_rows(q_out), _head_rows(k), _head_rows(v), _lib.dtype_code(dtype),
-                _lib.ptr(self._state.status), _lib.stream_handle(device)))
+                ctypes.byref(self.desc), ctypes.byref(batch.desc), turn, _head_rows(q), heads, _head_rows(q_out),
+                _head_rows(k), _head_rows(v), _lib.dtype_code(dtype), self._status, _stream(device)))
         return q_out
 
     def read(self, batch: PagedBatch, *, dtype: torch.dtype = torch.float16, k_out: Tensor | None = None,
@@ -273,13 +285,13 @@ class KvCache4:
             k_out = torch.empty(shape, dtype=dtype, device=device)
         if v_out is None:
             v_out = torch.empty(shape, dtype=dtype, device=device)
-        _rows(k_out, "k_out", *shape, dtype, device, written=True)
-        _rows(v_out, "v_out", *shape, dtype, device, written=True)
+        _rows(k_out, "k_out", shape, dtype, device, written=True)
+        _rows(v_out, "v_out", shape, dtype, device, written=True)
         if batch.rows:
             with _on(device):
                 _lib.check(_lib.library().dmoe_kv4_read(
                     ctypes.byref(self.desc), ctypes.byref(batch.desc), _head_rows(k_out), _head_rows(v_out),
-                    _lib.dtype_code(dtype), _lib.ptr(self._state.status), _lib.stream_handle(device)))
+                    _lib.dtype_code(dtype), self._status, _stream(device)))
         return k_out, v_out
 
     def attend(self, q: Tensor, batch: PagedBatch, *, scale: float | None = None, window: int = 0,
@@ -289,25 +301,25 @@ class KvCache4:
         that sees none becomes 0.  ``scale`` defaults to D ** -0.5.  Rows that
         no sequence owns are not written (in a new ``out`` they hold nothing)."""
         device = self._check(batch)
-        heads = q.shape[1] if q.ndim == 3 else 0
-        q = _rows(q, "q", batch.rows, heads, self.head_dim, None, device)
+        heads = _heads(q)
+        shape = (batch.rows, heads, self.head_dim)
+        q = _rows(q, "q", shape, None, device)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError("query heads must be a multiple of the key/value heads")
         if out is None:
-            out = torch.empty((batch.rows, heads, self.head_dim), dtype=q.dtype, device=device)
+            out = torch.empty(shape, dtype=q.dtype, device=device)
         else:
-            _rows(out, "out", batch.rows, heads, self.head_dim, q.dtype, device, written=True)
+            _rows(out, "out", shape, q.dtype, device, written=True)
         if batch.rows == 0:
             return out
         lib = _lib.library()
         cache, desc = ctypes.byref(self.desc), ctypes.byref(batch.desc)
         with _on(device):
             need = lib.dmoe_kv4_attention_workspace_bytes(cache, desc, heads)
-            scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+            scratch = torch.empty(need, dtype=torch.uint8, device=device)
             _lib.check(lib.dmoe_kv4_attention(
                 cache, desc, _head_rows(q), heads, self.head_dim ** -0.5 if scale is None else scale, window,
-                _head_rows(out), _lib.dtype_code(q.dtype), _lib.ptr(scratch), scratch.numel(),
-                _lib.ptr(self._state.status), _lib.stream_handle(device)))
+                _head_rows(out), _lib.dtype_code(q.dtype), scratch.data_ptr(), need, self._status, _stream(device)))
         return out
 
 
@@ -325,3 +337,8 @@ _HERE = _Here()
 def _on(device: torch.device):
     """The launches of a call go to its tensors' device, whichever is current."""
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    """hipStream_t of torch's current stream on ``device``."""
+    return torch._C._cuda_getCurrentRawStream(device.index)

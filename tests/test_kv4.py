@@ -150,7 +150,7 @@ def test_entry_points_refuse_bad_descriptors(entry, change, message):
     ("attend", dict(), dict(scale=float("inf")), "scale"),
     ("attend", dict(), dict(window=-1), "window"),
     ("attend", dict(), dict(ws=None), "workspace too small"),
-    ("attend", dict(), dict(ws_bytes=64), "workspace too small"),
+    ("attend", dict(batch=dict(table_cols=400, table_stride=400)), dict(ws_bytes=64), "workspace too small"),
     ("attend", dict(), dict(ws=FAKE + 8), "workspace must be 16-byte aligned"),
     ("attend", dict(), dict(q=_lib.HeadRows(FAKE, 512, 0)), "out rows overlap"),
 ])
@@ -163,7 +163,8 @@ def test_workspace_covers_more_rows_with_more_bytes():
     lib, by = _lib.library(), ctypes.byref
     sizes = []
     for rows, most in ((2, 1), (600, 300), (6000, 3000)):
-        cache, batch, _, _ = descriptors(batch=dict(rows=rows, max_rows=most, block_table=None, lengths=None))
+        cache, batch, _, _ = descriptors(batch=dict(rows=rows, max_rows=most, block_table=None, lengths=None,
+                                                    table_cols=900, table_stride=900))
         sizes.append(lib.dmoe_kv4_attention_workspace_bytes(by(cache), by(batch), 4))
     assert 0 < sizes[0] <= sizes[1] <= sizes[2]
     cache, batch, _, _ = descriptors(batch=dict(seqs=0))
