@@ -72,7 +72,9 @@ __device__ __forceinline__ void widen8(const v4i& raw, int dtype, float (&x)[8])
 
 // Two values as a word of a bf16 or fp16 row.
 __device__ __forceinline__ uint32_t narrow2(float a, float b, int dtype) {
-    return dtype == kBF16 ? f32_to_bf16(a) | (uint32_t)f32_to_bf16(b) << 16 : f32_to_f16(a) | (uint32_t)f32_to_f16(b) << 16;
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    return dtype == kBF16 ? __builtin_bit_cast(uint32_t, v2bf{(__bf16)a, (__bf16)b})
+                          : __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});
 }
 
 // A query row of which this lane holds N words of eight channels: into fp16

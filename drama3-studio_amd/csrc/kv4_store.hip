@@ -19,87 +19,116 @@ namespace dmoe {
 namespace {
 
 constexpr int kThreads = 256;
+// A workgroup takes several rows where that leaves this many of them: below, the chip is not full.
+constexpr int kFull = 512;
 
-// The sequence that owns row `row`, and the row's place in its cache; false if
-// no sequence owns it.  Every lane of the wave calls this with the same row.
-__device__ __forceinline__ bool locate_row(const Kv4Batch& b, int page_shift, int row, int* status, int& seq, int& pos) {
-    seq = row;
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// Where a row's token is kept.
+struct Place {
+    uint8_t* page;  // null: a table entry names no page
+    int pos;        // place in the sequence, -1 if no sequence owns the row or it has none
+};
+
+// Every lane of the wave calls this with the same row.
+__device__ __forceinline__ Place place_of(const Kv4Cache& c, const Kv4Batch& b, int row, int* status) {
+    Place none{nullptr, -1};
+    if (row >= b.rows) return none;
+    int seq = row;
     if (b.starts) {
         seq = 0;
-        for (int s = threadIdx.x & 63; s - (int)(threadIdx.x & 63) < b.seqs; s += kWave)
-            seq += __popcll(__ballot(s < b.seqs && b.starts[min(s, b.seqs - 1) + 1] <= row));
+        const int lane = threadIdx.x & 63;
+        for (int s = 0; s < b.seqs; s += kWave)
+            seq += __popcll(__ballot(s + lane < b.seqs && b.starts[min(s + lane, b.seqs - 1) + 1] <= row));
     }
-    if (seq >= b.seqs) return false;
+    if (seq >= b.seqs) return none;
     bool bad;
-    const Kv4Seq q = kv4_seq(b, page_shift, seq, bad);
+    const Kv4Seq q = kv4_seq(b, c.page_shift, seq, bad);
     if (bad && status) raise_status(status, kBadBatch);
-    pos = q.len - q.n + (row - q.row0);
-    return row >= q.row0 && row < q.row0 + q.n && pos >= 0;
+    const int pos = q.len - q.n + (row - q.row0);
+    if (row < q.row0 || row >= q.row0 + q.n || pos < 0) return none;
+    const int page = b.table[(int64_t)seq * b.table_stride + (pos >> c.page_shift)];
+    const bool off = (unsigned)page >= (unsigned)c.num_pages;
+    if (off && status) raise_status(status, kBadBatch);
+    return Place{off ? nullptr : c.pages + (int64_t)page * c.page_stride, pos};
 }
 
-// Page and slot of a token, or null where its table entry names no page.
-__device__ __forceinline__ uint8_t* token_page(const Kv4Cache& c, const Kv4Batch& b, int seq, int pos, int* status) {
-    const int page = b.table[(int64_t)seq * b.table_stride + (pos >> c.page_shift)];
-    if ((unsigned)page >= (unsigned)c.num_pages) {
-        if (status) raise_status(status, kBadBatch);
-        return nullptr;
-    }
-    return c.pages + (int64_t)page * c.page_stride;
-}
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ void unpack8(const v4i& raw, int dtype, float (&x)[8]) {
+    if (dtype == kBF16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t w = (uint32_t)raw[i];
-        x[2 * i] = dtype == kBF16 ? bf16_to_f32(w & 0xFFFF) : f16_to_f32(w & 0xFFFF);
-        x[2 * i + 1] = dtype == kBF16 ? bf16_to_f32(w >> 16) : f16_to_f32(w >> 16);
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float((uint32_t)raw[i] << 16);
+            x[2 * i + 1] = __uint_as_float((uint32_t)raw[i] & 0xFFFF0000u);
+        }
+    } else {
+        const v8h h = __builtin_bit_cast(v8h, raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
     }
 }
 
 __device__ __forceinline__ v4i pack8(const float (&x)[8], int dtype) {
-    v4i raw;
+    if (dtype == kBF16) {
+        v8bf h;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        raw[i] = dtype == kBF16 ? (int)(f32_to_bf16(x[2 * i]) | (uint32_t)f32_to_bf16(x[2 * i + 1]) << 16)
-                                : (int)(f32_to_f16(x[2 * i]) | (uint32_t)f32_to_f16(x[2 * i + 1]) << 16);
-    return raw;
+        for (int i = 0; i < 8; ++i) h[i] = (__bf16)x[i];
+        return __builtin_bit_cast(v4i, h);
+    }
+    v8h h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)x[i];
+    return __builtin_bit_cast(v4i, h);
 }
 
 // Eight codes of this lane's channels, low nibble first, and the scale word of
 // the 32 channels that it shares with the three lanes beside it.
 __device__ __forceinline__ uint32_t quantize8(float (&x)[8], uint32_t& scale_word, bool& odd) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);  // a NaN is the largest
+    odd = most > __float_as_uint(kKv4Limit);
+    if (odd) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] == x[i] ? fminf(fmaxf(x[i], -kKv4Limit), kKv4Limit) : 0.0f;
+    }
     float lo = 0.0f, hi = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float v = x[i] == x[i] ? fminf(fmaxf(x[i], -kKv4Limit), kKv4Limit) : 0.0f;
-        odd |= v != x[i];
-        x[i] = v;
-        lo = fminf(lo, v);
-        hi = fmaxf(hi, v);
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
     }
     lo = fminf(lo, dpp_f32<kDppXor1>(lo));
     hi = fmaxf(hi, dpp_f32<kDppXor1>(hi));
     lo = fminf(lo, dpp_f32<kDppXor2>(lo));
     hi = fmaxf(hi, dpp_f32<kDppXor2>(hi));
     const float r = hi - lo;
-    const float step = r / 15.0f;
-    float s;
-    if (step >= 0x1p-14f) {  // up to seven significant bits
-        s = __uint_as_float((__float_as_uint(step) + 0x1FFFFu) & ~0x1FFFFu);
-        if (15.0f * s < r) s = __uint_as_float(__float_as_uint(s) + 0x20000u);
-    } else {  // fp16 subnormals without their four lowest bits
+    // the next number of the scales' grid at or above about r / 15 -- seven
+    // significant bits, or fp16 subnormals without their four lowest -- and,
+    // as 15 s is exact, the smallest that reaches r
+    const float step = r * 0.06666667f;
+    float s, less, more;
+    if (step >= 0x1p-14f) {
+        const uint32_t b = (__float_as_uint(step) + 0x1FFFFu) & ~0x1FFFFu;
+        s = __uint_as_float(b);
+        less = __uint_as_float(b - 0x20000u);
+        more = __uint_as_float(b + 0x20000u);
+    } else {
         s = ceilf(step * 0x1p20f) * 0x1p-20f;
-        if (15.0f * s < r) s += 0x1p-20f;
+        less = s - 0x1p-20f;
+        more = s + 0x1p-20f;
     }
+    s = 15.0f * s < r ? more : less > 0.0f && 15.0f * less >= r ? less : s;
     scale_word = 0;
     uint32_t word = 0;
     if (s > 0.0f) {
-        const float y = 1.0f / s;
+        const float y = __builtin_amdgcn_rcpf(s), middle = 0.5f * s;
         const auto quotient = [&](float v) {
-            float t = __builtin_rintf(v * y);
-            const float left = __builtin_fmaf(-t, s, v), two = 2.0f * fabsf(left);
-            if (two > s || (two == s && ((int)t & 1))) t += left > 0.0f ? 1.0f : -1.0f;
-            return (int)t;
+            const float t = __builtin_rintf(v * y);
+            const float left = __builtin_fmaf(-t, s, v), off = fabsf(left);
+            const bool odd_tie = off == middle && ((int)t & 1);
+            return (int)t + (off > middle || odd_tie ? (left > 0.0f ? 1 : -1) : 0);
         };
         const int z = min(quotient(-lo), 15);
         scale_word = f32_to_f16(s) | (uint32_t)z;
@@ -109,16 +138,42 @@ __device__ __forceinline__ uint32_t quantize8(float (&x)[8], uint32_t& scale_wor
     return word;
 }
 
-// One row a workgroup (blockIdx.x), one 8-channel chunk of one head a thread:
-// query heads first, then key and value heads.
+// Rotates the channels c0..c0+7 of a head, x; y are those half a rotation
+// away, negative for the first of each pair (not used where pairs are
+// neighbours).
+template <class F>
+__device__ __forceinline__ void rotate8(const F (&turn)[144][2], bool interleaved, int half, int c0, float (&x)[8], const float (&y)[8]) {
+    if (interleaved) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const int f = (c0 + j) / 2;
+            const F c = turn[f + f / 8][0], s = turn[f + f / 8][1], u = x[j], w = x[j + 1];
+            x[j] = (float)(u * c - w * s);
+            x[j + 1] = (float)(w * c + u * s);
+        }
+        return;
+    }
+    const int f0 = c0 - (c0 >= half ? half : 0), at = f0 + f0 / 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const F c = turn[at + j][0], s = turn[at + j][1];
+        x[j] = (float)((F)x[j] * c + (F)y[j] * s);
+    }
+}
+
+// kRows rows a workgroup (blockIdx.x), one 8-channel chunk of one head a
+// thread: query heads first, then key and value heads.
+template <int kRows>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4AppendArgs a) {
-    __shared__ double turn[128][2];
-    const int dim = a.cache.dim, chunks = dim / 8;
-    const int row = blockIdx.x;
-    int seq, pos;
-    if (!locate_row(a.batch, a.cache.page_shift, row, a.status, seq, pos)) return;
+    // cosine and sine of each frequency, in 64 bits for keys, in 32 for queries; one entry in nine is left
+    // free, so that the chunks' entries lie in different banks
+    __shared__ double turn[kRows][144][2];
+    __shared__ float turn_q[kRows][144][2];
+    __shared__ Place places[kRows];
+    const int dim = a.cache.dim, chunks = dim / 8, log2 = __builtin_ctz(chunks);
+    const int row0 = blockIdx.x * kRows;
     const int unit = blockIdx.y * kThreads + threadIdx.x;
-    const int head = unit / chunks, chunk = unit % chunks;
+    const int head = unit >> log2, chunk = unit & (chunks - 1);
     const int kv = a.cache.kv_heads, heads = a.q_heads + 2 * kv;
     const bool is_v = head >= a.q_heads + kv, is_q = head < a.q_heads, live = head < heads;
     const int local = is_q ? head : is_v ? head - a.q_heads - kv : head - a.q_heads;
@@ -126,108 +181,136 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4AppendArgs a) {
     const int half = a.rotary.inv_freq ? a.rotary.dim / 2 : 0;
     const int c0 = chunk * 8;
     const bool turns = !is_v && c0 < 2 * half;
-    const bool apart = turns && !a.rotary.interleaved;  // the other channels of the pairs lie half a rotation away
-    v4i raw = {0, 0, 0, 0}, other = {0, 0, 0, 0};
+    // the lane with the other channels of the pairs; a head's lanes lie in one wave
+    const int partner = (threadIdx.x & 63) + (a.rotary.interleaved ? 0 : c0 < half ? half / 8 : -(half / 8));
+    v4i raw[kRows];
     if (live) {
-        const uint16_t* p = (const uint16_t*)src.p + (int64_t)row * src.row_stride + (int64_t)local * src.head_stride;
-        raw = *(const v4i*)(p + c0);
-        if (apart) other = *(const v4i*)(p + (c0 < half ? c0 + half : c0 - half));
-    }
-    for (int i = threadIdx.x; i < half; i += kThreads) {
-        double place = pos;
-        if (a.rotary.positions) {
-            const int axis = a.rotary.axis ? a.rotary.axis[i] : 0;
-            const int64_t at = (int64_t)min(axis, a.rotary.axes - 1) * a.rotary.axis_stride + row;
-            place = (double)load_id(a.rotary.positions, at, a.rotary.positions_dtype);
+        const uint16_t* p = (const uint16_t*)src.p + (int64_t)local * src.head_stride + c0;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const uint16_t* x = p + (int64_t)min(row0 + i, a.batch.rows - 1) * src.row_stride;
+            raw[i] = *(const v4i*)x;
         }
-        const double turns_of = place * (double)a.rotary.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
-        sincospi(2.0 * (turns_of - rint(turns_of)), &turn[i][1], &turn[i][0]);
+    }
+    for (int i = wave_index(); i < kRows; i += kThreads / kWave) {
+        const Place place = place_of(a.cache, a.batch, row0 + i, a.status);
+        if ((threadIdx.x & 63) == 0) places[i] = place;
+    }
+    if (!a.rotary.positions) __syncthreads();
+    for (int i = threadIdx.x; i < kRows * half; i += kThreads) {
+        const int row = i / half, f = i - row * half;
+        double place;
+        if (a.rotary.positions) {
+            const int axis = a.rotary.axis ? a.rotary.axis[f] : 0;
+            const int64_t at = (int64_t)min(axis, a.rotary.axes - 1) * a.rotary.axis_stride + min(row0 + row, a.batch.rows - 1);
+            place = (double)load_id(a.rotary.positions, at, a.rotary.positions_dtype);
+        } else {
+            place = (double)places[row].pos;
+        }
+        const double turns_of = place * (double)a.rotary.inv_freq[f] * 0.15915494309189533577;  // 1 / (2 pi)
+        double cosine, sine;
+        sincospi(2.0 * (turns_of - rint(turns_of)), &sine, &cosine);
+        const int at = f + f / 8;
+        turn[row][at][0] = cosine;
+        turn[row][at][1] = sine;
+        turn_q[row][at][0] = (float)cosine;
+        turn_q[row][at][1] = (float)sine;
     }
     __syncthreads();
     if (!live) return;
-    float x[8];
-    unpack8(raw, a.dtype, x);
-    if (turns) {
-        float y[8];
-        unpack8(other, a.dtype, y);
-        const bool second = c0 >= half;
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            if (apart) {
-                const double* t0 = turn[c0 + i - (second ? half : 0)];
-                const double* t1 = turn[c0 + i + 1 - (second ? half : 0)];
-                const double s0 = second ? t0[1] : -t0[1], s1 = second ? t1[1] : -t1[1];
-                x[i] = (float)((double)x[i] * t0[0] + (double)y[i] * s0);
-                x[i + 1] = (float)((double)x[i + 1] * t1[0] + (double)y[i + 1] * s1);
-            } else {
-                const double* t = turn[(c0 + i) / 2];
-                const double u = x[i], w = x[i + 1];
-                x[i] = (float)(u * t[0] - w * t[1]);
-                x[i + 1] = (float)(w * t[0] + u * t[1]);
-            }
+    for (int i = 0; i < kRows; ++i) {
+        const Place place = places[i];
+        if (place.pos < 0) continue;
+        float x[8];
+        unpack8(raw[i], a.dtype, x);
+        if (turns) {
+            float y[8];
+            v4i other;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) other[j] = __shfl(raw[i][j], partner, kWave) ^ (c0 < half ? (int)0x80008000 : 0);
+            unpack8(other, a.dtype, y);
+            if (is_q) rotate8<float>(turn_q[i], a.rotary.interleaved, half, c0, x, y);
+            else rotate8<double>(turn[i], a.rotary.interleaved, half, c0, x, y);
         }
+        if (is_q) {
+            uint16_t* o = (uint16_t*)a.q_out.p + (int64_t)(row0 + i) * a.q_out.row_stride + (int64_t)local * a.q_out.head_stride;
+            *(v4i*)(o + c0) = pack8(x, a.dtype);
+            continue;
+        }
+        uint32_t scale_word;
+        bool odd;
+        const uint32_t word = quantize8(x, scale_word, odd);
+        if (odd && a.status) raise_status(a.status, kNonFinite);
+        if (!place.page) continue;
+        const int size = 1 << a.cache.page_shift, slot = place.pos & (size - 1);
+        uint8_t* base = place.page + local * kv4_head_bytes(size, dim);
+        uint16_t* scales = (uint16_t*)(base + (int64_t)size * dim) + (is_v ? size * (dim / kKv4Group) : 0);
+        if (is_v) ((uint32_t*)(base + size * dim / 2))[(slot / 4 * chunks + chunk) * 4 + slot % 4] = word;
+        else ((uint32_t*)base)[slot * chunks + chunk] = word;
+        if (chunk % 4 == 0) scales[chunk / 4 * size + slot] = (uint16_t)scale_word;
     }
-    if (is_q) {
-        uint16_t* o = (uint16_t*)a.q_out.p + (int64_t)row * a.q_out.row_stride + (int64_t)local * a.q_out.head_stride;
-        *(v4i*)(o + c0) = pack8(x, a.dtype);
-        return;
-    }
-    uint8_t* page = token_page(a.cache, a.batch, seq, pos, a.status);
-    uint32_t scale_word;
-    bool odd = false;
-    const uint32_t word = quantize8(x, scale_word, odd);
-    if (odd && a.status) raise_status(a.status, kNonFinite);
-    if (!page) return;
-    const int size = 1 << a.cache.page_shift, slot = pos & (size - 1);
-    uint8_t* base = page + local * kv4_head_bytes(size, dim);
-    uint16_t* scales = (uint16_t*)(base + (int64_t)size * dim) + (is_v ? size * (dim / kKv4Group) : 0);
-    if (is_v) ((uint32_t*)(base + size * dim / 2))[(slot / 4 * chunks + chunk) * 4 + slot % 4] = word;
-    else ((uint32_t*)base)[slot * chunks + chunk] = word;
-    if (chunk % 4 == 0) scales[chunk / 4 * size + slot] = (uint16_t)scale_word;
 }
 
-// One row a workgroup, one 8-channel chunk of a key or value head a thread.
+// kRows rows a workgroup, one 8-channel chunk of a key or value head a thread.
+template <int kRows>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4ReadArgs a) {
-    const int dim = a.cache.dim, chunks = dim / 8, kv = a.cache.kv_heads;
-    const int row = blockIdx.x;
-    int seq, pos;
-    if (!locate_row(a.batch, a.cache.page_shift, row, a.status, seq, pos)) return;
+    __shared__ Place places[kRows];
+    const int dim = a.cache.dim, chunks = dim / 8, log2 = __builtin_ctz(chunks), kv = a.cache.kv_heads;
+    const int row0 = blockIdx.x * kRows;
     const int unit = blockIdx.y * kThreads + threadIdx.x;
-    const int head = unit / chunks, chunk = unit % chunks;
-    if (head >= 2 * kv) return;
-    const bool is_v = head >= kv;
+    const int head = unit >> log2, chunk = unit & (chunks - 1);
+    const bool is_v = head >= kv, live = head < 2 * kv;
     const int local = is_v ? head - kv : head;
-    const uint8_t* page = token_page(a.cache, a.batch, seq, pos, a.status);
-    float x[8] = {};
-    if (page) {
-        const int size = 1 << a.cache.page_shift, slot = pos & (size - 1);
-        const uint8_t* base = page + local * kv4_head_bytes(size, dim);
-        const uint16_t* scales = (const uint16_t*)(base + (int64_t)size * dim) + (is_v ? size * (dim / kKv4Group) : 0);
-        const uint32_t word = is_v ? ((const uint32_t*)(base + size * dim / 2))[(slot / 4 * chunks + chunk) * 4 + slot % 4]
-                                   : ((const uint32_t*)base)[slot * chunks + chunk];
-        const uint32_t sw = scales[chunk / 4 * size + slot];
-        const float s = f16_to_f32(sw & 0xFFF0);
-        const int z = sw & 15;
+    for (int i = wave_index(); i < kRows; i += kThreads / kWave) {
+        const Place place = place_of(a.cache, a.batch, row0 + i, a.status);
+        if ((threadIdx.x & 63) == 0) places[i] = place;
+    }
+    __syncthreads();
+    if (!live) return;
+    const int size = 1 << a.cache.page_shift;
+    const int64_t head_at = local * kv4_head_bytes(size, dim);
+    uint32_t word[kRows], scale[kRows];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)((int)(word >> (4 * i) & 15) - z) * s;
+    for (int i = 0; i < kRows; ++i) {
+        word[i] = scale[i] = 0;
+        const Place place = places[i];
+        if (!place.page) continue;
+        const int slot = place.pos & (size - 1);
+        const uint8_t* base = place.page + head_at;
+        const uint16_t* scales = (const uint16_t*)(base + (int64_t)size * dim) + (is_v ? size * (dim / kKv4Group) : 0);
+        word[i] = is_v ? ((const uint32_t*)(base + size * dim / 2))[(slot / 4 * chunks + chunk) * 4 + slot % 4]
+                       : ((const uint32_t*)base)[slot * chunks + chunk];
+        scale[i] = scales[chunk / 4 * size + slot];
     }
     const Kv4Rows& dst = is_v ? a.v : a.k;
-    uint16_t* o = (uint16_t*)dst.p + (int64_t)row * dst.row_stride + (int64_t)local * dst.head_stride;
-    *(v4i*)(o + chunk * 8) = pack8(x, a.dtype);
+    uint16_t* o = (uint16_t*)dst.p + (int64_t)local * dst.head_stride + chunk * 8;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        if (places[i].pos < 0) continue;
+        const float s = f16_to_f32(scale[i] & 0xFFF0);
+        const int z = scale[i] & 15;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (float)((int)(word[i] >> (4 * j) & 15) - z) * s;
+        *(v4i*)(o + (int64_t)(row0 + i) * dst.row_stride) = pack8(x, a.dtype);
+    }
 }
 
 }  // namespace
 
 void launch_kv4_append(const Kv4AppendArgs& a, hipStream_t st) {
     const int units = (a.q_heads + 2 * a.cache.kv_heads) * (a.cache.dim / 8);
-    const dim3 grid(a.batch.rows, (units + kThreads - 1) / kThreads);
-    kv4_append_kernel<<<grid, kThreads, 0, st>>>(a);
+    const unsigned parts = (units + kThreads - 1) / kThreads;
+    if ((int64_t)a.batch.rows * parts < 8 * kFull) kv4_append_kernel<1><<<dim3(a.batch.rows, parts), kThreads, 0, st>>>(a);
+    else kv4_append_kernel<8><<<dim3((a.batch.rows + 7) / 8, parts), kThreads, 0, st>>>(a);
 }
 
 void launch_kv4_read(const Kv4ReadArgs& a, hipStream_t st) {
     const int units = 2 * a.cache.kv_heads * (a.cache.dim / 8);
-    const dim3 grid(a.batch.rows, (units + kThreads - 1) / kThreads);
-    kv4_read_kernel<<<grid, kThreads, 0, st>>>(a);
+    const unsigned parts = (units + kThreads - 1) / kThreads;
+    if ((int64_t)a.batch.rows * parts < 8 * kFull) kv4_read_kernel<1><<<dim3(a.batch.rows, parts), kThreads, 0, st>>>(a);
+    else kv4_read_kernel<8><<<dim3((a.batch.rows + 7) / 8, parts), kThreads, 0, st>>>(a);
 }
 
 }  // namespace dmoe

@@ -135,9 +135,11 @@ def test_append_writes_the_reference_bytes_and_nothing_else(cuda, dim, hq, hkv, 
             placed.append(row), held_k.append(k), held_v.append(v)
     assert np.array_equal(cache.pages.cpu().numpy(), pages.raw)
     assert len(placed) == 1 + 5 + 16 + 33 + 2
-    # products and sum in 64 bits, one rounding to fp32 and one to the type
+    # cosine and sine, a product and a sum rounded to fp32 (2^-24 each, of at most |a| + |b| <= sqrt(2) times the
+    # pair's length, which is at most sqrt(2) times the head's largest value), then the result to the type
     err = np.abs(wide(q_out)[placed] - turned[placed, :hq])
-    assert (err <= (EPS[dtype] / 2 + 2.0 ** -23) * np.abs(turned[placed, :hq]) + 2.0 ** -25).all()
+    most = np.abs(x[placed, :hq]).max(-1, keepdims=True)
+    assert (err <= EPS[dtype] / 2 * np.abs(turned[placed, :hq]) + 4 * 2.0 ** -24 * 2 * most * (1 + EPS[dtype]) + 2.0 ** -25).all()
     missing = sorted(set(range(case.rows)) - set(placed))
     assert (q_out[missing] == 55.0).all()
     k, v = cache.read(batch)
