@@ -434,7 +434,7 @@ Kv4Shape kv4_attend_shape(const Kv4Batch& b, int page_size, int kv_heads, int di
     const int64_t most_rows = (int64_t)b.max_rows * group;
     s.tile_rows = most_rows <= 16 ? 16 : kv4_tile_rows(most_rows, dim);
     s.slots_log2 = most_rows <= 16 ? 11 : kv4_tile_slots_log2(most_rows, dim);
-    s.one_tile = most_rows <= s.tile_rows;
+    s.one_tile = most_rows <= 64;  // the kernel of many rows cuts into tiles also where one would do
     // a wave of few rows has little more to do for two blocks than for one; a
     // tile of many rows shorter than kKv4Whole is not worth joining
     const int64_t most_blocks = ((int64_t)b.table_cols * page_size + kKv4Block - 1) / kKv4Block;

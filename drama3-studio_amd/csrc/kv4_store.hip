@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kThreads = 256;
 // A workgroup takes several rows where that leaves this many of them: below, the chip is not full.
-constexpr int kFull = 512;
+constexpr int kFull = 1024;
 
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
