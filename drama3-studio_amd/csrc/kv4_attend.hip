@@ -39,21 +39,26 @@ struct Values {
 };
 
 // Pages of this lane's four key tokens and 16 value tokens of a block.  Tokens
-// behind the last visible one are read from wherever page 0 has them, and masked.
+// behind the last one are read from its page, and masked.
 struct Pages {
     int key, value;
 };
 __device__ __forceinline__ Pages pages_of(const Kv4AttendArgs& a, int seq, int block, int end, int r, int g) {
     const int32_t* table = a.batch.table + (int64_t)seq * a.batch.table_stride;
-    const int kt = block * kKv4Block + 4 * r, vt = block * kKv4Block + 16 * g, shift = a.cache.page_shift;
-    return Pages{kt < end ? table[kt >> shift] : 0, vt < end ? table[vt >> shift] : 0};
+    const int kt = min(block * kKv4Block + 4 * r, end - 1), vt = min(block * kKv4Block + 16 * g, end - 1), shift = a.cache.page_shift;
+    return Pages{table[kt >> shift], table[vt >> shift]};
+}
+
+// The part of a page that one head has; of page 0 where the table's entry is none.
+template <int D>
+__device__ __forceinline__ const uint8_t* part_of(const Kv4AttendArgs& a, int page, int head) {
+    if ((unsigned)page >= (unsigned)a.cache.num_pages) page = 0;
+    return a.cache.pages + (int64_t)page * a.cache.page_stride + (int64_t)head * kv4_head_bytes(1 << a.cache.page_shift, D);
 }
 
 template <int D>
-__device__ __forceinline__ void load_keys(const Kv4AttendArgs& a, int page, int head, int block, int r, int g, Keys<D>& keys) {
+__device__ __forceinline__ void load_keys(const Kv4AttendArgs& a, const uint8_t* base, int block, int r, int g, Keys<D>& keys) {
     const int size = 1 << a.cache.page_shift;
-    if ((unsigned)page >= (unsigned)a.cache.num_pages) page = 0;
-    const uint8_t* base = a.cache.pages + (int64_t)page * a.cache.page_stride + (int64_t)head * kv4_head_bytes(size, D);
     const int slot = (block * kKv4Block + 4 * r) & (size - 1);
     const uint8_t* codes = base + slot * (D / 2) + g * (D / 8);
     if constexpr (D == 64) {
@@ -76,11 +81,8 @@ __device__ __forceinline__ void load_keys(const Kv4AttendArgs& a, int page, int 
 }
 
 template <int D>
-__device__ __forceinline__ void load_values(const Kv4AttendArgs& a, int page, int head, int block, int r, int g, Values<D>& values) {
+__device__ __forceinline__ void load_values(const Kv4AttendArgs& a, const uint8_t* base, int block, int r, int g, Values<D>& values) {
     const int size = 1 << a.cache.page_shift;
-    values.bad = (unsigned)page >= (unsigned)a.cache.num_pages;
-    if (values.bad) page = 0;
-    const uint8_t* base = a.cache.pages + (int64_t)page * a.cache.page_stride + (int64_t)head * kv4_head_bytes(size, D);
     const int slot = (block * kKv4Block + 16 * g) & (size - 1);
 #pragma unroll
     for (int c = 0; c < Values<D>::kParts; ++c) {
@@ -137,15 +139,17 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendA
         const int place = p_first + min(r, max(packed, 1) - 1) / a.group;
         const bool goes_on = more && ahead.from < ahead.to;
         const auto pages_at = [&](int block) {  // also of the next segment's blocks, as if they lay behind this one's
-            if (block < to) return pages_of(a, it.seq, block, it.len, r, g);
-            const int there = ahead.from + block - to;
-            return more && there < ahead.to ? pages_of(a, ahead.seq, there, ahead.len, r, g) : Pages{};
+            const bool here = block < to || !goes_on;
+            return pages_of(a, here ? it.seq : ahead.seq, here ? block : ahead.from + block - to, here ? it.len : ahead.len, r, g);
         };
         if (!loaded && from < to) {
             const Pages now = pages_of(a, it.seq, from, it.len, r, g);
             pages = pages_at(from + 1);
-            load_keys<D>(a, now.key, it.head, from, r, g, keys);
-            load_values<D>(a, now.value, it.head, from, r, g, values);
+            load_keys<D>(a, part_of<D>(a, now.key, it.head), from, r, g, keys);
+            load_values<D>(a, part_of<D>(a, now.value, it.head), from, r, g, values);
+            values.bad = (unsigned)now.value >= (unsigned)a.cache.num_pages;
+        } else if (from + 1 == to) {
+            pages = pages_at(to);  // what follows a single block was not known before
         }
 
         v8h query[kSteps];
@@ -183,13 +187,17 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendA
                     s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, query[j], s[i], 0, 0, 0);
                 }
             }
-            // the next block, in this segment or the one after it
-            const bool here = block + 1 < to, next = here || goes_on;
-            const int next_head = here ? it.head : ahead.head, next_block = here ? block + 1 : ahead.from;
-            if (next) load_keys<D>(a, pages.key, next_head, next_block, r, g, keys);
-            const Pages after = pages_at(block + 2);
+            // The next block, in this segment or the one after it.  The last one of
+            // all is loaded once more: a load that only some blocks have would be
+            // waited for in all of them.
+            const bool here = block + 1 < to || !goes_on;
+            const int next_head = here ? it.head : ahead.head, next_block = here ? min(block + 1, to - 1) : ahead.from;
+            load_keys<D>(a, part_of<D>(a, pages.key, next_head), next_block, r, g, keys);
 
             // s[i][x]: token 16 g + 4 x + i of the block
+            v4u scales[kParts][2];
+#pragma unroll
+            for (int c = 0; c < kParts; ++c) scales[c][0] = values.scales[c][0], scales[c][1] = values.scales[c][1];
             const int first = block * kKv4Block;
             if (any_bad || first + kKv4Block - 1 > p_first || (a.window > 0 && first <= p_last - a.window)) {
                 // tokens 16 g + 0..15 of the block that the row sees: those in [low, high]
@@ -208,7 +216,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendA
                 for (int c = 0; c < kParts; ++c)
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
-                        values.scales[c][x / 4][x % 4] &= (2 * x < kept ? 0xFFFFu : 0u) | (2 * x + 1 < kept ? 0xFFFF0000u : 0u);
+                        scales[c][x / 4][x % 4] &= (2 * x < kept ? 0xFFFFu : 0u) | (2 * x + 1 < kept ? 0xFFFF0000u : 0u);
             }
             float top = s[0][0];
 #pragma unroll
@@ -245,7 +253,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendA
                 for (int h = 0; h < 2; ++h) {
                     Scales sc[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) sc[x] = scales_of(bits, values.scales[c][h][x]);
+                    for (int x = 0; x < 4; ++x) sc[x] = scales_of(bits, scales[c][h][x]);
                     // words of this lane's channels for tokens 8h..8h+7 of its 16
                     uint32_t w[8];
 #pragma unroll
@@ -272,8 +280,14 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendA
                         out[o + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(upper, p[h], out[o + 1], 0, 0, 0);
                     }
                 }
-            if (next) load_values<D>(a, pages.value, next_head, next_block, r, g, values);
-            pages = after;
+            // The pages after are loaded behind the last use of these: a copy of
+            // theirs left to the loop's end would wait for every load.
+            int64_t base = part_of<D>(a, pages.value, next_head) - a.cache.pages;
+            values.bad = (unsigned)pages.value >= (unsigned)a.cache.num_pages;
+            int after = block + 2;
+            asm("" : "+v"(base), "+s"(after));
+            pages = pages_at(after);
+            load_values<D>(a, a.cache.pages + base, next_block, r, g, values);
         }
         loaded = from < to && goes_on;
         if (more && ahead.n) load_query(ahead);

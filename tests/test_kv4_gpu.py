@@ -235,6 +235,21 @@ def test_several_rows_a_sequence(cuda, dim, hq, hkv, page, dtype, seqs, window):
         assert (out[at:at + empty] == 0).all()
 
 
+@pytest.mark.parametrize("dim,hq,hkv,seqs,longest", [
+    (64, 8, 4, 1300, 60), (64, 2, 2, 1400, 190), (128, 16, 8, 333, 64), (256, 4, 2, 1100, 100)])
+@pytest.mark.parametrize("window", [0, 40])
+def test_more_sequences_than_there_is_room_for(cuda, dim, hq, hkv, seqs, longest, window):
+    # one token each: several sequences, most of one block, come to one wave
+    print_case("kv4 crowd", dim, hq, hkv, seqs, longest, window)
+    lengths = torch.randint(1, longest + 1, (seqs,), generator=torch.Generator().manual_seed(seqs)).tolist()
+    case = Case(cuda, [(int(n % 11 != 0), n) for n in lengths], hq, hkv, dim, 64, torch.bfloat16, seed=seqs)
+    # any codes, scales of 2^-7 to 2^-6 with any zero point
+    case.raw.copy_(torch.randint(0, 256, case.raw.shape, dtype=torch.uint8, generator=case.g))
+    scales = case.raw[:, :, 64 * dim:].view(torch.int16)
+    scales.copy_(scales & 0x03FF | 0x2000)
+    check_attend(case, case.random(hq), window=window)
+
+
 def test_default_tables_and_strided_queries(cuda):
     """No starts: a row a sequence; q as a slice, heads first in memory, a broadcast row, an odd address."""
     print_case("kv4 attend strides")
