@@ -53,7 +53,7 @@ __device__ __forceinline__ Pages pages_of(const Kv4AttendArgs& a, int seq, int b
 template <int D>
 __device__ __forceinline__ const uint8_t* part_of(const Kv4AttendArgs& a, int page, int head) {
     if ((unsigned)page >= (unsigned)a.cache.num_pages) page = 0;
-    return a.cache.pages + (int64_t)page * a.cache.page_stride + (int64_t)head * kv4_head_bytes(1 << a.cache.page_shift, D);
+    return a.cache.pages + (int64_t)((uint64_t)(unsigned)page * (uint64_t)a.cache.page_stride) + (int64_t)head * kv4_head_bytes(1 << a.cache.page_shift, D);
 }
 
 template <int D>
@@ -106,9 +106,11 @@ __device__ __forceinline__ uint32_t key_word(const Keys<D>& keys, int token, int
 // row is a token and one of the group's heads).  Waves work alone, with no LDS
 // and no barrier.  Registers hold one block: its keys are replaced by the next
 // one's as soon as the scores are formed, its values when they have been
-// added, across segments too, so loads are always on their way.
+// added, across segments too, so loads are always on their way.  A head of 256
+// channels takes 300 registers for that: one wave a SIMD and half the shares
+// (16 sequences of 8000 tokens, 16 heads over 2: 35 us; two waves spill, 55 us).
 template <int D>
-__global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendArgs a) {
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_attend_rows_kernel(Kv4AttendArgs a) {
     constexpr int kSteps = D / 32;  // key steps of 32 channels
     constexpr int kOut = D / 16;    // 16-channel results
     constexpr int kParts = Keys<D>::kParts;
@@ -154,13 +156,11 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendA
 
         v8h query[kSteps];
         const float score_scale = scale_query(raw_query, groups_max(largest(raw_query, a.dtype)), a.dtype, a.scale_log2, query);
-        const float slack = kKv4Slack / score_scale;
-        // Scores are held less `base`, from which the first product starts: a
-        // maximum of the row, at most kKv4Slack (in powers of two) below the
-        // running one.  2^((S - base) scale) never overflows, however large
-        // the scores are, and sums are rarely scaled down.
-        float base = 0.0f, sum = 0.0f;
-        bool seen = false;
+        // Weights are taken from `base`, a maximum of the row so far or up to
+        // 2^7 times less; `shift` is 8 less base in powers of two, `huge` says
+        // that base's product with the scale has lost its digits.
+        float base = 0.0f, shift = kKv4Shift, sum = 0.0f;
+        bool seen = false, huge = false;
         v4f out[kOut];
 #pragma unroll
         for (int j = 0; j < kOut; ++j) out[j] = v4f{0, 0, 0, 0};
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendA
             v4f s[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[i] = v4f{-base, -base, -base, -base};
+                s[i] = v4f{0, 0, 0, 0};
                 Scales sc[kParts];
 #pragma unroll
                 for (int c = 0; c < kParts; ++c) {
@@ -218,35 +218,59 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendA
                     for (int x = 0; x < 8; ++x)
                         scales[c][x / 4][x % 4] &= (2 * x < kept ? 0xFFFFu : 0u) | (2 * x + 1 < kept ? 0xFFFF0000u : 0u);
             }
-            float top = s[0][0];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) top = fmaxf(top, s[i][x]);
-            top = groups_max(top);
-            const bool up = top > slack || (!seen && top > -__builtin_inff());
-            if (__any(up)) {
-                const float by = up ? top : 0.0f;
-                const float fade = seen ? __builtin_amdgcn_exp2f(-by * score_scale) : 0.0f;
-                base += by;
-                seen |= up;
-                sum *= fade;
-#pragma unroll
-                for (int j = 0; j < kOut; ++j) out[j] *= fade;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[i] -= by;
-            }
+            // P and this lane's part of its sum, of the weights as they are
+            // multiplied.  base * scale is rounded once for all of a row's tokens;
+            // where that is too rough, scores are first taken from the base.
             v8h p[2];
+            const auto weights = [&](bool rough) {
+                float part[2] = {};
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * h + x], score_scale, kKv4Shift));
-                        sum += e;
-                        p[h][4 * x + i] = (_Float16)e;
-                    }
+                        for (int i = 0; i < 4; i += 2) {
+                            float t[2];
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const float score = s[i + y][2 * h + x];
+                                t[y] = __builtin_fmaf(score, score_scale, shift);
+                                if (rough && huge) t[y] = __builtin_fmaf(score - base, score_scale, kKv4Shift);
+                            }
+                            const v2h e{(_Float16)__builtin_amdgcn_exp2f(t[0]), (_Float16)__builtin_amdgcn_exp2f(t[1])};
+                            part[x] = __builtin_amdgcn_fdot2(e, v2h{(_Float16)1.0f, (_Float16)1.0f}, part[x], false);
+                            p[h][4 * x + i] = e[0];
+                            p[h][4 * x + i + 1] = e[1];
+                        }
+                return part[0] + part[1];
+            };
+            // A score so far above the base that its weight leaves fp16 shows in
+            // the sum; then, and for a row's first tokens, the base is brought up
+            // to the maximum.  Else no maximum is needed.
+            float part = weights(false);
+            const bool mine = !seen || huge || !(part < 0x1p20f);
+            if (__any(mine)) {
+                float top = s[0][0];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) top = fmaxf(top, s[i][x]);
+                top = groups_max(top);
+                int either = (int)mine | __shfl_xor((int)mine, 16, kWave);
+                either |= __shfl_xor(either, 32, kWave);
+                if (either && (seen ? top > base : top > -__builtin_inff())) {
+                    const float fade = seen ? __builtin_amdgcn_exp2f((base - top) * score_scale) : 0.0f;
+                    base = top;
+                    shift = kKv4Shift - base * score_scale;
+                    huge = !(fabsf(shift) <= 0x1p20f);
+                    seen = true;
+                    sum *= fade;
+#pragma unroll
+                    for (int j = 0; j < kOut; ++j) out[j] *= fade;
+                }
+                part = __any(huge) ? weights(true) : weights(false);
+            }
+            sum += part;
 #pragma unroll
             for (int c = 0; c < kParts; ++c)
 #pragma unroll
@@ -305,7 +329,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_rows_kernel(Kv4AttendA
 #pragma unroll
                     for (int j = 0; j < kEach; j += 4)
                         *(v4f*)(o + 128 * c + kEach * x + j) = v4f{out[8 * c + j][x], out[8 * c + j + 1][x], out[8 * c + j + 2][x], out[8 * c + j + 3][x]};
-            if (g == 0) *(v2f*)(a.part_ml + at * 2) = v2f{seen ? base * score_scale : -__builtin_inff(), sum};
+            if (g == 0) *(v2f*)(a.part_ml + at * 2) = v2f{!seen ? -__builtin_inff() : huge ? base * score_scale : kKv4Shift - shift, sum};
         } else if (r < packed) {
             const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
             const int token = r / a.group, head = it.head * a.group + r % a.group;
@@ -447,7 +471,8 @@ Kv4Shape kv4_attend_shape(const Kv4Batch& b, int page_size, int kv_heads, int di
     Kv4Shape s{};
     const int64_t most_rows = (int64_t)b.max_rows * group;
     s.tile_rows = most_rows <= 16 ? 16 : kv4_tile_rows(most_rows, dim);
-    s.slots_log2 = most_rows <= 16 ? 11 : kv4_tile_slots_log2(most_rows, dim);
+    // shares of few rows: the waves that the chip holds
+    s.slots_log2 = most_rows > 16 ? kv4_tile_slots_log2(most_rows, dim) : dim == 256 ? 10 : 11;
     s.one_tile = most_rows <= 64;  // the kernel of many rows cuts into tiles also where one would do
     // a wave of few rows has little more to do for two blocks than for one; a
     // tile of many rows shorter than kKv4Whole is not worth joining

@@ -17,8 +17,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
-constexpr float kKv4Shift = 8.0f;  // P is held times 2^8,
-constexpr float kKv4Slack = 7.0f;  // and up to 2^7 times that: at most 2^15, half of fp16's range
+constexpr float kKv4Shift = 8.0f;  // P is held times 2^8; 2^16 is where fp16 ends
 
 __device__ __forceinline__ v2h as_h2(uint32_t w) { return __builtin_bit_cast(v2h, w); }
 
