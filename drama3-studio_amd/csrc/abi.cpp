@@ -1725,6 +1725,7 @@ int dmoe_kv4_attention(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, con
         require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
         a.slots_log2 = s.slots_log2;
         a.min_blocks = s.min_blocks;
+        a.cut = s.cut;
         a.tile_rows = s.tile_rows;
         a.part = static_cast<float*>(workspace);
         a.part_ml = a.part + s.part_bytes / sizeof(float);

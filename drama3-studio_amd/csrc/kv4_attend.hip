@@ -493,7 +493,7 @@ Kv4Shape kv4_attend_shape(const Kv4Batch& b, int page_size, int kv_heads, int di
     s.ml_bytes = (size_t)s.slots * s.tile_rows * 2 * sizeof(float);
     s.record_bytes = s.cut && s.one_tile ? (size_t)b.seqs * kv_heads * sizeof(Kv4Record) : 0;
     // counts of blocks are kept in 31 bits
-    if (most_blocks * s.tiles * kv_heads > INT32_MAX / 2) s.groups = 0;
+    if (std::max(most_blocks, (int64_t)s.min_blocks) * s.tiles * kv_heads > INT32_MAX / 2) s.groups = 0;
     return s;
 }
 

@@ -115,13 +115,18 @@ struct Kv4Shares {
             total += wave_total(s + me < seqs ? max(lane.blocks, 1) : 0);
         }
         const int slots = 1 << a.slots_log2;
-        share = max(a.min_blocks, (int)(((int64_t)total * kv + slots - 1) >> a.slots_log2));
-        int shares = 0;
-        for (int s = 0; s < seqs; s += kWave) {
-            if (!once) lane = kv4_lane(a, s + me);
-            shares += wave_total(s + me < seqs ? (max(lane.blocks, 1) + share - 1) / share : 0);
+        share = a.min_blocks;
+        int shares = seqs;
+        if (a.cut) {
+            share = max(share, (int)(((int64_t)total * kv + slots - 1) >> a.slots_log2));
+            shares = 0;
+            for (int s = 0; s < seqs; s += kWave) {
+                if (!once) lane = kv4_lane(a, s + me);
+                shares += wave_total(s + me < seqs ? (max(lane.blocks, 1) + share - 1) / share : 0);
+            }
         }
-        padded = (int64_t)shares * kv <= slots;
+        // where nothing is cut a tile has a share to itself, however many there are
+        padded = !a.cut || (int64_t)shares * kv <= slots;
         const int end = (padded ? shares * share : total) * kv;
         x = (int)min((int64_t)index * share, (int64_t)end);
         x_end = min(x + share, end);

@@ -235,14 +235,15 @@ def test_several_rows_a_sequence(cuda, dim, hq, hkv, page, dtype, seqs, window):
         assert (out[at:at + empty] == 0).all()
 
 
-@pytest.mark.parametrize("dim,hq,hkv,seqs,longest", [
-    (64, 8, 4, 1300, 60), (64, 2, 2, 1400, 190), (128, 16, 8, 333, 64), (256, 4, 2, 1100, 100)])
+@pytest.mark.parametrize("dim,hq,hkv,seqs,longest,rows", [
+    (64, 8, 4, 1300, 60, 1), (64, 2, 2, 1400, 190, 1), (128, 16, 8, 333, 64, 1), (256, 4, 2, 1100, 100, 1),
+    (64, 5, 5, 900, 128, 1), (64, 8, 2, 700, 200, 6), (128, 12, 1, 600, 700, 2), (256, 8, 2, 300, 120, 9)])
 @pytest.mark.parametrize("window", [0, 40])
-def test_more_sequences_than_there_is_room_for(cuda, dim, hq, hkv, seqs, longest, window):
-    # one token each: several sequences, most of one block, come to one wave
-    print_case("kv4 crowd", dim, hq, hkv, seqs, longest, window)
+def test_more_sequences_than_there_is_room_for(cuda, dim, hq, hkv, seqs, longest, rows, window):
+    # several short sequences come to one wave or workgroup where they may be cut, and have their own where not
+    print_case("kv4 crowd", dim, hq, hkv, seqs, longest, rows, window)
     lengths = torch.randint(1, longest + 1, (seqs,), generator=torch.Generator().manual_seed(seqs)).tolist()
-    case = Case(cuda, [(int(n % 11 != 0), n) for n in lengths], hq, hkv, dim, 64, torch.bfloat16, seed=seqs)
+    case = Case(cuda, [(min(n % 11, rows, n), n) for n in lengths], hq, hkv, dim, 64, torch.bfloat16, seed=seqs)
     # any codes, scales of 2^-7 to 2^-6 with any zero point
     case.raw.copy_(torch.randint(0, 256, case.raw.shape, dtype=torch.uint8, generator=case.g))
     scales = case.raw[:, :, 64 * dim:].view(torch.int16)
