@@ -1,4 +1,5 @@
-"""The MoE block of a Drama 3 decoder layer around the routed experts.
+"""The two halves of a Drama 3 decoder layer: attention over a 4-bit cache,
+and the MoE block around the routed experts.
 
 BackboneDecodeGraph splits a decoder layer's MoE half into _route_impl (router
 softmax / top-k on ``moe.gate(flat)``), _shared_impl (the sigmoid-gated shared
@@ -10,6 +11,11 @@ gate/up (``dmoe_moe_block_pre``), the routed experts through the FP8 or packed
 backend (``forward_routed``), and one launch for the shared down projection,
 gating and residual adds (``dmoe_moe_block_post``).  Weights and rows are
 bf16, the reference's compute dtype for these modules.
+
+``AttentionBlock`` is the half before it for a layer whose keys and values are
+kept in a ``KvCache4``: projections, ``append``, ``attend``, output projection
+and residual add, with no host sync either, so that a whole layer's decode
+step is captured in one hipGraph.
 """
 from __future__ import annotations
 
@@ -17,6 +23,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from .attention import KvCache4, PagedBatch, Rotary
 from .formats import QuantizedStore, StagedExperts
 
 
@@ -109,5 +116,62 @@ class MoeBlock:
         experts_out, weights, ids = self.backend.forward_routed(mlp_input, logits, self.top_k, self.experts,
                                                                 renormalize=self.norm_topk_prob)
         return self.post(act, sgate, experts_out, after_mixer, out=out), weights, ids
+
+    __call__ = forward
+
+
+class AttentionBlock:
+    """Attention half of a decoder layer over a paged 4-bit cache.
+
+    ``q_proj``, ``k_proj``, ``v_proj`` and ``o_proj`` are modules over rows
+    (``GPTQLinear``, ``torch.nn.Linear``); ``q_norm`` and ``k_norm``, if the
+    layer has them, are applied to [rows, heads, D] before the rotation.
+    ``cache`` is the layer's ``KvCache4``; ``rotary``, ``scale`` and
+    ``window`` are those of its ``append`` and ``attend``.
+    """
+
+    def __init__(self, q_proj, k_proj, v_proj, o_proj, cache: KvCache4, *, heads: int, rotary: Rotary | None = None,
+                 q_norm=None, k_norm=None, scale: float | None = None, window: int = 0):
+        self.heads = int(heads)
+        if self.heads < 1 or self.heads % cache.kv_heads:
+            raise ValueError("heads must be a multiple of the cache's key/value heads")
+        if window < 0:
+            raise ValueError("window must not be negative")
+        width, kv_width = self.heads * cache.head_dim, cache.kv_heads * cache.head_dim
+        for proj, name, side, size in ((q_proj, "q_proj", "out_features", width), (k_proj, "k_proj", "out_features", kv_width),
+                                       (v_proj, "v_proj", "out_features", kv_width), (o_proj, "o_proj", "in_features", width)):
+            if getattr(proj, side, size) != size:
+                raise ValueError(f"{name} must have {side} {size}")
+        self.q_proj, self.k_proj, self.v_proj, self.o_proj = q_proj, k_proj, v_proj, o_proj
+        self.q_norm, self.k_norm = q_norm, k_norm
+        self.cache, self.rotary, self.scale, self.window = cache, rotary, scale, int(window)
+
+    def forward(self, attn_input: Tensor, residual: Tensor, batch: PagedBatch, positions: Tensor | None = None) -> Tensor:
+        """residual + o_proj(attention of the batch's rows), the rows' keys and
+        values stored on the way.  Both inputs are [rows, hidden]; for rows that no
+        sequence owns, and those before a sequence's first token, the attention
+        is zero."""
+        if attn_input.ndim != 2 or attn_input.shape != residual.shape or attn_input.shape[0] != batch.rows:
+            raise ValueError(f"attn_input and residual must be [{batch.rows}, hidden]")
+        rows, dim = batch.rows, self.cache.head_dim
+        q = self.q_proj(attn_input).reshape(rows, self.heads, dim)
+        k = self.k_proj(attn_input).reshape(rows, self.cache.kv_heads, dim)
+        v = self.v_proj(attn_input).reshape(rows, self.cache.kv_heads, dim)
+        if self.q_norm is not None:
+            q = self.q_norm(q)
+        if self.k_norm is not None:
+            k = self.k_norm(k)
+        if self.rotary is not None:
+            # rows without a place stay zeros, which attention does not read
+            q = self.cache.append(k, v, batch, rotary=self.rotary, positions=positions, q=q, q_out=torch.zeros_like(
+                q, memory_format=torch.contiguous_format))
+        else:
+            self.cache.append(k, v, batch, positions=positions)
+        attended = torch.zeros((rows, self.heads, dim), dtype=q.dtype, device=q.device)
+        self.cache.attend(q, batch, scale=self.scale, window=self.window, out=attended)
+        out = self.o_proj(attended.reshape(rows, self.heads * dim))
+        if out.shape != residual.shape:
+            raise ValueError(f"o_proj must give {list(residual.shape)}, got {list(out.shape)}")
+        return residual + out
 
     __call__ = forward

@@ -12,6 +12,7 @@ import torch
 import kv4_reference as ref
 from drama_moe import _lib
 from drama_moe.attention import KvCache4, PagedBatch, Rotary
+from drama_moe.block import AttentionBlock
 
 
 def i32(*shape):
@@ -206,3 +207,30 @@ def test_reference_pages_return_what_was_put():
             for got, x in zip(pages.get(1, p), kv[p]):
                 assert np.array_equal(got, ref.value(*ref.quantize(x.astype(np.float32))))
         assert not pages.raw[0].any()
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"heads": 0}, "heads must be"), ({"heads": 3}, "heads must be"), ({"window": -1}, "window"),
+    ({"q_proj": (32, 128)}, "q_proj must have out_features 256"), ({"k_proj": (32, 256)}, "k_proj must have out_features 128"),
+    ({"v_proj": (32, 256)}, "v_proj must have out_features 128"), ({"o_proj": (128, 32)}, "o_proj must have in_features 256"),
+])
+def test_attention_block_refusals(change, message):
+    cache = KvCache4.allocate(4, 2, 64, page_size=16, device="cpu")
+    sizes = {"q_proj": (32, 256), "k_proj": (32, 128), "v_proj": (32, 128), "o_proj": (256, 32), **change}
+    projections = {n: torch.nn.Linear(*sizes[n]) for n in ("q_proj", "k_proj", "v_proj", "o_proj")}
+    options = {"heads": 4, **{n: v for n, v in change.items() if n in ("heads", "window")}}
+    with pytest.raises(ValueError, match=message):
+        AttentionBlock(**projections, cache=cache, **options)
+
+
+def test_attention_block_checks_its_rows():
+    cache = KvCache4.allocate(4, 2, 64, page_size=16, device="cpu")
+    block = AttentionBlock(torch.nn.Linear(32, 256), torch.nn.Linear(32, 128), torch.nn.Linear(32, 128),
+                           torch.nn.Linear(256, 32), cache, heads=4)
+    batch = PagedBatch(i32(2, 2), i32(2))
+    for x, residual in ((torch.zeros(2, 32), torch.zeros(2, 16)), (torch.zeros(3, 32), torch.zeros(3, 32)),
+                        (torch.zeros(2, 1, 32), torch.zeros(2, 1, 32))):
+        with pytest.raises(ValueError, match="attn_input and residual"):
+            block(x, residual, batch)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        block(torch.zeros(2, 32), torch.zeros(2, 32), batch)
