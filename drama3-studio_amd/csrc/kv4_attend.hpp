@@ -54,21 +54,6 @@ __device__ __forceinline__ v8h join(v2h a, v2h b, v2h c, v2h d) {
     return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Eight neighbouring elements of a bf16 or fp16 row as fp32.
-__device__ __forceinline__ void widen8(const v4i& raw, int dtype, float (&x)[8]) {
-    if (dtype == kBF16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float((uint32_t)raw[i] << 16);
-            x[2 * i + 1] = __uint_as_float((uint32_t)raw[i] & 0xFFFF0000u);
-        }
-    } else {
-        const v8h h = __builtin_bit_cast(v8h, raw);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
-    }
-}
-
 // Two values as a word of a bf16 or fp16 row.
 __device__ __forceinline__ uint32_t narrow2(float a, float b, int dtype) {
     typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
@@ -86,29 +71,36 @@ __device__ __forceinline__ float scale_query(const v4i (&raw)[N], float most, in
     if (most > 0.0f && most < __builtin_inff()) (void)frexpf(most, &e);
     e = max(-120, min(120, e));
     const float down = ldexpf(1.0f, -e);
+    const auto fill = [&](auto&& element) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        float x[8];
-        widen8(raw[j], dtype, x);
+        for (int j = 0; j < N; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= down;
-        query[j] = v8h{(_Float16)x[0], (_Float16)x[4], (_Float16)x[1], (_Float16)x[5],
-                       (_Float16)x[2], (_Float16)x[6], (_Float16)x[3], (_Float16)x[7]};
+            for (int i = 0; i < 4; ++i) {  // channels i and i + 4
+                query[j][2 * i] = (_Float16)(element(j, i) * down);
+                query[j][2 * i + 1] = (_Float16)(element(j, i + 4) * down);
+            }
+    };
+    if (dtype == kBF16) {
+        fill([&](int j, int i) { return __uint_as_float(i & 1 ? (uint32_t)raw[j][i / 2] & 0xFFFF0000u : (uint32_t)raw[j][i / 2] << 16); });
+    } else {
+        fill([&](int j, int i) { return (float)as_h2((uint32_t)raw[j][i / 2])[i & 1]; });
     }
     return fmaxf(scale_log2 * ldexpf(1.0f, e), 1e-35f);
 }
 
+// The largest magnitude of a query row's words, found among their bits: those
+// of both types grow with it (NaN above all).
 template <int N>
 __device__ __forceinline__ float largest(const v4i (&raw)[N], int dtype) {
-    float most = 0.0f;
+    typedef uint16_t v2s __attribute__((ext_vector_type(2)));
+    v2s most{0, 0};
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        float x[8];
-        widen8(raw[j], dtype, x);
+    for (int j = 0; j < N; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
-    }
-    return most;
+        for (int i = 0; i < 4; ++i)
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(v2s, (uint32_t)raw[j][i] & 0x7FFF7FFFu));
+    const uint32_t top = max((uint32_t)most[0], (uint32_t)most[1]);
+    return dtype == kBF16 ? __uint_as_float(top << 16) : (float)as_h2(top)[0];
 }
 
 // Largest / sum over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).

@@ -36,7 +36,7 @@ struct Tile {
     static constexpr int kKeyBytes = kKv4Block * (D * 2 + 16), kValueBytes = D * 144, kStage = kKeyBytes + kValueBytes;
 };
 template <int D>
-using Few = Tile<D, 2, D == 256 ? 1 : 2, D == 256 ? 2 : 1>;
+using Few = Tile<D, 2, 2, D == 256 ? 2 : 1>;
 template <int D>
 using Many = Tile<D, D == 256 ? 4 : 8, 1, D == 256 ? 2 : 1>;
 
@@ -212,8 +212,8 @@ struct Rows {
         hi = lane >> 5;
         const int wave = wave_index();
         group = wave % T::kGroups;
-        half = T::kHalves == 2 ? wave / T::kGroups : 0;
-        split = T::kSplit == 2 ? wave / T::kGroups : 0;
+        half = wave / T::kGroups % T::kHalves;
+        split = wave / T::kGroups / T::kHalves;
         const int packed = it.n * a.group;
         row_a = it.row_a;
         row_b = min(row_a + T::kRows, packed);
@@ -459,24 +459,24 @@ __device__ __forceinline__ void attend_few(const Kv4AttendArgs& a, const Kv4Segm
     float top = rows.top();
     if constexpr (T::kHalves == 2) {
         // the second halves' sums by way of LDS, a lane's values a row of its own length apart
-        static_assert(T::kGroups * kWave * (D / 2 + 2) * 4 <= 2 * T::kStage, "the halves are joined in the stages");
-        constexpr int kStride = T::kGroups * kWave;
-        float* share = (float*)lds.stage + 64 * rows.group + rows.lane;
+        constexpr int kValues = 16 * T::kOut, kStride = T::kGroups * T::kSplit * kWave;
+        static_assert(kStride * (kValues + 2) * 4 <= 2 * T::kStage, "the halves are joined in the stages");
+        float* share = (float*)lds.stage + kWave * (rows.group + T::kGroups * rows.split) + rows.lane;
         __syncthreads();
         if (rows.half) {
 #pragma unroll
             for (int c = 0; c < T::kOut; ++c)
 #pragma unroll
                 for (int x = 0; x < 16; ++x) share[(16 * c + x) * kStride] = rows.out[c][x];
-            share[D / 2 * kStride] = top;
-            share[(D / 2 + 1) * kStride] = rows.sum;
+            share[kValues * kStride] = top;
+            share[(kValues + 1) * kStride] = rows.sum;
         }
         __syncthreads();
         if (rows.half) return;
-        const float other = share[D / 2 * kStride], both = fmaxf(top, other);
+        const float other = share[kValues * kStride], both = fmaxf(top, other);
         const float f = top == both ? 1.0f : __builtin_amdgcn_exp2f(top - both);
         const float h = other == both ? 1.0f : __builtin_amdgcn_exp2f(other - both);
-        rows.sum = f * rows.sum + h * share[(D / 2 + 1) * kStride];
+        rows.sum = f * rows.sum + h * share[(kValues + 1) * kStride];
         top = both;
 #pragma unroll
         for (int c = 0; c < T::kOut; ++c)
@@ -487,7 +487,7 @@ __device__ __forceinline__ void attend_few(const Kv4AttendArgs& a, const Kv4Segm
 }
 
 template <class T>
-__global__ __launch_bounds__(T::kThreads, T::D == 256 ? 1 : 2) void kv4_attend_few_kernel(Kv4AttendArgs a) {
+__global__ __launch_bounds__(T::kThreads, 2) void kv4_attend_few_kernel(Kv4AttendArgs a) {
     __shared__ Stages<T> lds;
     Kv4Shares shares(a, blockIdx.x);
     Kv4Segment seg;
