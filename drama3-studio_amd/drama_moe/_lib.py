@@ -70,6 +70,7 @@ class HeadRows(ctypes.Structure):
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
+_CACHE, _BATCH, _HEADS = ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Batch), ctypes.POINTER(HeadRows)
 
 _SIGNATURES = {
     "dmoe_abi_version": ([], _I),
@@ -111,10 +112,10 @@ _SIGNATURES = {
     "dmoe_w4a16_linear": ([_P, _I, _L, _I, _P, _L, _P, _L, _I, _I, _P, _L, _P], _I),
     "dmoe_moe_block_pre": ([_P, _L, _I, _I, _P, _L, _I, _P, _P, _L, _P, _L, _I, _P, _L, _P, _P, _L, _P], _I),
     "dmoe_moe_block_post": ([_P, _L, _I, _I, _P, _L, _I, _P, _P, _L, _P, _L, _P, _L, _P], _I),
-    "dmoe_kv4_append": ([_P, _P, _P, _P, _I, _P, _P, _P, _I, _P, _P], _I),
-    "dmoe_kv4_read": ([_P, _P, _P, _P, _I, _P, _P], _I),
-    "dmoe_kv4_attention_workspace_bytes": ([_P, _P, _I], ctypes.c_size_t),
-    "dmoe_kv4_attention": ([_P, _P, _P, _I, ctypes.c_float, _I, _P, _I, _P, ctypes.c_size_t, _P, _P], _I),
+    "dmoe_kv4_append": ([_CACHE, _BATCH, ctypes.POINTER(RotaryDesc), _HEADS, _I, _HEADS, _HEADS, _HEADS, _I, _P, _P], _I),
+    "dmoe_kv4_read": ([_CACHE, _BATCH, _HEADS, _HEADS, _I, _P, _P], _I),
+    "dmoe_kv4_attention_workspace_bytes": ([_CACHE, _BATCH, _I], ctypes.c_size_t),
+    "dmoe_kv4_attention": ([_CACHE, _BATCH, _HEADS, _I, ctypes.c_float, _I, _HEADS, _I, _P, ctypes.c_size_t, _P, _P], _I),
     "dmoe_fp8_quantized_pairs": ([ctypes.POINTER(Fp8Bank), _P, _P, _L, _L, _I, _I, _I, _P, _I, _P,
                                   _I, _I, _I, _P, _P, ctypes.c_size_t, _P, _P], _I),
     "dmoe_combine_slots": ([_P, _L, _P, _I, _I, _I, _I, _I, _P, _I, _L, _P], _I),

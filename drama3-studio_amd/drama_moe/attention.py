@@ -16,8 +16,6 @@ graphs captured apart share nothing but the cache and the status word.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch import Tensor
 
@@ -29,9 +27,10 @@ MAX_SEQUENCES = 4096
 _HALVES = (torch.bfloat16, torch.float16)
 
 
-def _rows(t: Tensor, name: str, shape: tuple, dtype: torch.dtype | None, device, *, written: bool = False) -> Tensor:
+def _rows(t: Tensor, name: str, shape: tuple, dtype: torch.dtype | None, device, *, written: bool = False):
     """t as rows of ``shape`` [rows, heads, dim] with contiguous, 16-byte
-    aligned heads: itself, or (for one that is only read) a copy."""
+    aligned heads -- itself, or (for one that is only read) a copy -- and its
+    descriptor."""
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     if t.dtype not in _HALVES:
@@ -41,20 +40,15 @@ def _rows(t: Tensor, name: str, shape: tuple, dtype: torch.dtype | None, device,
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
     s0, s1, s2 = t.stride()
-    if s2 != 1 or (s0 % 8 and shape[0] > 1) or (s1 % 8 and shape[1] > 1) or t.data_ptr() % 16:
+    rows, heads = shape[0] > 1, shape[1] > 1
+    address = t.data_ptr()
+    if s2 != 1 or (s0 % 8 and rows) or (s1 % 8 and heads) or address % 16:
         if written:
             raise ValueError(f"{name} must have contiguous, 16-byte aligned heads")
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _head_rows(t: Tensor | None):
-    """Descriptor of a checked tensor (a dimension of one entry has no stride)."""
-    if t is None:
-        return None
-    rows, heads, _ = t.shape
-    s0, s1, _ = t.stride()
-    return ctypes.byref(_lib.HeadRows(t.data_ptr(), s0 if rows > 1 else 0, s1 if heads > 1 else 0))
+        t = t.clone(memory_format=torch.contiguous_format)
+        (s0, s1, _), address = t.stride(), t.data_ptr()
+    # a dimension of one entry has no stride
+    return t, _lib.HeadRows(address, s0 if rows else 0, s1 if heads else 0)
 
 
 def _heads(q: Tensor) -> int:
@@ -81,7 +75,7 @@ class PagedBatch:
     that no sequence owns -- behind the last one -- are left as they are.
     """
 
-    __slots__ = ("block_table", "lengths", "starts", "rows", "max_rows", "desc", "device")
+    __slots__ = ("block_table", "lengths", "starts", "rows", "max_rows", "desc", "device", "scratch")
 
     def __init__(self, block_table: Tensor, lengths: Tensor, starts: Tensor | None = None, *, rows: int | None = None,
                  max_rows: int | None = None):
@@ -118,6 +112,7 @@ class PagedBatch:
             raise ValueError("max_rows outside [1, rows]")
         self.block_table, self.lengths, self.starts = block_table, lengths, starts
         self.rows, self.max_rows, self.device = rows, max_rows, device
+        self.scratch = {}  # bytes that attention over this batch's sizes needs, by geometry
         # a table of one row may have any row stride
         self.desc = _lib.Kv4Batch(block_table.data_ptr(), max(block_table.stride(0), cols), lengths.data_ptr(),
                                   starts.data_ptr() if starts is not None else None, seqs, cols, rows, max_rows)
@@ -228,17 +223,16 @@ class KvCache4:
         rows, dim = batch.rows, self.head_dim
         dtype = k.dtype
         shape = (rows, self.kv_heads, dim)
-        k = _rows(k, "k", shape, None, device)
-        v = _rows(v, "v", shape, dtype, device)
-        heads = 0
+        k, k_rows = _rows(k, "k", shape, None, device)
+        v, v_rows = _rows(v, "v", shape, dtype, device)
+        heads, q_rows, out_rows = 0, None, None
         if q is not None:
             heads = _heads(q)
             shape = (rows, heads, dim)
-            q = _rows(q, "q", shape, dtype, device)
+            q, q_rows = _rows(q, "q", shape, dtype, device)
             if q_out is None:
                 q_out = torch.empty(shape, dtype=dtype, device=device)
-            else:
-                _rows(q_out, "q_out", shape, dtype, device, written=True)
+            q_out, out_rows = _rows(q_out, "q_out", shape, dtype, device, written=True)
         elif q_out is not None:
             raise ValueError("q_out needs q")
         turn = None
@@ -260,19 +254,18 @@ class KvCache4:
                     axes, stride = positions.shape[0], positions.stride(0)
                 if not axes:
                     raise ValueError("positions has no axis")
-            turn = ctypes.byref(_lib.RotaryDesc(
+            turn = _lib.RotaryDesc(
                 rotary.inv_freq.data_ptr(), rotary.axis.data_ptr() if rotary.axis is not None else None,
                 positions.data_ptr() if positions is not None else None, stride,
                 _lib.I32 if positions is not None and positions.dtype == torch.int32 else _lib.I64, axes, rotary.dim,
-                int(rotary.interleaved)))
+                int(rotary.interleaved))
         elif positions is not None:
             raise ValueError("positions need a rotary")
         if rows == 0:
             return q_out
         with _on(device):
             _lib.check(_lib.library().dmoe_kv4_append(
-                ctypes.byref(self.desc), ctypes.byref(batch.desc), turn, _head_rows(q), heads, _head_rows(q_out),
-                _head_rows(k), _head_rows(v), _lib.dtype_code(dtype), self._status, _stream(device)))
+                self.desc, batch.desc, turn, q_rows, heads, out_rows, k_rows, v_rows, _lib.dtype_code(dtype), self._status, _stream(device)))
         return q_out
 
     def read(self, batch: PagedBatch, *, dtype: torch.dtype = torch.float16, k_out: Tensor | None = None,
@@ -285,13 +278,12 @@ class KvCache4:
             k_out = torch.empty(shape, dtype=dtype, device=device)
         if v_out is None:
             v_out = torch.empty(shape, dtype=dtype, device=device)
-        _rows(k_out, "k_out", shape, dtype, device, written=True)
-        _rows(v_out, "v_out", shape, dtype, device, written=True)
+        k_out, k_rows = _rows(k_out, "k_out", shape, dtype, device, written=True)
+        v_out, v_rows = _rows(v_out, "v_out", shape, dtype, device, written=True)
         if batch.rows:
             with _on(device):
                 _lib.check(_lib.library().dmoe_kv4_read(
-                    ctypes.byref(self.desc), ctypes.byref(batch.desc), _head_rows(k_out), _head_rows(v_out),
-                    _lib.dtype_code(dtype), self._status, _stream(device)))
+                    self.desc, batch.desc, k_rows, v_rows, _lib.dtype_code(dtype), self._status, _stream(device)))
         return k_out, v_out
 
     def attend(self, q: Tensor, batch: PagedBatch, *, scale: float | None = None, window: int = 0,
@@ -303,23 +295,24 @@ class KvCache4:
         device = self._check(batch)
         heads = _heads(q)
         shape = (batch.rows, heads, self.head_dim)
-        q = _rows(q, "q", shape, None, device)
+        q, q_rows = _rows(q, "q", shape, None, device)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError("query heads must be a multiple of the key/value heads")
         if out is None:
             out = torch.empty(shape, dtype=q.dtype, device=device)
-        else:
-            _rows(out, "out", shape, q.dtype, device, written=True)
+        out, out_rows = _rows(out, "out", shape, q.dtype, device, written=True)
         if batch.rows == 0:
             return out
         lib = _lib.library()
-        cache, desc = ctypes.byref(self.desc), ctypes.byref(batch.desc)
         with _on(device):
-            need = lib.dmoe_kv4_attention_workspace_bytes(cache, desc, heads)
+            need = batch.scratch.get((heads, self.kv_heads, self.head_dim, self.page_size))
+            if need is None:
+                need = lib.dmoe_kv4_attention_workspace_bytes(self.desc, batch.desc, heads)
+                batch.scratch[heads, self.kv_heads, self.head_dim, self.page_size] = need
             scratch = torch.empty(need, dtype=torch.uint8, device=device)
             _lib.check(lib.dmoe_kv4_attention(
-                cache, desc, _head_rows(q), heads, self.head_dim ** -0.5 if scale is None else scale, window,
-                _head_rows(out), _lib.dtype_code(q.dtype), scratch.data_ptr(), need, self._status, _stream(device)))
+                self.desc, batch.desc, q_rows, heads, self.head_dim ** -0.5 if scale is None else scale, window,
+                out_rows, _lib.dtype_code(q.dtype), scratch.data_ptr(), need, self._status, _stream(device)))
         return out
 
 
