@@ -19,7 +19,9 @@ namespace dmoe {
 namespace {
 
 constexpr int kThreads = 256;
-// A workgroup takes several rows where that leaves this many of them: below, the chip is not full.
+// A workgroup takes eight rows where that leaves this many of them: below, the
+// chip is not full (2300 rows of 20 heads of 256 channels: 21 us one by one,
+// 25 us by eight; 8192 rows of 48 heads of 128: 74 us one by one, 55 by eight).
 constexpr int kFull = 1024;
 
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
@@ -162,9 +164,15 @@ __device__ __forceinline__ void rotate8(const F (&turn)[144][2], bool interleave
 }
 
 // kRows rows a workgroup (blockIdx.x), one 8-channel chunk of one head a
-// thread: query heads first, then key and value heads.
+// thread: query heads first, then key and value heads.  A row alone takes
+// workgroups of 256 threads, small enough that many run at once (64 rows of
+// 48 heads of 128 channels: 5 us; of up to 1024 threads 8 us); eight rows take
+// all their heads together, so that their angles are formed once, not three
+// times, and a row's tables are read once.  8192 such rows: 55 us, 177 MB read
+// and written at 3.2 TB/s, of which a third is the vector unit's (quantizer,
+// 64-bit keys, angles) and the rest loads that wait for few of them.
 template <int kRows>
-__global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4AppendArgs a) {
+__global__ __launch_bounds__(kRows == 1 ? kThreads : 1024) void kv4_append_kernel(Kv4AppendArgs a) {
     // cosine and sine of each frequency, in 64 bits for keys, in 32 for queries; one entry in nine is left
     // free, so that the chunks' entries lie in different banks
     __shared__ double turn[kRows][144][2];
@@ -172,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4AppendArgs a) {
     __shared__ Place places[kRows];
     const int dim = a.cache.dim, chunks = dim / 8, log2 = __builtin_ctz(chunks);
     const int row0 = blockIdx.x * kRows;
-    const int unit = blockIdx.y * kThreads + threadIdx.x;
+    const int unit = blockIdx.y * (int)blockDim.x + threadIdx.x;
     const int head = unit >> log2, chunk = unit & (chunks - 1);
     const int kv = a.cache.kv_heads, heads = a.q_heads + 2 * kv;
     const bool is_v = head >= a.q_heads + kv, is_q = head < a.q_heads, live = head < heads;
@@ -192,12 +200,12 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4AppendArgs a) {
             raw[i] = *(const v4i*)x;
         }
     }
-    for (int i = wave_index(); i < kRows; i += kThreads / kWave) {
+    for (int i = wave_index(); i < kRows; i += (int)blockDim.x / kWave) {
         const Place place = place_of(a.cache, a.batch, row0 + i, a.status);
         if ((threadIdx.x & 63) == 0) places[i] = place;
     }
     if (!a.rotary.positions) __syncthreads();
-    for (int i = threadIdx.x; i < kRows * half; i += kThreads) {
+    for (int i = threadIdx.x; i < kRows * half; i += (int)blockDim.x) {
         const int row = i / half, f = i - row * half;
         double place;
         if (a.rotary.positions) {
@@ -252,7 +260,9 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4AppendArgs a) {
     }
 }
 
-// kRows rows a workgroup, one 8-channel chunk of a key or value head a thread.
+// kRows rows a workgroup, one 8-channel chunk of a key or value head a thread:
+// bound by memory (30001 rows of 8 + 8 heads of 128 channels: 33 us, 158 MB at
+// 4.8 TB/s, what a copy reaches).
 template <int kRows>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4ReadArgs a) {
     __shared__ Place places[kRows];
@@ -301,9 +311,13 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4ReadArgs a) {
 
 void launch_kv4_append(const Kv4AppendArgs& a, hipStream_t st) {
     const int units = (a.q_heads + 2 * a.cache.kv_heads) * (a.cache.dim / 8);
-    const unsigned parts = (units + kThreads - 1) / kThreads;
-    if ((int64_t)a.batch.rows * parts < 8 * kFull) kv4_append_kernel<1><<<dim3(a.batch.rows, parts), kThreads, 0, st>>>(a);
-    else kv4_append_kernel<8><<<dim3((a.batch.rows + 7) / 8, parts), kThreads, 0, st>>>(a);
+    const int small = (units + kThreads - 1) / kThreads;
+    if ((int64_t)a.batch.rows * small < 8 * kFull) {
+        kv4_append_kernel<1><<<dim3(a.batch.rows, small), kThreads, 0, st>>>(a);
+        return;
+    }
+    const int parts = (units + 1023) / 1024, threads = ((units + parts - 1) / parts + kWave - 1) / kWave * kWave;
+    kv4_append_kernel<8><<<dim3((a.batch.rows + 7) / 8, parts), threads, 0, st>>>(a);
 }
 
 void launch_kv4_read(const Kv4ReadArgs& a, hipStream_t st) {
