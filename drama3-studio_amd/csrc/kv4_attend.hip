@@ -1,11 +1,12 @@
 // Attention of a batch's rows over the 4-bit paged cache.
 //
-// One pass over keys and values with the running maximum m and sum l of each
-// row's softmax: per block of 64 tokens S = K Q^T, P = 2^(S - m), O += V^T P^T.
-// Both products are 16x16x32 fp16 MFMAs, kept transposed so that a lane holds
-// everything of ONE row in both results (column = lane % 16): the row's scale, maximum
-// and sum are plain registers, and P leaves the first product in the lanes
-// where the second takes it, with no exchange between lanes.  For that the
+// One pass over keys and values with a base m (a maximum of the row so far)
+// and the sum l of each row's softmax: per block of 64 tokens S = K Q^T,
+// P = 2^(S - m), O += V^T P^T.  Both products are 16x16x32 fp16 MFMAs, kept
+// transposed so that a lane holds everything of ONE row in both results
+// (column = lane % 16): the row's scale, base and sum are plain registers, and
+// P leaves the first product in the lanes where the second takes it, with no
+// exchange between lanes.  For that the
 // four 16-token tiles of a block take tokens 4r + i (tile i, operand row r):
 // the results of lane group g = lane / 16 are then tokens 16g..16g+15, the
 // eight-token slices that the second product's operand wants.
@@ -109,6 +110,14 @@ __device__ __forceinline__ uint32_t key_word(const Keys<D>& keys, int token, int
 // added, across segments too, so loads are always on their way.  A head of 256
 // channels takes 300 registers for that: one wave a SIMD and half the shares
 // (16 sequences of 8000 tokens, 16 heads over 2: 35 us; two waves spill, 55 us).
+//
+// 32 heads over 8 of 128 channels: 131072 tokens of one sequence take 36 us,
+// 151 MB at 4.2 TB/s, as many more 30 us (5.1 TB/s); 64 sequences, 120 MB,
+// 38 us.  What is lost is the start (lengths, then pages, then codes, each
+// read behind the other) and waits: two waves a SIMD keep the vector unit busy
+// half of the time -- 430 of a block's 640 instructions decode its codes -- and
+// wait for loads 40% of it.  Three waves spill (60 us for the one sequence),
+// twice as many shares add to the start (62 us with the join instead of 51).
 template <int D>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_attend_rows_kernel(Kv4AttendArgs a) {
     constexpr int kSteps = D / 32;  // key steps of 32 channels
@@ -156,8 +165,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_attend_rows_ke
 
         v8h query[kSteps];
         const float score_scale = scale_query(raw_query, groups_max(largest(raw_query, a.dtype)), a.dtype, a.scale_log2, query);
-        // Weights are taken from `base`, a maximum of the row so far or up to
-        // 2^7 times less; `shift` is 8 less base in powers of two, `huge` says
+        // Weights are taken from `base`, a maximum of the row so far or less than
+        // 2^8 times below one; `shift` is 8 less base in powers of two, `huge` says
         // that base's product with the scale has lost its digits.
         float base = 0.0f, shift = kKv4Shift, sum = 0.0f;
         bool seen = false, huge = false;
@@ -469,6 +478,10 @@ void launch_dim(const Kv4AttendArgs& a, const Kv4Shape& s, hipStream_t st) {
 
 Kv4Shape kv4_attend_shape(const Kv4Batch& b, int page_size, int kv_heads, int dim, int group) {
     Kv4Shape s{};
+    // Up to 16 packed rows go to waves that work alone, up to 64 to workgroups
+    // that decode a block once for all of them, more to tiles of 128 or 256.
+    // One sequence of 131072 tokens with 4 packed rows: 51 us so, 88 us with the
+    // workgroups of 64; 12 sequences with 20 rows: 41 us, 72 us with the tiles.
     const int64_t most_rows = (int64_t)b.max_rows * group;
     s.tile_rows = most_rows <= 16 ? 16 : kv4_tile_rows(most_rows, dim);
     // shares of few rows: the waves that the chip holds

@@ -167,10 +167,11 @@ struct Decoder {
     }
 };
 
-// N products with their operands loaded three ahead, and beside(i) behind
-// product i: the matrix unit takes 32 cycles for one, in which the wave can
-// issue some six vector instructions.  The compiler left to itself puts the
-// products together and the vector instructions behind them.
+// N products with their operands loaded two ahead (three measure the same and
+// take more registers), and beside(i) behind product i: the matrix unit takes
+// 32 cycles for one, in which the wave can issue some six vector instructions.
+// The compiler left to itself puts the products together and the vector
+// instructions behind them.
 template <int N, class Load, class Product, class Beside>
 __device__ __forceinline__ void products(Load&& load, Product&& product, Beside&& beside) {
     constexpr int kAhead = 2;
@@ -397,7 +398,11 @@ struct alignas(16) Stages {
 };
 
 // A segment of a tile of up to 64 rows: block after block, the next one's
-// pieces decoded behind the products.
+// pieces decoded before the products, with the loads of the one after behind
+// them.  12 sequences, 40 packed rows a key/value head of 256 channels, 4096 tokens:
+// 27 us, 18 MB.  Two thirds are the start and the end (pages, first pieces,
+// partial sums); a further 4096 tokens take 12 us, in which the vector unit is
+// the bound, since a block is decoded for few rows.
 template <class T>
 __device__ __forceinline__ void attend_few(const Kv4AttendArgs& a, const Kv4Segment& it, Stages<T>& lds) {
     constexpr int D = T::D, kMine = 2 * T::kPieces / T::kThreads;  // pieces of a thread, keys then values
@@ -505,8 +510,9 @@ __global__ __launch_bounds__(T::kThreads, 2) void kv4_attend_few_kernel(Kv4Atten
 // two stages of each are enough.
 //
 // Bound by the vector unit: a block of 64 tokens takes a wave 32 products of
-// 32 cycles and some 330 vector instructions, 32 of them exponentials of 16
-// cycles, on a unit that two waves share.  2048 rows behind 12288 tokens, 16
+// 32 cycles and some 260 vector instructions, 32 of them exponentials, on a
+// unit that two waves share, and keeps LDS busy more than half of the time;
+// the matrix unit works 40% of it.  2048 rows behind 12288 tokens, 16
 // heads over 2 of 128 channels: 293 us, 880 TFLOP/s.  Two waves in turn, one
 // with its products and one with its vector instructions, took 332 us: a
 // wave alone issues a vector instruction only every fifth cycle.
