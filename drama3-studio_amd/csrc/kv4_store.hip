@@ -243,7 +243,9 @@ __global__ __launch_bounds__(kRows == 1 ? kThreads : 1024) void kv4_append_kerne
         }
         if (is_q) {
             uint16_t* o = (uint16_t*)a.q_out.p + (int64_t)(row0 + i) * a.q_out.row_stride + (int64_t)local * a.q_out.head_stride;
-            *(v4i*)(o + c0) = pack8(x, a.dtype);
+            const v4i y = pack8(x, a.dtype);
+            if (kRows > 1) __builtin_nontemporal_store(y, (v4i*)(o + c0));  // more than a cache holds: 62 us with the read back, 70 without
+            else *(v4i*)(o + c0) = y;
             continue;
         }
         uint32_t scale_word;
@@ -261,8 +263,9 @@ __global__ __launch_bounds__(kRows == 1 ? kThreads : 1024) void kv4_append_kerne
 }
 
 // kRows rows a workgroup, one 8-channel chunk of a key or value head a thread:
-// bound by memory (30001 rows of 8 + 8 heads of 128 channels: 33 us, 158 MB at
-// 4.8 TB/s, what a copy reaches).
+// bound by memory.  Rows are written past the caches (30001 rows of 8 + 8
+// heads of 128 channels, 157 MB: 31 us, 5.1 TB/s, more than a copy reaches;
+// 50 us with ordinary stores).
 template <int kRows>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4ReadArgs a) {
     __shared__ Place places[kRows];
@@ -303,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4ReadArgs a) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = (float)((int)(word[i] >> (4 * j) & 15) - z) * s;
-        *(v4i*)(o + (int64_t)(row0 + i) * dst.row_stride) = pack8(x, a.dtype);
+        __builtin_nontemporal_store(pack8(x, a.dtype), (v4i*)(o + (int64_t)(row0 + i) * dst.row_stride));
     }
 }
 
