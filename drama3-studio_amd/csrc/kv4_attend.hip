@@ -394,6 +394,8 @@ __global__ __launch_bounds__(kThreads) void kv4_join_kernel(Kv4AttendArgs a, int
     }
     const int lane_row = threadIdx.x / kLanes, c0 = threadIdx.x % kLanes * 4;
     if (pieces <= 1) return;
+    // offsets that go back can name more rows than there are: such tiles' pieces have no place
+    if (first < 0 || first + (pieces - 1) * step + odd >= a.slots) return;
     const int row_b = min(a.tile_rows, n * a.group - row_a);
     int row = kRowEach ? (int)blockIdx.y * rows + lane_row : (int)blockIdx.y;
     const int row_end = kRowEach ? min(row_b, ((int)blockIdx.y + 1) * rows) : min(row_b, row + 1);

@@ -123,8 +123,9 @@ class Rotary:
 
     Pair i -- channels (i, i + R/2) of R, or (2i, 2i + 1) with ``interleaved``
     -- turns by ``position * inv_freq[i]``, where the position is that of
-    axis ``axis[i]`` (uint8 [R/2]; None: one axis).  ``sections`` makes such
-    an axis table from frequency counts.  Angles are formed in 64 bits.
+    axis ``axis[i]`` (uint8 [R/2]; None: the first), the last one where there
+    are fewer.  ``sections`` makes such an axis table from frequency counts.
+    Angles are formed in 64 bits.
     """
 
     __slots__ = ("inv_freq", "axis", "dim", "interleaved")
@@ -298,6 +299,8 @@ class KvCache4:
         q, q_rows = _rows(q, "q", shape, None, device)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError("query heads must be a multiple of the key/value heads")
+        if not -2 ** 31 <= window < 2 ** 31:
+            raise ValueError("window must fit 32 bits")
         if out is None:
             out = torch.empty(shape, dtype=q.dtype, device=device)
         out, out_rows = _rows(out, "out", shape, q.dtype, device, written=True)

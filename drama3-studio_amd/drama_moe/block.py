@@ -135,8 +135,8 @@ class AttentionBlock:
         self.heads = int(heads)
         if self.heads < 1 or self.heads % cache.kv_heads:
             raise ValueError("heads must be a multiple of the cache's key/value heads")
-        if window < 0:
-            raise ValueError("window must not be negative")
+        if not 0 <= window < 2 ** 31:
+            raise ValueError("window outside [0, 2^31)")
         width, kv_width = self.heads * cache.head_dim, cache.kv_heads * cache.head_dim
         for proj, name, side, size in ((q_proj, "q_proj", "out_features", width), (k_proj, "k_proj", "out_features", kv_width),
                                        (v_proj, "v_proj", "out_features", kv_width), (o_proj, "o_proj", "in_features", width)):
@@ -162,9 +162,7 @@ class AttentionBlock:
         if self.k_norm is not None:
             k = self.k_norm(k)
         if self.rotary is not None:
-            # rows without a place stay zeros, which attention does not read
-            q = self.cache.append(k, v, batch, rotary=self.rotary, positions=positions, q=q, q_out=torch.zeros_like(
-                q, memory_format=torch.contiguous_format))
+            q = self.cache.append(k, v, batch, rotary=self.rotary, positions=positions, q=q)
         else:
             self.cache.append(k, v, batch, positions=positions)
         attended = torch.zeros((rows, self.heads, dim), dtype=q.dtype, device=q.device)

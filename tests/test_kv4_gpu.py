@@ -366,6 +366,30 @@ def test_pages_out_of_range_and_odd_batches_are_flagged_and_skipped(cuda, rows):
         assert (out[rows - 1:2 * rows] == 77.0).all() and not (out[2 * rows:] == 77.0).any()
 
 
+@pytest.mark.parametrize("rows", [1, 10, 40])
+def test_offsets_that_go_back(cuda, rows):
+    """Every second sequence ends before it starts and is skipped; the others, all alike, own the same rows."""
+    print_case("kv4 offsets back", rows)
+    case = Case(cuda, [(rows, 3000)], 8, 2, 64, 64, torch.bfloat16, seed=rows).fill()
+    cache, batch = case.device()
+    q = case.random(8).to(cuda)
+    cache.status()
+    want = cache.attend(q, batch)
+    assert cache.status() == 0
+    n = 40
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    table = case.table.to(cuda).expand(2 * n - 1, -1).contiguous()
+    back = PagedBatch(table, i32([3000] * (2 * n - 1)), i32([0, rows] * n), rows=rows, max_rows=rows)
+    got = torch.full_like(want, 5.0)
+    cache.attend(q, back, out=got)
+    assert cache.status() == BAD
+    # other cuts of the same tokens: two roundings of the result, of weights and of sums apart
+    bound = case.expected(q.cpu(), 64 ** -0.5)[1]
+    assert (np.abs(wide(got) - wide(want)) <= 2 * bound).all()
+    with pytest.raises(ValueError, match="window must fit"):
+        cache.attend(q, batch, window=2 ** 32 + 5)
+
+
 def test_places_beyond_32_bits(cuda):
     """Pages behind 4 GiB of others; a row buffer whose rows lie far apart."""
     print_case("kv4 far pages")
