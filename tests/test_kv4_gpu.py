@@ -198,6 +198,34 @@ def test_values_no_code_can_stand_for(cuda):
     assert k[1, 0, 3] == 0 and k[2, 0, 5] == 15 * 2208 and v[1, 0, 40] == -15 * 2208
 
 
+def test_ranges_at_and_beside_every_scale(cuda):
+    """Groups whose range is 15 times a number of the scales' grid, exactly or the next fp16 value up or down."""
+    print_case("kv4 scale grid")
+    grid = [m * 2.0 ** (k - 6) for k in range(-14, 11) for m in range(64, 128)] + [m * 2.0 ** -20 for m in range(1, 64)]
+    ranges = (15 * torch.tensor(grid, dtype=torch.float64)).half()
+    assert (ranges.double() == 15 * torch.tensor(grid, dtype=torch.float64))[:64 * 25].all()
+    bits = ranges.view(torch.int16)
+    tops = torch.cat([ranges, (bits + 1).view(torch.float16), (bits - 1).view(torch.float16)])
+    assert torch.isfinite(tops).all()
+    heads, dim = 8, 64
+    rows = -(-len(tops) // (heads * 2))
+    k = torch.zeros(rows * heads * 2, 32, dtype=torch.float16)
+    k[:len(tops), 5] = tops                    # all above zero
+    v = torch.zeros_like(k)
+    v[:len(tops), 9] = -tops                   # all below
+    middle = torch.rand(k.shape, generator=torch.Generator().manual_seed(1)) * tops.max()
+    k[:, 16:] = torch.minimum(middle[:, 16:].half(), k[:, 5:6])
+    v[:, 16:] = -torch.minimum(middle[:, 16:].half() * 0.01, -v[:, 9:10])
+    k, v = k.reshape(rows, heads, dim), v.reshape(rows, heads, dim)
+    case = Case(cuda, [(rows, rows)], heads, heads, dim, 16, torch.float16, seed=2)
+    cache, batch = case.device()
+    cache.append(k.to(cuda), v.to(cuda), batch)
+    pages = ref.Pages(case.raw.numpy(), 16, dim)
+    for p in range(rows):
+        pages.put(int(case.table[0, p // 16]), p % 16, wide(k)[p].astype(np.float32), wide(v)[p])
+    assert np.array_equal(cache.pages.cpu().numpy(), pages.raw)
+
+
 # ------------------------------------------------------------------- attention
 
 EDGES = [(1, 1), (1, 2), (1, 16), (1, 17), (1, 63), (1, 64), (1, 65), (1, 128), (1, 300), (1, 1100)]
@@ -249,6 +277,18 @@ def test_more_sequences_than_there_is_room_for(cuda, dim, hq, hkv, seqs, longest
     scales = case.raw[:, :, 64 * dim:].view(torch.int16)
     scales.copy_(scales & 0x03FF | 0x2000)
     check_attend(case, case.random(hq), window=window)
+
+
+@pytest.mark.parametrize("dim,group,rows", [
+    (128, 1, 16), (128, 1, 17), (64, 8, 2), (64, 8, 3), (256, 1, 64), (256, 1, 65), (128, 32, 2), (128, 13, 5),
+    (64, 1, 256), (64, 1, 257), (128, 8, 32), (128, 8, 33), (256, 2, 64), (256, 2, 65), (64, 128, 1), (128, 300, 1)])
+def test_rows_at_the_edges_of_a_tile(cuda, dim, group, rows):
+    print_case("kv4 tile edges", dim, group, rows)
+    case = Case(cuda, [(rows, 1200), (rows, rows), (max(1, rows // 2), 65)], group, 1, dim, 32, torch.float16,
+                seed=dim + group + rows).fill()
+    q = case.random(group)
+    q[0] *= 200.0  # scores that leave fp16 as weights of the base before
+    check_attend(case, q, scale=dim ** -0.5)
 
 
 def test_default_tables_and_strided_queries(cuda):
