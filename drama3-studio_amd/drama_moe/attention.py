@@ -51,6 +51,13 @@ def _rows(t: Tensor, name: str, shape: tuple, dtype: torch.dtype | None, device,
     return t, _lib.HeadRows(address, s0 if rows else 0, s1 if heads else 0)
 
 
+def _new(shape: tuple, dtype: torch.dtype, device):
+    """New rows of ``shape`` and their descriptor."""
+    t = torch.empty(shape, dtype=dtype, device=device)
+    rows, heads, dim = shape
+    return t, _lib.HeadRows(t.data_ptr(), heads * dim if rows > 1 else 0, dim if heads > 1 else 0)
+
+
 def _heads(q: Tensor) -> int:
     return q.shape[1] if q.ndim == 3 else 0
 
@@ -232,8 +239,9 @@ class KvCache4:
             shape = (rows, heads, dim)
             q, q_rows = _rows(q, "q", shape, dtype, device)
             if q_out is None:
-                q_out = torch.empty(shape, dtype=dtype, device=device)
-            q_out, out_rows = _rows(q_out, "q_out", shape, dtype, device, written=True)
+                q_out, out_rows = _new(shape, dtype, device)
+            else:
+                _, out_rows = _rows(q_out, "q_out", shape, dtype, device, written=True)
         elif q_out is not None:
             raise ValueError("q_out needs q")
         turn = None
@@ -275,12 +283,12 @@ class KvCache4:
         batch's rows: keys as rotated, exact in fp16."""
         device = self._check(batch)
         shape = (batch.rows, self.kv_heads, self.head_dim)
-        if k_out is None:
-            k_out = torch.empty(shape, dtype=dtype, device=device)
-        if v_out is None:
-            v_out = torch.empty(shape, dtype=dtype, device=device)
-        k_out, k_rows = _rows(k_out, "k_out", shape, dtype, device, written=True)
-        v_out, v_rows = _rows(v_out, "v_out", shape, dtype, device, written=True)
+        if dtype not in _HALVES:
+            raise ValueError(f"k_out must be bf16 or fp16, got {dtype}")
+        k_out, k_rows = _new(shape, dtype, device) if k_out is None else _rows(k_out, "k_out", shape, dtype, device,
+                                                                               written=True)
+        v_out, v_rows = _new(shape, dtype, device) if v_out is None else _rows(v_out, "v_out", shape, dtype, device,
+                                                                               written=True)
         if batch.rows:
             with _on(device):
                 _lib.check(_lib.library().dmoe_kv4_read(
@@ -302,8 +310,9 @@ class KvCache4:
         if not -2 ** 31 <= window < 2 ** 31:
             raise ValueError("window must fit 32 bits")
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=device)
-        out, out_rows = _rows(out, "out", shape, q.dtype, device, written=True)
+            out, out_rows = _new(shape, q.dtype, device)
+        else:
+            _, out_rows = _rows(out, "out", shape, q.dtype, device, written=True)
         if batch.rows == 0:
             return out
         lib = _lib.library()
@@ -332,7 +341,7 @@ _HERE = _Here()
 
 def _on(device: torch.device):
     """The launches of a call go to its tensors' device, whichever is current."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _stream(device: torch.device) -> int:
