@@ -182,6 +182,7 @@ __device__ __forceinline__ void products(Load&& load, Product&& product, Beside&
     for (int i = 0; i < N; ++i) {
         if (i + kAhead < N) operand[(i + kAhead) % (kAhead + 1)] = load(i + kAhead);
         product(i, operand[i % (kAhead + 1)]);
+        __builtin_amdgcn_sched_barrier(0);
         beside(i);
         __builtin_amdgcn_sched_barrier(0);
     }
