@@ -398,8 +398,8 @@ struct Rows {
 
     // The same by way of LDS, `kStoreBytes` for each wave, so that whole rows
     // are stored, and past the caches: nine prompts of up to 2000 tokens, 32
-    // heads, take 181 us so, 187 with eight bytes of 32 rows at a time (214 with
-    // those past the caches).
+    // heads, take 175 us so, 7 us more with eight bytes of 32 rows at a time (33
+    // more with those past the caches).
     static constexpr int kRowBytes = 64 * T::kOut + 16, kStoreBytes = 32 * kRowBytes;
     __device__ __forceinline__ void store(float top, uint8_t* lds) const {
         if (!it.whole) return store_part(top);
@@ -541,8 +541,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void kv4_attend_few_kernel(Kv4Atten
 // 32 cycles and some 260 vector instructions, 32 of them exponentials, on a
 // unit that two waves share, and keeps LDS busy more than half of the time;
 // the matrix unit works 40% of it.  2048 rows behind 12288 tokens, 16
-// heads over 2 of 128 channels: 293 us, 880 TFLOP/s.  Two waves in turn, one
-// with its products and one with its vector instructions, took 332 us: a
+// heads over 2 of 128 channels: 284 us, 907 TFLOP/s.  Two waves in turn, one
+// with its products and one with its vector instructions, took 324 us: a
 // wave alone issues a vector instruction only every fifth cycle.
 template <class T>
 __global__ __launch_bounds__(T::kThreads, 2) void kv4_attend_many_kernel(Kv4AttendArgs a) {
