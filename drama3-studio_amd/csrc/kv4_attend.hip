@@ -440,11 +440,12 @@ __global__ __launch_bounds__(kThreads) void kv4_join_kernel(Kv4AttendArgs a, int
             __syncthreads();
             if (lane_row) return;  // of one row only
             float most = top;
+#pragma unroll
             for (int i = 1; i < kAtOnce; ++i) most = fmaxf(most, sum_m[i]);
             const float f = top == most ? 1.0f : __builtin_amdgcn_exp2f(top - most);
             sum *= f;
             v *= f;
-#pragma unroll 4
+#pragma unroll 8
             for (int i = 1; i < kAtOnce; ++i) {
                 const float h = sum_m[i] == most ? 1.0f : __builtin_amdgcn_exp2f(sum_m[i] - most);
                 sum = __builtin_fmaf(h, sum_l[i], sum);

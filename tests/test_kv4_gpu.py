@@ -226,6 +226,41 @@ def test_ranges_at_and_beside_every_scale(cuda):
     assert np.array_equal(cache.pages.cpu().numpy(), pages.raw)
 
 
+@pytest.mark.parametrize("dim,hq,hkv,rot,interleaved,dtype", [
+    (128, 60, 2, 1.0, False, torch.bfloat16), (128, 80, 3, 0.5, True, torch.float16), (64, 50, 20, 1.0, False, torch.bfloat16),
+    (256, 33, 16, 0.25, False, torch.float16)])
+def test_a_large_call_is_its_small_ones(cuda, dim, hq, hkv, rot, interleaved, dtype):
+    """Thousands of rows in one call against the same rows, up to 400 of one sequence a call."""
+    print_case("kv4 large append", dim, hq, hkv, rot, interleaved, dtype)
+    seqs = [(2000, 2000), (3, 700), (0, 5), (1337, 1400), (65, 65)]
+    case = Case(cuda, seqs, hq, hkv, dim, 32, dtype, seed=hq, behind=7, fill=0)
+    qkv = case.random(hq + 2 * hkv).to(cuda)
+    half = int(dim * rot) // 2
+    rotary = Rotary((10000.0 ** (-torch.arange(half) / half)).to(cuda), axis=Rotary.sections([half - 3, 2, 1], device=cuda),
+                    interleaved=interleaved)
+    positions = torch.randint(0, 90000, (3, case.rows), generator=case.g).to(cuda)
+    cache, batch = case.device()
+    cut = lambda at: (qkv[at, hq:hq + hkv], qkv[at, hq + hkv:])  # noqa: E731
+    q_out = torch.full((case.rows, hq, dim), 3.0, dtype=dtype, device=cuda)
+    cache.append(*cut(slice(None)), batch, rotary=rotary, positions=positions, q=qkv[:, :hq], q_out=q_out)
+    k, v = (torch.full((case.rows, hkv, dim), 4.0, dtype=dtype, device=cuda) for _ in range(2))
+    cache.read(batch, dtype=dtype, k_out=k, v_out=v)
+    assert cache.status() == 0 and (q_out[-7:] == 3.0).all() and (k[-7:] == 4.0).all() and (v[-7:] == 4.0).all()
+    pages = cache.pages.clone()
+    cache.pages.zero_()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    for s, (n, length) in enumerate(seqs):
+        for first in range(0, n, 400):
+            count = min(400, n - first)
+            at = slice(int(case.starts[s]) + first, int(case.starts[s]) + first + count)
+            part = PagedBatch(batch.block_table[s:s + 1], i32(length - n + first + count), i32(0, count), rows=count)
+            got = cache.append(*cut(at), part, rotary=rotary, positions=positions[:, at].contiguous(), q=qkv[at, :hq])
+            assert torch.equal(got, q_out[at])
+            kk, vv = cache.read(part, dtype=dtype)
+            assert torch.equal(kk, k[at]) and torch.equal(vv, v[at])
+    assert torch.equal(cache.pages, pages)
+
+
 # ------------------------------------------------------------------- attention
 
 EDGES = [(1, 1), (1, 2), (1, 16), (1, 17), (1, 63), (1, 64), (1, 65), (1, 128), (1, 300), (1, 1100)]
