@@ -471,9 +471,10 @@ void launch_dim(const Kv4AttendArgs& a, const Kv4Shape& s, hipStream_t st) {
     // cut (1200 tiles, none cut: 128 rows 2 us less than 64, 256 rows 4 us, but a cut tile's rows follow each other)
     const unsigned each = tiles > 512 ? 128 : kThreads / (D / 4);
     const dim3 row_each(tiles, (rows + each - 1) / each);
-    // few rows: many pieces each, and few workgroups unless there are many tiles
+    // few rows: many pieces each, and few workgroups unless there are many tiles; a workgroup a row while that does
+    // not fill the chip (12 sequences with 40 rows: 29 us with the attention, 32 with four rows a workgroup)
     if (a.tile_rows <= 16 && tiles <= 32) kv4_join_kernel<D, true, false, 1024><<<dim3(tiles, rows), 1024, 0, st>>>(a, 1);
-    else if (a.tile_rows <= 16) kv4_join_kernel<D, true, false, kThreads><<<dim3(tiles, rows), kThreads, 0, st>>>(a, 1);
+    else if (a.tile_rows <= 16 || (s.one_tile && (int64_t)tiles * rows <= 4096)) kv4_join_kernel<D, true, false, kThreads><<<dim3(tiles, rows), kThreads, 0, st>>>(a, 1);
     else if (s.one_tile) kv4_join_kernel<D, true, true, kThreads><<<row_each, kThreads, 0, st>>>(a, each);
     else kv4_join_kernel<D, false, true, kThreads><<<row_each, kThreads, 0, st>>>(a, each);
 }
