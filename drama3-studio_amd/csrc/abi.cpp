@@ -1604,7 +1604,7 @@ dmoe::Kv4Batch to_kernel(const DmoeKv4Batch* b, bool tables = true) {
     require(b->rows >= 1 && b->rows <= (1 << 24), "row count outside [1, 2^24]");
     require(b->max_rows >= 1 && b->max_rows <= b->rows, "max_rows outside [1, rows]");
     require(b->starts || b->rows >= b->seqs, "one row a sequence needs at least as many rows as sequences");
-    require(b->table_cols >= 1 && b->table_stride >= b->table_cols, "bad block_table geometry");
+    require(b->table_cols >= 1 && (b->table_stride == 0 || b->table_stride >= b->table_cols), "bad block_table geometry");
     return {b->block_table, b->table_stride, b->lengths, b->starts, b->seqs, b->table_cols, b->rows, b->max_rows};
 }
 

@@ -72,7 +72,7 @@ class PagedBatch:
     """Rows of a call over paged sequences.
 
     ``block_table`` [S, pages] int32 names the pages of each sequence's
-    tokens, ``lengths`` [S] int32 counts its tokens with the call's rows among
+    tokens (sequences on the same pages may share a row: ``row.expand(S, -1)``), ``lengths`` [S] int32 counts its tokens with the call's rows among
     them, and ``starts`` [S + 1] int32 are the offsets of each sequence's rows
     in the row buffers (None: row s is sequence s).  With n rows, a
     sequence's rows are its last n tokens.  ``rows`` is the row count of the
@@ -95,6 +95,10 @@ class PagedBatch:
             raise ValueError(f"sequence count outside [1, {MAX_SEQUENCES}]")
         if cols < 1:
             raise ValueError("block_table has no pages")
+        # sequences on the same pages may share one row of the table (stride 0)
+        stride = block_table.stride(0) if seqs > 1 else cols
+        if 0 < stride < cols:
+            raise ValueError("block_table rows overlap")
         device = lengths.device
         if block_table.device != device:
             raise ValueError("batch tables must share a device")
@@ -120,8 +124,7 @@ class PagedBatch:
         self.block_table, self.lengths, self.starts = block_table, lengths, starts
         self.rows, self.max_rows, self.device = rows, max_rows, device
         self.scratch = {}  # bytes that attention over this batch's sizes needs, by geometry
-        # a table of one row may have any row stride
-        self.desc = _lib.Kv4Batch(block_table.data_ptr(), max(block_table.stride(0), cols), lengths.data_ptr(),
+        self.desc = _lib.Kv4Batch(block_table.data_ptr(), stride, lengths.data_ptr(),
                                   starts.data_ptr() if starts is not None else None, seqs, cols, rows, max_rows)
 
 

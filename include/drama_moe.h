@@ -504,7 +504,8 @@ typedef struct DmoeKv4Cache {
 /* The rows of a call.  Sequence s owns rows starts[s] .. starts[s+1] - 1
  * (starts [seqs + 1]; NULL: row s) of the rows buffers; they are the LAST
  * tokens of its lengths[s] tokens: with n rows, row i has place lengths[s] - n
- * + i.  Its token p lies in page block_table[s * table_stride + p / page_size].
+ * + i.  Its token p lies in page block_table[s * table_stride + p / page_size];
+ * table_stride is at least table_cols, or 0 where all sequences share one row.
  * `rows` is the row count of the buffers, max_rows the most rows of a sequence
  * (sizes the launch).  Tables are device memory and may differ at each replay
  * of a captured call; at most 4096 sequences.  Places below 0 (a

@@ -52,6 +52,37 @@ def test_python_refusals(make, message):
         make()
 
 
+@pytest.mark.parametrize("seqs,cols,size,stride", [
+    (3, 5, 5, 0), (2, 1, 1, 0), (4096, 2, 2, 0),          # one row for all: row.expand(seqs, cols)
+    (1, 5, 5, 0), (1, 5, 5, 1), (1, 5, 5, 400),           # one sequence, whatever its row stride is
+    (3, 5, 15, 5), (3, 5, 19, 7), (3, 1, 3, 1)])
+def test_tables_are_read_where_they_lie(seqs, cols, size, stride):
+    """The descriptor's places of all entries are those of the tensor."""
+    table = torch.arange(size, dtype=torch.int32).as_strided((seqs, cols), (stride, 1))
+    desc = PagedBatch(table, i32(seqs)).desc
+    assert (desc.seqs, desc.table_cols) == (seqs, cols)
+    places = np.arange(seqs)[:, None] * desc.table_stride + np.arange(cols)
+    assert places.max() < size and np.array_equal(places, table.numpy())
+
+
+@pytest.mark.parametrize("seqs,cols,stride", [(3, 5, 2), (2, 5, 4), (3, 2, 1)])
+def test_tables_whose_rows_overlap_are_refused(seqs, cols, stride):
+    table = i32((seqs - 1) * stride + cols).as_strided((seqs, cols), (stride, 1))
+    with pytest.raises(ValueError, match="rows overlap"):
+        PagedBatch(table, i32(seqs))
+
+
+@pytest.mark.parametrize("stride,accepted", [(0, True), (1, False), (3, False), (4, True), (9, True)])
+def test_entry_points_take_one_table_row_for_all_sequences(stride, accepted):
+    cache, batch, _, _ = descriptors(batch=dict(table_stride=stride, block_table=None, lengths=None))
+    size = _lib.library().dmoe_kv4_attention_workspace_bytes(ctypes.byref(cache), ctypes.byref(batch), 4)
+    assert (size > 0) == accepted
+    if not accepted:
+        for entry in ("append", "read", "attend"):
+            assert call(entry, descriptors(batch=dict(table_stride=stride))) == -1
+            assert "block_table geometry" in _lib.library().dmoe_last_error().decode()
+
+
 def test_there_is_no_cpu_path():
     cache = KvCache4.allocate(4, 2, 64, page_size=16, device="cpu")
     batch = PagedBatch(i32(1, 2), i32(1))

@@ -511,6 +511,30 @@ def test_shared_prefix_pages_and_strided_layers(cuda):
     assert torch.equal(inner.attend(q, batch), want)
 
 
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_one_table_row_for_all_sequences(cuda, rows):
+    """A table expanded from one row is its copy: sequences on the same pages, each at places of its own."""
+    print_case("kv4 expanded table", rows)
+    case = Case(cuda, [(rows, 300)], 4, 2, 64, 16, torch.bfloat16, seed=rows + 50).fill()
+    n = 5
+    cache, _ = case.device()
+    lengths = torch.tensor([300, 60, 107, 154, 201], dtype=torch.int32, device=cuda)
+    starts = torch.arange(0, n * rows + 1, rows, dtype=torch.int32, device=cuda)
+    q, k, v = (case.random(h, rows=n * rows).to(cuda) for h in (4, 2, 2))
+    table = case.table.to(cuda)
+    before, results = cache.pages.clone(), []
+    cache.status()
+    for t in (table.expand(n, -1), table.expand(n, -1).contiguous()):
+        cache.pages.copy_(before)
+        batch = PagedBatch(t, lengths, starts, rows=n * rows, max_rows=rows)
+        first = cache.attend(q, batch)
+        cache.append(k, v, batch)
+        results.append((first, cache.pages.clone(), *cache.read(batch), cache.attend(q, batch, window=50)))
+    assert cache.status() == 0 and not torch.equal(results[0][1], before)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 # --------------------------------------------------------------- as it is used
 
 def decode_step(cache, batch, qkv, hq, hkv, rotary):
