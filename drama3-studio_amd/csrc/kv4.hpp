@@ -21,10 +21,11 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "kv4_places.hpp"
+
 namespace dmoe {
 
 constexpr int kKv4Group = 32;          // channels a scale word
-constexpr int kKv4Block = 64;          // tokens an attention step takes
 constexpr int kKv4Whole = 16;          // sequences of up to this many blocks are not cut
 constexpr int kKv4MaxSeqs = 4096;
 constexpr float kKv4Limit = 32640.0f;  // values beyond are stored as this: 15 s = 2 * 32640 is the largest span in fp16

@@ -46,7 +46,7 @@ struct Pages {
 };
 __device__ __forceinline__ Pages pages_of(const Kv4AttendArgs& a, int seq, int block, int end, int r, int g) {
     const int32_t* table = a.batch.table + (int64_t)seq * a.batch.table_stride;
-    const int kt = min(block * kKv4Block + 4 * r, end - 1), vt = min(block * kKv4Block + 16 * g, end - 1), shift = a.cache.page_shift;
+    const int kt = kv4_token(block, 4 * r, end), vt = kv4_token(block, 16 * g, end), shift = a.cache.page_shift;
     return Pages{table[kt >> shift], table[vt >> shift]};
 }
 

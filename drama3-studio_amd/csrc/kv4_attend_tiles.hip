@@ -89,7 +89,7 @@ __device__ __forceinline__ Place piece_place(bool is_v, int at, int page_shift) 
 template <int D>
 __device__ __forceinline__ void load_page(const Kv4AttendArgs& a, const int32_t* table, bool is_v, int at, int block, int end,
                                           Piece& piece) {
-    int token = min(block * kKv4Block + piece_token<D>(is_v, at), end - 1);  // behind the end: the last token's
+    int token = kv4_token(block, piece_token<D>(is_v, at), end);  // behind the end: the last token's
     // has the page copied before this load: a copy left to the loop's end would wait for the load
     asm("" : "+v"(piece.page), "+v"(token));
     piece.next = *(const int32_t*)((const char*)table + (uint32_t)(token >> a.cache.page_shift) * 4u);
@@ -139,7 +139,7 @@ struct Decoder {
         uint32_t w0 = piece.scales[0], w1 = piece.scales[1];
         if (is_v) {
             // slots that hold no token may hold anything; their values must be numbers
-            const int kept = (unsigned)piece.page >= (unsigned)a.cache.num_pages ? 0 : end - block * kKv4Block - token;
+            const int kept = (unsigned)piece.page >= (unsigned)a.cache.num_pages ? 0 : kv4_left(block, token, end);
             w0 &= (kept > 0 ? 0xFFFFu : 0u) | (kept > 1 ? 0xFFFF0000u : 0u);
             w1 &= (kept > 2 ? 0xFFFFu : 0u) | (kept > 3 ? 0xFFFF0000u : 0u);
             const int word = at % (D / 8), quad = token / 4;

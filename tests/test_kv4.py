@@ -4,12 +4,15 @@ tests use."""
 from __future__ import annotations
 
 import ctypes
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
 import torch
 
 import kv4_reference as ref
+from conftest import ROOT
 from drama_moe import _lib
 from drama_moe.attention import KvCache4, PagedBatch, Rotary
 from drama_moe.block import AttentionBlock
@@ -203,6 +206,27 @@ def test_workspace_covers_more_rows_with_more_bytes():
     assert lib.dmoe_kv4_attention_workspace_bytes(by(cache), by(batch), 4) == 0
     cache, batch, _, _ = descriptors()
     assert lib.dmoe_kv4_attention_workspace_bytes(by(cache), by(batch), 5) == 0
+
+
+def places_check(tmp_path, header):
+    (tmp_path / "kv4_places.hpp").write_text(header)
+    exe = tmp_path / "places_check"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fwrapv", "-Wall", "-Werror", "-I", str(tmp_path),
+                    str(ROOT / "tests" / "kv4_places_check.cpp"), "-o", str(exe)], check=True)
+    return subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_places_of_tokens_up_to_the_longest_sequence(tmp_path):
+    header = (ROOT / "drama3-studio_amd" / "csrc" / "kv4_places.hpp").read_text()
+    run = places_check(tmp_path, header)
+    assert run.returncode == 0 and run.stdout.startswith("ok "), run.stdout + run.stderr
+    # the check sees a place formed in 31 bits before it is cut
+    signed = header.replace("const uint32_t token = (uint32_t)block * kKv4Block + (uint32_t)at, last = (uint32_t)end - 1;",
+                            "const int32_t token = block * kKv4Block + at, last = end - 1;")
+    assert signed != header
+    run = places_check(tmp_path, signed)
+    assert run.returncode == 1 and "differ" in run.stdout
 
 
 # --------------------------------------------------------------- the reference

@@ -535,6 +535,38 @@ def test_one_table_row_for_all_sequences(cuda, rows):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dim,hq,hkv", [(64, 2, 2), (128, 4, 1), (256, 1, 1)])
+@pytest.mark.parametrize("rows", [1, 3, 20, 70])
+def test_the_last_of_the_longest_sequence(cuda, dim, hq, hkv, rows):
+    """2^31 - 1 tokens, of which a window sees the last: blocks and places at the end of 31 bits."""
+    print_case("kv4 longest", dim, hq, hkv, rows)
+    page, longest, window = 256, 2 ** 31 - 1, 300
+    cols = -(-longest // page)
+    table = torch.full((1, cols), 4, dtype=torch.int32, device=cuda)
+    table[0, -4:] = torch.tensor([3, 0, 2, 1], dtype=torch.int32)
+    cache = KvCache4.allocate(5, hkv, dim, page_size=page, device=cuda)
+    base, n = (cols - 4) * page, 900
+    g = torch.Generator().manual_seed(dim + rows)
+    k, v = (torch.randn(n, hkv, dim, generator=g).half() for _ in range(2))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    cache.status()
+    cache.append(k.to(cuda), v.to(cuda), PagedBatch(table, i32(longest), i32(0, n), rows=n))
+    pages = ref.Pages(np.zeros(cache.pages.shape, np.uint8), page, dim)
+    own, places = [3, 0, 2, 1], range(longest - base - n, longest - base)
+    for i, p in enumerate(places):
+        pages.put(own[p // page], p % page, wide(k)[i], wide(v)[i])
+    assert np.array_equal(cache.pages.cpu().numpy(), pages.raw)
+    batch = PagedBatch(table, i32(longest), i32(0, rows), rows=rows)
+    q = torch.randn(rows, hq, dim, generator=g).half()
+    out = cache.attend(q.to(cuda), batch, window=window)
+    held = [np.stack(x) for x in zip(*(pages.get(own[p // page], p % page) for p in range(longest - base)))]
+    want, size, terms = ref.attention(wide(q), *held, longest - base, dim ** -0.5, window)
+    bound = ref.tolerance(want, size, terms, dim, window, EPS[torch.float16])
+    assert cache.status() == 0 and (np.abs(wide(out) - want) <= bound).all()
+    got = cache.read(batch)
+    assert all(np.array_equal(wide(x), y[-rows:]) for x, y in zip(got, held))
+
+
 # --------------------------------------------------------------- as it is used
 
 def decode_step(cache, batch, qkv, hq, hkv, rotary):
