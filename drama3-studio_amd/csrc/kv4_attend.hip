@@ -176,7 +176,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_attend_rows_ke
 
         for (int block = from; block < to; ++block) {
             const bool any_bad = __any(values.bad);
-            if (any_bad && a.status) raise_status(a.status, kBadBatch);
+            if (any_bad && a.status && __any(values.bad && block * kKv4Block + 16 * g + 15 >= kv4_lowest(p_first, a.window)))
+                raise_status(a.status, kBadBatch);  // a page that a row would see
             v4f s[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

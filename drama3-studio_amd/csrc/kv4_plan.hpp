@@ -55,10 +55,15 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 __device__ __forceinline__ int wave_total(int v) { return of_lane(wave_scan(v), kWave - 1); }
 
+// The first token that a row at place p sees; no row behind it sees an earlier one.
+__device__ __forceinline__ int kv4_lowest(int p, int window) {
+    return window > 0 ? (int)max((int64_t)0, (int64_t)p - window + 1) : 0;
+}
+
 // First and last (exclusive) block that rows i0..i1 of a sequence see.
 __device__ __forceinline__ void kv4_blocks(const Kv4Seq& q, int window, int i0, int i1, int& b0, int& b1) {
     const int p0 = q.len - q.n + i0, p1 = q.len - q.n + i1;
-    b0 = window > 0 ? max(0, (int)max((int64_t)0, (int64_t)p0 - window + 1)) / kKv4Block : 0;
+    b0 = kv4_lowest(p0, window) / kKv4Block;
     b1 = p1 < 0 ? b0 : max(b0, p1 / kKv4Block + 1);
 }
 

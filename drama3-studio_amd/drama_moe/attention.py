@@ -302,7 +302,8 @@ class KvCache4:
                out: Tensor | None = None) -> Tensor:
         """Attention of queries [rows, heads, D] over the cache: a row sees the
         tokens up to its own place, with ``window`` only that many of them; one
-        that sees none becomes 0.  ``scale`` defaults to D ** -0.5.  Rows that
+        that sees none becomes 0.  Table entries behind the windows of all rows
+        may name no page.  ``scale`` defaults to D ** -0.5.  Rows that
         no sequence owns are not written (in a new ``out`` they hold nothing)."""
         device = self._check(batch)
         heads = _heads(q)

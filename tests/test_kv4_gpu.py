@@ -567,6 +567,25 @@ def test_the_last_of_the_longest_sequence(cuda, dim, hq, hkv, rows):
     assert all(np.array_equal(wide(x), y[-rows:]) for x, y in zip(got, held))
 
 
+@pytest.mark.parametrize("dim,hq,hkv,page,window,rows", [
+    (128, 16, 2, 16, 70, 1), (64, 4, 4, 32, 33, 1), (256, 2, 1, 16, 100, 3), (128, 4, 1, 32, 65, 12),
+    (64, 10, 2, 16, 40, 9), (256, 8, 1, 16, 50, 5), (128, 2, 1, 16, 90, 150), (256, 3, 3, 32, 130, 130),
+    (64, 4, 1, 16, 64, 200)])
+def test_pages_behind_a_window_may_be_given_back(cuda, dim, hq, hkv, page, window, rows):
+    """Table entries of which no row sees a token name no page: nothing is flagged.  The first one in sight is."""
+    print_case("kv4 window pages", dim, hq, hkv, page, window, rows)
+    lengths = [rows + x for x in (0, 257, 300, 313, 326, 350)]
+    case = Case(cuda, [(rows, length) for length in lengths], hq, hkv, dim, page, torch.bfloat16, seed=dim + rows).fill()
+    q = case.random(hq)
+    gone = [max(0, length - rows - window + 1) // page for length in lengths]
+    for s, count in enumerate(gone):
+        case.table[s, :count] = torch.tensor([-1, len(case.raw), 2 ** 31 - 1, -2 ** 31]).repeat(99)[:count].int()
+    assert gone[0] == 0 and min(gone[1:]) > 0
+    check_attend(case, q, window=window)
+    case.table[3, gone[3]] = -1
+    check_attend(case, q, window=window, status=BAD)
+
+
 # --------------------------------------------------------------- as it is used
 
 def decode_step(cache, batch, qkv, hq, hkv, rotary):
