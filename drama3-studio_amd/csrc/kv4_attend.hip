@@ -219,14 +219,15 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_attend_rows_ke
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
                         s[i][x] = ((4 * x + i > high) | (4 * x + i < low)) ? -__builtin_inff() : s[i][x];
-                // slots that hold no token may hold anything: a weight of zero
-                // times a value that is no number would reach the sum
-                const int kept = values.bad ? 0 : it.len - at;
+                // slots that hold no token, or one that no row sees, may hold anything: a
+                // weight of zero times a value that is no number would reach the sum
+                const int kept = values.bad ? 0 : it.len - at, gone = kv4_lowest(p_first, a.window) - at;
 #pragma unroll
                 for (int c = 0; c < kParts; ++c)
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
-                        scales[c][x / 4][x % 4] &= (2 * x < kept ? 0xFFFFu : 0u) | (2 * x + 1 < kept ? 0xFFFF0000u : 0u);
+                        scales[c][x / 4][x % 4] &= (((2 * x < kept) & (2 * x >= gone)) ? 0xFFFFu : 0u) |
+                                                   (((2 * x + 1 < kept) & (2 * x + 1 >= gone)) ? 0xFFFF0000u : 0u);
             }
             // P and this lane's part of its sum, of the weights as they are
             // multiplied.  base * scale is rounded once for all of a row's tokens;

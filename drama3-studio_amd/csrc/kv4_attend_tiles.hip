@@ -128,16 +128,21 @@ struct Decoder {
     int place;
 
     // keys, values: the places of their stages
-    __device__ __forceinline__ Decoder(const Kv4AttendArgs& a, const CodeBits& bits, bool is_v, int at, int block, int end,
-                                       const Piece& piece, int keys, int values)
+    __device__ __forceinline__ Decoder(const Kv4AttendArgs& a, const CodeBits& bits, bool is_v, int at, int block, int lowest,
+                                       int end, const Piece& piece, int keys, int values)
         : x(0), y(0), held(0) {
         const int token = piece_token<D>(is_v, at);
         uint32_t w0 = piece.scales[0], w1 = piece.scales[1];
         if (is_v) {
-            // slots that hold no token may hold anything; their values must be numbers
+            // slots that hold no token, or one that no row sees, may hold anything; their values must be numbers
             const int kept = (unsigned)piece.page >= (unsigned)a.cache.num_pages ? 0 : kv4_left(block, token, end);
             w0 &= (kept > 0 ? 0xFFFFu : 0u) | (kept > 1 ? 0xFFFF0000u : 0u);
             w1 &= (kept > 2 ? 0xFFFFu : 0u) | (kept > 3 ? 0xFFFF0000u : 0u);
+            if (kv4_left(block, 0, lowest) > 0) {
+                const int gone = kv4_left(block, token, lowest);
+                w0 &= (gone > 0 ? 0u : 0xFFFFu) | (gone > 1 ? 0u : 0xFFFF0000u);
+                w1 &= (gone > 2 ? 0u : 0xFFFFu) | (gone > 3 ? 0u : 0xFFFF0000u);
+            }
             const int word = at % (D / 8), quad = token / 4;
             // 16 tokens of an operand step: lanes 0..31 take tokens 0..3 and 8..11 of them, lanes 32..63 the others
             place = values + value_at(8 * word, quad / 4 * 2 + (quad & 1)) + (quad >> 1 & 1) * 8;
@@ -195,7 +200,8 @@ struct Rows {
     int row_a, row_b;              // the tile's packed rows
     int wave_a, wave_b;            // this wave's, maybe none
     int place;                     // of this lane's token
-    int end, p_first, p_last;
+    int lowest, end;               // the tokens that any row of the tile sees
+    int p_first, p_last;           // places of this wave's rows
     v8h query[kSteps];
     float score_scale;             // of the scores in powers of two
     float base, shift;             // the maximum that weights are taken from; 8 - base in powers of two
@@ -218,6 +224,7 @@ struct Rows {
         wave_a = row_a + 32 * group;
         wave_b = min(wave_a + 32, row_b);
         place = it.len - it.n + min(wave_a + r, packed - 1) / a.group;
+        lowest = kv4_lowest(it.len - it.n + row_a / a.group, a.window);
         end = it.len - it.n + (row_b - 1) / a.group + 1;
         p_first = it.len - it.n + wave_a / a.group;
         p_last = it.len - it.n + (wave_b - 1) / a.group;
@@ -255,9 +262,8 @@ struct Rows {
     // Reports entries of the table that name no page, of tokens in the blocks
     // [from, to) which a row of the tile would see.
     __device__ __forceinline__ void report(const int32_t* table, int from, int to) const {
-        const int lowest = max(from * kKv4Block, kv4_lowest(it.len - it.n + row_a / a.group, a.window));
         const int shift = a.cache.page_shift, last = kv4_token(to - 1, kKv4Block - 1, end) >> shift;
-        for (int i = (lowest >> shift) + (int)threadIdx.x; i <= last; i += T::kThreads)
+        for (int i = (max(from * kKv4Block, lowest) >> shift) + (int)threadIdx.x; i <= last; i += T::kThreads)
             if ((unsigned)table[i] >= (unsigned)a.cache.num_pages) raise_status(a.status, kBadBatch);
     }
 
@@ -463,7 +469,7 @@ __device__ __forceinline__ void attend_few(const Kv4AttendArgs& a, const Kv4Segm
         uint8_t* stage = lds.stage[(block - from) & 1];
         each([&](bool is_v, int at, Piece& x) {
             if (!is_v) store_page<D>(a, at, x, lds.parts[(block - from) & 1]);
-            Decoder<D> decoder(a, bits, is_v, at, block, rows.end, x, 0, T::kKeyBytes);
+            Decoder<D> decoder(a, bits, is_v, at, block, rows.lowest, rows.end, x, 0, T::kKeyBytes);
 #pragma unroll
             for (int u = 0; u < 16; ++u) decoder.step(bits, is_v, x, u, stage);
         });
@@ -581,7 +587,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void kv4_attend_many_kernel(Kv4Atte
     };
     const auto decoder = [&](int m, int block) {
         const int n = (block - from) & 1;
-        return Decoder<D>(a, bits, is_v, m * kSide + (int)threadIdx.x % min(kSide, T::kPieces), block, rows.end, piece[m],
+        return Decoder<D>(a, bits, is_v, m * kSide + (int)threadIdx.x % min(kSide, T::kPieces), block, rows.lowest, rows.end, piece[m],
                           n * T::kKeyBytes, 2 * T::kKeyBytes + n * T::kValueBytes);
     };
     const auto store = [&](int block) {

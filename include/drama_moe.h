@@ -515,7 +515,7 @@ typedef struct DmoeKv4Cache {
  * table_cols pages is skipped, and a token whose page is outside
  * [0, num_pages) is not stored, read as 0, and seen by no row; both raise
  * DMOE_STATUS_BAD_BATCH, in attention where a row would see the token: table
- * entries behind the windows of all rows may hold anything. */
+ * entries behind the windows of all rows, and slots there, may hold anything. */
 typedef struct DmoeKv4Batch {
     const int32_t* block_table;
     int64_t table_stride;

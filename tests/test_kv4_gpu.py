@@ -586,6 +586,39 @@ def test_pages_behind_a_window_may_be_given_back(cuda, dim, hq, hkv, page, windo
     check_attend(case, q, window=window, status=BAD)
 
 
+@pytest.mark.parametrize("dim,hq,hkv,page,window,rows", [
+    (128, 16, 2, 16, 70, 1), (64, 4, 4, 256, 33, 1), (256, 2, 1, 128, 100, 3), (128, 4, 1, 32, 65, 12),
+    (64, 10, 2, 64, 40, 9), (256, 8, 1, 16, 50, 5), (128, 2, 1, 64, 90, 150), (256, 3, 3, 128, 130, 130),
+    (64, 4, 1, 16, 64, 200)])
+def test_slots_behind_a_window_may_hold_anything(cuda, dim, hq, hkv, page, window, rows):
+    """Tokens that no row sees were never stored: their slots, and pages named in their place, hold bytes of 255 (scales
+    that are no number)."""
+    print_case("kv4 window slots", dim, hq, hkv, page, window, rows)
+    lengths = [rows + x for x in (0, 257, 300, 313, 326, 350, 366)]
+    case = Case(cuda, [(rows, length) for length in lengths], hq, hkv, dim, page, torch.bfloat16, seed=dim + page)
+    clean = ref.Pages(case.raw.numpy().copy(), page, dim)
+    pages = ref.Pages(case.raw.numpy(), page, dim)
+    for s, length in enumerate(lengths):
+        kv = wide(torch.randn(length, 2, hkv, dim, generator=case.g)).astype(np.float32)
+        lowest = max(0, length - rows - window + 1)
+        for p in range(length):
+            at = (int(case.table[s, p // page]), p % page)
+            clean.put(*at, *kv[p])
+            if p >= lowest:
+                pages.put(*at, *kv[p])
+    q = case.random(hq)
+    stored = case.raw.clone()
+    case.raw = torch.from_numpy(clean.raw)
+    want = check_attend(case, q, window=window)
+    case.raw = stored
+    for s, length in enumerate(lengths):
+        case.table[s, :max(0, length - rows - window + 1) // page] = case.unused[s % 2]
+    cache, batch = case.device()
+    cache.status()
+    got = cache.attend(q.to(cuda), batch, window=window)
+    assert torch.isfinite(got).all() and torch.equal(got, want) and cache.status() == 0
+
+
 # --------------------------------------------------------------- as it is used
 
 def decode_step(cache, batch, qkv, hq, hkv, rotary):
