@@ -1726,6 +1726,7 @@ int dmoe_kv4_attention(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, con
         a.slots_log2 = s.slots_log2;
         a.min_blocks = s.min_blocks;
         a.cut = s.cut;
+        a.groups = s.groups;
         a.slots = s.slots;
         a.tile_rows = s.tile_rows;
         a.part = static_cast<float*>(workspace);

@@ -89,7 +89,7 @@ struct Kv4AttendArgs {
     int slots_log2;         // work is cut for 2^slots_log2 workgroups,
     int min_blocks;         // in pieces of at least this many blocks
     bool cut;               // if at all: without, there is no room for partial sums
-    int64_t slots;          // of the partial sums
+    int64_t groups, slots;  // workgroups; places for partial sums
     int tile_rows;          // packed rows (token, head of the group) of a tile
     float* part;            // [slots][tile_rows][D] unnormalised sums of the pieces of a cut tile
     float* part_ml;         // [slots][tile_rows][2] running maximum and sum

@@ -372,6 +372,7 @@ __global__ __launch_bounds__(kThreads) void kv4_join_kernel(Kv4AttendArgs a, int
     const int kv = a.cache.kv_heads;
     int pieces, head, row0, n, row_a;
     int64_t first, step, odd;  // slots of the first piece and between them, and what the first lies behind that
+    int64_t group = 0;         // of the last piece
     if constexpr (kOneTile) {
         const Kv4Record rec = a.records[blockIdx.x];
         pieces = rec.pieces;
@@ -390,14 +391,15 @@ __global__ __launch_bounds__(kThreads) void kv4_join_kernel(Kv4AttendArgs a, int
         row0 = it.row0;
         n = it.n;
         row_a = it.tile * a.tile_rows;
-        first = it.first;
+        first = it.slot;
         step = kv;
         odd = 0;
+        group = it.first + (pieces - 1) * step;
     }
     const int lane_row = threadIdx.x / kLanes, c0 = threadIdx.x % kLanes * 4;
     if (pieces <= 1) return;
-    // offsets that go back can name more rows than there are: such tiles' pieces have no place
-    if (first < 0 || first + (pieces - 1) * step + odd >= a.slots) return;
+    // offsets that go back can name more rows than there are: such tiles' pieces have no place or no workgroup
+    if (first < 0 || first + (pieces - 1) * step + odd >= a.slots || group < 0 || group >= a.groups) return;
     const int row_b = min(a.tile_rows, n * a.group - row_a);
     int row = kRowEach ? (int)blockIdx.y * rows + lane_row : (int)blockIdx.y;
     const int row_end = kRowEach ? min(row_b, ((int)blockIdx.y + 1) * rows) : min(row_b, row + 1);
@@ -508,7 +510,10 @@ Kv4Shape kv4_attend_shape(const Kv4Batch& b, int page_size, int kv_heads, int di
     // shares: as many as wanted, or one a sequence and head where nothing is cut
     const int64_t shares = s.cut ? cuts : std::max(cuts, (int64_t)b.seqs * kv_heads);
     s.groups = !s.one_tile ? s.tiles * kv_heads + (s.cut ? cuts : 0) : waves ? (shares + kWaves - 1) / kWaves : shares;
-    s.slots = !s.cut ? 0 : s.one_tile ? 2 * cuts : s.groups;
+    // Partial sums: two for each share that there can be.  Of many rows only cut tiles have them, and a tile is cut if
+    // its blocks are more than a piece, which has at least a workgroup's average work: less than two pieces a workgroup.
+    const int64_t most_shares = (int64_t)b.seqs * kv_heads * ((most_blocks + s.min_blocks - 1) / s.min_blocks);
+    s.slots = !s.cut ? 0 : s.one_tile ? 2 * std::min(cuts, most_shares) : std::min(s.groups, 2 * cuts);
     s.part_bytes = (size_t)s.slots * s.tile_rows * dim * sizeof(float);
     s.ml_bytes = (size_t)s.slots * s.tile_rows * 2 * sizeof(float);
     s.record_bytes = s.cut && s.one_tile ? (size_t)b.seqs * kv_heads * sizeof(Kv4Record) : 0;

@@ -379,7 +379,7 @@ struct Rows {
     }
 
     __device__ __forceinline__ void store_part(float top) const {
-        if (wave_a + r >= row_b) return;
+        if (wave_a + r >= row_b || it.slot < 0 || it.slot >= a.slots) return;  // see the join
         const int c0 = 32 * T::kOut * split + 4 * hi;
         const int64_t at = it.slot * a.tile_rows + 32 * group + r;
         float* o = a.part + at * D + c0;

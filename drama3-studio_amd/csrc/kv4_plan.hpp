@@ -177,7 +177,8 @@ struct Kv4Shares {
 struct Kv4Item {
     int seq, head, tile, split, splits;
     int row0, n, len;
-    int first;  // workgroup of the tile's first piece; its pieces lie kv_heads apart
+    int first;  // workgroup of the tile's first piece; its pieces lie kv_heads apart,
+    int slot;   // as do their partial sums, which only cut tiles have
     bool live;
 };
 
@@ -201,12 +202,13 @@ __device__ Kv4Item kv4_item(const Kv4AttendArgs& a, int index) {
     it.live = false;
     it.head = index % kv;
     const int want = index / kv;
-    int before = 0, pieces_before = 0;
+    int before = 0, pieces_before = 0, slots_before = 0;
     for (int s = 0; s < seqs; s += kWave) {
         if (!once) load(s);
         const int splits = l.blocks <= kKv4Whole ? 1 : (l.blocks + piece - 1) / piece;
         const int mine = kTiles ? tiles : tiles * splits;
-        const int upto = wave_scan(mine), pieces = wave_scan(tiles * splits);
+        const int cut = splits > 1 ? tiles * splits : 0;
+        const int upto = wave_scan(mine), pieces = wave_scan(tiles * splits), slots = wave_scan(cut);
         const unsigned long long past = __ballot(before + upto > want);
         if (past) {
             const int who = __ffsll(past) - 1;
@@ -220,12 +222,14 @@ __device__ Kv4Item kv4_item(const Kv4AttendArgs& a, int index) {
             it.tile = kTiles ? at : at / it.splits;
             it.split = kTiles ? 0 : at % it.splits;
             it.first = (first + it.tile * it.splits) * kv + it.head;
+            it.slot = (slots_before + of_lane(slots - cut, who) + it.tile * it.splits) * kv + it.head;
             it.tile = of_lane(tiles, who) - 1 - it.tile;  // the last rows see the most
             it.live = true;
             return it;
         }
         before += of_lane(upto, kWave - 1);
         pieces_before += of_lane(pieces, kWave - 1);
+        slots_before += of_lane(slots, kWave - 1);
     }
     return it;
 }
@@ -234,7 +238,7 @@ __device__ Kv4Item kv4_item(const Kv4AttendArgs& a, int index) {
 __device__ __forceinline__ bool kv4_piece(const Kv4AttendArgs& a, Kv4Segment& g) {
     const Kv4Item it = kv4_item<false>(a, blockIdx.x);
     if (!it.live) return false;
-    g = Kv4Segment{it.seq, it.head, it.row0, it.n, it.len, it.tile * a.tile_rows, 0, 0, it.splits == 1, (int64_t)blockIdx.x};
+    g = Kv4Segment{it.seq, it.head, it.row0, it.n, it.len, it.tile * a.tile_rows, 0, 0, it.splits == 1, it.slot + (int64_t)it.split * a.cache.kv_heads};
     const int last = min(g.row_a + a.tile_rows, g.n * a.group) - 1;
     int b0, b1;
     kv4_blocks(Kv4Seq{g.row0, g.n, g.len}, a.window, g.row_a / a.group, last / a.group, b0, b1);

@@ -208,6 +208,25 @@ def test_workspace_covers_more_rows_with_more_bytes():
     assert lib.dmoe_kv4_attention_workspace_bytes(by(cache), by(batch), 5) == 0
 
 
+@pytest.mark.parametrize("dim,kv_heads,heads", [(64, 4, 4), (128, 8, 32), (256, 2, 16)])
+def test_workspace_is_bounded(dim, kv_heads, heads):
+    """Room for partial sums of what can be cut: two for each of 256 workgroups' tiles of 128 or 256 rows and 2 (D + 2)
+    fp32 at most, however many rows there are; for few rows no more than the table has blocks."""
+    lib, by = _lib.library(), ctypes.byref
+
+    def need(seqs, rows, most, cols):
+        cache, batch, _, _ = descriptors(dict(page_stride=kv_heads * 16 * (dim + dim // 8), kv_heads=kv_heads, head_dim=dim),
+                                         dict(seqs=seqs, rows=rows, max_rows=most, table_cols=cols, table_stride=cols))
+        return lib.dmoe_kv4_attention_workspace_bytes(by(cache), by(batch), heads)
+
+    tile = (128 if dim == 256 else 256) * (dim + 2) * 4
+    for seqs, rows, most in ((1, 32768, 32768), (1, 131072, 131072), (40, 1 << 20, 100000)):
+        assert 0 < need(seqs, rows, most, most // 16) <= 2 * 256 * tile
+    for cols in (12, 44):  # a wave's share is two blocks of 64 tokens or more; each leaves two partial sums of 16 rows
+        group = heads // kv_heads
+        assert 0 < need(1, 1, 1, cols) <= 2 * kv_heads * -(-cols * 16 // 128) * 16 * (dim + 2) * 4 + kv_heads * 16, group
+
+
 def places_check(tmp_path, header):
     (tmp_path / "kv4_places.hpp").write_text(header)
     exe = tmp_path / "places_check"

@@ -619,6 +619,21 @@ def test_slots_behind_a_window_may_hold_anything(cuda, dim, hq, hkv, page, windo
     assert torch.isfinite(got).all() and torch.equal(got, want) and cache.status() == 0
 
 
+@pytest.mark.parametrize("dim,hq,hkv,window", [(64, 4, 2, 0), (128, 8, 1, 0), (128, 2, 2, 1500), (256, 2, 1, 0)])
+@pytest.mark.parametrize("order", ["long last", "long first", "many between"])
+def test_cut_and_whole_tiles_in_one_batch(cuda, dim, hq, hkv, window, order):
+    """Sequences of many rows: some end in one piece, some are cut, more than 64 of them."""
+    print_case("kv4 mixed cuts", dim, hq, hkv, window, order)
+    short, long = [(9, 9), (1, 70), (0, 12), (40, 41)], [(130, 2600), (3, 3000), (1, 1990)]
+    seqs = {"long last": short + [(140, 150)] + long, "long first": long + short,
+            "many between": long[:1] + short * 17 + long[1:] + short}[order]
+    case = Case(cuda, seqs, hq, hkv, dim, 64, torch.bfloat16, seed=dim + hq + len(seqs), behind=2)
+    case.raw.copy_(torch.randint(0, 256, case.raw.shape, dtype=torch.uint8, generator=case.g))
+    scales = case.raw[:, :, 64 * dim:].view(torch.int16)
+    scales.copy_(scales & 0x03FF | 0x2000)  # 2^-7 to 2^-6 with any zero point
+    check_attend(case, case.random(hq), window=window)
+
+
 # --------------------------------------------------------------- as it is used
 
 def decode_step(cache, batch, qkv, hq, hkv, rotary):
