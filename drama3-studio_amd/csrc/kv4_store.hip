@@ -46,13 +46,25 @@ __device__ __forceinline__ Place place_of(const Kv4Cache& c, const Kv4Batch& b, 
     if (seq >= b.seqs) return none;
     bool bad;
     const Kv4Seq q = kv4_seq(b, c.page_shift, seq, bad);
-    if (bad && status) raise_status(status, kBadBatch);
+    if (bad && status && !b.starts) raise_status(status, kBadBatch);
     const int pos = q.len - q.n + (row - q.row0);
     if (row < q.row0 || row >= q.row0 + q.n || pos < 0) return none;
     const int page = b.table[(int64_t)seq * b.table_stride + (pos >> c.page_shift)];
     const bool off = (unsigned)page >= (unsigned)c.num_pages;
     if (off && status) raise_status(status, kBadBatch);
     return Place{off ? nullptr : c.pages + (int64_t)page * c.page_stride, pos};
+}
+
+// Reports a batch's bad sequences, also those that none of the buffers' rows
+// belongs to: the last wave of one workgroup, beside the wave that finds a
+// row's place.
+__device__ __forceinline__ void report_sequences(const Kv4Cache& c, const Kv4Batch& b, int* status) {
+    if (!b.starts || !status || blockIdx.x || blockIdx.y || wave_index() != (int)blockDim.x / kWave - 1) return;
+    for (int s = threadIdx.x & 63; s < b.seqs; s += kWave) {
+        bool bad;
+        kv4_seq(b, c.page_shift, s, bad);
+        if (bad) raise_status(status, kBadBatch);
+    }
 }
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -204,6 +216,7 @@ __global__ __launch_bounds__(kRows == 1 ? kThreads : 1024) void kv4_append_kerne
         const Place place = place_of(a.cache, a.batch, row0 + i, a.status);
         if ((threadIdx.x & 63) == 0) places[i] = place;
     }
+    report_sequences(a.cache, a.batch, a.status);
     if (!a.rotary.positions) __syncthreads();
     for (int i = threadIdx.x; i < kRows * half; i += (int)blockDim.x) {
         const int row = i / half, f = i - row * half;
@@ -279,6 +292,7 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4ReadArgs a) {
         const Place place = place_of(a.cache, a.batch, row0 + i, a.status);
         if ((threadIdx.x & 63) == 0) places[i] = place;
     }
+    report_sequences(a.cache, a.batch, a.status);
     __syncthreads();
     if (!live) return;
     const int size = 1 << a.cache.page_shift;

@@ -74,7 +74,7 @@ class PagedBatch:
     ``block_table`` [S, pages] int32 names the pages of each sequence's
     tokens (sequences on the same pages may share a row: ``row.expand(S, -1)``), ``lengths`` [S] int32 counts its tokens with the call's rows among
     them, and ``starts`` [S + 1] int32 are the offsets of each sequence's rows
-    in the row buffers (None: row s is sequence s).  With n rows, a
+    in the row buffers, which must not decrease (None: row s is sequence s).  With n rows, a
     sequence's rows are its last n tokens.  ``rows`` is the row count of the
     buffers and ``max_rows`` the most rows a sequence has (default: ``rows``;
     1 without ``starts``).  The three tables stay the caller's: their contents

@@ -510,7 +510,8 @@ typedef struct DmoeKv4Cache {
  * (sizes the launch).  Tables are device memory and may differ at each replay
  * of a captured call; at most 4096 sequences.  Places below 0 (a
  * sequence of fewer tokens than rows) hold no token.  Rows that no sequence
- * owns are neither read nor written.  A sequence whose rows do not lie in
+ * owns are neither read nor written.  starts must not decrease: where it does,
+ * rows may be left out.  A sequence whose rows do not lie in
  * [0, rows], that has more than max_rows rows, or whose tokens do not fit its
  * table_cols pages is skipped, and a token whose page is outside
  * [0, num_pages) is not stored, read as 0, and seen by no row; both raise

@@ -441,6 +441,36 @@ def test_pages_out_of_range_and_odd_batches_are_flagged_and_skipped(cuda, rows):
         assert (out[rows - 1:2 * rows] == 77.0).all() and not (out[2 * rows:] == 77.0).any()
 
 
+@pytest.mark.parametrize("heads,count", [(2, 6), (60, 3000)])
+@pytest.mark.parametrize("what", ["behind the buffers", "back", "too long without rows", "negative without rows"])
+def test_odd_sequences_without_rows_are_flagged(cuda, heads, count, what):
+    """A sequence that is out of range is flagged by every call, also where none of the buffers' rows is its."""
+    print_case("kv4 odd sequences", heads, count, what)
+    case = Case(cuda, [(count, count)], heads, 2, 64, 64, torch.bfloat16, seed=count, fill=0)
+    cache, batch = case.device()
+    q, k, v = (case.random(h).to(cuda) for h in (heads, 2, 2))
+    cache.status()
+    cache.append(k, v, batch)
+    stored, held = cache.pages.clone(), cache.read(batch)
+    assert cache.status() == 0
+    starts, lengths = {"behind the buffers": ([0, count, count, count + 4], [count, 0, 4]),
+                       "back": ([0, count, count, 1], [count, 0, 0]),
+                       "too long without rows": ([0, count, count, count], [count, 0, 2 ** 30]),
+                       "negative without rows": ([0, count, count, count], [count, -1, 0])}[what]
+    table = case.table.to(cuda).expand(3, -1)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    odd = PagedBatch(table, i32(lengths), i32(starts), rows=count)
+    cache.pages.zero_()
+    cache.append(k, v, odd, q=q)
+    assert cache.status() == BAD
+    k_out, v_out = cache.read(odd)
+    assert cache.status() == BAD
+    if what != "back":  # where offsets go back, rows may be left out
+        assert torch.equal(cache.pages, stored) and torch.equal(k_out, held[0]) and torch.equal(v_out, held[1])
+    cache.attend(q, odd)
+    assert cache.status() == BAD
+
+
 @pytest.mark.parametrize("rows", [1, 10, 40])
 def test_offsets_that_go_back(cuda, rows):
     """Every second sequence ends before it starts and is skipped; the others, all alike, own the same rows."""
