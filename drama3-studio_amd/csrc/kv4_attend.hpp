@@ -70,7 +70,9 @@ __device__ __forceinline__ float scale_query(const v4i (&raw)[N], float most, in
     int e = 0;
     if (most > 0.0f && most < __builtin_inff()) (void)frexpf(most, &e);
     e = max(-120, min(120, e));
-    const float down = ldexpf(1.0f, -e);
+    // an infinity or NaN makes all of the row's scores no number: else an infinity whose
+    // scores are all minus infinity would look like a row that sees nothing
+    const float down = most < __builtin_inff() ? ldexpf(1.0f, -e) : __builtin_nanf("");
     const auto fill = [&](auto&& element) {
 #pragma unroll
         for (int j = 0; j < N; ++j)

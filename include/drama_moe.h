@@ -566,7 +566,8 @@ DMOE_API size_t dmoe_kv4_attention_workspace_bytes(const DmoeKv4Cache* cache, co
 
 /* out row = softmax over the tokens its row sees of (scale q . k), times the
  * values.  A row at place p sees tokens 0 .. p, with window > 0 only p -
- * window + 1 .. p; one that sees nothing becomes 0.  q_heads a multiple of
+ * window + 1 .. p; one that sees nothing becomes 0, else one whose query holds
+ * an infinity or NaN becomes NaN.  q_heads a multiple of
  * kv_heads, query head h reads key/value head h / (q_heads / kv_heads).
  * Sums and softmax statistics are fp32; weights are rounded to fp16.  The
  * result of a row depends on the batch it is computed in (the order of its

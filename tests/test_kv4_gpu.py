@@ -376,6 +376,31 @@ def test_odd_queries(cuda, rows):
     assert torch.isfinite(out[:, 3:]).all()
 
 
+@pytest.mark.parametrize("dim,rows,length", [(64, 1, 40), (128, 1, 900), (256, 6, 1300), (64, 40, 300), (128, 40, 2000),
+                                             (256, 20, 900), (128, 150, 200), (64, 300, 2500), (256, 140, 1200)])
+def test_infinite_queries_whose_scores_are_all_negative(cuda, dim, rows, length):
+    """A query with an infinity is no number in its result, also where every score is minus infinity; a row that sees
+    no token is zero all the same."""
+    print_case("kv4 infinite queries", dim, rows, length)
+    case = Case(cuda, [(rows, length), (3, 1)], 4, 2, dim, 64, torch.bfloat16, seed=dim + rows, fill=0)
+    cache, batch = case.device()
+    for s, count in enumerate((length, 1)):
+        k, v = (torch.randn(count, 2, dim, generator=case.g).to(cuda).bfloat16() for _ in range(2))
+        k[:, :, 5] = -2.0
+        cache.append(k, v, PagedBatch(batch.block_table[s:s + 1], batch.lengths[s:s + 1],
+                                      torch.tensor([0, count], dtype=torch.int32, device=cuda), rows=count))
+    q = case.random(4).to(cuda)
+    want = cache.attend(q, batch)
+    odd = [(0, 1), (rows - 1, 3), (rows, 0), (rows + 2, 2)]  # the last two of the second sequence's: its first row sees nothing
+    for row, head in odd:
+        q[row, head, 5] = float("inf")
+    got = cache.attend(q, batch)
+    for row, head in odd:
+        assert (got[row, head] == 0).all() if row == rows else torch.isnan(got[row, head]).all()
+        got[row, head] = want[row, head]
+    assert torch.equal(got, want)
+
+
 def test_scores_far_apart_and_many_equal(cuda):
     """Maxima that come first, last and in the middle; equal scores everywhere."""
     print_case("kv4 score ranges")
