@@ -12,7 +12,8 @@ The reference leaves attention to the model it drives, with a bf16 cache of
 ``sequence_capacity`` tokens (src/drama_low_vram/backbone_graph.py:123-128).
 No call synchronizes the host, every call can be captured in a hipGraph, and
 scratch is allocated for each call by torch, so calls on several streams and
-graphs captured apart share nothing but the cache and the status word.
+graphs captured apart share nothing but the cache and the status word.  There is
+no backward: with gradients enabled, inputs that need them are refused.
 """
 from __future__ import annotations
 
@@ -56,6 +57,15 @@ def _new(shape: tuple, dtype: torch.dtype, device):
     t = torch.empty(shape, dtype=dtype, device=device)
     rows, heads, dim = shape
     return t, _lib.HeadRows(t.data_ptr(), heads * dim if rows > 1 else 0, dim if heads > 1 else 0)
+
+
+def _no_gradients(names: str, *tensors: Tensor | None) -> None:
+    """Refuses inputs whose gradients the kernels, which have no backward, would lose."""
+    if torch.is_grad_enabled():
+        for i, t in enumerate(tensors):
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{names.split()[i]} needs gradients, which attention over the cache does not have: "
+                                 "call it under torch.no_grad()")
 
 
 def _heads(q: Tensor) -> int:
@@ -273,6 +283,7 @@ class KvCache4:
                 int(rotary.interleaved))
         elif positions is not None:
             raise ValueError("positions need a rotary")
+        _no_gradients("k v q q_out", k, v, q, q_out)
         if rows == 0:
             return q_out
         with _on(device):
@@ -292,6 +303,7 @@ class KvCache4:
                                                                                written=True)
         v_out, v_rows = _new(shape, dtype, device) if v_out is None else _rows(v_out, "v_out", shape, dtype, device,
                                                                                written=True)
+        _no_gradients("k_out v_out", k_out, v_out)
         if batch.rows:
             with _on(device):
                 _lib.check(_lib.library().dmoe_kv4_read(
@@ -313,6 +325,7 @@ class KvCache4:
             raise ValueError("query heads must be a multiple of the key/value heads")
         if not -2 ** 31 <= window < 2 ** 31:
             raise ValueError("window must fit 32 bits")
+        _no_gradients("q out", q, out)
         if out is None:
             out, out_rows = _new(shape, q.dtype, device)
         else:

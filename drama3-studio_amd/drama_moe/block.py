@@ -23,7 +23,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .attention import KvCache4, PagedBatch, Rotary
+from .attention import KvCache4, PagedBatch, Rotary, _no_gradients
 from .formats import QuantizedStore, StagedExperts
 
 
@@ -125,7 +125,9 @@ class AttentionBlock:
 
     ``q_proj``, ``k_proj``, ``v_proj`` and ``o_proj`` are modules over rows
     (``GPTQLinear``, ``torch.nn.Linear``); ``q_norm`` and ``k_norm``, if the
-    layer has them, are applied to [rows, heads, D] before the rotation.
+    layer has them, are applied to [rows, heads, D] before the rotation.  It has
+    no backward: with gradients enabled, inputs or projections that need them are
+    refused.
     ``cache`` is the layer's ``KvCache4``; ``rotary``, ``scale`` and
     ``window`` are those of its ``append`` and ``attend``.
     """
@@ -153,6 +155,7 @@ class AttentionBlock:
         is zero."""
         if attn_input.ndim != 2 or attn_input.shape != residual.shape or attn_input.shape[0] != batch.rows:
             raise ValueError(f"attn_input and residual must be [{batch.rows}, hidden]")
+        _no_gradients("attn_input", attn_input)
         rows, dim = batch.rows, self.cache.head_dim
         q = self.q_proj(attn_input).reshape(rows, self.heads, dim)
         k = self.k_proj(attn_input).reshape(rows, self.cache.kv_heads, dim)

@@ -297,6 +297,18 @@ def test_attention_block_refusals(change, message):
         AttentionBlock(**projections, cache=cache, **options)
 
 
+def test_attention_block_refuses_inputs_that_need_gradients():
+    cache = KvCache4.allocate(4, 2, 64, page_size=16, device="cpu")
+    block = AttentionBlock(torch.nn.Linear(32, 256), torch.nn.Linear(32, 128), torch.nn.Linear(32, 128),
+                           torch.nn.Linear(256, 32), cache, heads=4)
+    batch = PagedBatch(i32(2, 2), i32(2))
+    x = torch.zeros(2, 32, requires_grad=True)
+    with pytest.raises(ValueError, match="attn_input needs gradients"):
+        block(x, x, batch)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="ROCm GPU"):
+        block(x, x, batch)
+
+
 def test_attention_block_checks_its_rows():
     cache = KvCache4.allocate(4, 2, 64, page_size=16, device="cpu")
     block = AttentionBlock(torch.nn.Linear(32, 256), torch.nn.Linear(32, 128), torch.nn.Linear(32, 128),

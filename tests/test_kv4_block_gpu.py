@@ -144,6 +144,25 @@ def test_layer_in_prompts_then_captured_decode_steps(cuda):
     assert layer.cache.status() == 0
 
 
+def test_projections_that_need_gradients_are_refused(cuda):
+    print_case("kv4 layer gradients")
+    cache = KvCache4.allocate(8, 2, 64, page_size=16, device=cuda)
+    linear = lambda k, n: torch.nn.Linear(k, n, bias=False, device=cuda, dtype=torch.float16)  # noqa: E731
+    block = AttentionBlock(linear(64, 256), linear(64, 128), linear(64, 128), linear(256, 64), cache, heads=4)
+    x = torch.randn(20, 64, device=cuda, dtype=torch.float16)
+    batch = PagedBatch(i32(cuda, 3, 5).reshape(1, 2), i32(cuda, 20), i32(cuda, 0, 20), rows=20)
+    with pytest.raises(ValueError, match="k needs gradients"):
+        block(x, x, batch)
+    assert not cache.pages.any()
+    with torch.no_grad():
+        assert torch.isfinite(block(x, x, batch)).all()
+    for p in (block.q_proj, block.k_proj, block.v_proj):
+        p.requires_grad_(False)
+    out = block(x, x, batch)  # the output projection alone learns, which its own backward serves
+    out.float().sum().backward()
+    assert block.o_proj.weight.grad is not None
+
+
 def test_norms_plain_linears_and_no_rotation(cuda):
     print_case("kv4 layer linears")
     torch.manual_seed(9)

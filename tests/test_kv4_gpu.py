@@ -782,6 +782,29 @@ def test_calls_on_two_streams_at_once(cuda):
         assert torch.equal(a, b)
 
 
+def test_inputs_that_need_gradients_are_refused(cuda):
+    cache = KvCache4.allocate(4, 2, 64, page_size=16, device=cuda)
+    batch = PagedBatch(*(torch.ones(s, dtype=torch.int32, device=cuda) for s in ((2, 2), (2,))))
+    k, grad = (torch.ones(2, 2, 64, dtype=torch.bfloat16, device=cuda).requires_grad_(x) for x in (False, True))
+    pages = cache.pages.clone()
+    calls = [(lambda: cache.append(grad, k, batch), "k needs"), (lambda: cache.append(k, grad, batch), "v needs"),
+             (lambda: cache.append(k, k, batch, q=grad), "q needs"), (lambda: cache.attend(grad, batch), "q needs"),
+             (lambda: cache.append(k, k, batch, q=k, q_out=grad), "q_out needs"),
+             (lambda: cache.attend(k, batch, out=grad), "out needs"),
+             (lambda: cache.read(batch, dtype=torch.bfloat16, k_out=grad), "k_out needs")]
+    for call, message in calls:
+        with pytest.raises(ValueError, match=message + " gradients"):
+            call()
+    assert torch.equal(cache.pages, pages)
+    want = cache.append(k, k, batch, q=k), cache.attend(k, batch)
+    with torch.no_grad():
+        got = cache.append(grad, grad, batch, q=grad), cache.attend(grad, batch)
+    with torch.inference_mode():
+        again = cache.append(grad, grad, batch, q=grad), cache.attend(grad, batch)
+    for a, b, c in zip(want, got, again):
+        assert torch.equal(a, b) and torch.equal(a, c) and not b.requires_grad
+
+
 def test_calls_that_are_refused(cuda):
     cache = KvCache4.allocate(4, 2, 64, page_size=16, device=cuda)
     batch = PagedBatch(*(torch.ones(s, dtype=torch.int32, device=cuda) for s in ((2, 2), (2,))))
