@@ -25,6 +25,7 @@ from .offload import _device_of, device_state
 
 GROUP = 32            # channels a scale word
 MAX_SEQUENCES = 4096
+MAX_ROWS = 1 << 24
 _HALVES = (torch.bfloat16, torch.float16)
 
 
@@ -129,6 +130,8 @@ class PagedBatch:
             max_rows = 1 if max_rows is None else int(max_rows)
             if rows < seqs:
                 raise ValueError("rows must cover every sequence")
+        if rows > MAX_ROWS:  # the descriptor has 32 bits for it
+            raise ValueError(f"row count outside [0, {MAX_ROWS}]")
         if rows and not 1 <= max_rows <= rows:
             raise ValueError("max_rows outside [1, rows]")
         self.block_table, self.lengths, self.starts = block_table, lengths, starts

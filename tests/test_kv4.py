@@ -35,6 +35,9 @@ def i32(*shape):
     (lambda: PagedBatch(i32(2, 3), i32(2), rows=1), "cover every sequence"),
     (lambda: PagedBatch(i32(2, 3), i32(2), i32(3), rows=4, max_rows=5), "max_rows outside"),
     (lambda: PagedBatch(i32(2, 3), i32(2), i32(3), rows=4, max_rows=0), "max_rows outside"),
+    (lambda: PagedBatch(i32(2, 3), i32(2), i32(3), rows=2 ** 24 + 1), "row count"),
+    (lambda: PagedBatch(i32(2, 3), i32(2), i32(3), rows=2 ** 32 + 6, max_rows=6), "row count"),
+    (lambda: PagedBatch(i32(2, 3), i32(2), rows=2 ** 32 + 6), "row count"),
     (lambda: KvCache4(torch.zeros(4, 2, 16 * 72, dtype=torch.uint8), page_size=16, head_dim=80), "head_dim"),
     (lambda: KvCache4(torch.zeros(4, 2, 24 * 72, dtype=torch.uint8), page_size=24, head_dim=64), "power of two"),
     (lambda: KvCache4(torch.zeros(4, 2, 16 * 72 + 1, dtype=torch.uint8), page_size=16, head_dim=64), "pages must be"),
