@@ -26,7 +26,8 @@
 namespace dmoe {
 
 constexpr int kKv4Group = 32;          // channels a scale word
-constexpr int kKv4Whole = 16;          // sequences of up to this many blocks are not cut
+constexpr int kKv4Whole = 16;          // blocks up to which a sequence with tiles of many rows, or a batch whose
+                                       // table has no more for its tiles of 17..64 rows, is not cut
 constexpr int kKv4MaxSeqs = 4096;
 constexpr float kKv4Limit = 32640.0f;  // values beyond are stored as this: 15 s = 2 * 32640 is the largest span in fp16
 

@@ -116,7 +116,7 @@ __device__ __forceinline__ uint32_t key_word(const Keys<D>& keys, int token, int
 // 38 us.  What is lost is the start (lengths, then pages, then codes, each
 // read behind the other) and waits: two waves a SIMD keep the vector unit busy
 // two thirds of the time -- 430 of a block's 700 instructions decode its codes
-// -- and wait for loads 40% of it.  Three waves spill (60 us for the one sequence),
+// -- and wait for loads 37% of it.  Three waves spill (60 us for the one sequence),
 // twice as many shares add to the start (62 us with the join instead of 51).
 template <int D>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void kv4_attend_rows_kernel(Kv4AttendArgs a) {

@@ -3,8 +3,12 @@
 // Codes become fp16 without conversions: a nibble put into the mantissa of
 // 1024 (low) or 64 (high) is 1024 + c or 64 + c, from which 1024 + z or 64 + z
 // is taken exactly; times s it is exact again.  Queries are scaled by a power
-// of two per row into fp16 (exact), P is shifted by 2^8, which keeps weights
-// down to 2^-22 normal, and is rounded to fp16 with the sums in fp32.
+// of two per row into fp16, the row's largest channel to [0.5, 1): channels of
+// 2^-14 of that power (fp16 rows; 2^-17 for bf16, which has fewer digits) keep
+// all their digits, smaller ones become multiples of 2^-24 of it.  So a score
+// is at most 2^-25 of the power times the sum of its |k| off, times the scale.
+// P is shifted by 2^8, which keeps weights down to 2^-22 normal, and is rounded
+// to fp16 with the sums in fp32.
 #pragma once
 
 #include "common.hpp"
@@ -61,7 +65,7 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b, int dtype) {
                           : __builtin_bit_cast(uint32_t, v2h{(_Float16)a, (_Float16)b});
 }
 
-// A query row of which this lane holds N words of eight channels: into fp16
+// A query row of which this lane holds N words of eight channels: to fp16
 // by the power of two that brings the row's largest value `most` to [0.5, 1),
 // channels in the order in which low_pair / high_pair take a code word's.
 // Returns the factor that takes the scores back, times scale_log2.

@@ -379,7 +379,7 @@ struct Rows {
     }
 
     __device__ __forceinline__ void store_part(float top) const {
-        if (wave_a + r >= row_b || it.slot < 0 || it.slot >= a.slots) return;  // see the join
+        if (wave_a + r >= row_b || it.slot < 0 || it.slot >= a.slots) return;  // no place: offsets that go back
         const int c0 = 32 * T::kOut * split + 4 * hi;
         const int64_t at = it.slot * a.tile_rows + 32 * group + r;
         float* o = a.part + at * D + c0;
@@ -552,8 +552,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void kv4_attend_few_kernel(Kv4Atten
 // Bound by the vector unit: a block of 64 tokens takes a wave 32 products of
 // 32 cycles and some 260 vector instructions, 32 of them exponentials, on a
 // unit that two waves share, and keeps LDS busy more than half of the time;
-// the matrix unit works 40% of it.  2048 rows behind 12288 tokens, 16
-// heads over 2 of 128 channels: 284 us, 907 TFLOP/s.  Two waves in turn, one
+// the matrix unit works 44% of it.  2048 rows behind 14336 tokens, 16
+// heads over 2 of 128 channels: 281 us, 917 TFLOP/s.  Two waves in turn, one
 // with its products and one with its vector instructions, took 324 us: a
 // wave alone issues a vector instruction only every fifth cycle.
 template <class T>

@@ -13,7 +13,8 @@
 // without needing more workgroups than there are, shares end with them.
 //
 // Many rows: tiles of different length, each cut into pieces of at most the
-// average work of a workgroup, the longest tiles of a sequence first.
+// average work of a workgroup, the longest tiles of a sequence first.  Only
+// the pieces of cut tiles have a place for a partial sum.
 #pragma once
 
 #include "common.hpp"

@@ -19,9 +19,10 @@ namespace dmoe {
 namespace {
 
 constexpr int kThreads = 256;
-// A workgroup takes eight rows where that leaves this many of them: below, the
-// chip is not full (2300 rows of 20 heads of 256 channels: 21 us one by one,
-// 25 us by eight; 8192 rows of 48 heads of 128: 74 us one by one, 55 by eight).
+// Rows go eight to a workgroup where one by one they would make eight times
+// this many workgroups of 256 threads: with fewer the chip is not full (2300
+// rows of 20 heads of 256 channels: 6900 workgroups, 21 us one by one, 25 us by
+// eight; 8192 rows of 48 heads of 128: 24576, 74 us one by one, 55 by eight).
 constexpr int kFull = 1024;
 
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }

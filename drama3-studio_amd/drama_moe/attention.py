@@ -91,6 +91,8 @@ class PagedBatch:
     1 without ``starts``).  The three tables stay the caller's: their contents
     may change between calls and between replays of a captured call.  Rows
     that no sequence owns -- behind the last one -- are left as they are.
+    ``max_rows`` picks the attention kernel for all sequences: a prompt and
+    single tokens are better attended as two batches.
     """
 
     __slots__ = ("block_table", "lengths", "starts", "rows", "max_rows", "desc", "device", "scratch")

@@ -559,9 +559,10 @@ DMOE_API int dmoe_kv4_append(const DmoeKv4Cache* cache, const DmoeKv4Batch* batc
 DMOE_API int dmoe_kv4_read(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, const DmoeHeadRows* k_out,
                            const DmoeHeadRows* v_out, int dtype, int* status, void* stream);
 
-/* Scratch bytes of dmoe_kv4_attention for this batch's seqs, rows and max_rows
- * (0 if they are out of range).  It needs no clearing and holds nothing
- * between calls; calls that overlap need one each. */
+/* Scratch bytes of dmoe_kv4_attention for this batch's seqs, rows, max_rows and
+ * table_cols, the cache's page_size, kv_heads and head_dim, and q_heads (0 if
+ * they are out of range); a call with a wider table may need more.  It needs no
+ * clearing and holds nothing between calls; calls that overlap need one each. */
 DMOE_API size_t dmoe_kv4_attention_workspace_bytes(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, int q_heads);
 
 /* out row = softmax over the tokens its row sees of (scale q . k), times the
@@ -571,7 +572,12 @@ DMOE_API size_t dmoe_kv4_attention_workspace_bytes(const DmoeKv4Cache* cache, co
  * kv_heads, query head h reads key/value head h / (q_heads / kv_heads).
  * Sums and softmax statistics are fp32; weights are rounded to fp16.  The
  * result of a row depends on the batch it is computed in (the order of its
- * partial sums), not on the run. */
+ * partial sums; with 17 to 64 packed rows -- a token's heads of one key/value
+ * head -- also on the table's width), not on the run.  Queries are held in
+ * fp16 times a power of two per row: a channel below 2^-14 of its row's largest
+ * is rounded to 2^-24 of the power of two above that.  max_rows picks the
+ * kernel for the whole batch: one sequence of many rows takes those of one row
+ * along into tiles of 128 or 256, so such batches are better called in two. */
 DMOE_API int dmoe_kv4_attention(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, const DmoeHeadRows* q,
                                 int q_heads, float scale, int window, const DmoeHeadRows* out, int dtype,
                                 void* workspace, size_t workspace_bytes, int* status, void* stream);
