@@ -145,6 +145,11 @@ struct Kv4Shares {
         const int kv = a.cache.kv_heads;
         unsigned long long past;
         while (!(past = __ballot((int64_t)upto * kv > x))) {
+            // lengths written over while the kernel runs can leave less than was counted: the wave ends all the same
+            if (s0 + kWave >= a.batch.seqs) {
+                x = x_end;
+                return false;
+            }
             const int before = of_lane(upto, kWave - 1);
             s0 += kWave;
             lane = kv4_lane(a, s0 + (int)(threadIdx.x & 63));

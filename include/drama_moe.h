@@ -508,7 +508,7 @@ typedef struct DmoeKv4Cache {
  * table_stride is at least table_cols, or 0 where all sequences share one row.
  * `rows` is the row count of the buffers, max_rows the most rows of a sequence
  * (sizes the launch).  Tables are device memory and may differ at each replay
- * of a captured call; at most 4096 sequences.  Places below 0 (a
+ * of a captured call, but not while a call runs; at most 4096 sequences.  Places below 0 (a
  * sequence of fewer tokens than rows) hold no token.  Rows that no sequence
  * owns are neither read nor written.  starts must not decrease: where it does,
  * rows may be left out.  A sequence whose rows do not lie in
