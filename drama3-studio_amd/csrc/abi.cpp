@@ -15,6 +15,7 @@
 #include <stdexcept>
 #include <string>
 
+#include "int8.hpp"
 #include "kernels.hpp"
 #include "kv4.hpp"
 #include "layout.hpp"
@@ -1733,6 +1734,310 @@ int dmoe_kv4_attention(const DmoeKv4Cache* cache, const DmoeKv4Batch* batch, con
         a.part_ml = a.part + s.part_bytes / sizeof(float);
         a.records = s.record_bytes ? reinterpret_cast<dmoe::Kv4Record*>(a.part_ml + s.ml_bytes / sizeof(float)) : nullptr;
         dmoe::launch_kv4_attend(a, s, as_stream(stream));
+    });
+}
+
+}  // extern "C"
+
+// ------------------------------------------------ rows and products in 8 bits
+namespace {
+
+constexpr int64_t kMaxRowStride = (int64_t)1 << 38;  // products with a row count stay in 64 bits
+
+int elem_size(int dtype) { return dtype == DMOE_F32 ? 4 : 2; }
+
+void check_rows8_size(int rows, int cols) {
+    require(rows >= 0 && rows <= dmoe::kRows8MaxRows, "row count outside [0, 2^24]");
+    require(cols >= 1 && cols <= dmoe::kInt8MaxK, "column count outside [1, 65536]");
+}
+
+dmoe::Rows to_kernel(const DmoeRows* r, int rows, int64_t cols, const char* what) {
+    const auto need = [&](bool ok, const char* why) {
+        if (!ok) throw AbiError(std::string(what) + why);
+    };
+    need(r != nullptr && r->data != nullptr, " rows are required");
+    need(is_float_dtype(r->dtype), " must be fp32, bf16 or fp16");
+    need(reinterpret_cast<uintptr_t>(r->data) % elem_size(r->dtype) == 0, " must be aligned to its elements");
+    need(r->row_stride < kMaxRowStride && (rows <= 1 || r->row_stride >= cols), " has a row stride out of range");
+    dmoe::Rows k;
+    k.p = r->data;
+    k.stride = rows > 1 ? r->row_stride : 0;
+    k.dtype = r->dtype;
+    return k;
+}
+
+// Rows that are only read may all be one row (stride 0).
+dmoe::Rows read_rows(const DmoeRows* r, int rows, int64_t cols, const char* what) {
+    DmoeRows one = r ? *r : DmoeRows{};
+    if (r && r->row_stride == 0) one.row_stride = cols;
+    dmoe::Rows k = to_kernel(r ? &one : nullptr, rows, cols, what);
+    if (r->row_stride == 0) k.stride = 0;
+    return k;
+}
+
+dmoe::Rows8 to_kernel(const DmoeQuantRows* q, int rows, int cols) {
+    require(q != nullptr && q->values != nullptr && q->scales != nullptr, "rows in 8 bits and their scales are required");
+    require(q->format >= DMOE_ROWS_INT8 && q->format <= DMOE_ROWS_E4M3_GROUP, "unknown format of rows in 8 bits");
+    require(q->format != DMOE_ROWS_E4M3_GROUP || cols % 128 == 0, "groups of 128 need a multiple of 128 columns");
+    require(reinterpret_cast<uintptr_t>(q->values) % 16 == 0 && reinterpret_cast<uintptr_t>(q->scales) % 4 == 0,
+            "rows in 8 bits must be 16-byte aligned");
+    // the last row too is as long as the columns rounded up
+    require(q->row_stride % 16 == 0 && q->row_stride >= dmoe::padded_k(cols) && q->row_stride < ((int64_t)1 << 23),
+            "rows in 8 bits need a row stride of whole 16 bytes, at least the columns rounded up to 128, below 2^23");
+    dmoe::Rows8 k;
+    k.q = static_cast<uint8_t*>(q->values);
+    k.stride = q->row_stride;
+    k.scales = q->scales;
+    k.format = q->format;
+    (void)rows;
+    return k;
+}
+
+void check_weight(const DmoeInt8Weight* w) {
+    require(w != nullptr && w->values != nullptr && w->scales != nullptr, "INT8 weight values and scales are required");
+    require(w->n >= 1 && w->n <= (1 << 24), "INT8 weight rows outside [1, 2^24]");
+    require(w->k >= 1 && w->k <= dmoe::kInt8MaxK, "INT8 weight columns outside [1, 65536]");
+    require(reinterpret_cast<uintptr_t>(w->values) % 16 == 0 && reinterpret_cast<uintptr_t>(w->scales) % 4 == 0 &&
+                w->row_stride % 16 == 0 && w->row_stride >= w->k && w->row_stride < ((int64_t)1 << 23),
+            "INT8 weight rows must be 16-byte aligned, with a row stride below 2^23");
+}
+
+dmoe::Int8Args int8_args(const DmoeInt8Weight& w, int rows, bool gated, int* status) {
+    dmoe::Int8Args a{};
+    a.rows = rows;
+    a.k = w.k;
+    a.w = w.values;
+    a.w_stride = w.row_stride;
+    a.ws = w.scales;
+    a.n = gated ? w.n / 2 : w.n;
+    a.gated = gated;
+    a.status = status;
+    return a;
+}
+
+void set_rows(dmoe::Int8Args& a, const dmoe::Rows& x) {
+    a.x = x.p;
+    a.x_stride = x.stride;
+    a.x_dtype = x.dtype;
+}
+void set_rows(dmoe::Int8Args& a, const dmoe::Rows8& q) {
+    a.xq = q.q;
+    a.xq_stride = q.stride;
+    a.xs = q.scales;
+}
+
+size_t rows8_bytes(int rows, int k) { return ((size_t)rows * dmoe::padded_k(k) + (size_t)rows * 4 + 255) / 256 * 256; }
+
+dmoe::Rows8 rows8_at(void* base, int rows, int k) {
+    dmoe::Rows8 q;
+    q.q = static_cast<uint8_t*>(base);
+    q.stride = dmoe::padded_k(k);
+    q.scales = reinterpret_cast<float*>(q.q + (size_t)rows * q.stride);
+    q.format = dmoe::kRowsInt8;
+    return q;
+}
+
+void quantize_into(const dmoe::Rows& x, int rows, int cols, const dmoe::Rows8& q, int* status, hipStream_t stream) {
+    dmoe::NormArgs n{};
+    n.x = x.p;
+    n.x_stride = x.stride;
+    n.dtype = x.dtype;
+    n.rows = rows;
+    n.cols = cols;
+    n.q = q;
+    n.status = status;
+    dmoe::launch_rows8(n, stream);
+}
+
+void product(const dmoe::Int8Args& a, hipStream_t stream) {
+    if (a.rows <= dmoe::kInt8FewRows) dmoe::launch_int8_few(a, stream);
+    else dmoe::launch_int8_tiles(a, device_cus(), stream);
+}
+
+// The rows of a product: as they are, or quantized at `place` where its kernel does not do that itself.
+void set_input(dmoe::Int8Args& a, const dmoe::Rows& x, void* place, int* status, hipStream_t stream) {
+    if (dmoe::int8_few_quantizes(a.rows, a.k)) {
+        set_rows(a, x);
+        return;
+    }
+    const dmoe::Rows8 q = rows8_at(place, a.rows, a.k);
+    quantize_into(x, a.rows, a.k, q, status, stream);
+    set_rows(a, q);
+}
+
+size_t input_bytes(int rows, int k) { return dmoe::int8_few_quantizes(rows, k) ? 0 : rows8_bytes(rows, k); }
+
+void check_workspace(const void* workspace, size_t have, size_t need) {
+    require(need == 0 || (workspace != nullptr && have >= need), "workspace too small");
+    require(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
+}
+
+bool sizes_fit(int rows, int k) { return rows >= 1 && rows <= dmoe::kRows8MaxRows && k >= 1 && k <= dmoe::kInt8MaxK; }
+
+}  // namespace
+
+extern "C" {
+
+int dmoe_rms_norm(const DmoeRows* x, const DmoeRows* residual, int rows, int cols, const void* weight, int weight_dtype,
+                  float offset, double eps, const DmoeRows* hidden, const DmoeRows* out, const DmoeQuantRows* quantized,
+                  int* status, void* stream) {
+    return checked([&] {
+        check_rows8_size(rows, cols);
+        require(weight != nullptr && is_float_dtype(weight_dtype), "norm weight must be fp32, bf16 or fp16");
+        require(reinterpret_cast<uintptr_t>(weight) % elem_size(weight_dtype) == 0, "norm weight must be aligned to its elements");
+        require(std::isfinite(offset) && std::isfinite(eps) && eps >= 0.0, "offset and eps must be finite, eps not negative");
+        require(out != nullptr || quantized != nullptr, "the norm has no output");
+        require(hidden == nullptr || residual != nullptr, "hidden rows need a residual");
+        dmoe::NormArgs a{};
+        const dmoe::Rows in = read_rows(x, rows, cols, "x");
+        a.x = in.p;
+        a.x_stride = in.stride;
+        a.dtype = in.dtype;
+        a.rows = rows;
+        a.cols = cols;
+        a.weight = weight;
+        a.weight_dtype = weight_dtype;
+        a.offset = offset;
+        a.eps = eps;
+        a.status = status;
+        if (residual) {
+            const dmoe::Rows r = read_rows(residual, rows, cols, "residual");
+            require(r.dtype == in.dtype, "residual must have the type of x");
+            a.residual = r.p;
+            a.residual_stride = r.stride;
+        }
+        if (hidden) {
+            const dmoe::Rows h = to_kernel(hidden, rows, cols, "hidden");
+            require(h.dtype == in.dtype, "hidden must have the type of x");
+            a.hidden = h.p;
+            a.hidden_stride = h.stride;
+        }
+        if (out) {
+            const dmoe::Rows y = to_kernel(out, rows, cols, "out");
+            require(y.dtype == in.dtype, "out must have the type of x");
+            a.y = y.p;
+            a.y_stride = y.stride;
+        }
+        if (quantized) a.q = to_kernel(quantized, rows, cols);
+        if (rows) dmoe::launch_rows8(a, as_stream(stream));
+    });
+}
+
+int dmoe_int8_quantize(const DmoeRows* x, int rows, int cols, const DmoeQuantRows* quantized, int* status, void* stream) {
+    return checked([&] {
+        check_rows8_size(rows, cols);
+        const dmoe::Rows in = read_rows(x, rows, cols, "x");
+        const dmoe::Rows8 q = to_kernel(quantized, rows, cols);
+        require(q.format == DMOE_ROWS_INT8, "rows are quantized to 8-bit integers");
+        if (rows) quantize_into(in, rows, cols, q, status, as_stream(stream));
+    });
+}
+
+int dmoe_rows8_read(const DmoeQuantRows* quantized, int rows, int cols, const DmoeRows* out, void* stream) {
+    return checked([&] {
+        check_rows8_size(rows, cols);
+        dmoe::Dequant8Args a{};
+        a.q = to_kernel(quantized, rows, cols);
+        const dmoe::Rows o = to_kernel(out, rows, cols, "out");
+        a.rows = rows;
+        a.cols = cols;
+        a.out = o.p;
+        a.out_stride = o.stride;
+        a.dtype = o.dtype;
+        if (rows) dmoe::launch_dequant8(a, as_stream(stream));
+    });
+}
+
+size_t dmoe_int8_linear_workspace_bytes(int rows, int k) { return sizes_fit(rows, k) ? input_bytes(rows, k) : 0; }
+
+int dmoe_int8_linear(const DmoeRows* x, const DmoeQuantRows* quantized, int rows, const DmoeInt8Weight* weight,
+                     const float* bias, const DmoeRows* residual, const DmoeRows* out, void* workspace,
+                     size_t workspace_bytes, int* status, void* stream) {
+    return checked([&] {
+        check_weight(weight);
+        check_rows8_size(rows, weight->k);
+        require((x != nullptr) != (quantized != nullptr), "rows come either quantized or not");
+        dmoe::Int8Args a = int8_args(*weight, rows, false, status);
+        const dmoe::Rows o = to_kernel(out, rows, a.n, "out");
+        a.out = o.p;
+        a.out_stride = o.stride;
+        a.out_dtype = o.dtype;
+        require(bias == nullptr || reinterpret_cast<uintptr_t>(bias) % 4 == 0, "bias must be aligned fp32");
+        a.bias = bias;
+        if (residual) {
+            const dmoe::Rows r = read_rows(residual, rows, a.n, "residual");
+            require(r.dtype == o.dtype, "residual must have the type of out");
+            a.residual = r.p;
+            a.residual_stride = r.stride;
+        }
+        if (quantized) {
+            const dmoe::Rows8 q = to_kernel(quantized, rows, a.k);
+            require(q.format == DMOE_ROWS_INT8, "products take rows of 8-bit integers");
+            if (!rows) return;
+            set_rows(a, q);
+        } else {
+            const dmoe::Rows in = read_rows(x, rows, a.k, "x");
+            if (!rows) return;
+            check_workspace(workspace, workspace_bytes, input_bytes(rows, a.k));
+            set_input(a, in, workspace, status, as_stream(stream));
+        }
+        product(a, as_stream(stream));
+    });
+}
+
+size_t dmoe_int8_feed_forward_workspace_bytes(int rows, int k, int inter, int out_dtype) {
+    if (!sizes_fit(rows, k) || !sizes_fit(rows, inter) || !is_float_dtype(out_dtype)) return 0;
+    const size_t hidden = ((size_t)rows * inter * elem_size(out_dtype) + 255) / 256 * 256;
+    return hidden + std::max(input_bytes(rows, k), input_bytes(rows, inter));
+}
+
+int dmoe_int8_feed_forward(const DmoeRows* x, const DmoeQuantRows* quantized, int rows, const DmoeInt8Weight* gate_up,
+                           const DmoeInt8Weight* down, int activation, const DmoeRows* residual, const DmoeRows* out,
+                           void* workspace, size_t workspace_bytes, int* status, void* stream) {
+    return checked([&] {
+        check_weight(gate_up);
+        check_weight(down);
+        check_rows8_size(rows, gate_up->k);
+        require(gate_up->n % 2 == 0 && gate_up->n / 2 == down->k, "gate_up must be [2 * inter, k] for down [n, inter]");
+        require((int64_t)gate_up->n * gate_up->row_stride < (int64_t)1 << 31, "gate_up must be smaller than 2 GiB");
+        require(activation == DMOE_ACT_SILU || activation == DMOE_ACT_GELU_TANH, "unknown activation");
+        require((x != nullptr) != (quantized != nullptr), "rows come either quantized or not");
+        dmoe::Int8Args up = int8_args(*gate_up, rows, true, status), back = int8_args(*down, rows, false, status);
+        up.gelu = activation == DMOE_ACT_GELU_TANH;
+        const dmoe::Rows o = to_kernel(out, rows, back.n, "out");
+        back.out = o.p;
+        back.out_stride = o.stride;
+        back.out_dtype = o.dtype;
+        if (residual) {
+            const dmoe::Rows r = read_rows(residual, rows, back.n, "residual");
+            require(r.dtype == o.dtype, "residual must have the type of out");
+            back.residual = r.p;
+            back.residual_stride = r.stride;
+        }
+        dmoe::Rows in;
+        dmoe::Rows8 in8;
+        if (quantized) {
+            in8 = to_kernel(quantized, rows, up.k);
+            require(in8.format == DMOE_ROWS_INT8, "products take rows of 8-bit integers");
+        } else {
+            in = read_rows(x, rows, up.k, "x");
+        }
+        if (!rows) return;
+        check_workspace(workspace, workspace_bytes, dmoe_int8_feed_forward_workspace_bytes(rows, up.k, up.n, o.dtype));
+        // the hidden rows, then a place for the rows in 8 bits: the input's until the first product has read them
+        dmoe::Rows hidden;
+        hidden.p = workspace;
+        hidden.stride = up.n;
+        hidden.dtype = o.dtype;
+        void* place = static_cast<char*>(workspace) + ((size_t)rows * up.n * elem_size(o.dtype) + 255) / 256 * 256;
+        if (quantized) set_rows(up, in8);
+        else set_input(up, in, place, status, as_stream(stream));
+        up.out = hidden.p;
+        up.out_stride = hidden.stride;
+        up.out_dtype = hidden.dtype;
+        product(up, as_stream(stream));
+        set_input(back, hidden, place, status, as_stream(stream));
+        product(back, as_stream(stream));
     });
 }
 

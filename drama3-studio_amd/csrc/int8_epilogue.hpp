@@ -1,0 +1,22 @@
+// What the products of 8-bit integers make of an int32 sum.
+#pragma once
+
+#include "common.hpp"
+
+namespace dmoe {
+
+// A sum in units of its matrix row's scale and its activation row's: the
+// small one of the two first, so that neither product leaves fp32's range
+// where the result does not.
+__device__ __forceinline__ float int8_value(int sum, float channel, float row) { return (float)sum * channel * row; }
+
+// act(z): z / (1 + exp(-z)), or gelu in its tanh form, which is
+// z / (1 + exp(-2 sqrt(2 / pi) (z + 0.044715 z^3))).
+__device__ __forceinline__ float int8_gate(float z, int gelu) {
+    constexpr float kGelu = 1.5957691216057308f;
+    const float y = gelu ? kGelu * (z + 0.044715f * z * z * z) : z;
+    // exp(-y) beyond fp32's range: z / inf is the right 0
+    return __fdividef(z, 1.0f + __expf(-y));
+}
+
+}  // namespace dmoe

@@ -1,0 +1,208 @@
+// Rows of the residual stream between two blocks of a decoder layer, in one
+// pass: the residual's addition, the root-mean-square norm, and the next
+// block's input in 8 bits with scales; the row quantizer alone; and what rows
+// in 8 bits stand for.
+//
+//   h = T(x + residual);  g = fl32(offset + weight);  u = fl32(h g)
+//   y = u r,  r = 1 / sqrt(sum(h^2) / cols + eps)
+//   integers: s = fl32(max(fl32(max|u| r), 1e-12) fl32(1/127)), codes round(u r / s)
+//   E4M3:     s = fl32(max(fl32(max|u| r), 1e-10) fl32(1/448)), codes the numbers nearest u r / s
+//
+// r > 0 is the same for a row, so the row's largest |y| comes from its largest
+// |u|: one reduction carries the sum and the maximum, and the row's values
+// stay in registers between the two halves.  The sum and r are of 64 bits, so
+// that scales and codes are those of the formula and do not depend on how a
+// row was cut; the codes are decided in 32 bits except next to a border.
+#include <algorithm>
+
+#include "rows8_util.hpp"
+
+namespace dmoe {
+
+namespace {
+
+// T threads hold a row, V vectors of eight columns each; several rows a
+// workgroup where a wave holds one.
+template <int DT, int T, int V, bool NORM>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
+    constexpr int kRowsPer = T < 256 ? 256 / T : 1;
+    constexpr int kWaves = T / kWave;
+    constexpr int kBytes = elem_bytes<DT>();
+    const int t = threadIdx.x % T;
+    const int64_t row = (int64_t)blockIdx.x * kRowsPer + threadIdx.x / T;
+    if (row >= a.rows) return;  // whole waves; a row of several waves is a whole workgroup
+    const char* x = (const char*)a.x + row * a.x_stride * kBytes;
+    float u[V][8];
+    int top = 0;
+    int group_top[V];
+    double sum = 0.0;
+    float res[V][8];
+#pragma unroll
+    for (int v = 0; v < V; ++v) load_cols8<DT>(x, (v * T + t) * 8, a.cols, u[v]);
+    if (NORM && a.residual) {
+        const char* r = (const char*)a.residual + row * a.residual_stride * kBytes;
+#pragma unroll
+        for (int v = 0; v < V; ++v) load_cols8<DT>(r, (v * T + t) * 8, a.cols, res[v]);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[v][j] = round_through(u[v][j] + res[v][j], DT);
+        if (a.hidden) {
+            char* h = (char*)a.hidden + row * a.hidden_stride * kBytes;
+#pragma unroll
+            for (int v = 0; v < V; ++v) store_cols8<DT>(h, (v * T + t) * 8, a.cols, u[v]);
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if constexpr (NORM) {
+            float g[8];
+            const int col = (v * T + t) * 8;
+            if (a.weight_dtype == kBF16) load_cols8<kBF16>(a.weight, col, a.cols, g);
+            else if (a.weight_dtype == kF16) load_cols8<kF16>(a.weight, col, a.cols, g);
+            else load_cols8<kF32>(a.weight, col, a.cols, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // squares of 16-bit types are exact in 32 bits
+                sum += DT == kF32 ? (double)u[v][j] * (double)u[v][j] : (double)(u[v][j] * u[v][j]);
+                u[v][j] *= a.offset + g[j];
+            }
+        }
+        int m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, magnitude(u[v][j]));
+        group_top[v] = m;
+        top = max(top, m);
+    }
+    top = wave_max_bits(top);
+    if constexpr (NORM) {
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
+    }
+    if constexpr (kWaves > 1) {
+        __shared__ double sums[kWaves];
+        __shared__ int tops[kWaves];
+        const int wave = t / kWave;
+        if (t % kWave == 0) {
+            if (NORM) sums[wave] = sum;
+            tops[wave] = top;
+        }
+        __syncthreads();
+        sum = NORM ? sums[0] : 0.0;
+        top = tops[0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            if (NORM) sum += sums[w];
+            top = max(top, tops[w]);
+        }
+    }
+    const double by = NORM ? 1.0 / sqrt(sum / a.cols + a.eps) : 1.0;
+    if (NORM && a.y) {
+        char* y = (char*)a.y + row * a.y_stride * kBytes;
+        const float r = (float)by;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float o[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = u[v][j] * r;
+            store_cols8<DT>(y, (v * T + t) * 8, a.cols, o);
+        }
+    }
+    if (a.q.format == kRowsNone) return;
+    uint8_t* q = a.q.q + row * a.q.stride;
+    if (a.q.format == kRowsE4M3Group) {  // cols % 128 == 0: sixteen lanes hold a group
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int col = (v * T + t) * 8;
+            const float top32 = (float)((double)__int_as_float(row_max_bits(group_top[v])) * by);
+            const bool fine = finite_bits(top32);
+            const float scale = e4m3_scale(top32);
+            if (col >= a.cols) continue;
+            *(uint64_t*)(q + col) = fine ? e4m3_codes8(u[v], (float)(by / (double)scale), by, scale) : 0;
+            if (t % 16 == 0) {
+                a.q.scales[row * (a.cols / 128) + col / 128] = fine ? scale : __builtin_nanf("");
+                if (!fine) raise_status(a.status, kNonFinite);
+            }
+        }
+        return;
+    }
+    const float top32 = (float)((double)__int_as_float(top) * by);
+    const bool fine = finite_bits(top32), e4m3 = a.q.format == kRowsE4M3;
+    const float scale = e4m3 ? e4m3_scale(top32) : int8_scale(top32);
+    const float each = (float)(by / (double)scale);
+    const int end = padded_k(a.cols);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int col = (v * T + t) * 8;  // columns from cols on are zeros
+        if (col < end)
+            *(uint64_t*)(q + col) = !fine ? 0 : e4m3 ? e4m3_codes8(u[v], each, by, scale) : int8_codes8(u[v], each, by, scale);
+    }
+    if (t == 0) {
+        a.q.scales[row] = fine ? scale : __builtin_nanf("");
+        if (!fine) raise_status(a.status, kNonFinite);
+    }
+}
+
+template <int DT, int T, int V>
+void launch_rows8_as(const NormArgs& a, hipStream_t stream) {
+    const int per = T < 256 ? 256 / T : 1;
+    const dim3 grid((unsigned)((a.rows + per - 1) / per)), block(T < 256 ? 256 : T);
+    if (a.weight) hipLaunchKernelGGL((rows8_kernel<DT, T, V, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((rows8_kernel<DT, T, V, false>), grid, block, 0, stream, a);
+}
+
+template <int DT>
+void launch_rows8_of(const NormArgs& a, hipStream_t stream) {
+    const int end = padded_k(a.cols);
+    if (end <= 512) launch_rows8_as<DT, 64, 1>(a, stream);
+    else if (end <= 1024) launch_rows8_as<DT, 64, 2>(a, stream);
+    else if (end <= 2048) launch_rows8_as<DT, 256, 1>(a, stream);
+    else if (end <= 4096) launch_rows8_as<DT, 256, 2>(a, stream);
+    else if (end <= 8192) launch_rows8_as<DT, 256, 4>(a, stream);
+    else if (end <= 16384) launch_rows8_as<DT, 1024, 2>(a, stream);
+    else if (end <= 32768) launch_rows8_as<DT, 1024, 4>(a, stream);
+    else launch_rows8_as<DT, 1024, 8>(a, stream);
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void dequant8_kernel(Dequant8Args a, int per_row, int64_t total) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int64_t row = i / per_row;
+    const int col = (int)(i - row * per_row) * 8;
+    const uint8_t* q = a.q.q + row * a.q.stride + col;
+    const float scale = a.q.scales[a.q.format == kRowsE4M3Group ? row * (a.cols / 128) + col / 128 : row];
+    float v[8];
+    const uint64_t w = *(const uint64_t*)q;  // rows are readable to a multiple of sixteen columns
+    if (a.q.format == kRowsInt8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)(int8_t)(w >> (8 * j)) * scale;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const v2f two = fp8x2_to_f32((uint32_t)(j < 2 ? w : w >> 32), j % 2 != 0);
+            v[2 * j] = two[0] * scale;
+            v[2 * j + 1] = two[1] * scale;
+        }
+    }
+    store_cols8<DT>((char*)a.out + row * a.out_stride * elem_bytes<DT>(), col, a.cols, v);
+}
+
+}  // namespace
+
+void launch_rows8(const NormArgs& a, hipStream_t stream) {
+    if (a.dtype == kBF16) launch_rows8_of<kBF16>(a, stream);
+    else if (a.dtype == kF16) launch_rows8_of<kF16>(a, stream);
+    else launch_rows8_of<kF32>(a, stream);
+}
+
+void launch_dequant8(const Dequant8Args& a, hipStream_t stream) {
+    const int per_row = (a.cols + 7) / 8;
+    const int64_t total = (int64_t)a.rows * per_row;
+    const dim3 grid((unsigned)((total + 255) / 256)), block(256);
+    if (a.dtype == kBF16) hipLaunchKernelGGL(dequant8_kernel<kBF16>, grid, block, 0, stream, a, per_row, total);
+    else if (a.dtype == kF16) hipLaunchKernelGGL(dequant8_kernel<kF16>, grid, block, 0, stream, a, per_row, total);
+    else hipLaunchKernelGGL(dequant8_kernel<kF32>, grid, block, 0, stream, a, per_row, total);
+}
+
+}  // namespace dmoe

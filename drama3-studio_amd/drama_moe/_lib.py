@@ -63,6 +63,20 @@ class RotaryDesc(ctypes.Structure):
                 ("dim", ctypes.c_int32), ("interleaved", ctypes.c_int32)]
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class QuantRowsDesc(ctypes.Structure):
+    _fields_ = [("values", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("scales", ctypes.c_void_p),
+                ("format", ctypes.c_int32)]
+
+
+class Int8WeightDesc(ctypes.Structure):
+    _fields_ = [("values", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("scales", ctypes.c_void_p),
+                ("n", ctypes.c_int32), ("k", ctypes.c_int32)]
+
+
 class HeadRows(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
@@ -70,6 +84,7 @@ class HeadRows(ctypes.Structure):
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
+_ROWS, _QROWS, _INT8 = ctypes.POINTER(Rows), ctypes.POINTER(QuantRowsDesc), ctypes.POINTER(Int8WeightDesc)
 _CACHE, _BATCH, _HEADS = ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Batch), ctypes.POINTER(HeadRows)
 
 _SIGNATURES = {
@@ -116,6 +131,13 @@ _SIGNATURES = {
     "dmoe_kv4_read": ([_CACHE, _BATCH, _HEADS, _HEADS, _I, _P, _P], _I),
     "dmoe_kv4_attention_workspace_bytes": ([_CACHE, _BATCH, _I], ctypes.c_size_t),
     "dmoe_kv4_attention": ([_CACHE, _BATCH, _HEADS, _I, ctypes.c_float, _I, _HEADS, _I, _P, ctypes.c_size_t, _P, _P], _I),
+    "dmoe_rms_norm": ([_ROWS, _ROWS, _I, _I, _P, _I, ctypes.c_float, ctypes.c_double, _ROWS, _ROWS, _QROWS, _P, _P], _I),
+    "dmoe_int8_quantize": ([_ROWS, _I, _I, _QROWS, _P, _P], _I),
+    "dmoe_rows8_read": ([_QROWS, _I, _I, _ROWS, _P], _I),
+    "dmoe_int8_linear_workspace_bytes": ([_I, _I], ctypes.c_size_t),
+    "dmoe_int8_linear": ([_ROWS, _QROWS, _I, _INT8, _P, _ROWS, _ROWS, _P, ctypes.c_size_t, _P, _P], _I),
+    "dmoe_int8_feed_forward_workspace_bytes": ([_I, _I, _I, _I], ctypes.c_size_t),
+    "dmoe_int8_feed_forward": ([_ROWS, _QROWS, _I, _INT8, _INT8, _I, _ROWS, _ROWS, _P, ctypes.c_size_t, _P, _P], _I),
     "dmoe_fp8_quantized_pairs": ([ctypes.POINTER(Fp8Bank), _P, _P, _L, _L, _I, _I, _I, _P, _I, _P,
                                   _I, _I, _I, _P, _P, ctypes.c_size_t, _P, _P], _I),
     "dmoe_combine_slots": ([_P, _L, _P, _I, _I, _I, _I, _I, _P, _I, _L, _P], _I),

@@ -664,6 +664,91 @@ DMOE_API int dmoe_silu_table(float* table, void* stream);
  * fixed unlikely value. */
 DMOE_API int dmoe_stream_read(const void* data, int64_t bytes, uint32_t* sink, void* stream);
 
+/* ------------------------------------------------ rows and products in 8 bits
+ *
+ * What a decoder layer does between its blocks and in its dense ones, on 8-bit
+ * integers: the norm with the residual's addition and the next block's input in
+ * 8 bits, the row quantizer, the product with a matrix of 8-bit integers, the
+ * gated feed-forward block on two of them.  No counterpart in the reference,
+ * whose norms, dense linears and feed-forward blocks are torch modules
+ * (backbone_graph.py:297-330).  T is the type of a call's rows, fl32 a rounding
+ * to 32 bits; ties go to even. */
+
+/* Formats of rows in 8 bits.  INT8: one scale a row,
+ * s = fl32(max(fl32(max |y|), 1e-12) * fl32(1/127)), codes round(y / s) within +-127.  E4M3: one scale a
+ * row, s = fl32(max(fl32(max |y|), 1e-10) * fl32(1/448)), codes the nearest E4M3
+ * numbers.  E4M3_GROUP: such a scale for every 128 columns (a multiple of them).
+ * Codes are those of the exact quotients.  A row (group) with an infinity or
+ * NaN has codes of 0 and a scale of NaN and raises DMOE_STATUS_NON_FINITE. */
+enum { DMOE_ROWS_INT8 = 1, DMOE_ROWS_E4M3 = 2, DMOE_ROWS_E4M3_GROUP = 3 };
+
+/* Rows of a float type; row_stride in elements, data aligned to an element. */
+typedef struct DmoeRows {
+    void* data;
+    int64_t row_stride;
+    int32_t dtype;
+} DmoeRows;
+
+/* Rows in 8 bits: values 16-byte aligned, row_stride in bytes, a multiple of
+ * 16 that holds the columns rounded up to a multiple of 128; the columns in
+ * between are zeros (calls that write such rows write them).  scales
+ * [rows], or [rows, columns / 128]. */
+typedef struct DmoeQuantRows {
+    void* values;
+    int64_t row_stride;
+    float* scales;
+    int32_t format;
+} DmoeQuantRows;
+
+/* Matrix [n, k] of 8-bit integers with a scale a row: rows 16-byte aligned,
+ * row_stride in bytes, a multiple of 16; a row is readable to a multiple of
+ * 16 columns, whatever lies there. */
+typedef struct DmoeInt8Weight {
+    const int8_t* values;
+    int64_t row_stride;
+    const float* scales;
+    int32_t n, k;
+} DmoeInt8Weight;
+
+/* h = T(x + residual) (x without residual), y = h * g / sqrt(mean(h^2) + eps)
+ * with g = fl32(offset + weight) and fl32(h * g) the value that is scaled.
+ * x, residual, hidden and out [rows, cols] have one type; weight [cols] has
+ * any.  hidden (wanted only with residual; it may be residual's or x's buffer
+ * itself), out and quantized may each be NULL, not both of the last.  cols in
+ * [1, 65536]. */
+DMOE_API int dmoe_rms_norm(const DmoeRows* x, const DmoeRows* residual, int rows, int cols, const void* weight,
+                           int weight_dtype, float offset, double eps, const DmoeRows* hidden, const DmoeRows* out,
+                           const DmoeQuantRows* quantized, int* status, void* stream);
+
+/* Rows x [rows, cols] to 8-bit integers (quantized->format DMOE_ROWS_INT8). */
+DMOE_API int dmoe_int8_quantize(const DmoeRows* x, int rows, int cols, const DmoeQuantRows* quantized, int* status,
+                                void* stream);
+
+/* out [rows, cols] = T(code * scale) of rows in 8 bits. */
+DMOE_API int dmoe_rows8_read(const DmoeQuantRows* quantized, int rows, int cols, const DmoeRows* out, void* stream);
+
+/* out [rows, n] = T(sum(codes * codes) * row scale * channel scale + bias + residual):
+ * sums exact in int32, the rest in fp32.  Rows come quantized (quantized,
+ * DMOE_ROWS_INT8) or as x of a float type, never both; x is quantized on the
+ * way, in the workspace of dmoe_int8_linear_workspace_bytes (0: none needed).
+ * bias fp32 [n] and residual (of out's type; it may be out's buffer itself) may
+ * be NULL.  k in [1, 65536]. */
+DMOE_API size_t dmoe_int8_linear_workspace_bytes(int rows, int k);
+DMOE_API int dmoe_int8_linear(const DmoeRows* x, const DmoeQuantRows* quantized, int rows, const DmoeInt8Weight* weight,
+                              const float* bias, const DmoeRows* residual, const DmoeRows* out, void* workspace,
+                              size_t workspace_bytes, int* status, void* stream);
+
+/* Gated feed-forward block: a = T(act(gate) * up) of the products with
+ * gate_up [2 * inter, k] (gate rows first; act DMOE_ACT_SILU z / (1 + exp(-z)) or
+ * DMOE_ACT_GELU_TANH), then out [rows, down->n] = T(product of a's 8-bit codes
+ * with down [n, inter] + residual). */
+enum { DMOE_ACT_SILU = 0, DMOE_ACT_GELU_TANH = 1 };
+DMOE_API size_t dmoe_int8_feed_forward_workspace_bytes(int rows, int k, int inter, int out_dtype);
+DMOE_API int dmoe_int8_feed_forward(const DmoeRows* x, const DmoeQuantRows* quantized, int rows,
+                                    const DmoeInt8Weight* gate_up, const DmoeInt8Weight* down, int activation,
+                                    const DmoeRows* residual, const DmoeRows* out, void* workspace,
+                                    size_t workspace_bytes, int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
