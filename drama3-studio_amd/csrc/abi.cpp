@@ -1802,6 +1802,9 @@ void check_weight(const DmoeInt8Weight* w) {
             "INT8 weight rows must be 16-byte aligned, with a row stride below 2^23");
 }
 
+// tile counts stay in 32 bits
+void check_result(int rows, int n) { require((int64_t)rows * n < (int64_t)1 << 40, "the product's result is too large"); }
+
 dmoe::Int8Args int8_args(const DmoeInt8Weight& w, int rows, bool gated, int* status) {
     dmoe::Int8Args a{};
     a.rows = rows;
@@ -1849,28 +1852,45 @@ void quantize_into(const dmoe::Rows& x, int rows, int cols, const dmoe::Rows8& q
     dmoe::launch_rows8(n, stream);
 }
 
-void product(const dmoe::Int8Args& a, hipStream_t stream) {
-    if (a.rows <= dmoe::kInt8FewRows) dmoe::launch_int8_few(a, stream);
-    else dmoe::launch_int8_tiles(a, device_cus(), stream);
+dmoe::Int8Plan plan_of(const dmoe::Int8Args& a) { return dmoe::int8_plan(a.rows, a.n, a.k, a.gated != 0); }
+
+// Whether a product's kernel quantizes its rows itself.
+bool takes_floats(int rows, int n, int k, bool gated) {
+    return dmoe::int8_plan(rows, n, k, gated).shape == dmoe::kInt8Few && dmoe::int8_few_quantizes(rows, k);
 }
 
-// The rows of a product: as they are, or quantized at `place` where its kernel does not do that itself.
-void set_input(dmoe::Int8Args& a, const dmoe::Rows& x, void* place, int* status, hipStream_t stream) {
-    if (dmoe::int8_few_quantizes(a.rows, a.k)) {
-        set_rows(a, x);
-        return;
+// Bytes of a product's rows in 8 bits where it needs a place for them, and of its shares' sums behind that.
+size_t input_bytes(int rows, int n, int k, bool gated) { return takes_floats(rows, n, k, gated) ? 0 : rows8_bytes(rows, k); }
+size_t product_bytes(int rows, int n, int k, bool gated) {
+    return input_bytes(rows, n, k, gated) + dmoe::int8_part_bytes(rows, n, k, gated);
+}
+
+// The product of rows of a float type (x) or in 8 bits (q): x as it is where the kernel quantizes it, else at `place`.
+void product(dmoe::Int8Args& a, const dmoe::Rows* x, const dmoe::Rows8* q, void* place, hipStream_t stream) {
+    const dmoe::Int8Plan plan = plan_of(a);
+    char* at = static_cast<char*>(place);
+    if (q) {
+        set_rows(a, *q);
+    } else if (takes_floats(a.rows, a.n, a.k, a.gated)) {
+        set_rows(a, *x);
+    } else {
+        const dmoe::Rows8 made = rows8_at(at, a.rows, a.k);
+        quantize_into(*x, a.rows, a.k, made, a.status, stream);
+        set_rows(a, made);
+        at += rows8_bytes(a.rows, a.k);
     }
-    const dmoe::Rows8 q = rows8_at(place, a.rows, a.k);
-    quantize_into(x, a.rows, a.k, q, status, stream);
-    set_rows(a, q);
+    a.splits = plan.splits;
+    a.part = reinterpret_cast<int*>(at);
+    if (plan.shape == dmoe::kInt8Few) dmoe::launch_int8_few(a, stream);
+    else dmoe::launch_int8_tiles(a, plan, stream);
 }
-
-size_t input_bytes(int rows, int k) { return dmoe::int8_few_quantizes(rows, k) ? 0 : rows8_bytes(rows, k); }
 
 void check_workspace(const void* workspace, size_t have, size_t need) {
     require(need == 0 || (workspace != nullptr && have >= need), "workspace too small");
     require(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
 }
+
+size_t hidden_bytes(int rows, int inter, int dtype) { return ((size_t)rows * inter * elem_size(dtype) + 255) / 256 * 256; }
 
 bool sizes_fit(int rows, int k) { return rows >= 1 && rows <= dmoe::kRows8MaxRows && k >= 1 && k <= dmoe::kInt8MaxK; }
 
@@ -1948,7 +1968,10 @@ int dmoe_rows8_read(const DmoeQuantRows* quantized, int rows, int cols, const Dm
     });
 }
 
-size_t dmoe_int8_linear_workspace_bytes(int rows, int k) { return sizes_fit(rows, k) ? input_bytes(rows, k) : 0; }
+size_t dmoe_int8_linear_workspace_bytes(int rows, int n, int k, int quantized) {
+    if (!sizes_fit(rows, k) || n < 1 || n > (1 << 24)) return 0;
+    return quantized ? dmoe::int8_part_bytes(rows, n, k, false) : product_bytes(rows, n, k, false);
+}
 
 int dmoe_int8_linear(const DmoeRows* x, const DmoeQuantRows* quantized, int rows, const DmoeInt8Weight* weight,
                      const float* bias, const DmoeRows* residual, const DmoeRows* out, void* workspace,
@@ -1957,6 +1980,7 @@ int dmoe_int8_linear(const DmoeRows* x, const DmoeQuantRows* quantized, int rows
         check_weight(weight);
         check_rows8_size(rows, weight->k);
         require((x != nullptr) != (quantized != nullptr), "rows come either quantized or not");
+        check_result(rows, weight->n);
         dmoe::Int8Args a = int8_args(*weight, rows, false, status);
         const dmoe::Rows o = to_kernel(out, rows, a.n, "out");
         a.out = o.p;
@@ -1970,25 +1994,24 @@ int dmoe_int8_linear(const DmoeRows* x, const DmoeQuantRows* quantized, int rows
             a.residual = r.p;
             a.residual_stride = r.stride;
         }
+        dmoe::Rows in;
+        dmoe::Rows8 in8;
         if (quantized) {
-            const dmoe::Rows8 q = to_kernel(quantized, rows, a.k);
-            require(q.format == DMOE_ROWS_INT8, "products take rows of 8-bit integers");
-            if (!rows) return;
-            set_rows(a, q);
+            in8 = to_kernel(quantized, rows, a.k);
+            require(in8.format == DMOE_ROWS_INT8, "products take rows of 8-bit integers");
         } else {
-            const dmoe::Rows in = read_rows(x, rows, a.k, "x");
-            if (!rows) return;
-            check_workspace(workspace, workspace_bytes, input_bytes(rows, a.k));
-            set_input(a, in, workspace, status, as_stream(stream));
+            in = read_rows(x, rows, a.k, "x");
         }
-        product(a, as_stream(stream));
+        if (!rows) return;
+        check_workspace(workspace, workspace_bytes, dmoe_int8_linear_workspace_bytes(rows, a.n, a.k, quantized != nullptr));
+        product(a, quantized ? nullptr : &in, quantized ? &in8 : nullptr, workspace, as_stream(stream));
     });
 }
 
-size_t dmoe_int8_feed_forward_workspace_bytes(int rows, int k, int inter, int out_dtype) {
-    if (!sizes_fit(rows, k) || !sizes_fit(rows, inter) || !is_float_dtype(out_dtype)) return 0;
-    const size_t hidden = ((size_t)rows * inter * elem_size(out_dtype) + 255) / 256 * 256;
-    return hidden + std::max(input_bytes(rows, k), input_bytes(rows, inter));
+size_t dmoe_int8_feed_forward_workspace_bytes(int rows, int n, int k, int inter, int out_dtype) {
+    if (!sizes_fit(rows, k) || !sizes_fit(rows, inter) || n < 1 || n > (1 << 24) || !is_float_dtype(out_dtype)) return 0;
+    return hidden_bytes(rows, inter, out_dtype) +
+           std::max(product_bytes(rows, inter, k, true), product_bytes(rows, n, inter, false));
 }
 
 int dmoe_int8_feed_forward(const DmoeRows* x, const DmoeQuantRows* quantized, int rows, const DmoeInt8Weight* gate_up,
@@ -2002,6 +2025,7 @@ int dmoe_int8_feed_forward(const DmoeRows* x, const DmoeQuantRows* quantized, in
         require((int64_t)gate_up->n * gate_up->row_stride < (int64_t)1 << 31, "gate_up must be smaller than 2 GiB");
         require(activation == DMOE_ACT_SILU || activation == DMOE_ACT_GELU_TANH, "unknown activation");
         require((x != nullptr) != (quantized != nullptr), "rows come either quantized or not");
+        check_result(rows, std::max(gate_up->n, down->n));
         dmoe::Int8Args up = int8_args(*gate_up, rows, true, status), back = int8_args(*down, rows, false, status);
         up.gelu = activation == DMOE_ACT_GELU_TANH;
         const dmoe::Rows o = to_kernel(out, rows, back.n, "out");
@@ -2023,21 +2047,19 @@ int dmoe_int8_feed_forward(const DmoeRows* x, const DmoeQuantRows* quantized, in
             in = read_rows(x, rows, up.k, "x");
         }
         if (!rows) return;
-        check_workspace(workspace, workspace_bytes, dmoe_int8_feed_forward_workspace_bytes(rows, up.k, up.n, o.dtype));
-        // the hidden rows, then a place for the rows in 8 bits: the input's until the first product has read them
+        check_workspace(workspace, workspace_bytes,
+                        dmoe_int8_feed_forward_workspace_bytes(rows, back.n, up.k, up.n, o.dtype));
+        // the hidden rows, then the place of each product in turn
         dmoe::Rows hidden;
         hidden.p = workspace;
         hidden.stride = up.n;
         hidden.dtype = o.dtype;
-        void* place = static_cast<char*>(workspace) + ((size_t)rows * up.n * elem_size(o.dtype) + 255) / 256 * 256;
-        if (quantized) set_rows(up, in8);
-        else set_input(up, in, place, status, as_stream(stream));
+        void* place = static_cast<char*>(workspace) + hidden_bytes(rows, up.n, o.dtype);
         up.out = hidden.p;
         up.out_stride = hidden.stride;
         up.out_dtype = hidden.dtype;
-        product(up, as_stream(stream));
-        set_input(back, hidden, place, status, as_stream(stream));
-        product(back, as_stream(stream));
+        product(up, quantized ? nullptr : &in, quantized ? &in8 : nullptr, place, as_stream(stream));
+        product(back, &hidden, nullptr, place, as_stream(stream));
     });
 }
 

@@ -80,16 +80,64 @@ struct Int8Args {
     void* out;
     int64_t out_stride;
     int out_dtype;
+    int splits;            // shares of K whose sums meet in `part` [splits, rows, int8_part_cols]
+    int* part;
     int* status;
 };
+
+// Columns of a share's row of sums: whole pieces of eight, gate and up behind each other.
+__host__ __device__ inline int64_t int8_part_cols(int n, bool gated) { return (int64_t)((n + 7) / 8 * 8) * (gated ? 2 : 1); }
 
 void launch_rows8(const NormArgs& a, hipStream_t stream);
 void launch_dequant8(const Dequant8Args& a, hipStream_t stream);
 
-constexpr int kInt8FewRows = 64;    // rows that the kernel of few rows takes
-// Whether that kernel quantizes `rows` rows of k columns itself.
+// How a product is cut.
+enum Int8Shape : int { kInt8Few, kInt8Tiles64x128, kInt8Tiles128Deep, kInt8Tiles128, kInt8Tiles256 };
+struct Int8Plan {
+    Int8Shape shape;
+    int splits;  // shares of K, tiles of 64 x 128 only
+};
+
+constexpr int kInt8FewRows = 64;  // rows that the kernel of few rows takes
+
+// Every result is the same bits whichever is taken.  Measured on MI355X (256 CUs), us:
+// * Few rows: each workgroup of sixteen columns reads all rows, from L2.  Up to 72 MB of that beside the matrix it is
+//   faster than tiles (64 rows, K 4096, N 4096, 67 MB: 11.7 against 12.1; 13 rows: 5.7 against 12.5), above it slower
+//   (47 rows, K 4096, gated N 11008, 132 MB: 37 against 19).
+// * 64 x 128 as long as they do not outnumber the CUs (512 rows, K 4096, N 4096, 256 tiles: 13.7, 128 x 128 15.5;
+//   1024 rows, 512 tiles: 24.6 against 20.2).  Their steps along K take about 0.3 each, so where there are over twenty
+//   a share, up to four workgroups share a tile (47 rows, K 11008, N 4096: 27.7 in one, 18.6 in two, 15.4 in four);
+//   with fewer steps joining costs what it saves (64 rows, K 4096: 12.5, 12.1, 12.2).
+// * 128 x 128 with a deep ring where they do not outnumber the CUs (1024 rows, K 4096, N 4096: 20.2, with a ring of
+//   two stages 24.3), else two workgroups a CU (2048 rows: 36 against 38.7).
+// * 256 x 256 where their rounds take less: a round of one a CU takes as long as 1 / 0.64 rounds of two 128 x 128
+//   (8192 rows, K 4096, N 4096: 113 against 135; 2048 rows: 42 against 36).
+inline Int8Plan int8_plan(int rows, int n, int k, bool gated) {
+    constexpr int64_t kCus = 256;
+    const auto tiles = [&](int tm, int tn) {
+        const int cols = gated ? tn / 2 : tn;
+        return ((int64_t)rows + tm - 1) / tm * (((int64_t)n + cols - 1) / cols);
+    };
+    const int64_t again = ((int64_t)n + 15) / 16 * rows * k;
+    if (rows <= kInt8FewRows && again <= 72000000) return {kInt8Few, 1};
+    const int64_t small = tiles(64, 128), middle = tiles(128, 128), large = tiles(256, 256);
+    if (small <= kCus) {
+        const int64_t steps = (k + 127) / 128, most = kCus / small < steps / 20 ? kCus / small : steps / 20;
+        return {kInt8Tiles64x128, most < 1 ? 1 : most > 4 ? 4 : (int)most};
+    }
+    if (middle <= kCus) return {kInt8Tiles128Deep, 1};
+    if ((large + kCus - 1) / kCus * 100 <= (middle + 2 * kCus - 1) / (2 * kCus) * 64) return {kInt8Tiles256, 1};
+    return {kInt8Tiles128, 1};
+}
+
+inline size_t int8_part_bytes(int rows, int n, int k, bool gated) {
+    const Int8Plan p = int8_plan(rows, n, k, gated);
+    return p.splits > 1 ? (size_t)p.splits * rows * int8_part_cols(n, gated) * sizeof(int) : 0;
+}
+
+// Whether the kernel of few rows quantizes `rows` rows of k columns itself.
 bool int8_few_quantizes(int rows, int k);
 void launch_int8_few(const Int8Args& a, hipStream_t stream);
-void launch_int8_tiles(const Int8Args& a, int cus, hipStream_t stream);
+void launch_int8_tiles(const Int8Args& a, const Int8Plan& plan, hipStream_t stream);
 
 }  // namespace dmoe

@@ -25,9 +25,9 @@ constexpr int kFewSumPitch = 17;    // ints from one row's sums to the next row'
 constexpr int kFewQuantRows = 4, kFewQuantVectors = 4;
 constexpr int kFewQuantBytes = 32768;
 
-template <int DT>
+template <int DT, int W>
 __device__ __forceinline__ void quantize_to_lds(const Int8Args& a, uint8_t* lds, int pitch, float* lds_scale, int* tops) {
-    const int waves = kFewWaves;
+    const int waves = W;
     const int slots = a.rows == 1 ? 1 : a.rows == 2 ? 2 : 4;  // wave groups, one a row
     const int per = waves / slots, threads = per * kWave;
     const int wave = threadIdx.x / kWave, group = wave / per, t = threadIdx.x - group * threads;
@@ -63,17 +63,16 @@ __device__ __forceinline__ void quantize_to_lds(const Int8Args& a, uint8_t* lds,
     lds_barrier();
 }
 
-// U K blocks of a wave are in flight at a time.
-template <int NT, int MT, bool GATED, bool QUANT>
-__global__ __launch_bounds__(kFewWaves * kWave) void int8_few_kernel(Int8Args a) {
+// A wave's next U blocks are on their way while it multiplies U.
+template <int NT, int MT, int U, int W, bool GATED, bool QUANT>
+__global__ __launch_bounds__(W * kWave) void int8_few_kernel(Int8Args a) {
     constexpr int kCols = GATED ? NT * 8 : NT * 16;
-    constexpr int U = NT * MT >= 8 ? 1 : NT >= 4 ? 2 : 4;
     __shared__ int sums[NT * MT * 16 * kFewSumPitch];
     __shared__ alignas(16) uint8_t xl[QUANT ? kFewQuantBytes : 16];
     __shared__ float xl_scale[QUANT ? kFewQuantRows : 1];
-    __shared__ int tops[QUANT ? kFewWaves : 1];
+    __shared__ int tops[QUANT ? W : 1];
     const int lane = threadIdx.x % kWave, r = lane % 16, c = lane / 16;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), waves = kFewWaves;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n0 = blockIdx.x * kCols;
     const int blocks = (a.k + kFewBlock - 1) / kFewBlock;
     const int last = ((a.k + 15) / 16 - 1) * 16;  // the last piece of a matrix row; rows' zeros stand against what repeats
@@ -83,24 +82,37 @@ __global__ __launch_bounds__(kFewWaves * kWave) void int8_few_kernel(Int8Args a)
         const int col = min(n0 + (GATED ? j % (NT / 2) : j) * 16 + r, a.n - 1);
         wrow[j] = (const uint8_t*)a.w + (int64_t)(GATED && j >= NT / 2 ? col + a.n : col) * a.w_stride;
     }
-    v4i wf[U][NT][2];
-    const auto fetch = [&](int b0) {
+    // a lane beyond the rows reads the last one again: its sums are columns of their own, which nothing takes
+    const uint8_t* xrow[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) xrow[m] = QUANT ? nullptr : a.xq + (int64_t)min(m * 16 + r, a.rows - 1) * a.xq_stride;
+    const int pitch = padded_k(a.k) + 16;
+    const uint8_t* xlds = xl + (QUANT ? min(r, a.rows - 1) * pitch : 0);
+    struct Group {
+        v4i w[U][NT][2], x[QUANT ? 1 : U][QUANT ? 1 : MT][2];
+    };
+    const auto fetch = [&](Group& g, int b0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int at = min(b0 + u * waves, blocks - 1) * kFewBlock + c * 16;
+            const int at = min(b0 + u * W, blocks - 1) * kFewBlock + c * 16;
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) wf[u][j][h] = *(const v4i*)(wrow[j] + min(at + h * 64, last));
+                for (int j = 0; j < NT; ++j) g.w[u][j][h] = *(const v4i*)(wrow[j] + min(at + h * 64, last));
+                if constexpr (!QUANT) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) g.x[u][m][h] = *(const v4i*)(xrow[m] + at + h * 64);
+                }
+            }
         }
     };
-    fetch(wave);
-    for (int i = threadIdx.x; i < NT * MT * 16 * kFewSumPitch; i += kFewWaves * kWave) sums[i] = 0;
-    const int pitch = padded_k(a.k) + 16;
+    Group now, next;
+    fetch(now, wave);
+    for (int i = threadIdx.x; i < NT * MT * 16 * kFewSumPitch; i += W * kWave) sums[i] = 0;
     if constexpr (QUANT) {
-        if (a.x_dtype == kBF16) quantize_to_lds<kBF16>(a, xl, pitch, xl_scale, tops);
-        else if (a.x_dtype == kF16) quantize_to_lds<kF16>(a, xl, pitch, xl_scale, tops);
-        else quantize_to_lds<kF32>(a, xl, pitch, xl_scale, tops);
+        if (a.x_dtype == kBF16) quantize_to_lds<kBF16, W>(a, xl, pitch, xl_scale, tops);
+        else if (a.x_dtype == kF16) quantize_to_lds<kF16, W>(a, xl, pitch, xl_scale, tops);
+        else quantize_to_lds<kF32, W>(a, xl, pitch, xl_scale, tops);
     } else {
         lds_barrier();
     }
@@ -109,30 +121,33 @@ __global__ __launch_bounds__(kFewWaves * kWave) void int8_few_kernel(Int8Args a)
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[j][m] = v4i{0, 0, 0, 0};
-    const v4i zero = {0, 0, 0, 0};
-    for (int b0 = wave; b0 < blocks; b0 += U * waves) {
-        if (b0 != wave) fetch(b0);
+    const auto multiply = [&](const Group& g, int b0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int b = b0 + u * waves;
-            if (b < blocks) {
-                const int at = b * kFewBlock + c * 16;
+            const int b = b0 + u * W;
+            if (b >= blocks) continue;  // the same for the wave
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const int row = m * 16 + r;
-                    v4i xf[2];
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if constexpr (QUANT) xf[h] = row < a.rows ? *(const v4i*)(xl + row * pitch + at + h * 64) : zero;
-                        else xf[h] = row < a.rows ? *(const v4i*)(a.xq + (int64_t)row * a.xq_stride + at + h * 64) : zero;
-                    }
+                for (int h = 0; h < 2; ++h) {
+                    const v4i xf = QUANT ? *(const v4i*)(xlds + b * kFewBlock + c * 16 + h * 64) : g.x[QUANT ? 0 : u][QUANT ? 0 : m][h];
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) acc[j][m] = mfma_i8(wf[u][j][h], xf[h], acc[j][m]);
+                    for (int j = 0; j < NT; ++j) acc[j][m] = mfma_i8(g.w[u][j][h], xf, acc[j][m]);
                 }
-            }
         }
+    };
+    int b0 = wave;
+    while (true) {
+        const bool more = b0 + U * W < blocks;
+        if (more) fetch(next, b0 + U * W);
+        multiply(now, b0);
+        if (!more) break;
+        b0 += U * W;
+        const bool again = b0 + U * W < blocks;
+        if (again) fetch(now, b0 + U * W);
+        multiply(next, b0);
+        if (!again) break;
+        b0 += U * W;
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -141,7 +156,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void int8_few_kernel(Int8Args a)
 #pragma unroll
             for (int i = 0; i < 4; ++i) atomicAdd(&sums[((j * MT + m) * 16 + r) * kFewSumPitch + 4 * c + i], acc[j][m][i]);
     lds_barrier();
-    for (int i = threadIdx.x; i < MT * 16 * kCols; i += kFewWaves * kWave) {
+    for (int i = threadIdx.x; i < MT * 16 * kCols; i += W * kWave) {
         const int row = i / kCols, col = i % kCols, n = n0 + col;
         if (row >= a.rows || n >= a.n) continue;
         const int j = col / 16, m = row / 16;
@@ -156,24 +171,24 @@ __global__ __launch_bounds__(kFewWaves * kWave) void int8_few_kernel(Int8Args a)
     }
 }
 
-template <int NT, int MT, bool GATED>
+template <int NT, int MT, int U, int W, bool GATED>
 void launch_few_as(const Int8Args& a, hipStream_t stream) {
     constexpr int kCols = GATED ? NT * 8 : NT * 16;
-    const dim3 grid((unsigned)((a.n + kCols - 1) / kCols)), block(kFewWaves * kWave);
+    const dim3 grid((unsigned)((a.n + kCols - 1) / kCols)), block(W * kWave);
     if constexpr (MT == 1) {
         if (a.xq == nullptr) {
-            hipLaunchKernelGGL((int8_few_kernel<NT, MT, GATED, true>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((int8_few_kernel<NT, MT, U, W, GATED, true>), grid, block, 0, stream, a);
             return;
         }
     }
-    hipLaunchKernelGGL((int8_few_kernel<NT, MT, GATED, false>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((int8_few_kernel<NT, MT, U, W, GATED, false>), grid, block, 0, stream, a);
 }
 
 template <int NT, bool GATED>
 void launch_few_of(const Int8Args& a, hipStream_t stream) {
-    if (a.rows <= 16) launch_few_as<NT, 1, GATED>(a, stream);
-    else if (a.rows <= 32) launch_few_as<NT, 2, GATED>(a, stream);
-    else launch_few_as<NT, 4, GATED>(a, stream);
+    if (a.rows <= 16) launch_few_as<NT, 1, 2, kFewWaves, GATED>(a, stream);
+    else if (a.rows <= 32) launch_few_as<NT, 2, 1, kFewWaves, GATED>(a, stream);
+    else launch_few_as<NT, 4, 1, kFewWaves, GATED>(a, stream);
 }
 
 }  // namespace

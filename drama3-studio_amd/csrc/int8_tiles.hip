@@ -3,10 +3,10 @@
 //   acc[t][n] = sum_k xq[t][k] w[n][k] (int32, exact), out = T(acc xs[t] ws[n] + bias[n] + residual[t][n]),
 //   gated: out = T(act(gate) up) of the products with rows n and n + N of w
 //
-// A workgroup of four waves owns B x B sums (gated: B / 2 gate and B / 2 up
-// rows of the matrix against B rows, 32 of each in turn, so that a gate's sum
-// and its up's meet in one lane); a wave owns a quarter in registers and
-// multiplies 32x32x32.  Both operands go through LDS in a ring of stages of BK
+// A workgroup of four waves owns TM x TN sums (gated: TN / 2 gate and TN / 2 up
+// rows of the matrix, 32 of each in turn, so that a gate's sum and its up's
+// meet in one lane); a wave owns a quarter in registers and multiplies
+// 32x32x32.  Both operands go through LDS in a ring of stages of BK
 // columns, filled by direct copies that no register waits for.
 #include <algorithm>
 
@@ -38,167 +38,273 @@ __device__ __forceinline__ v16i mfma_i8_32(const v4i& a, const v4i& b, const v16
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
 }
 
-template <int B, int BK, int S, bool GATED>
+// TM rows by TN matrix rows a workgroup, WM of its four waves along the rows;
+// a ring of S stages of BK columns; a stage's copies in EARLY parts of a step.
+template <int TM_, int TN_, int WM_, int BK_, int S_, int EARLY_>
+struct Shape {
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, BK = BK_, S = S_, EARLY = EARLY_;
+};
+
+template <class G, bool GATED>
 struct Tile {
-    static constexpr int kF = B / 64;              // 32-row fragments of a wave and side
-    static constexpr int kChunks = BK / 16;
-    static constexpr int kUnit = B * BK;           // bytes of one side's stage
-    static constexpr int kCopies = kUnit / 4096;   // copies of a wave for it
-    static constexpr int kCopyRows = 1024 / BK;    // rows of a copy
-    static constexpr int kSteps = BK / 32;         // matrix instructions along a stage
-    static constexpr int kCols = GATED ? B / 2 : B;
+    static constexpr int kWN = 4 / G::WM;
+    static constexpr int kFM = G::TM / G::WM / 32, kFN = G::TN / kWN / 32;  // 32-row fragments of a wave
+    static_assert(!GATED || kFN % 2 == 0, "a wave has gate and up fragments in turn");
+    static constexpr int kChunks = G::BK / 16;
+    static constexpr int kUnitX = G::TM * G::BK, kUnitW = G::TN * G::BK, kStage = kUnitX + kUnitW;  // bytes
+    static constexpr int kCopiesX = kUnitX / 4096, kCopiesW = kUnitW / 4096;   // of a wave for a stage
+    static constexpr int kCopies = kCopiesX + kCopiesW;
+    static constexpr int kCopyRows = 1024 / G::BK;  // rows of a copy
+    static constexpr int kSteps = G::BK / 32;       // matrix instructions along a stage
+    static constexpr int kCols = GATED ? G::TN / 2 : G::TN;
+    static constexpr int kSlots = G::EARLY * kFN;   // places of copies between matrix instructions
+    // copies [first(p), first(p + 1)) go to place p
+    static constexpr int first(int place) { return place * kCopies / kSlots; }
+    // workgroups a CU that LDS has room for
+    static constexpr int kPerCu = 2 * G::S * kStage <= 160 * 1024 ? 2 : 1;
     // a chunk's place in its row: eight lanes of consecutive rows and one chunk fall on all banks
     static __device__ __forceinline__ int place(int row, int chunk) {
-        return BK == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
+        return G::BK == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
     }
 };
 
-template <int B, int BK, int S, bool GATED>
-__global__ __launch_bounds__(256, B == 256 ? 1 : 2) void int8_tile_kernel(Int8Args a, int row_tiles, int col_tiles) {
-    using T = Tile<B, BK, S, GATED>;
-    constexpr int F = T::kF;
-    __shared__ alignas(1024) uint8_t lds[S * 2 * T::kUnit];
+// With DT kI32 a workgroup takes one of a.splits shares of K and leaves its
+// sums to the join.
+template <class G, bool GATED, int DT>
+__global__ __launch_bounds__(256, (Tile<G, GATED>::kPerCu)) void int8_tile_kernel(Int8Args a, int row_tiles, int col_tiles) {
+    using T = Tile<G, GATED>;
+    constexpr int FM = T::kFM, FN = T::kFN, BK = G::BK, S = G::S;
+    constexpr bool kSplit = DT == kI32;
+    __shared__ alignas(1024) uint8_t lds[S * T::kStage];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     // an XCD takes a contiguous share of the tiles and walks them kTileGroup row tiles at a time, column by column, so
     // that what runs on it at one time shares rows and matrix through its L2
-    int m0, n0;
+    int m0, n0, split = 0;
     {
-        const int total = row_tiles * col_tiles, x = blockIdx.x % kTileXcd, j = blockIdx.x / kTileXcd;
+        const int total = row_tiles * col_tiles * (kSplit ? a.splits : 1), x = blockIdx.x % kTileXcd, j = blockIdx.x / kTileXcd;
         const int lo = (int)((int64_t)x * total / kTileXcd), hi = (int)((int64_t)(x + 1) * total / kTileXcd);
         if (lo + j >= hi) return;
-        const int tile = lo + j, group = tile / (kTileGroup * col_tiles), at = tile - group * kTileGroup * col_tiles;
+        int tile = lo + j;
+        if constexpr (kSplit) {
+            split = tile % a.splits;
+            tile /= a.splits;
+        }
+        const int group = tile / (kTileGroup * col_tiles), at = tile - group * kTileGroup * col_tiles;
         const int wide = min(kTileGroup, row_tiles - group * kTileGroup);
-        m0 = (group * kTileGroup + at % wide) * B;
+        m0 = (group * kTileGroup + at % wide) * G::TM;
         n0 = at / wide * T::kCols;
     }
-    const int steps = (a.k + BK - 1) / BK;
+    int steps = (a.k + BK - 1) / BK, k0 = 0;
+    if constexpr (kSplit) {
+        k0 = split * steps / a.splits * BK;
+        steps = (split + 1) * steps / a.splits - k0 / BK;
+    }
     const int kw = (a.k + 15) / 16 * 16;  // readable columns of a matrix row
-    // copies: lane l of copy j brings the chunk that place() wants at its spot
-    uint32_t off_x[T::kCopies], off_w[T::kCopies];
-    const int chunk_of = lane % T::kChunks;
-    int src[T::kCopies];
+    // copies: lane l of copy j brings the chunk that place() wants at its spot, the same one for every j
+    uint32_t off_x[T::kCopiesX], off_w[T::kCopiesW];
+    const uint32_t src = T::place(lane / T::kChunks, lane % T::kChunks) * 16;
 #pragma unroll
-    for (int j = 0; j < T::kCopies; ++j) {
-        const int row = (wave * T::kCopies + j) * T::kCopyRows + lane / T::kChunks;
-        src[j] = T::place(row, chunk_of) * 16;
-        off_x[j] = (uint32_t)(min(m0 + row, a.rows - 1) - m0) * (uint32_t)a.xq_stride + src[j];
+    for (int j = 0; j < T::kCopiesX; ++j) {
+        const int row = (wave * T::kCopiesX + j) * T::kCopyRows + lane / T::kChunks;
+        off_x[j] = (uint32_t)(min(m0 + row, a.rows - 1) - m0) * (uint32_t)a.xq_stride + src;
+    }
+#pragma unroll
+    for (int j = 0; j < T::kCopiesW; ++j) {
+        const int row = (wave * T::kCopiesW + j) * T::kCopyRows + lane / T::kChunks;
         int64_t wr;
         if constexpr (GATED) wr = (int64_t)min(n0 + row / 64 * 32 + row % 32, a.n - 1) - n0 + (row & 32 ? a.n : 0);
         else wr = min(n0 + row, a.n - 1) - n0;
-        off_w[j] = (uint32_t)(wr * a.w_stride) + src[j];
+        off_w[j] = (uint32_t)(wr * a.w_stride) + src;
     }
-    const uint8_t* base_x = a.xq + (int64_t)m0 * a.xq_stride;
-    const uint8_t* base_w = (const uint8_t*)a.w + (int64_t)n0 * a.w_stride;
+    // behind a matrix row's last chunk its first of this stage again: the rows hold zeros there
+    const uint32_t last_back = k0 + (steps - 1) * BK + (int)src >= kw ? src : 0u;
+    const uint8_t* base_x = a.xq + (int64_t)m0 * a.xq_stride + k0;
+    const uint8_t* base_w = (const uint8_t*)a.w + (int64_t)n0 * a.w_stride + k0;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    const auto copy_x = [&](int step, int j) {
-        copy_to_lds(base_x + (int64_t)step * BK, off_x[j],
-                    lds0 + (step % S) * 2 * T::kUnit + (wave * T::kCopies + j) * 1024);
-    };
-    const auto copy_w = [&](int step, int j) {
-        // behind the matrix row's last chunk its first of this stage again: the rows hold zeros there
-        const uint32_t back = step * BK + src[j] >= kw ? (uint32_t)src[j] : 0u;
-        copy_to_lds(base_w + (int64_t)step * BK, off_w[j] - back,
-                    lds0 + (step % S) * 2 * T::kUnit + T::kUnit + (wave * T::kCopies + j) * 1024);
-    };
-    const auto copy_stage = [&](int step) {
-#pragma unroll
-        for (int j = 0; j < T::kCopies; ++j) {
-            copy_x(step, j);
-            copy_w(step, j);
+    const auto copy = [&](int step, int stage, int i) {  // copy i of a stage: rows, then matrix
+        const uint32_t to = lds0 + stage * T::kStage;
+        if (i < T::kCopiesX) {
+            copy_to_lds(base_x + (int64_t)step * BK, off_x[i], to + (wave * T::kCopiesX + i) * 1024);
+        } else {
+            const int j = i - T::kCopiesX;
+            copy_to_lds(base_w + (int64_t)step * BK, off_w[j] - (step == steps - 1 ? last_back : 0u),
+                        to + T::kUnitX + (wave * T::kCopiesW + j) * 1024);
         }
     };
     // operands: lane l holds row l % 32, chunk 2 s + l / 32 of step s
-    const int wave_m = wave % 2 * (B / 2), wave_n = wave / 2 * (B / 2);
+    const int wave_m = wave % G::WM * (FM * 32), wave_n = wave / G::WM;
     const int r = lane % 32, half = lane / 32;
     int at_x[T::kSteps], at_w[T::kSteps];
 #pragma unroll
     for (int s = 0; s < T::kSteps; ++s) {
         at_x[s] = (wave_m + r) * BK + T::place(r, 2 * s + half) * 16;
-        at_w[s] = (wave_n + r) * BK + T::place(r, 2 * s + half) * 16 + T::kUnit;
+        at_w[s] = (wave_n * FN * 32 + r) * BK + T::place(r, 2 * s + half) * 16 + T::kUnitX;
     }
-    v4i xf[2][F], wf[2][F];
-    const auto read = [&](int to, int stage, int s) {
-        const uint8_t* p = lds + stage * 2 * T::kUnit;
+    v4i xf[2][FM], wf[2][FN];
+    constexpr int kReading = FN > 1 ? FN / 2 : 1;  // groups of matrix instructions that read the next operands
+    const auto read = [&](int to, int stage, int s, int g) {
+        const uint8_t* p = lds + stage * T::kStage;
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            xf[to][f] = *(const v4i*)(p + at_x[s] + f * 32 * BK);
-            wf[to][f] = *(const v4i*)(p + at_w[s] + f * 32 * BK);
-        }
+        for (int f = g * FM / kReading; f < (g + 1) * FM / kReading; ++f) xf[to][f] = *(const v4i*)(p + at_x[s] + f * 32 * BK);
+#pragma unroll
+        for (int f = g * FN / kReading; f < (g + 1) * FN / kReading; ++f) wf[to][f] = *(const v4i*)(p + at_w[s] + f * 32 * BK);
     };
-    v16i acc[F][F];  // [matrix fragment][row fragment]: lane l holds row l % 32 and matrix rows 8 (i / 4) + 4 (l / 32) + i % 4
+    // what the results need is loaded first and held: eight columns of the matrix a lane, the rows' scales
+    constexpr int kRaw = FN * 32, kPitch = kRaw + 4;  // sums of a row in LDS, and four ints against bank conflicts
+    constexpr int kOut = GATED ? kRaw / 2 : kRaw, kVectors = kOut / 8, kRowsAt = kWave / kVectors;
+    static_assert((4 * 32 * kPitch + 4 * FM * 32) * 4 <= S * T::kStage, "sums and scales fit the ring");
+    const int cc = lane % kVectors * 8, n = n0 + wave_n * kOut + cc;
+    // column cc of the outputs in a row of sums: gate and up fragments lie in turn
+    const int from = GATED ? cc / 32 * 64 + cc % 32 : cc;
+    float ws[GATED ? 2 : 1][8], bias[8], xs[(FM + 1) / 2];
+    if constexpr (!kSplit) {
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+        for (int e = 0; e < 8; ++e) {
+            const int ne = min(n + e, a.n - 1);
+            ws[0][e] = a.ws[ne];
+            if constexpr (GATED) ws[1][e] = a.ws[ne + a.n];
+            bias[e] = a.bias ? a.bias[ne] : 0.0f;
+        }
 #pragma unroll
-        for (int j = 0; j < F; ++j)
+        for (int i = 0; i < (FM + 1) / 2; ++i) xs[i] = a.xs[min(m0 + wave_m + i * kWave + lane, a.rows - 1)];
+    }
+    v16i acc[FN][FM];  // [matrix fragment][row fragment]: lane l holds row l % 32 and matrix rows 8 (i / 4) + 4 (l / 32) + i % 4
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    const auto multiply = [&](int from) {
+    // of the ring's last stage the first part only, as a step's end would: step 0 goes on with it
+    constexpr int kFirst = T::first(FN);
 #pragma unroll
-        for (int i = 0; i < F; ++i)
+    for (int s = 0; s < S; ++s)
+        if (s < steps) {
 #pragma unroll
-            for (int j = 0; j < F; ++j) acc[i][j] = mfma_i8_32(wf[from][i], xf[from][j], acc[i][j]);
-    };
-    for (int s = 0; s < S && s < steps; ++s) copy_stage(s);
-    tile_wait<0>();
-    read(0, 0, 0);
-    for (int t = 0; t < steps; ++t) {
-        const int stage = t % S;
+            for (int i = 0; i < (s + 1 < S ? T::kCopies : kFirst); ++i) copy(s, s, i);
+        }
+    if (steps >= S) tile_wait<(S - 2) * T::kCopies + kFirst>();
+    else tile_wait<0>();
+#pragma unroll
+    for (int g = 0; g < kReading; ++g) read(0, 0, 0, g);
+    // One step of BK columns out of `stage`, the next one's first operands out of `next`.  The copies of a stage start
+    // behind the barrier that frees its place, in this step's last part, and go on in the next step's first ones: a few
+    // between matrix instructions, which do not wait for them.
+    int stage = 0;
+    const auto step_of = [&](int t, auto copying, auto behind) {
+        constexpr bool kCopying = decltype(copying)::value;  // stage t + S exists
+        constexpr int kBehind = decltype(behind)::value;     // copies that may be on their way at the barrier
+        const int next = stage + 1 == S ? 0 : stage + 1, before = stage == 0 ? S - 1 : stage - 1;
 #pragma unroll
         for (int s = 0; s < T::kSteps; ++s) {
-            if (s + 1 < T::kSteps) {
-                read((s + 1) % 2, stage, s + 1);
-            } else {
-                // every wave has read stage t, and stage t + 1 has come: younger ones may be on their way
-                if (t + S - 1 < steps) tile_wait<(S - 2) * 2 * T::kCopies>();
-                else tile_wait<0>();
-                if (t + S < steps) copy_stage(t + S);
-                if (t + 1 < steps) read(0, (t + 1) % S, 0);
-            }
-            multiply(s % 2);
-        }
-    }
-    // every wave is behind its last read of the ring: each takes a part of it for its results, 32 rows at a time
-    constexpr int kWaveCols = GATED ? B / 4 : B / 2, kPitch = kWaveCols + 4;
-    static_assert(4 * 32 * kPitch * 4 <= S * 2 * T::kUnit, "results fit the ring");
-    float* mine = (float*)lds + wave * 32 * kPitch;
-    const int col0 = n0 + wave / 2 * kWaveCols;
+            const bool last = s + 1 == T::kSteps;
+            if (last) tile_wait<kBehind>();  // every wave has read this stage, and the next has come
+            const int part = last ? 0 : s + 1;  // of the copies: the first starts stage t + S, the others end stage t + S - 1
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
-        const int row0 = m0 + wave_m + j * 32;
-        const float xs = a.xs[min(row0 + r, a.rows - 1)];
-        constexpr int kFragments = GATED ? F / 2 : F;
+            for (int g = 0; g < FN; ++g) {
+                if (g < kReading) read((s + 1) % 2, last ? next : stage, last ? 0 : s + 1, g);
+                if (part < G::EARLY && (kCopying || part > 0)) {
+                    if (part == 0 || t + S - 1 < steps) {
 #pragma unroll
-        for (int i = 0; i < kFragments; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int col = i * 32 + q * 8 + half * 4;
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int n = min(col0 + col + e, a.n - 1);
-                    if constexpr (GATED) {
-                        const float gate = int8_value(acc[2 * i][j][q * 4 + e], a.ws[n], xs);
-                        v[e] = int8_gate(gate, a.gelu) * int8_value(acc[2 * i + 1][j][q * 4 + e], a.ws[n + a.n], xs);
-                    } else {
-                        v[e] = int8_value(acc[i][j][q * 4 + e], a.ws[n], xs);
+                        for (int c = T::first(part * FN + g); c < T::first(part * FN + g + 1); ++c) {
+                            if (part == 0) copy(t + S, stage, c);
+                            else copy(t + S - 1, before, c);
+                        }
                     }
                 }
-                *(v4f*)(mine + r * kPitch + col) = v4f{v[0], v[1], v[2], v[3]};
-            }
-        constexpr int kVectors = kWaveCols / 8, kRowsAt = kWave / kVectors;
-#pragma unroll 1
-        for (int p = 0; p < 32 / kRowsAt; ++p) {
-            const int rr = p * kRowsAt + lane / kVectors, cc = lane % kVectors * 8, n = col0 + cc;
-            const int64_t row = row0 + rr;
-            const v4f lo = *(const v4f*)(mine + rr * kPitch + cc), hi = *(const v4f*)(mine + rr * kPitch + cc + 4);
-            if (row >= a.rows || n >= a.n) continue;
-            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if (a.bias) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += a.bias[min(n + e, a.n - 1)];
+                for (int j = 0; j < FM; ++j) acc[g][j] = mfma_i8_32(wf[s % 2][g], xf[s % 2][j], acc[g][j]);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            const auto finish = [&](auto dt) {
-                constexpr int DT = decltype(dt)::value;
+        }
+        stage = next;
+    };
+    int t = 0;
+    for (; t + S < steps; ++t) step_of(t, std::true_type{}, std::integral_constant<int, (S - 2) * T::kCopies>{});
+    for (; t < steps; ++t) step_of(t, std::false_type{}, std::integral_constant<int, 0>{});
+    // Every wave is behind its last read of the ring: each takes a part of it and turns its sums over there, 32 rows at
+    // a time, so that a lane gets eight columns of a row and the scales, bias and store of whole pieces.
+    int* mine = (int*)lds + wave * 32 * kPitch;
+    float* mine_xs = (float*)lds + 4 * 32 * kPitch + wave * FM * 32;
+    if constexpr (!kSplit) {
+#pragma unroll
+        for (int i = 0; i < (FM + 1) / 2; ++i)
+            if (i * kWave + lane < FM * 32) mine_xs[i * kWave + lane] = xs[i];
+    }
+    constexpr int kPasses = 32 / kRowsAt;
+    const auto put = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *(v4i*)(mine + r * kPitch + i * 32 + q * 8 + half * 4) =
+                    v4i{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+    };
+    const auto sums = [&](int rr, int h, int* raw) {
+        *(v4i*)raw = *(const v4i*)(mine + rr * kPitch + from + h * 32);
+        *(v4i*)(raw + 4) = *(const v4i*)(mine + rr * kPitch + from + h * 32 + 4);
+    };
+    if constexpr (kSplit) {
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            put(j);
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p) {
+                const int rr = p * kRowsAt + lane / kVectors;
+                const int64_t row = m0 + wave_m + j * 32 + rr;
+                if (row >= a.rows || n >= a.n) continue;
+                int* to = a.part + ((int64_t)split * a.rows + row) * int8_part_cols(a.n, GATED) + n;
+#pragma unroll
+                for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+                    int raw[8];
+                    sums(rr, h, raw);
+                    *(v4i*)(to + h * int8_part_cols(a.n, false)) = *(v4i*)raw;
+                    *(v4i*)(to + h * int8_part_cols(a.n, false) + 4) = *(v4i*)(raw + 4);
+                }
+            }
+        }
+    } else {
+        const auto values = [&](int j, int rr, float* v) {
+            int raw[GATED ? 2 : 1][8];
+#pragma unroll
+            for (int h = 0; h < (GATED ? 2 : 1); ++h) sums(rr, h, raw[h]);
+            const float by = mine_xs[j * 32 + rr];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = int8_value(raw[0][e], ws[0][e], by);
+                if constexpr (GATED) v[e] = int8_gate(v[e], a.gelu) * int8_value(raw[GATED][e], ws[GATED][e], by);
+            }
+        };
+        char* out = (char*)a.out + ((int64_t)(m0 + wave_m + lane / kVectors) * a.out_stride + n) * elem_bytes<DT>();
+        const int64_t pass = a.out_stride * kRowsAt * elem_bytes<DT>();
+        if (m0 + G::TM <= a.rows && n0 + T::kCols <= a.n && !a.bias && !a.residual) {  // nothing to ask for
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                put(j);
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) {
+                    float v[8];
+                    values(j, p * kRowsAt + lane / kVectors, v);
+                    put_cols8<DT>(out, v);
+                    out += pass;
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            put(j);
+#pragma unroll 1
+            for (int p = 0; p < kPasses; ++p) {
+                const int rr = p * kRowsAt + lane / kVectors;
+                const int64_t row = m0 + wave_m + j * 32 + rr;
+                if (row >= a.rows || n >= a.n) continue;
+                float v[8];
+                values(j, rr, v);
+                if (a.bias) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += bias[e];
+                }
                 if (a.residual) {
                     float add[8];
                     load_cols8<DT>((const char*)a.residual + row * a.residual_stride * elem_bytes<DT>(), n, a.n, add);
@@ -206,29 +312,87 @@ __global__ __launch_bounds__(256, B == 256 ? 1 : 2) void int8_tile_kernel(Int8Ar
                     for (int e = 0; e < 8; ++e) v[e] += add[e];
                 }
                 store_cols8<DT>((char*)a.out + row * a.out_stride * elem_bytes<DT>(), n, a.n, v);
-            };
-            if (a.out_dtype == kBF16) finish(std::integral_constant<int, kBF16>{});
-            else if (a.out_dtype == kF16) finish(std::integral_constant<int, kF16>{});
-            else finish(std::integral_constant<int, kF32>{});
+            }
         }
     }
 }
 
-template <int B, int BK, int S>
+// The shares' sums of eight columns a thread, added up and finished.
+template <bool GATED, int DT>
+__global__ __launch_bounds__(256) void int8_join_kernel(Int8Args a, int per_row) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (int64_t)a.rows * per_row) return;
+    const int64_t row = at / per_row;
+    const int n = (int)(at - row * per_row) * 8, cols = int8_part_cols(a.n, GATED);
+    const int* p = a.part + row * cols + n;
+    int sum[GATED ? 2 : 1][8] = {};
+    for (int s = 0; s < a.splits; ++s, p += (int64_t)a.rows * cols)
+#pragma unroll
+        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+            const v4i lo = *(const v4i*)(p + h * (cols / 2)), hi = *(const v4i*)(p + h * (cols / 2) + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sum[h][e] += lo[e];
+                sum[h][4 + e] += hi[e];
+            }
+        }
+    const float by = a.xs[row];
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int ne = min(n + e, a.n - 1);
+        v[e] = int8_value(sum[0][e], a.ws[ne], by);
+        if constexpr (GATED) v[e] = int8_gate(v[e], a.gelu) * int8_value(sum[GATED][e], a.ws[ne + a.n], by);
+        if (a.bias) v[e] += a.bias[ne];
+    }
+    if (a.residual) {
+        float add[8];
+        load_cols8<DT>((const char*)a.residual + row * a.residual_stride * elem_bytes<DT>(), n, a.n, add);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += add[e];
+    }
+    store_cols8<DT>((char*)a.out + row * a.out_stride * elem_bytes<DT>(), n, a.n, v);
+}
+
+template <class G, bool GATED>
+void launch_tiles_of(const Int8Args& a, hipStream_t stream) {
+    constexpr int kCols = Tile<G, GATED>::kCols;
+    const int64_t row_tiles = (a.rows + G::TM - 1) / G::TM, col_tiles = (a.n + kCols - 1) / kCols;
+    const int64_t total = row_tiles * col_tiles * a.splits;
+    const dim3 grid((unsigned)((total + kTileXcd - 1) / kTileXcd * kTileXcd)), block(256);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a, (int)row_tiles, (int)col_tiles); };
+    if (a.splits == 1) {
+        if (a.out_dtype == kBF16) go(int8_tile_kernel<G, GATED, kBF16>);
+        else if (a.out_dtype == kF16) go(int8_tile_kernel<G, GATED, kF16>);
+        else go(int8_tile_kernel<G, GATED, kF32>);
+        return;
+    }
+    if constexpr (G::TM == 64) {
+        go(int8_tile_kernel<G, GATED, kI32>);
+        const int per_row = (a.n + 7) / 8;
+        const dim3 join((unsigned)(((int64_t)a.rows * per_row + 255) / 256));
+        const auto end = [&](auto kernel) { hipLaunchKernelGGL(kernel, join, block, 0, stream, a, per_row); };
+        if (a.out_dtype == kBF16) end(int8_join_kernel<GATED, kBF16>);
+        else if (a.out_dtype == kF16) end(int8_join_kernel<GATED, kF16>);
+        else end(int8_join_kernel<GATED, kF32>);
+    }
+}
+
+template <class G>
 void launch_tiles_as(const Int8Args& a, hipStream_t stream) {
-    const int cols = a.gated ? B / 2 : B;
-    const int64_t row_tiles = (a.rows + B - 1) / B, col_tiles = (a.n + cols - 1) / cols;
-    const dim3 grid((unsigned)((row_tiles * col_tiles + kTileXcd - 1) / kTileXcd * kTileXcd)), block(256);
-    if (a.gated) hipLaunchKernelGGL((int8_tile_kernel<B, BK, S, true>), grid, block, 0, stream, a, (int)row_tiles, (int)col_tiles);
-    else hipLaunchKernelGGL((int8_tile_kernel<B, BK, S, false>), grid, block, 0, stream, a, (int)row_tiles, (int)col_tiles);
+    if (a.gated) launch_tiles_of<G, true>(a, stream);
+    else launch_tiles_of<G, false>(a, stream);
 }
 
 }  // namespace
 
-void launch_int8_tiles(const Int8Args& a, int cus, hipStream_t stream) {
-    const int64_t large = (int64_t)((a.rows + 255) / 256) * ((a.n * (a.gated ? 2 : 1) + 255) / 256);
-    if (large >= cus) launch_tiles_as<256, 128, 2>(a, stream);
-    else launch_tiles_as<128, 128, 2>(a, stream);
+void launch_int8_tiles(const Int8Args& a, const Int8Plan& plan, hipStream_t stream) {
+    switch (plan.shape) {
+        case kInt8Tiles64x128: return launch_tiles_as<Shape<64, 128, 2, 128, 4, 2>>(a, stream);
+        case kInt8Tiles128Deep: return launch_tiles_as<Shape<128, 128, 2, 128, 4, 2>>(a, stream);
+        case kInt8Tiles128: return launch_tiles_as<Shape<128, 128, 2, 128, 2, 2>>(a, stream);
+        default: return launch_tiles_as<Shape<256, 256, 2, 128, 2, 2>>(a, stream);
+    }
 }
 
 }  // namespace dmoe

@@ -43,27 +43,38 @@ __device__ __forceinline__ void load_cols8(const void* row, int col, int cols, f
     }
 }
 
+// Two values rounded to a 16-bit type by the hardware's conversion (for bf16 one instruction for both).
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (DT == kBF16) {
+        typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, v2{(__bf16)lo, (__bf16)hi});
+    } else {
+        typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, v2{(_Float16)lo, (_Float16)hi});
+    }
+}
+
+// Eight values to where they lie; past the caches, whose lines the call itself has no more use for.
+template <int DT>
+__device__ __forceinline__ void put_cols8(void* p, const float* v) {
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    typedef v4u any16 __attribute__((aligned(2)));
+    if constexpr (DT == kF32) {
+        __builtin_nontemporal_store(v4u{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])},
+                                    (any16*)p);
+        __builtin_nontemporal_store(v4u{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])},
+                                    (any16*)p + 1);
+    } else {
+        __builtin_nontemporal_store(v4u{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])},
+                                    (any16*)p);
+    }
+}
+
 template <int DT>
 __device__ __forceinline__ void store_cols8(void* row, int col, int cols, const float* v) {
     if (col + 8 <= cols) {
-        char* p = (char*)row + (int64_t)col * elem_bytes<DT>();
-        Any16 a;
-        if constexpr (DT == kF32) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) a.w[j] = __float_as_uint(v[j]);
-            *(Any16*)p = a;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) a.w[j] = __float_as_uint(v[4 + j]);
-            *(Any16*)(p + 16) = a;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint16_t lo = DT == kBF16 ? f32_to_bf16(v[2 * j]) : f32_to_f16(v[2 * j]);
-                const uint16_t hi = DT == kBF16 ? f32_to_bf16(v[2 * j + 1]) : f32_to_f16(v[2 * j + 1]);
-                a.w[j] = lo | (uint32_t)hi << 16;
-            }
-            *(Any16*)p = a;
-        }
+        put_cols8<DT>((char*)row + (int64_t)col * elem_bytes<DT>(), v);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)

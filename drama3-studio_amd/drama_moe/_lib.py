@@ -134,9 +134,9 @@ _SIGNATURES = {
     "dmoe_rms_norm": ([_ROWS, _ROWS, _I, _I, _P, _I, ctypes.c_float, ctypes.c_double, _ROWS, _ROWS, _QROWS, _P, _P], _I),
     "dmoe_int8_quantize": ([_ROWS, _I, _I, _QROWS, _P, _P], _I),
     "dmoe_rows8_read": ([_QROWS, _I, _I, _ROWS, _P], _I),
-    "dmoe_int8_linear_workspace_bytes": ([_I, _I], ctypes.c_size_t),
+    "dmoe_int8_linear_workspace_bytes": ([_I, _I, _I, _I], ctypes.c_size_t),
     "dmoe_int8_linear": ([_ROWS, _QROWS, _I, _INT8, _P, _ROWS, _ROWS, _P, ctypes.c_size_t, _P, _P], _I),
-    "dmoe_int8_feed_forward_workspace_bytes": ([_I, _I, _I, _I], ctypes.c_size_t),
+    "dmoe_int8_feed_forward_workspace_bytes": ([_I, _I, _I, _I, _I], ctypes.c_size_t),
     "dmoe_int8_feed_forward": ([_ROWS, _QROWS, _I, _INT8, _INT8, _I, _ROWS, _ROWS, _P, ctypes.c_size_t, _P, _P], _I),
     "dmoe_fp8_quantized_pairs": ([ctypes.POINTER(Fp8Bank), _P, _P, _L, _L, _I, _I, _I, _P, _I, _P,
                                   _I, _I, _I, _P, _P, ctypes.c_size_t, _P, _P], _I),

@@ -263,9 +263,8 @@ def int8_linear(x: Tensor | QuantRows, weight: Int8Weight, *, bias: Tensor | Non
     if rows:
         lib = _lib.library()
         with _on(device):
-            quant, need = isinstance(x, QuantRows), 0
-            if not quant:
-                need = lib.dmoe_int8_linear_workspace_bytes(rows, weight.shape[1])
+            quant = isinstance(x, QuantRows)
+            need = lib.dmoe_int8_linear_workspace_bytes(rows, n, weight.shape[1], quant)
             scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
             _lib.check(lib.dmoe_int8_linear(
                 None if quant else _desc(rows_in), rows_in.desc if quant else None, rows, weight.desc,
@@ -297,7 +296,7 @@ def int8_feed_forward(x: Tensor | QuantRows, gate_up: Int8Weight, down: Int8Weig
         lib = _lib.library()
         with _on(device):
             quant = isinstance(x, QuantRows)
-            need = lib.dmoe_int8_feed_forward_workspace_bytes(rows, width, inter, _lib.dtype_code(dtype))
+            need = lib.dmoe_int8_feed_forward_workspace_bytes(rows, n, width, inter, _lib.dtype_code(dtype))
             scratch = torch.empty(need, dtype=torch.uint8, device=device)
             _lib.check(lib.dmoe_int8_feed_forward(
                 None if quant else _desc(rows_in), rows_in.desc if quant else None, rows, gate_up.desc, down.desc,

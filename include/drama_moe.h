@@ -730,10 +730,11 @@ DMOE_API int dmoe_rows8_read(const DmoeQuantRows* quantized, int rows, int cols,
 /* out [rows, n] = T(sum(codes * codes) * row scale * channel scale + bias + residual):
  * sums exact in int32, the rest in fp32.  Rows come quantized (quantized,
  * DMOE_ROWS_INT8) or as x of a float type, never both; x is quantized on the
- * way, in the workspace of dmoe_int8_linear_workspace_bytes (0: none needed).
+ * way.  The workspace (256-byte aligned, any contents; nothing is kept in it)
+ * has dmoe_int8_linear_workspace_bytes, which may be none.
  * bias fp32 [n] and residual (of out's type; it may be out's buffer itself) may
  * be NULL.  k in [1, 65536]. */
-DMOE_API size_t dmoe_int8_linear_workspace_bytes(int rows, int k);
+DMOE_API size_t dmoe_int8_linear_workspace_bytes(int rows, int n, int k, int quantized);
 DMOE_API int dmoe_int8_linear(const DmoeRows* x, const DmoeQuantRows* quantized, int rows, const DmoeInt8Weight* weight,
                               const float* bias, const DmoeRows* residual, const DmoeRows* out, void* workspace,
                               size_t workspace_bytes, int* status, void* stream);
@@ -743,7 +744,7 @@ DMOE_API int dmoe_int8_linear(const DmoeRows* x, const DmoeQuantRows* quantized,
  * DMOE_ACT_GELU_TANH), then out [rows, down->n] = T(product of a's 8-bit codes
  * with down [n, inter] + residual). */
 enum { DMOE_ACT_SILU = 0, DMOE_ACT_GELU_TANH = 1 };
-DMOE_API size_t dmoe_int8_feed_forward_workspace_bytes(int rows, int k, int inter, int out_dtype);
+DMOE_API size_t dmoe_int8_feed_forward_workspace_bytes(int rows, int n, int k, int inter, int out_dtype);
 DMOE_API int dmoe_int8_feed_forward(const DmoeRows* x, const DmoeQuantRows* quantized, int rows,
                                     const DmoeInt8Weight* gate_up, const DmoeInt8Weight* down, int activation,
                                     const DmoeRows* residual, const DmoeRows* out, void* workspace,

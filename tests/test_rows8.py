@@ -242,14 +242,18 @@ def test_entry_points_refuse(call, message):
 
 def test_workspaces_cover_what_calls_hold():
     lib = _lib.library()
-    for count, k in ((1, 1 << 16), (5, 100), (65, 4096), (1 << 24, 65536)):
-        need = lib.dmoe_int8_linear_workspace_bytes(count, k)
-        assert need >= count * (-(-k // 128) * 128 + 4) and need % 256 == 0
-        both = lib.dmoe_int8_feed_forward_workspace_bytes(count, k, 1000, _lib.F32)
-        assert both >= need + count * 4000
-    assert lib.dmoe_int8_linear_workspace_bytes(0, 128) == 0 and lib.dmoe_int8_linear_workspace_bytes(1, 65537) == 0
-    assert lib.dmoe_int8_feed_forward_workspace_bytes(4, 128, 0, _lib.F32) == 0
-    assert lib.dmoe_int8_feed_forward_workspace_bytes(4, 128, 128, _lib.I32) == 0
+    for count, k in ((17, 1 << 16), (5, 100), (65, 4096), (1 << 24, 65536)):
+        need = lib.dmoe_int8_linear_workspace_bytes(count, 512, k, 0)
+        assert need >= count * (-(-k // 128) * 128 + 4) and need % 32 == 0
+        assert need > lib.dmoe_int8_linear_workspace_bytes(count, 512, k, 1)
+        both = lib.dmoe_int8_feed_forward_workspace_bytes(count, 512, k, 1000, _lib.F32)
+        assert both >= need - 4 * 4 * 512 * count + count * 4000
+    # shares of K leave their sums: up to four of them, whole pieces of eight columns
+    assert lib.dmoe_int8_linear_workspace_bytes(60, 4090, 11008, 1) == 4 * 60 * 4096 * 4
+    assert lib.dmoe_int8_linear_workspace_bytes(0, 512, 128, 0) == 0 and lib.dmoe_int8_linear_workspace_bytes(1, 512, 65537, 0) == 0
+    assert lib.dmoe_int8_linear_workspace_bytes(4, 0, 128, 0) == 0
+    assert lib.dmoe_int8_feed_forward_workspace_bytes(4, 512, 128, 0, _lib.F32) == 0
+    assert lib.dmoe_int8_feed_forward_workspace_bytes(4, 512, 128, 128, _lib.I32) == 0
 
 
 # ------------------------------------------------------------------ the reference
