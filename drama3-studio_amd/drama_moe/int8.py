@@ -29,7 +29,7 @@ from .offload import _device_of, device_state
 
 MAX_K = 65536
 MAX_ROWS = 1 << 24
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_FLOATS = {t: _lib.dtype_code(t) for t in (torch.bfloat16, torch.float16, torch.float32)}
 INT8, E4M3, E4M3_GROUP = 1, 2, 3
 GROUP = 128  # columns of an E4M3 group
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
@@ -52,21 +52,25 @@ def _check_float(t: Tensor, name: str) -> None:
 
 def _flat(t: Tensor, name: str, cols: int | None = None) -> Tensor:
     """t [..., cols] as rows [rows, cols] with contiguous columns."""
-    if t.ndim < 1 or (cols is not None and t.shape[-1] != cols):
-        raise ValueError(f"{name} must be [..., {cols if cols is not None else 'columns'}], got {list(t.shape)}")
-    _check_float(t, name)
-    if t.ndim != 2:
+    shape = t.shape
+    if len(shape) < 1 or (cols is not None and shape[-1] != cols):
+        raise ValueError(f"{name} must be [..., {cols if cols is not None else 'columns'}], got {list(shape)}")
+    if t.dtype not in _FLOATS:
+        _check_float(t, name)
+    if len(shape) != 2:
         rows = 1
-        for size in t.shape[:-1]:
+        for size in shape[:-1]:
             rows *= size
-        t = t.reshape(rows, t.shape[-1])
-    if t.shape[1] > 1 and t.stride(1) != 1 or 0 < t.stride(0) < t.shape[1] and t.shape[0] > 1:
+        t = t.reshape(rows, shape[-1])
+        shape = t.shape
+    down, across = t.stride()
+    if (across != 1 and shape[1] > 1) or (0 < down < shape[1] and shape[0] > 1):
         t = t.contiguous()
     return t
 
 
 def _desc(t: Tensor) -> _lib.Rows:
-    return _lib.Rows(t.data_ptr(), t.stride(0), _lib.dtype_code(t.dtype))
+    return _lib.Rows(t.data_ptr(), t.stride(0), _FLOATS[t.dtype])
 
 
 def _check_sizes(rows: int, cols: int) -> None:
@@ -74,6 +78,12 @@ def _check_sizes(rows: int, cols: int) -> None:
         raise ValueError(f"row count outside [0, {MAX_ROWS}]")
     if not 1 <= cols <= MAX_K:
         raise ValueError(f"column count outside [1, {MAX_K}]")
+
+
+def _gpu(device: torch.device, t: Tensor) -> torch.device:
+    if device.type != "cuda":
+        _device_of(t)  # raises: there is no CPU path
+    return device
 
 
 def _same_device(device: torch.device, **tensors) -> None:
@@ -91,7 +101,7 @@ class QuantRows:
     object is made; later writes to ``values`` given do not reach the copy.
     """
 
-    __slots__ = ("values", "scales", "format", "desc")
+    __slots__ = ("shape", "format", "device", "desc", "_held", "_values", "_scales")
     ndim = 2
     requires_grad = False
 
@@ -110,42 +120,57 @@ class QuantRows:
         stride = values.stride(0)
         if cols % GROUP or values.stride(1) != 1 or stride % 16 or not cols <= stride < 1 << 23 or values.data_ptr() % 16:
             held = torch.zeros((rows, _padded(cols)), dtype=torch.int8, device=values.device)
-            held[:, :cols] = values.view(torch.int8) if values.element_size() == 1 else values
+            held[:, :cols] = values.view(torch.int8)
             values = held.view(values.dtype)[:, :cols]
-        self._set(values, scales.contiguous(), E4M3_GROUP if grouped else INT8 if values.dtype is torch.int8 else E4M3)
-
-    def _set(self, values: Tensor, scales: Tensor, fmt: int) -> None:
-        self.values, self.scales, self.format = values, scales, fmt
-        self.desc = _lib.QuantRowsDesc(values.data_ptr(), values.stride(0), scales.data_ptr(), fmt)
+        scales = scales.contiguous()
+        self._values, self._scales, self._held = values, scales, None
+        self.shape, self.device = values.shape, values.device
+        self.format = E4M3_GROUP if grouped else INT8 if values.dtype is torch.int8 else E4M3
+        self.desc = _lib.QuantRowsDesc(values.data_ptr(), values.stride(0), scales.data_ptr(), self.format)
 
     @classmethod
     def _new(cls, rows: int, cols: int, fmt: int, device) -> QuantRows:
-        """Rows for a call to write."""
+        """Rows for a call to write: one piece of memory, the scales behind the values."""
         self = cls.__new__(cls)
         width = _padded(cols)
-        values = torch.empty((rows, width), dtype=torch.int8 if fmt == INT8 else FP8_DTYPE, device=device)
-        scales = torch.empty((rows, cols // GROUP) if fmt == E4M3_GROUP else rows, dtype=torch.float32, device=device)
-        self._set(values if width == cols else values[:, :cols], scales, fmt)
+        self._held = held = torch.empty(rows * (width + 4 * (cols // GROUP if fmt == E4M3_GROUP else 1)), dtype=torch.int8,
+                                        device=device)
+        self._values = self._scales = None
+        self.shape, self.device, self.format = torch.Size((rows, cols)), device, fmt
+        at = held.data_ptr()
+        self.desc = _lib.QuantRowsDesc(at, width, at + rows * width, fmt)
         return self
 
     @property
-    def shape(self) -> torch.Size:
-        return self.values.shape
+    def values(self) -> Tensor:
+        if self._values is None:
+            rows, cols = self.shape
+            width = _padded(cols)
+            values = self._held[:rows * width].view(rows, width)[:, :cols]
+            self._values = values if self.format == INT8 else values.view(FP8_DTYPE)
+        return self._values
 
     @property
-    def device(self) -> torch.device:
-        return self.values.device
+    def scales(self) -> Tensor:
+        if self._scales is None:
+            rows, cols = self.shape
+            scales = self._held[rows * _padded(cols):].view(torch.float32)
+            self._scales = scales.view(rows, cols // GROUP) if self.format == E4M3_GROUP else scales
+        return self._scales
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> Tensor:
         """[rows, columns]: what the codes stand for, code * scale rounded to ``dtype``."""
         if dtype not in _FLOATS:
             raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
-        device = _device_of(self.values)
-        rows, cols = self.values.shape
-        out = torch.empty((rows, cols), dtype=dtype, device=device)
+        device = self.device
+        if device.type != "cuda":
+            _device_of(self.values)
+        rows, cols = self.shape
+        out = torch.empty(self.shape, dtype=dtype, device=device)
         if rows:
             with _on(device):
-                _lib.check(_lib.library().dmoe_rows8_read(self.desc, rows, cols, _desc(out), _stream(device)))
+                _lib.check(_lib.library().dmoe_rows8_read(
+                    self.desc, rows, cols, _lib.Rows(out.data_ptr(), cols, _FLOATS[dtype]), _stream(device)))
         return out
 
 
@@ -157,7 +182,7 @@ def quantize_rows(x: Tensor) -> QuantRows:
     x = _flat(x, "x")
     rows, cols = x.shape
     _check_sizes(rows, cols)
-    device = _device_of(x)
+    device = _gpu(x.device, x)
     q = QuantRows._new(rows, cols, INT8, device)
     if rows:
         with _on(device):
@@ -174,34 +199,33 @@ class Int8Weight:
     multiple of 16, say) are copied once, when the object is made.
     """
 
-    __slots__ = ("values", "scales", "desc")
+    __slots__ = ("values", "scales", "shape", "device", "desc")
 
     def __init__(self, values: Tensor, scales: Tensor):
         if values.dtype is not torch.int8 or values.ndim != 2 or not values.numel():
             raise ValueError("INT8 weight values must be int8 [N, K]")
-        n, k = values.shape
+        self.shape = n, k = values.shape
         if k > MAX_K or n > MAX_ROWS:
             raise ValueError(f"INT8 weight outside [{MAX_ROWS}, {MAX_K}]")
-        if scales.dtype is not torch.float32 or scales.numel() != n or scales.shape not in ((n,), (n, 1)):
+        if scales.dtype is not torch.float32 or scales.shape not in ((n,), (n, 1)):
             raise ValueError("INT8 weight scales must be fp32 [N]")
-        if scales.device != values.device:
+        self.device = values.device
+        if scales.device != self.device:
             raise ValueError("values and scales must share a device")
-        stride, width = values.stride(0) if n > 1 else max(values.stride(0), -(-k // 16) * 16), -(-k // 16) * 16
-        if (k > 1 and values.stride(1) != 1) or stride % 16 or not width <= stride < 1 << 23 or values.data_ptr() % 16 \
-                or values.data_ptr() + (n - 1) * stride + width > _storage_end(values):
+        width = (k + 15) // 16 * 16
+        stride, across = values.stride()
+        if n == 1:
+            stride = max(stride, width)
+        at = values.data_ptr()
+        if (across != 1 and k > 1) or stride % 16 or at % 16 or not width <= stride < 1 << 23 \
+                or (width > k and at + (n - 1) * stride + width > _storage_end(values)):
             held = torch.zeros((n, width), dtype=torch.int8, device=values.device)
             held[:, :k] = values
-            values, stride = held[:, :k], width
-        self.values, self.scales = values, scales.reshape(n).contiguous()
-        self.desc = _lib.Int8WeightDesc(values.data_ptr(), stride, self.scales.data_ptr(), n, k)
-
-    @property
-    def shape(self) -> torch.Size:
-        return self.values.shape
-
-    @property
-    def device(self) -> torch.device:
-        return self.values.device
+            values, stride, at = held[:, :k], width, held.data_ptr()
+        if scales.ndim != 1 or not scales.is_contiguous():
+            scales = scales.reshape(n).contiguous()
+        self.values, self.scales = values, scales
+        self.desc = _lib.Int8WeightDesc(at, stride, scales.data_ptr(), n, k)
 
     @classmethod
     def quantize(cls, weight: Tensor) -> Int8Weight:
@@ -213,18 +237,19 @@ class Int8Weight:
         return cls((w / scales.double()[:, None]).round().clamp(-127, 127).to(torch.int8), scales)
 
 
-def _input(x, weight: Int8Weight, name: str):
-    """(rows as a tensor or QuantRows, leading shape, row count)."""
-    k = weight.shape[1]
+def _input(x, k: int):
+    """(descriptor of float rows, descriptor of rows in 8 bits, leading shape, row count, what they point into)."""
     if isinstance(x, QuantRows):
         if x.format != INT8:
-            raise ValueError(f"{name} must be rows of 8-bit integers")
-        if x.shape[1] != k:
-            raise ValueError(f"{name} must have {k} columns, got {x.shape[1]}")
-        return x, x.shape[:1], x.shape[0]
-    flat = _flat(x, name, k)
-    _check_sizes(flat.shape[0], k)
-    return flat, x.shape[:-1], flat.shape[0]
+            raise ValueError("x must be rows of 8-bit integers")
+        rows, cols = x.shape
+        if cols != k:
+            raise ValueError(f"x must have {k} columns, got {cols}")
+        return None, x.desc, x.shape[:1], rows, x
+    flat = _flat(x, "x", k)
+    rows = flat.shape[0]
+    _check_sizes(rows, k)
+    return _desc(flat), None, x.shape[:-1], rows, flat
 
 
 def _out_dtype(x, dtype: torch.dtype | None, residual: Tensor | None) -> torch.dtype:
@@ -235,9 +260,7 @@ def _out_dtype(x, dtype: torch.dtype | None, residual: Tensor | None) -> torch.d
     return dtype
 
 
-def _residual(residual: Tensor | None, lead: torch.Size, cols: int, dtype: torch.dtype) -> Tensor | None:
-    if residual is None:
-        return None
+def _residual(residual: Tensor, lead: torch.Size, cols: int, dtype: torch.dtype) -> Tensor:
     if residual.shape != (*lead, cols) or residual.dtype is not dtype:
         raise ValueError(f"residual must be {dtype} {[*lead, cols]}")
     return _flat(residual, "residual")
@@ -248,27 +271,27 @@ def int8_linear(x: Tensor | QuantRows, weight: Int8Weight, *, bias: Tensor | Non
     """[..., N] = x w^T (+ bias fp32 [N]) (+ residual [..., N]) in ``dtype``
     (default: the residual's, else x's, else bf16).  x [..., K] is quantized
     on the way, or ``QuantRows`` of 8-bit integers."""
-    n = weight.shape[0]
+    n, k = weight.shape
     dtype = _out_dtype(x, dtype, residual)
     _no_gradients("x bias residual", x, bias, residual)
-    rows_in, lead, rows = _input(x, weight, "x")
-    device = _device_of(weight.values)
-    _same_device(device, x=x, bias=bias, residual=residual)
+    floats, quant, lead, rows, held = _input(x, k)
+    device = _gpu(weight.device, weight.values)
+    if x.device != device or bias is not None or residual is not None:
+        _same_device(device, x=x, bias=bias, residual=residual)
     if bias is not None:
         if bias.dtype is not torch.float32 or bias.shape != (n,):
             raise ValueError(f"bias must be fp32 [{n}]")
         bias = bias.contiguous()
-    add = _residual(residual, lead, n, dtype)
+    add = _residual(residual, lead, n, dtype) if residual is not None else None
     out = torch.empty((rows, n), dtype=dtype, device=device)
     if rows:
         lib = _lib.library()
         with _on(device):
-            quant = isinstance(x, QuantRows)
-            need = lib.dmoe_int8_linear_workspace_bytes(rows, n, weight.shape[1], quant)
+            need = lib.dmoe_int8_linear_workspace_bytes(rows, n, k, quant is not None)
             scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
             _lib.check(lib.dmoe_int8_linear(
-                None if quant else _desc(rows_in), rows_in.desc if quant else None, rows, weight.desc,
-                bias.data_ptr() if bias is not None else None, _desc(add) if add is not None else None, _desc(out),
+                floats, quant, rows, weight.desc, bias.data_ptr() if bias is not None else None,
+                _desc(add) if add is not None else None, _lib.Rows(out.data_ptr(), n, _FLOATS[dtype]),
                 scratch.data_ptr() if need else None, need, device_state(device).status.data_ptr(), _stream(device)))
     return out if len(lead) == 1 else out.reshape(*lead, n)
 
@@ -280,28 +303,29 @@ def int8_feed_forward(x: Tensor | QuantRows, gate_up: Int8Weight, down: Int8Weig
     then the up rows, ``down`` is [N, I].  The hidden rows are rounded to
     ``dtype`` and then to 8-bit integers with a scale a row; ``activation`` is
     "silu" or "gelu_tanh"."""
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")
-    (n, inter), width = down.shape, gate_up.shape[1]
-    if gate_up.shape[0] != 2 * inter:
+    (n, inter), (both, k) = down.shape, gate_up.shape
+    if both != 2 * inter:
         raise ValueError(f"gate_up must be [{2 * inter}, K] for down [{n}, {inter}]")
     dtype = _out_dtype(x, dtype, residual)
     _no_gradients("x residual", x, residual)
-    rows_in, lead, rows = _input(x, gate_up, "x")
-    device = _device_of(gate_up.values)
-    _same_device(device, x=x, down=down, residual=residual)
-    add = _residual(residual, lead, n, dtype)
+    floats, quant, lead, rows, held = _input(x, k)
+    device = _gpu(gate_up.device, gate_up.values)
+    if x.device != device or down.device != device or residual is not None:
+        _same_device(device, x=x, down=down, residual=residual)
+    add = _residual(residual, lead, n, dtype) if residual is not None else None
     out = torch.empty((rows, n), dtype=dtype, device=device)
     if rows:
-        lib = _lib.library()
+        lib, code = _lib.library(), _FLOATS[dtype]
         with _on(device):
-            quant = isinstance(x, QuantRows)
-            need = lib.dmoe_int8_feed_forward_workspace_bytes(rows, n, width, inter, _lib.dtype_code(dtype))
+            need = lib.dmoe_int8_feed_forward_workspace_bytes(rows, n, k, inter, code)
             scratch = torch.empty(need, dtype=torch.uint8, device=device)
             _lib.check(lib.dmoe_int8_feed_forward(
-                None if quant else _desc(rows_in), rows_in.desc if quant else None, rows, gate_up.desc, down.desc,
-                ACTIVATIONS[activation], _desc(add) if add is not None else None, _desc(out), scratch.data_ptr(), need,
-                device_state(device).status.data_ptr(), _stream(device)))
+                floats, quant, rows, gate_up.desc, down.desc, act, _desc(add) if add is not None else None,
+                _lib.Rows(out.data_ptr(), n, code), scratch.data_ptr(), need, device_state(device).status.data_ptr(),
+                _stream(device)))
     return out if len(lead) == 1 else out.reshape(*lead, n)
 
 

@@ -20,8 +20,9 @@ from torch import Tensor
 
 from . import _lib
 from .attention import _no_gradients, _on, _stream
-from .int8 import E4M3, E4M3_GROUP, GROUP, INT8, QuantRows, _check_float, _check_sizes, _desc, _flat, _same_device
-from .offload import _device_of, device_state
+from .int8 import (_FLOATS, E4M3, E4M3_GROUP, GROUP, INT8, QuantRows, _check_float, _check_sizes, _desc, _flat, _gpu,
+                   _same_device)
+from .offload import device_state
 
 QUANT_FORMATS = {"int8": INT8, "fp8": E4M3, "fp8-128": E4M3_GROUP}
 
@@ -45,11 +46,14 @@ def rms_norm(x: Tensor, weight: Tensor, *, residual: Tensor | None = None, eps: 
     (default: without ``quant``).  Sums are of 64 bits, y is rounded once, and
     the codes are of y before that.  A row with an infinity or NaN gets codes
     of 0 and a scale of NaN, and raises the device status bit."""
+    fmt = None
+    if quant is not None:
+        fmt = QUANT_FORMATS.get(quant)
+        if fmt is None:
+            raise ValueError(f"quant must be one of {sorted(QUANT_FORMATS)}")
     if rows is None:
-        rows = quant is None
-    if quant is not None and quant not in QUANT_FORMATS:
-        raise ValueError(f"quant must be one of {sorted(QUANT_FORMATS)}")
-    if not rows and quant is None:
+        rows = fmt is None
+    elif not rows and fmt is None:
         raise ValueError("the norm has no output: neither rows nor quant")
     _no_gradients("x weight residual", x, weight, residual)
     flat = _flat(x, "x")
@@ -57,28 +61,37 @@ def rms_norm(x: Tensor, weight: Tensor, *, residual: Tensor | None = None, eps: 
     _check_sizes(count, cols)
     if weight.shape != (cols,):
         raise ValueError(f"weight must be [{cols}]")
-    _check_float(weight, "weight")
-    if quant == "fp8-128" and cols % GROUP:
+    dtype, shape = x.dtype, x.shape
+    if weight.dtype not in _FLOATS:
+        _check_float(weight, "weight")
+    if fmt == E4M3_GROUP and cols % GROUP:
         raise ValueError("groups of 128 need a multiple of 128 columns")
-    if residual is not None and (residual.shape != x.shape or residual.dtype is not x.dtype):
-        raise ValueError(f"residual must be {x.dtype} {list(x.shape)}")
-    device = _device_of(x)
+    add = None
+    if residual is not None:
+        if residual.shape != shape or residual.dtype is not dtype:
+            raise ValueError(f"residual must be {dtype} {list(shape)}")
+        add = _flat(residual, "residual")
+    device = _gpu(x.device, x)
     _same_device(device, weight=weight, residual=residual)
-    weight = weight.contiguous()
-    add = _flat(residual, "residual") if residual is not None else None
-    hidden = torch.empty((count, cols), dtype=x.dtype, device=device) if residual is not None else None
-    y = torch.empty((count, cols), dtype=x.dtype, device=device) if rows else None
-    q = QuantRows._new(count, cols, QUANT_FORMATS[quant], device) if quant is not None else None
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    hidden = x if add is None else flat.new_empty((count, cols))
+    y = flat.new_empty((count, cols)) if rows else None
+    q = QuantRows._new(count, cols, fmt, device) if fmt is not None else None
     if count:
+        code = _FLOATS[dtype]
         with _on(device):
             _lib.check(_lib.library().dmoe_rms_norm(
                 _desc(flat), _desc(add) if add is not None else None, count, cols, weight.data_ptr(),
-                _lib.dtype_code(weight.dtype), offset, eps, _desc(hidden) if hidden is not None else None,
-                _desc(y) if y is not None else None, q.desc if q is not None else None,
+                _FLOATS[weight.dtype], offset, eps, _lib.Rows(hidden.data_ptr(), cols, code) if add is not None else None,
+                _lib.Rows(y.data_ptr(), cols, code) if rows else None, q.desc if q is not None else None,
                 device_state(device).status.data_ptr(), _stream(device)))
-    shape = x.shape
-    return Normed(x if hidden is None else hidden if len(shape) == 2 else hidden.view(shape),
-                  y if y is None or len(shape) == 2 else y.view(shape), q)
+    if len(shape) != 2:
+        if add is not None:
+            hidden = hidden.view(shape)
+        if rows:
+            y = y.view(shape)
+    return Normed(hidden, y, q)
 
 
 class RmsNorm(torch.nn.Module):
