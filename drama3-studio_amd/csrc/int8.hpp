@@ -92,24 +92,26 @@ void launch_rows8(const NormArgs& a, hipStream_t stream);
 void launch_dequant8(const Dequant8Args& a, hipStream_t stream);
 
 // How a product is cut.
-enum Int8Shape : int { kInt8Few, kInt8Tiles64x128, kInt8Tiles128Deep, kInt8Tiles128, kInt8Tiles256 };
+enum Int8Shape : int { kInt8Few, kInt8Tiles64, kInt8Tiles64x128, kInt8Tiles128Deep, kInt8Tiles128, kInt8Tiles256 };
+constexpr int kInt8MaxSplits = 4;
 struct Int8Plan {
     Int8Shape shape;
-    int splits;  // shares of K, tiles of 64 x 128 only
+    int splits;  // shares of K, tiles of 64 x 64 only
 };
 
 constexpr int kInt8FewRows = 64;  // rows that the kernel of few rows takes
 
-// Every result is the same bits whichever is taken.  Measured on MI355X (256 CUs), us:
-// * Few rows: each workgroup of sixteen columns reads all rows, from L2.  Up to 72 MB of that beside the matrix it is
-//   faster than tiles (64 rows, K 4096, N 4096, 67 MB: 11.7 against 12.1; 13 rows: 5.7 against 12.5), above it slower
-//   (47 rows, K 4096, gated N 11008, 132 MB: 37 against 19).
-// * 64 x 128 as long as they do not outnumber the CUs (512 rows, K 4096, N 4096, 256 tiles: 13.7, 128 x 128 15.5;
-//   1024 rows, 512 tiles: 24.6 against 20.2).  Their steps along K take about 0.3 each, so where there are over twenty
-//   a share, up to four workgroups share a tile (47 rows, K 11008, N 4096: 27.7 in one, 18.6 in two, 15.4 in four);
-//   with fewer steps joining costs what it saves (64 rows, K 4096: 12.5, 12.1, 12.2).
-// * 128 x 128 with a deep ring where they do not outnumber the CUs (1024 rows, K 4096, N 4096: 20.2, with a ring of
-//   two stages 24.3), else two workgroups a CU (2048 rows: 36 against 38.7).
+// Every result is the same bits whichever is taken.  Measured on MI355X (256 CUs) with matrices that are in no cache, us:
+// * Few rows: each workgroup of sixteen columns reads all rows, from L2.  Up to 72 MB of that it is as fast as tiles or
+//   faster (13 rows, K 4096, N 4096: 6.6 against 13.5; 64 rows, 67 MB: 13.0 against 13.6), above it slower (47 rows,
+//   132 MB: K 4096, gated N 11008 39 against 24; K 11008, N 4096 25 against 16.5).
+// * 64 x 64 while they do not outnumber the CUs (256 rows, K 4096, N 4096, 256 tiles: 13.8, 64 x 128 17.4, 128 x 128
+//   22.5).  A step along K takes about 0.3, so where there are over twenty a share, up to four workgroups share a tile
+//   (47 rows, K 11008, N 4096: 28.4 in one, 20.8 in two, 16.5 in four); with fewer, joining costs what it saves (128
+//   rows, K 4096, N 4096: 13.6, 14.3, 16.7).
+// * 64 x 128 while they do not (47 rows, K 4096, gated N 11008, 172 tiles: 24.2, 64 x 64 26.2, 128 x 128 26.5).
+// * 128 x 128 with a deep ring while they do not (509 rows, K 2048, N 5003, 160 tiles: 14.3, 64 x 128 19.4), then with a
+//   ring of two stages, two workgroups a CU (2048 rows, K 4096, N 4096: 36 against 38.7, the matrix in the caches).
 // * 256 x 256 where their rounds take less: a round of one a CU takes as long as 1 / 0.64 rounds of two 128 x 128
 //   (8192 rows, K 4096, N 4096: 113 against 135; 2048 rows: 42 against 36).
 inline Int8Plan int8_plan(int rows, int n, int k, bool gated) {
@@ -120,11 +122,12 @@ inline Int8Plan int8_plan(int rows, int n, int k, bool gated) {
     };
     const int64_t again = ((int64_t)n + 15) / 16 * rows * k;
     if (rows <= kInt8FewRows && again <= 72000000) return {kInt8Few, 1};
-    const int64_t small = tiles(64, 128), middle = tiles(128, 128), large = tiles(256, 256);
+    const int64_t small = tiles(64, 64), middle = tiles(128, 128), large = tiles(256, 256);
     if (small <= kCus) {
         const int64_t steps = (k + 127) / 128, most = kCus / small < steps / 20 ? kCus / small : steps / 20;
-        return {kInt8Tiles64x128, most < 1 ? 1 : most > 4 ? 4 : (int)most};
+        return {kInt8Tiles64, most < 1 ? 1 : most > kInt8MaxSplits ? kInt8MaxSplits : (int)most};
     }
+    if (tiles(64, 128) <= kCus) return {kInt8Tiles64x128, 1};
     if (middle <= kCus) return {kInt8Tiles128Deep, 1};
     if ((large + kCus - 1) / kCus * 100 <= (middle + 2 * kCus - 1) / (2 * kCus) * 64) return {kInt8Tiles256, 1};
     return {kInt8Tiles128, 1};

@@ -8,8 +8,8 @@
 // streaming 16-byte pieces of one row into 16x16x64 matrix instructions, and
 // add their sums in LDS: integer sums, so their order does not matter.  Up to
 // four rows that are not quantized yet are quantized by every workgroup for
-// itself while its first matrix pieces are on their way (a row is at most
-// 64 KB from L2, less than a launch of its own costs).
+// itself while its first matrix pieces are on their way (one row, K 2048, N
+// 2560: 3.6 us against 3.3 and a launch of the quantizer, about 2.5).
 #include <algorithm>
 
 #include "rows8_util.hpp"
@@ -19,53 +19,69 @@ namespace dmoe {
 
 namespace {
 
-constexpr int kFewWaves = 8;
 constexpr int kFewBlock = 128;      // columns of a K block
 constexpr int kFewSumPitch = 17;    // ints from one row's sums to the next row's: 16 and one against bank conflicts
-constexpr int kFewQuantRows = 4, kFewQuantVectors = 4;
+constexpr int kFewQuantRows = 4;
 constexpr int kFewQuantBytes = 32768;
 
+// The call's rows to 8-bit integers in LDS, a row by each group of waves.  A
+// thread holds its first eight columns, asked for before the matrix's loads
+// (they would be waited for too); longer rows are read twice rather than
+// held, which would cost those loads their registers.
 template <int DT, int W>
-__device__ __forceinline__ void quantize_to_lds(const Int8Args& a, uint8_t* lds, int pitch, float* lds_scale, int* tops) {
-    const int waves = W;
-    const int slots = a.rows == 1 ? 1 : a.rows == 2 ? 2 : 4;  // wave groups, one a row
-    const int per = waves / slots, threads = per * kWave;
-    const int wave = threadIdx.x / kWave, group = wave / per, t = threadIdx.x - group * threads;
-    const int row = min(group, a.rows - 1), end = padded_k(a.k);
-    const char* x = (const char*)a.x + (int64_t)row * a.x_stride * elem_bytes<DT>();
-    float u[kFewQuantVectors][8];
-    int top = 0;
-#pragma unroll
-    for (int v = 0; v < kFewQuantVectors; ++v) {
-        load_cols8<DT>(x, (v * threads + t) * 8, a.k, u[v]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, magnitude(u[v][j]));
+struct RowsToLds {
+    int group, t, threads, row;
+    const char* x;
+    Cols8<DT> first;
+
+    __device__ __forceinline__ RowsToLds(const Int8Args& a, bool wanted) {
+        if (!wanted) return;
+        const int slots = a.rows == 1 ? 1 : a.rows == 2 ? 2 : 4;
+        threads = W / slots * kWave;
+        group = threadIdx.x / threads;
+        t = threadIdx.x - group * threads;
+        row = min(group, a.rows - 1);
+        x = (const char*)a.x + (int64_t)row * a.x_stride * elem_bytes<DT>();
+        first = load_raw8<DT>(x, t * 8, a.k);
     }
-    top = wave_max_bits(top);
-    if (threadIdx.x % kWave == 0) tops[wave] = top;
-    lds_barrier();
-    top = tops[group * per];
-    for (int w = 1; w < per; ++w) top = max(top, tops[group * per + w]);
-    const float top32 = __int_as_float(top);
-    const bool fine = finite_bits(top32);
-    const float scale = int8_scale(top32), each = __fdiv_rn(1.0f, scale);
-    if (group < a.rows) {
+
+    __device__ __forceinline__ void quantize(const Int8Args& a, uint8_t* lds, int pitch, float* lds_scale, int* tops) const {
+        const int per = threads / kWave, end = padded_k(a.k);
+        int top = magnitude8<DT>(first);
+#pragma unroll 1
+        for (int col = (t + threads) * 8; col < a.k; col += threads * 8) top = max(top, magnitude8<DT>(load_raw8<DT>(x, col, a.k)));
+        top = wave_max_bits(top);
+        if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
+        lds_barrier();
+        top = tops[group * per];
+        for (int w = 1; w < per; ++w) top = max(top, tops[group * per + w]);
+        const float top32 = __int_as_float(top);
+        const bool fine = finite_bits(top32);
+        const Units units = units_of(1.0, int8_scale(top32));
+        if (group < a.rows) {
+            Cols8<DT> c = first;
+#pragma unroll 1
+            for (int col = t * 8; col < end; col += threads * 8) {
+                if (col != t * 8) c = load_raw8<DT>(x, col, a.k);
+                float u[8];
 #pragma unroll
-        for (int v = 0; v < kFewQuantVectors; ++v) {
-            const int col = (v * threads + t) * 8;
-            if (col < end) *(uint64_t*)(lds + row * pitch + col) = fine ? int8_codes8(u[v], each, 1.0, scale) : 0;
+                for (int j = 0; j < 8; ++j) u[j] = col_of<DT>(c, j);
+                *(uint64_t*)(lds + row * pitch + col) = fine ? int8_codes8(u, units) : 0;
+            }
+            if (t == 0) {
+                lds_scale[row] = fine ? units.scale : __builtin_nanf("");
+                if (!fine && blockIdx.x == 0) raise_status(a.status, kNonFinite);
+            }
         }
-        if (t == 0) {
-            lds_scale[row] = fine ? scale : __builtin_nanf("");
-            if (!fine && blockIdx.x == 0) raise_status(a.status, kNonFinite);
-        }
+        lds_barrier();
     }
-    lds_barrier();
-}
+};
 
 // A wave's next U blocks are on their way while it multiplies U.
-template <int NT, int MT, int U, int W, bool GATED, bool QUANT>
-__global__ __launch_bounds__(W * kWave) void int8_few_kernel(Int8Args a) {
+// DT is the type of rows that are not quantized yet, kI32 where they are.
+template <int NT, int MT, int U, int W, bool GATED, int DT>
+__global__ __launch_bounds__(W * kWave, (W > 8 ? 4 : NT * MT <= 2 ? 6 : NT * MT <= 4 ? 4 : 2)) void int8_few_kernel(Int8Args a) {
+    constexpr bool QUANT = DT != kI32;
     constexpr int kCols = GATED ? NT * 8 : NT * 16;
     __shared__ int sums[NT * MT * 16 * kFewSumPitch];
     __shared__ alignas(16) uint8_t xl[QUANT ? kFewQuantBytes : 16];
@@ -106,16 +122,18 @@ __global__ __launch_bounds__(W * kWave) void int8_few_kernel(Int8Args a) {
             }
         }
     };
+    const RowsToLds<QUANT ? DT : kBF16, W> rows(a, QUANT);
     Group now, next;
     fetch(now, wave);
+    // what the first result of a thread needs beside its sum
+    const int my_row = threadIdx.x / kCols, my_n = min(n0 + (int)threadIdx.x % kCols, a.n - 1);
+    const int safe_row = min(my_row, a.rows - 1);
+    const float my_ws = a.ws[my_n], my_up = GATED ? a.ws[my_n + a.n] : 0.0f, my_xs = QUANT ? 0.0f : a.xs[safe_row];
+    const float my_bias = a.bias ? a.bias[my_n] : 0.0f;
+    const float my_add = a.residual ? load_as_f32(a.residual, (int64_t)safe_row * a.residual_stride + my_n, a.out_dtype) : 0.0f;
     for (int i = threadIdx.x; i < NT * MT * 16 * kFewSumPitch; i += W * kWave) sums[i] = 0;
-    if constexpr (QUANT) {
-        if (a.x_dtype == kBF16) quantize_to_lds<kBF16, W>(a, xl, pitch, xl_scale, tops);
-        else if (a.x_dtype == kF16) quantize_to_lds<kF16, W>(a, xl, pitch, xl_scale, tops);
-        else quantize_to_lds<kF32, W>(a, xl, pitch, xl_scale, tops);
-    } else {
-        lds_barrier();
-    }
+    if constexpr (QUANT) rows.quantize(a, xl, pitch, xl_scale, tops);
+    else lds_barrier();
     v4i acc[NT][MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -156,18 +174,23 @@ __global__ __launch_bounds__(W * kWave) void int8_few_kernel(Int8Args a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) atomicAdd(&sums[((j * MT + m) * 16 + r) * kFewSumPitch + 4 * c + i], acc[j][m][i]);
     lds_barrier();
-    for (int i = threadIdx.x; i < MT * 16 * kCols; i += W * kWave) {
-        const int row = i / kCols, col = i % kCols, n = n0 + col;
-        if (row >= a.rows || n >= a.n) continue;
-        const int j = col / 16, m = row / 16;
-        const float xs = QUANT ? xl_scale[QUANT ? row : 0] : a.xs[row];
+    const auto finish = [&](int row, int col, float ws, float up, float xs, float bias, float add) {
+        const int j = col / 16, m = row / 16, n = n0 + col;
         const int* s = &sums[((j * MT + m) * 16 + row % 16) * kFewSumPitch + col % 16];
-        float v = int8_value(s[0], a.ws[n], xs);
-        if constexpr (GATED)
-            v = int8_gate(v, a.gelu) * int8_value(s[NT / 2 * MT * 16 * kFewSumPitch], a.ws[n + a.n], xs);
-        if (a.bias) v += a.bias[n];
-        if (a.residual) v += load_as_f32(a.residual, (int64_t)row * a.residual_stride + n, a.out_dtype);
+        float v = int8_value(s[0], ws, xs);
+        if constexpr (GATED) v = int8_gate(v, a.gelu) * int8_value(s[NT / 2 * MT * 16 * kFewSumPitch], up, xs);
+        if (a.bias) v += bias;
+        if (a.residual) v += add;
         store_from_f32(a.out, (int64_t)row * a.out_stride + n, a.out_dtype, v);
+    };
+    if (my_row < min(a.rows, MT * 16) && n0 + (int)threadIdx.x % kCols < a.n)
+        finish(my_row, threadIdx.x % kCols, my_ws, my_up, QUANT ? xl_scale[QUANT ? my_row : 0] : my_xs, my_bias, my_add);
+    for (int i = threadIdx.x + W * kWave; i < min(a.rows, MT * 16) * kCols; i += W * kWave) {
+        const int row = i / kCols, col = i % kCols, n = n0 + col;
+        if (n >= a.n) continue;
+        finish(row, col, a.ws[n], GATED ? a.ws[n + a.n] : 0.0f, QUANT ? xl_scale[QUANT ? row : 0] : a.xs[row],
+               a.bias ? a.bias[n] : 0.0f,
+               a.residual ? load_as_f32(a.residual, (int64_t)row * a.residual_stride + n, a.out_dtype) : 0.0f);
     }
 }
 
@@ -175,33 +198,38 @@ template <int NT, int MT, int U, int W, bool GATED>
 void launch_few_as(const Int8Args& a, hipStream_t stream) {
     constexpr int kCols = GATED ? NT * 8 : NT * 16;
     const dim3 grid((unsigned)((a.n + kCols - 1) / kCols)), block(W * kWave);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
     if constexpr (MT == 1) {
         if (a.xq == nullptr) {
-            hipLaunchKernelGGL((int8_few_kernel<NT, MT, U, W, GATED, true>), grid, block, 0, stream, a);
+            if (a.x_dtype == kBF16) go(int8_few_kernel<NT, MT, U, W, GATED, kBF16>);
+            else if (a.x_dtype == kF16) go(int8_few_kernel<NT, MT, U, W, GATED, kF16>);
+            else go(int8_few_kernel<NT, MT, U, W, GATED, kF32>);
             return;
         }
     }
-    hipLaunchKernelGGL((int8_few_kernel<NT, MT, U, W, GATED, false>), grid, block, 0, stream, a);
+    go(int8_few_kernel<NT, MT, U, W, GATED, kI32>);
 }
 
-template <int NT, bool GATED>
+template <int NT, int W, bool GATED>
 void launch_few_of(const Int8Args& a, hipStream_t stream) {
-    if (a.rows <= 16) launch_few_as<NT, 1, 2, kFewWaves, GATED>(a, stream);
-    else if (a.rows <= 32) launch_few_as<NT, 2, 1, kFewWaves, GATED>(a, stream);
-    else launch_few_as<NT, 4, 1, kFewWaves, GATED>(a, stream);
+    if (a.rows <= 16) launch_few_as<NT, 1, 1, W, GATED>(a, stream);
+    else if (a.rows <= 32) launch_few_as<NT, 2, 1, W, GATED>(a, stream);
+    else launch_few_as<NT, 4, 1, W, GATED>(a, stream);
 }
 
 }  // namespace
 
 bool int8_few_quantizes(int rows, int k) {
-    if (rows > kFewQuantRows || rows * (padded_k(k) + 16) > kFewQuantBytes) return false;
-    const int slots = rows == 1 ? 1 : rows == 2 ? 2 : 4;
-    return padded_k(k) <= kFewQuantVectors * 8 * (kFewWaves / slots) * kWave;
+    return rows <= kFewQuantRows && rows * (padded_k(k) + 16) <= kFewQuantBytes;
 }
 
+// Sixteen waves a workgroup where those are few (one row, K 5632, N 2048, 128 workgroups: 5.6 us, with eight waves 6.2;
+// 16 rows, K 11008, N 4096, 256 workgroups: 15.2 against 14.1).  A second K block on its way costs the registers of a
+// workgroup a CU (13 rows, K 4096, N 4096: 8.0 us against 6.6).
 void launch_int8_few(const Int8Args& a, hipStream_t stream) {
-    if (a.gated) launch_few_of<2, true>(a, stream);
-    else launch_few_of<1, false>(a, stream);
+    if (a.gated) launch_few_of<2, 8, true>(a, stream);
+    else if (a.n <= 16 * 192) launch_few_of<1, 16, false>(a, stream);
+    else launch_few_of<1, 8, false>(a, stream);
 }
 
 }  // namespace dmoe

@@ -3,7 +3,7 @@
 //   acc[t][n] = sum_k xq[t][k] w[n][k] (int32, exact), out = T(acc xs[t] ws[n] + bias[n] + residual[t][n]),
 //   gated: out = T(act(gate) up) of the products with rows n and n + N of w
 //
-// A workgroup of four waves owns TM x TN sums (gated: TN / 2 gate and TN / 2 up
+// A workgroup, mostly of four waves, owns TM x TN sums (gated: TN / 2 gate and TN / 2 up
 // rows of the matrix, 32 of each in turn, so that a gate's sum and its up's
 // meet in one lane); a wave owns a quarter in registers and multiplies
 // 32x32x32.  Both operands go through LDS in a ring of stages of BK
@@ -38,21 +38,22 @@ __device__ __forceinline__ v16i mfma_i8_32(const v4i& a, const v4i& b, const v16
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
 }
 
-// TM rows by TN matrix rows a workgroup, WM of its four waves along the rows;
-// a ring of S stages of BK columns; a stage's copies in EARLY parts of a step.
-template <int TM_, int TN_, int WM_, int BK_, int S_, int EARLY_>
+// TM rows by TN matrix rows a workgroup, WM of its waves along the rows and WN
+// along the matrix; a ring of S stages of BK columns; a stage's copies in EARLY
+// parts of a step.
+template <int TM_, int TN_, int WM_, int WN_, int BK_, int S_, int EARLY_>
 struct Shape {
-    static constexpr int TM = TM_, TN = TN_, WM = WM_, BK = BK_, S = S_, EARLY = EARLY_;
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, BK = BK_, S = S_, EARLY = EARLY_;
+    static constexpr int kWaves = WM * WN, kThreads = kWaves * kWave;
 };
 
 template <class G, bool GATED>
 struct Tile {
-    static constexpr int kWN = 4 / G::WM;
-    static constexpr int kFM = G::TM / G::WM / 32, kFN = G::TN / kWN / 32;  // 32-row fragments of a wave
+    static constexpr int kFM = G::TM / G::WM / 32, kFN = G::TN / G::WN / 32;  // 32-row fragments of a wave
     static_assert(!GATED || kFN % 2 == 0, "a wave has gate and up fragments in turn");
     static constexpr int kChunks = G::BK / 16;
     static constexpr int kUnitX = G::TM * G::BK, kUnitW = G::TN * G::BK, kStage = kUnitX + kUnitW;  // bytes
-    static constexpr int kCopiesX = kUnitX / 4096, kCopiesW = kUnitW / 4096;   // of a wave for a stage
+    static constexpr int kCopiesX = kUnitX / 1024 / G::kWaves, kCopiesW = kUnitW / 1024 / G::kWaves;  // of a wave for a stage
     static constexpr int kCopies = kCopiesX + kCopiesW;
     static constexpr int kCopyRows = 1024 / G::BK;  // rows of a copy
     static constexpr int kSteps = G::BK / 32;       // matrix instructions along a stage
@@ -60,8 +61,8 @@ struct Tile {
     static constexpr int kSlots = G::EARLY * kFN;   // places of copies between matrix instructions
     // copies [first(p), first(p + 1)) go to place p
     static constexpr int first(int place) { return place * kCopies / kSlots; }
-    // workgroups a CU that LDS has room for
-    static constexpr int kPerCu = 2 * G::S * kStage <= 160 * 1024 ? 2 : 1;
+    // waves a SIMD that LDS has room for, in workgroups of at least a wave each
+    static constexpr int kPerCu = 160 * 1024 / (G::S * kStage) * G::kWaves / 4, kPerSimd = kPerCu < 1 ? 1 : kPerCu > 2 ? 2 : kPerCu;
     // a chunk's place in its row: eight lanes of consecutive rows and one chunk fall on all banks
     static __device__ __forceinline__ int place(int row, int chunk) {
         return G::BK == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
@@ -71,7 +72,7 @@ struct Tile {
 // With DT kI32 a workgroup takes one of a.splits shares of K and leaves its
 // sums to the join.
 template <class G, bool GATED, int DT>
-__global__ __launch_bounds__(256, (Tile<G, GATED>::kPerCu)) void int8_tile_kernel(Int8Args a, int row_tiles, int col_tiles) {
+__global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_tile_kernel(Int8Args a, int row_tiles, int col_tiles) {
     using T = Tile<G, GATED>;
     constexpr int FM = T::kFM, FN = T::kFN, BK = G::BK, S = G::S;
     constexpr bool kSplit = DT == kI32;
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(256, (Tile<G, GATED>::kPerCu)) void int8_tile_kerne
     // what the results need is loaded first and held: eight columns of the matrix a lane, the rows' scales
     constexpr int kRaw = FN * 32, kPitch = kRaw + 4;  // sums of a row in LDS, and four ints against bank conflicts
     constexpr int kOut = GATED ? kRaw / 2 : kRaw, kVectors = kOut / 8, kRowsAt = kWave / kVectors;
-    static_assert((4 * 32 * kPitch + 4 * FM * 32) * 4 <= S * T::kStage, "sums and scales fit the ring");
+    static_assert(G::kWaves * (32 * kPitch + FM * 32) * 4 <= S * T::kStage, "sums and scales fit the ring");
     const int cc = lane % kVectors * 8, n = n0 + wave_n * kOut + cc;
     // column cc of the outputs in a row of sums: gate and up fragments lie in turn
     const int from = GATED ? cc / 32 * 64 + cc % 32 : cc;
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(256, (Tile<G, GATED>::kPerCu)) void int8_tile_kerne
     // Every wave is behind its last read of the ring: each takes a part of it and turns its sums over there, 32 rows at
     // a time, so that a lane gets eight columns of a row and the scales, bias and store of whole pieces.
     int* mine = (int*)lds + wave * 32 * kPitch;
-    float* mine_xs = (float*)lds + 4 * 32 * kPitch + wave * FM * 32;
+    float* mine_xs = (float*)lds + G::kWaves * 32 * kPitch + wave * FM * 32;
     if constexpr (!kSplit) {
 #pragma unroll
         for (int i = 0; i < (FM + 1) / 2; ++i)
@@ -275,20 +276,41 @@ __global__ __launch_bounds__(256, (Tile<G, GATED>::kPerCu)) void int8_tile_kerne
                 if constexpr (GATED) v[e] = int8_gate(v[e], a.gelu) * int8_value(raw[GATED][e], ws[GATED][e], by);
             }
         };
-        char* out = (char*)a.out + ((int64_t)(m0 + wave_m + lane / kVectors) * a.out_stride + n) * elem_bytes<DT>();
-        const int64_t pass = a.out_stride * kRowsAt * elem_bytes<DT>();
-        if (m0 + G::TM <= a.rows && n0 + T::kCols <= a.n && !a.bias && !a.residual) {  // nothing to ask for
+        // whole pieces of eight columns: nothing waits for anything but the residual, which is asked for a strip ahead
+        const auto whole = [&](auto more) {
+            constexpr bool kMore = decltype(more)::value;  // bias or residual
 #pragma unroll
             for (int j = 0; j < FM; ++j) {
+                float add[kMore ? kPasses : 1][8];
+                if (kMore && a.residual) {
+#pragma unroll
+                    for (int p = 0; p < (kMore ? kPasses : 0); ++p) {
+                        const int64_t row = min(m0 + wave_m + j * 32 + p * kRowsAt + lane / kVectors, a.rows - 1);
+                        load_cols8<DT>((const char*)a.residual + row * a.residual_stride * elem_bytes<DT>(), n, n + 8, add[p]);
+                    }
+                }
                 put(j);
 #pragma unroll
                 for (int p = 0; p < kPasses; ++p) {
+                    const int rr = p * kRowsAt + lane / kVectors;
+                    const int64_t row = m0 + wave_m + j * 32 + rr;
                     float v[8];
-                    values(j, p * kRowsAt + lane / kVectors, v);
-                    put_cols8<DT>(out, v);
-                    out += pass;
+                    values(j, rr, v);
+                    if (kMore && a.bias) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] += bias[e];
+                    }
+                    if (kMore && a.residual) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] += add[kMore ? p : 0][e];
+                    }
+                    if (row < a.rows) put_cols8<DT>((char*)a.out + (row * a.out_stride + n) * elem_bytes<DT>(), v);
                 }
             }
+        };
+        if (n0 + T::kCols <= a.n) {
+            if (a.bias || a.residual) whole(std::true_type{});
+            else whole(std::false_type{});
             return;
         }
 #pragma unroll
@@ -326,14 +348,18 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Int8Args a, int per_row)
     const int n = (int)(at - row * per_row) * 8, cols = int8_part_cols(a.n, GATED);
     const int* p = a.part + row * cols + n;
     int sum[GATED ? 2 : 1][8] = {};
-    for (int s = 0; s < a.splits; ++s, p += (int64_t)a.rows * cols)
 #pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-            const v4i lo = *(const v4i*)(p + h * (cols / 2)), hi = *(const v4i*)(p + h * (cols / 2) + 4);
+    for (int s = 0; s < kInt8MaxSplits; ++s)
+        if (s < a.splits) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sum[h][e] += lo[e];
-                sum[h][4 + e] += hi[e];
+            for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+                const int* q = p + (int64_t)s * a.rows * cols + h * (cols / 2);
+                const v4i lo = *(const v4i*)q, hi = *(const v4i*)(q + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sum[h][e] += lo[e];
+                    sum[h][4 + e] += hi[e];
+                }
             }
         }
     const float by = a.xs[row];
@@ -359,7 +385,7 @@ void launch_tiles_of(const Int8Args& a, hipStream_t stream) {
     constexpr int kCols = Tile<G, GATED>::kCols;
     const int64_t row_tiles = (a.rows + G::TM - 1) / G::TM, col_tiles = (a.n + kCols - 1) / kCols;
     const int64_t total = row_tiles * col_tiles * a.splits;
-    const dim3 grid((unsigned)((total + kTileXcd - 1) / kTileXcd * kTileXcd)), block(256);
+    const dim3 grid((unsigned)((total + kTileXcd - 1) / kTileXcd * kTileXcd)), block(G::kThreads);
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a, (int)row_tiles, (int)col_tiles); };
     if (a.splits == 1) {
         if (a.out_dtype == kBF16) go(int8_tile_kernel<G, GATED, kBF16>);
@@ -367,11 +393,11 @@ void launch_tiles_of(const Int8Args& a, hipStream_t stream) {
         else go(int8_tile_kernel<G, GATED, kF32>);
         return;
     }
-    if constexpr (G::TM == 64) {
+    if constexpr (G::TN == 64) {
         go(int8_tile_kernel<G, GATED, kI32>);
         const int per_row = (a.n + 7) / 8;
         const dim3 join((unsigned)(((int64_t)a.rows * per_row + 255) / 256));
-        const auto end = [&](auto kernel) { hipLaunchKernelGGL(kernel, join, block, 0, stream, a, per_row); };
+        const auto end = [&](auto kernel) { hipLaunchKernelGGL(kernel, join, dim3(256), 0, stream, a, per_row); };
         if (a.out_dtype == kBF16) end(int8_join_kernel<GATED, kBF16>);
         else if (a.out_dtype == kF16) end(int8_join_kernel<GATED, kF16>);
         else end(int8_join_kernel<GATED, kF32>);
@@ -388,10 +414,11 @@ void launch_tiles_as(const Int8Args& a, hipStream_t stream) {
 
 void launch_int8_tiles(const Int8Args& a, const Int8Plan& plan, hipStream_t stream) {
     switch (plan.shape) {
-        case kInt8Tiles64x128: return launch_tiles_as<Shape<64, 128, 2, 128, 4, 2>>(a, stream);
-        case kInt8Tiles128Deep: return launch_tiles_as<Shape<128, 128, 2, 128, 4, 2>>(a, stream);
-        case kInt8Tiles128: return launch_tiles_as<Shape<128, 128, 2, 128, 2, 2>>(a, stream);
-        default: return launch_tiles_as<Shape<256, 256, 2, 128, 2, 2>>(a, stream);
+        case kInt8Tiles64: return launch_tiles_as<Shape<64, 64, 2, 1, 128, 4, 2>>(a, stream);
+        case kInt8Tiles64x128: return launch_tiles_as<Shape<64, 128, 2, 2, 128, 4, 2>>(a, stream);
+        case kInt8Tiles128Deep: return launch_tiles_as<Shape<128, 128, 2, 2, 128, 4, 2>>(a, stream);
+        case kInt8Tiles128: return launch_tiles_as<Shape<128, 128, 2, 2, 128, 2, 2>>(a, stream);
+        default: return launch_tiles_as<Shape<256, 256, 2, 2, 128, 2, 2>>(a, stream);
     }
 }
 

@@ -32,53 +32,55 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
     const int64_t row = (int64_t)blockIdx.x * kRowsPer + threadIdx.x / T;
     if (row >= a.rows) return;  // whole waves; a row of several waves is a whole workgroup
     const char* x = (const char*)a.x + row * a.x_stride * kBytes;
+    Cols8<DT> h[V];
     float u[V][8];
-    int top = 0;
-    int group_top[V];
+    int top = 0, group_top[V];
     double sum = 0.0;
-    float res[V][8];
 #pragma unroll
-    for (int v = 0; v < V; ++v) load_cols8<DT>(x, (v * T + t) * 8, a.cols, u[v]);
+    for (int v = 0; v < V; ++v) h[v] = load_raw8<DT>(x, (v * T + t) * 8, a.cols);
     if (NORM && a.residual) {
         const char* r = (const char*)a.residual + row * a.residual_stride * kBytes;
+        Cols8<DT> add[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) load_cols8<DT>(r, (v * T + t) * 8, a.cols, res[v]);
+        for (int v = 0; v < V; ++v) add[v] = load_raw8<DT>(r, (v * T + t) * 8, a.cols);
 #pragma unroll
-        for (int v = 0; v < V; ++v)
+        for (int v = 0; v < V; ++v) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) u[v][j] = round_through(u[v][j] + res[v][j], DT);
+            for (int j = 0; j < 8; ++j) u[v][j] = col_of<DT>(h[v], j) + col_of<DT>(add[v], j);
+            h[v] = cols_of<DT>(u[v]);
+        }
         if (a.hidden) {
-            char* h = (char*)a.hidden + row * a.hidden_stride * kBytes;
+            char* to = (char*)a.hidden + row * a.hidden_stride * kBytes;
 #pragma unroll
-            for (int v = 0; v < V; ++v) store_cols8<DT>(h, (v * T + t) * 8, a.cols, u[v]);
+            for (int v = 0; v < V; ++v) store_raw8<DT>(to, (v * T + t) * 8, a.cols, h[v]);
         }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[v][j] = col_of<DT>(h[v], j);
         if constexpr (NORM) {
             float g[8];
             const int col = (v * T + t) * 8;
             if (a.weight_dtype == kBF16) load_cols8<kBF16>(a.weight, col, a.cols, g);
             else if (a.weight_dtype == kF16) load_cols8<kF16>(a.weight, col, a.cols, g);
             else load_cols8<kF32>(a.weight, col, a.cols, g);
+            int m = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 // squares of 16-bit types are exact in 32 bits
                 sum += DT == kF32 ? (double)u[v][j] * (double)u[v][j] : (double)(u[v][j] * u[v][j]);
                 u[v][j] *= a.offset + g[j];
+                m = max(m, magnitude(u[v][j]));
             }
+            group_top[v] = m;
+        } else {
+            group_top[v] = magnitude8<DT>(h[v]);
         }
-        int m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, magnitude(u[v][j]));
-        group_top[v] = m;
-        top = max(top, m);
+        top = max(top, group_top[v]);
     }
     top = wave_max_bits(top);
-    if constexpr (NORM) {
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) sum += __shfl_xor(sum, o, kWave);
-    }
+    if constexpr (NORM) sum = wave_sum_f64(sum);
     if constexpr (kWaves > 1) {
         __shared__ double sums[kWaves];
         __shared__ int tops[kWaves];
@@ -96,7 +98,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
             top = max(top, tops[w]);
         }
     }
-    const double by = NORM ? 1.0 / sqrt(sum / a.cols + a.eps) : 1.0;
+    const double by = NORM ? rsqrt_f64(sum / a.cols + a.eps) : 1.0;
     if (NORM && a.y) {
         char* y = (char*)a.y + row * a.y_stride * kBytes;
         const float r = (float)by;
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
             const bool fine = finite_bits(top32);
             const float scale = e4m3_scale(top32);
             if (col >= a.cols) continue;
-            *(uint64_t*)(q + col) = fine ? e4m3_codes8(u[v], (float)(by / (double)scale), by, scale) : 0;
+            *(uint64_t*)(q + col) = fine ? e4m3_codes8(u[v], units_of(by, scale)) : 0;
             if (t % 16 == 0) {
                 a.q.scales[row * (a.cols / 128) + col / 128] = fine ? scale : __builtin_nanf("");
                 if (!fine) raise_status(a.status, kNonFinite);
@@ -129,13 +131,13 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
     const float top32 = (float)((double)__int_as_float(top) * by);
     const bool fine = finite_bits(top32), e4m3 = a.q.format == kRowsE4M3;
     const float scale = e4m3 ? e4m3_scale(top32) : int8_scale(top32);
-    const float each = (float)(by / (double)scale);
+    const Units units = units_of(by, scale);
     const int end = padded_k(a.cols);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int col = (v * T + t) * 8;  // columns from cols on are zeros
         if (col < end)
-            *(uint64_t*)(q + col) = !fine ? 0 : e4m3 ? e4m3_codes8(u[v], each, by, scale) : int8_codes8(u[v], each, by, scale);
+            *(uint64_t*)(q + col) = !fine ? 0 : e4m3 ? e4m3_codes8(u[v], units) : int8_codes8(u[v], units);
     }
     if (t == 0) {
         a.q.scales[row] = fine ? scale : __builtin_nanf("");
@@ -151,17 +153,24 @@ void launch_rows8_as(const NormArgs& a, hipStream_t stream) {
     else hipLaunchKernelGGL((rows8_kernel<DT, T, V, false>), grid, block, 0, stream, a);
 }
 
+// Rows that do not fill the chip get more threads each: their time is a row's.
 template <int DT>
 void launch_rows8_of(const NormArgs& a, hipStream_t stream) {
     const int end = padded_k(a.cols);
-    if (end <= 512) launch_rows8_as<DT, 64, 1>(a, stream);
-    else if (end <= 1024) launch_rows8_as<DT, 64, 2>(a, stream);
-    else if (end <= 2048) launch_rows8_as<DT, 256, 1>(a, stream);
-    else if (end <= 4096) launch_rows8_as<DT, 256, 2>(a, stream);
-    else if (end <= 8192) launch_rows8_as<DT, 256, 4>(a, stream);
-    else if (end <= 16384) launch_rows8_as<DT, 1024, 2>(a, stream);
-    else if (end <= 32768) launch_rows8_as<DT, 1024, 4>(a, stream);
-    else launch_rows8_as<DT, 1024, 8>(a, stream);
+    if (end <= 512) return launch_rows8_as<DT, 64, 1>(a, stream);
+    if (end <= 2048 && (end > 1024 || a.rows <= 1024)) return launch_rows8_as<DT, 256, 1>(a, stream);
+    if (end <= 1024) return launch_rows8_as<DT, 64, 2>(a, stream);
+    if (a.rows <= 512 || end > 16384) {
+        if (end <= 8192) return launch_rows8_as<DT, 1024, 1>(a, stream);
+        if (end <= 16384) return launch_rows8_as<DT, 1024, 2>(a, stream);
+        if (end <= 32768) return launch_rows8_as<DT, 1024, 4>(a, stream);
+        return launch_rows8_as<DT, 1024, 8>(a, stream);
+    }
+    if (end <= 4096) return launch_rows8_as<DT, 256, 2>(a, stream);
+    if (end <= 6144) return launch_rows8_as<DT, 256, 3>(a, stream);
+    if (end <= 8192) return launch_rows8_as<DT, 256, 4>(a, stream);
+    if (end <= 12288) return launch_rows8_as<DT, 256, 6>(a, stream);
+    return launch_rows8_as<DT, 256, 8>(a, stream);
 }
 
 template <int DT>
