@@ -1,5 +1,5 @@
-"""The two halves of a Drama 3 decoder layer: attention over a 4-bit cache,
-and the MoE block around the routed experts.
+"""The halves of a decoder layer: attention over a 4-bit cache, the MoE block
+around the routed experts, and the feed-forward block of a dense layer.
 
 BackboneDecodeGraph splits a decoder layer's MoE half into _route_impl (router
 softmax / top-k on ``moe.gate(flat)``), _shared_impl (the sigmoid-gated shared
@@ -15,7 +15,10 @@ bf16, the reference's compute dtype for these modules.
 ``AttentionBlock`` is the half before it for a layer whose keys and values are
 kept in a ``KvCache4``: projections, ``append``, ``attend``, output projection
 and residual add, with no host sync either, so that a whole layer's decode
-step is captured in one hipGraph.
+step is captured in one hipGraph.  ``DenseBlock`` is the other half of a layer
+without experts: residual add, norm and gated feed-forward on 8-bit integers.
+What ``norm.RmsNorm`` gives feeds all three: rows and the sum for ``MoeBlock``,
+rows in 8 bits for projections that are ``Int8Linear`` and for ``DenseBlock``.
 """
 from __future__ import annotations
 
@@ -25,6 +28,8 @@ from torch import Tensor
 from . import _lib
 from .attention import KvCache4, PagedBatch, Rotary, _no_gradients
 from .formats import QuantizedStore, StagedExperts
+from .int8 import Int8FeedForward, Int8Linear, QuantRows
+from .norm import RmsNorm
 
 
 def _bf16_rows(t: Tensor, name: str, cols: int, rows: int | None = None) -> Tensor:
@@ -124,7 +129,9 @@ class AttentionBlock:
     """Attention half of a decoder layer over a paged 4-bit cache.
 
     ``q_proj``, ``k_proj``, ``v_proj`` and ``o_proj`` are modules over rows
-    (``GPTQLinear``, ``torch.nn.Linear``); ``q_norm`` and ``k_norm``, if the
+    (``GPTQLinear``, ``Int8Linear``, ``torch.nn.Linear``); where the first three
+    are ``Int8Linear``, ``attn_input`` may be a norm's ``QuantRows``, and an
+    ``Int8Linear`` ``o_proj`` adds the residual itself; ``q_norm`` and ``k_norm``, if the
     layer has them, are applied to [rows, heads, D] before the rotation.  It has
     no backward: with gradients enabled, inputs or projections that need them are
     refused.
@@ -148,7 +155,8 @@ class AttentionBlock:
         self.q_norm, self.k_norm = q_norm, k_norm
         self.cache, self.rotary, self.scale, self.window = cache, rotary, scale, int(window)
 
-    def forward(self, attn_input: Tensor, residual: Tensor, batch: PagedBatch, positions: Tensor | None = None) -> Tensor:
+    def forward(self, attn_input: Tensor | QuantRows, residual: Tensor, batch: PagedBatch,
+                positions: Tensor | None = None) -> Tensor:
         """residual + o_proj(attention of the batch's rows), the rows' keys and
         values stored on the way.  Both inputs are [rows, hidden]; for rows that no
         sequence owns, and those before a sequence's first token, the attention
@@ -156,6 +164,9 @@ class AttentionBlock:
         if attn_input.ndim != 2 or attn_input.shape != residual.shape or attn_input.shape[0] != batch.rows:
             raise ValueError(f"attn_input and residual must be [{batch.rows}, hidden]")
         _no_gradients("attn_input", attn_input)
+        if isinstance(attn_input, QuantRows) and not all(isinstance(p, Int8Linear)
+                                                         for p in (self.q_proj, self.k_proj, self.v_proj)):
+            raise ValueError("attn_input in 8 bits needs Int8Linear projections")
         rows, dim = batch.rows, self.cache.head_dim
         q = self.q_proj(attn_input).reshape(rows, self.heads, dim)
         k = self.k_proj(attn_input).reshape(rows, self.cache.kv_heads, dim)
@@ -170,9 +181,38 @@ class AttentionBlock:
             self.cache.append(k, v, batch, positions=positions)
         attended = torch.zeros((rows, self.heads, dim), dtype=q.dtype, device=q.device)
         self.cache.attend(q, batch, scale=self.scale, window=self.window, out=attended)
-        out = self.o_proj(attended.reshape(rows, self.heads * dim))
+        attended = attended.reshape(rows, self.heads * dim)
+        if isinstance(self.o_proj, Int8Linear) and residual.shape[1] == self.o_proj.out_features:
+            return self.o_proj(attended, residual=residual)
+        out = self.o_proj(attended)
         if out.shape != residual.shape:
             raise ValueError(f"o_proj must give {list(residual.shape)}, got {list(out.shape)}")
         return residual + out
+
+    __call__ = forward
+
+
+class DenseBlock:
+    """Feed-forward half of a decoder layer without experts, on 8-bit integers.
+
+    ``norm`` makes the block's input of the residual stream, with
+    ``quant="int8"`` in 8 bits, which the first product then takes as it is;
+    ``ffn`` is the ``Int8FeedForward``.  It has no backward.
+    """
+
+    def __init__(self, norm: RmsNorm, ffn: Int8FeedForward):
+        if norm.quant not in (None, "int8"):
+            raise ValueError("the norm of a dense block gives rows or 8-bit integers")
+        if norm.weight.shape[0] != ffn.gate_up.in_features or ffn.down.out_features != ffn.gate_up.in_features:
+            raise ValueError("norm and feed-forward block must have one width")
+        self.norm, self.ffn = norm, ffn
+
+    def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
+        """h + feed-forward(norm(h)) with h = x + residual (x itself without one), [..., hidden]."""
+        made = self.norm(x, residual)
+        if made.quant is None:
+            return self.ffn(made.rows, residual=made.hidden)
+        out = self.ffn(made.quant, residual=made.hidden.reshape(made.quant.shape), dtype=x.dtype)
+        return out.reshape(x.shape)
 
     __call__ = forward

@@ -25,7 +25,7 @@ from torch import Tensor
 from . import _lib
 from .attention import _no_gradients, _on, _stream
 from .formats import FP8_DTYPE
-from .offload import _device_of, device_state
+from .offload import _STATES, _device_of, device_state
 
 MAX_K = 65536
 MAX_ROWS = 1 << 24
@@ -84,6 +84,13 @@ def _gpu(device: torch.device, t: Tensor) -> torch.device:
     if device.type != "cuda":
         _device_of(t)  # raises: there is no CPU path
     return device
+
+
+def _status(device: torch.device) -> int:
+    """Address of the device's status word, which a capture must not be the first to need: it would lie in the graph's memory."""
+    if device not in _STATES and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the device's status word does not exist yet: run this call once eagerly before capturing it")
+    return device_state(device).status.data_ptr()
 
 
 def _same_device(device: torch.device, **tensors) -> None:
@@ -187,7 +194,7 @@ def quantize_rows(x: Tensor) -> QuantRows:
     if rows:
         with _on(device):
             _lib.check(_lib.library().dmoe_int8_quantize(_desc(x), rows, cols, q.desc,
-                                                         device_state(device).status.data_ptr(), _stream(device)))
+                                                         _status(device), _stream(device)))
     return q
 
 
@@ -292,7 +299,7 @@ def int8_linear(x: Tensor | QuantRows, weight: Int8Weight, *, bias: Tensor | Non
             _lib.check(lib.dmoe_int8_linear(
                 floats, quant, rows, weight.desc, bias.data_ptr() if bias is not None else None,
                 _desc(add) if add is not None else None, _lib.Rows(out.data_ptr(), n, _FLOATS[dtype]),
-                scratch.data_ptr() if need else None, need, device_state(device).status.data_ptr(), _stream(device)))
+                scratch.data_ptr() if need else None, need, _status(device), _stream(device)))
     return out if len(lead) == 1 else out.reshape(*lead, n)
 
 
@@ -324,7 +331,7 @@ def int8_feed_forward(x: Tensor | QuantRows, gate_up: Int8Weight, down: Int8Weig
             scratch = torch.empty(need, dtype=torch.uint8, device=device)
             _lib.check(lib.dmoe_int8_feed_forward(
                 floats, quant, rows, gate_up.desc, down.desc, act, _desc(add) if add is not None else None,
-                _lib.Rows(out.data_ptr(), n, code), scratch.data_ptr(), need, device_state(device).status.data_ptr(),
+                _lib.Rows(out.data_ptr(), n, code), scratch.data_ptr(), need, _status(device),
                 _stream(device)))
     return out if len(lead) == 1 else out.reshape(*lead, n)
 
@@ -332,11 +339,16 @@ def int8_feed_forward(x: Tensor | QuantRows, gate_up: Int8Weight, down: Int8Weig
 class Int8Linear(torch.nn.Module):
     """Dense linear on 8-bit integers: ``weight`` int8 [N, K] with fp32
     ``scales`` [N] and an optional ``bias`` [N]; ``forward`` takes rows
-    [..., K] or ``QuantRows`` (so one norm's output serves several).  The
+    [..., K] or ``QuantRows`` (so one norm's output serves several), and
+    ``dtype`` is what ``QuantRows`` give where the call does not say.  The
     buffer ``qweight`` has K rounded up to a multiple of 16."""
 
-    def __init__(self, weight: Tensor, scales: Tensor, bias: Tensor | None = None, *, device=None):
+    def __init__(self, weight: Tensor, scales: Tensor, bias: Tensor | None = None, *, device=None,
+                 dtype: torch.dtype = torch.bfloat16):
         super().__init__()
+        if dtype not in _FLOATS:
+            raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
+        self.dtype = dtype
         device = weight.device if device is None else torch.device(device)
         held = Int8Weight(weight.to(device), scales.to(device))
         self.out_features, self.in_features = held.shape
@@ -350,39 +362,44 @@ class Int8Linear(torch.nn.Module):
         return Int8Weight(self.qweight[:, :self.in_features], self.scales)
 
     @classmethod
-    def from_linear(cls, linear: torch.nn.Linear, *, device=None) -> Int8Linear:
+    def from_linear(cls, linear: torch.nn.Linear, *, device=None, dtype: torch.dtype = torch.bfloat16) -> Int8Linear:
         """The nearest 8-bit integers of a float linear."""
         held = Int8Weight.quantize(linear.weight)
-        return cls(held.values, held.scales, linear.bias, device=device)
+        return cls(held.values, held.scales, linear.bias, device=device, dtype=dtype)
 
     def forward(self, x: Tensor | QuantRows, *, residual: Tensor | None = None, dtype: torch.dtype | None = None) -> Tensor:
+        if dtype is None and residual is None and isinstance(x, QuantRows):
+            dtype = self.dtype
         return int8_linear(x, self._weight(), bias=self.bias, residual=residual, dtype=dtype)
 
 
 class Int8FeedForward(torch.nn.Module):
     """Gated feed-forward block on 8-bit integers: ``gate_up`` int8 [2 * I, K]
-    (gate rows first), ``down`` int8 [N, I], each with its fp32 scales."""
+    (gate rows first), ``down`` int8 [N, I], each with its fp32 scales; ``dtype``
+    as ``Int8Linear``'s."""
 
     def __init__(self, gate_up: Tensor, gate_up_scales: Tensor, down: Tensor, down_scales: Tensor, *,
-                 activation: str = "silu", device=None):
+                 activation: str = "silu", device=None, dtype: torch.dtype = torch.bfloat16):
         super().__init__()
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")
         if gate_up.ndim != 2 or down.ndim != 2 or gate_up.shape[0] != 2 * down.shape[1]:
             raise ValueError("gate_up must be [2 * I, K] for down [N, I]")
         self.activation = activation
-        self.gate_up = Int8Linear(gate_up, gate_up_scales, device=device)
-        self.down = Int8Linear(down, down_scales, device=device)
+        self.gate_up = Int8Linear(gate_up, gate_up_scales, device=device, dtype=dtype)
+        self.down = Int8Linear(down, down_scales, device=device, dtype=dtype)
 
     @classmethod
     def from_linears(cls, gate: torch.nn.Linear, up: torch.nn.Linear, down: torch.nn.Linear, *, activation: str = "silu",
-                     device=None) -> Int8FeedForward:
+                     device=None, dtype: torch.dtype = torch.bfloat16) -> Int8FeedForward:
         """The nearest 8-bit integers of a float block's three linears, which have no bias."""
         if any(linear.bias is not None for linear in (gate, up, down)):
             raise ValueError("the linears of a gated feed-forward block have no bias here")
         w, v = Int8Weight.quantize(torch.cat([gate.weight, up.weight])), Int8Weight.quantize(down.weight)
-        return cls(w.values, w.scales, v.values, v.scales, activation=activation, device=device)
+        return cls(w.values, w.scales, v.values, v.scales, activation=activation, device=device, dtype=dtype)
 
     def forward(self, x: Tensor | QuantRows, *, residual: Tensor | None = None, dtype: torch.dtype | None = None) -> Tensor:
+        if dtype is None and residual is None and isinstance(x, QuantRows):
+            dtype = self.down.dtype
         return int8_feed_forward(x, self.gate_up._weight(), self.down._weight(), activation=self.activation,
                                  residual=residual, dtype=dtype)

@@ -21,8 +21,7 @@ from torch import Tensor
 from . import _lib
 from .attention import _no_gradients, _on, _stream
 from .int8 import (_FLOATS, E4M3, E4M3_GROUP, GROUP, INT8, QuantRows, _check_float, _check_sizes, _desc, _flat, _gpu,
-                   _same_device)
-from .offload import device_state
+                   _same_device, _status)
 
 QUANT_FORMATS = {"int8": INT8, "fp8": E4M3, "fp8-128": E4M3_GROUP}
 
@@ -85,7 +84,7 @@ def rms_norm(x: Tensor, weight: Tensor, *, residual: Tensor | None = None, eps: 
                 _desc(flat), _desc(add) if add is not None else None, count, cols, weight.data_ptr(),
                 _FLOATS[weight.dtype], offset, eps, _lib.Rows(hidden.data_ptr(), cols, code) if add is not None else None,
                 _lib.Rows(y.data_ptr(), cols, code) if rows else None, q.desc if q is not None else None,
-                device_state(device).status.data_ptr(), _stream(device)))
+                _status(device), _stream(device)))
     if len(shape) != 2:
         if add is not None:
             hidden = hidden.view(shape)

@@ -9,6 +9,8 @@ import torch
 
 import rows8_reference as ref
 from drama_moe import _lib
+from drama_moe.attention import KvCache4, PagedBatch
+from drama_moe.block import AttentionBlock, DenseBlock
 from drama_moe.int8 import (Int8FeedForward, Int8Linear, Int8Weight, QuantRows, int8_feed_forward, int8_linear,
                             quantize_rows)
 from drama_moe.norm import RmsNorm, rms_norm
@@ -295,3 +297,32 @@ def test_reference_feed_forward_brackets_a_plain_one():
     c, s = ref.int8(ref.through(ref.act(first[:, :48], "silu")[0] * first[:, 48:], BF16))
     out, _ = ref.product(c, s, v, vs)
     assert (low <= out).all() and (out <= high).all()
+
+
+# ------------------------------------------------------------------ blocks
+
+def test_dense_block_refusals():
+    ffn = Int8FeedForward(i8(8, 32), torch.ones(8), i8(32, 4), torch.ones(32))
+    with pytest.raises(ValueError, match="one width"):
+        DenseBlock(RmsNorm(torch.ones(31), quant="int8"), ffn)
+    with pytest.raises(ValueError, match="one width"):
+        DenseBlock(RmsNorm(torch.ones(32)), Int8FeedForward(i8(8, 32), torch.ones(8), i8(33, 4), torch.ones(33)))
+    with pytest.raises(ValueError, match="rows or 8-bit integers"):
+        DenseBlock(RmsNorm(torch.ones(32), quant="fp8"), ffn)
+    block = DenseBlock(RmsNorm(torch.ones(32), quant="int8"), ffn)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        block(torch.zeros(2, 32))
+
+
+def test_attention_block_takes_rows_in_8_bits_for_8_bit_projections_only():
+    cache = KvCache4.allocate(4, 2, 64, page_size=16, device="cpu")
+    batch = PagedBatch(torch.ones(2, 2).int(), torch.ones(2).int())
+    x, residual = QuantRows(i8(2, 32), torch.ones(2)), torch.zeros(2, 32)
+    linear = [torch.nn.Linear(32, 256), torch.nn.Linear(32, 128), torch.nn.Linear(32, 128), torch.nn.Linear(256, 32)]
+    with torch.no_grad(), pytest.raises(ValueError, match="needs Int8Linear projections"):
+        AttentionBlock(*linear, cache, heads=4)(x, residual, batch)
+    with pytest.raises(ValueError, match="attn_input and residual"):
+        AttentionBlock(*linear, cache, heads=4)(x, residual[:, :16], batch)
+    eight = [Int8Linear.from_linear(m) for m in linear]
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        AttentionBlock(*eight, cache, heads=4)(x, residual, batch)
