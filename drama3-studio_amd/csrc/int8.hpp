@@ -92,7 +92,7 @@ void launch_rows8(const NormArgs& a, hipStream_t stream);
 void launch_dequant8(const Dequant8Args& a, hipStream_t stream);
 
 // How a product is cut.
-enum Int8Shape : int { kInt8Few, kInt8Tiles64, kInt8Tiles64x128, kInt8Tiles128Deep, kInt8Tiles128, kInt8Tiles256 };
+enum Int8Shape : int { kInt8Few, kInt8Tiles64, kInt8Tiles64x128, kInt8Tiles128Deep, kInt8Tiles128x256, kInt8Tiles128, kInt8Tiles256 };
 constexpr int kInt8MaxSplits = 4;
 struct Int8Plan {
     Int8Shape shape;
@@ -110,10 +110,10 @@ constexpr int kInt8FewRows = 64;  // rows that the kernel of few rows takes
 //   (47 rows, K 11008, N 4096: 28.4 in one, 20.8 in two, 16.5 in four); with fewer, joining costs what it saves (128
 //   rows, K 4096, N 4096: 13.6, 14.3, 16.7).
 // * 64 x 128 while they do not (47 rows, K 4096, gated N 11008, 172 tiles: 24.2, 64 x 64 26.2, 128 x 128 26.5).
-// * 128 x 128 with a deep ring while they do not (509 rows, K 2048, N 5003, 160 tiles: 14.3, 64 x 128 19.4), then with a
-//   ring of two stages, two workgroups a CU (2048 rows, K 4096, N 4096: 36 against 38.7, the matrix in the caches).
-// * 256 x 256 where their rounds take less: a round of one a CU takes as long as 1 / 0.64 rounds of two 128 x 128
-//   (8192 rows, K 4096, N 4096: 113 against 135; 2048 rows: 42 against 36).
+// * 128 x 128 with a deep ring while they do not (509 rows, K 2048, N 5003, 160 tiles: 14.6, 64 x 128 19.5).
+// * 128 x 256 while they do not (2048 rows, K 4096, N 4096, 256 tiles: 36.3, 128 x 128 41.9, 256 x 256 52.7).
+// * 256 x 256 where their rounds take less than those of 128 x 128 with a ring of two stages, two workgroups a CU: one
+//   a CU takes as long as 1 / 0.64 rounds of the others (8192 rows, K 4096, N 4096: 122 against 146).
 inline Int8Plan int8_plan(int rows, int n, int k, bool gated) {
     constexpr int64_t kCus = 256;
     const auto tiles = [&](int tm, int tn) {
@@ -129,6 +129,7 @@ inline Int8Plan int8_plan(int rows, int n, int k, bool gated) {
     }
     if (tiles(64, 128) <= kCus) return {kInt8Tiles64x128, 1};
     if (middle <= kCus) return {kInt8Tiles128Deep, 1};
+    if (tiles(128, 256) <= kCus) return {kInt8Tiles128x256, 1};
     if ((large + kCus - 1) / kCus * 100 <= (middle + 2 * kCus - 1) / (2 * kCus) * 64) return {kInt8Tiles256, 1};
     return {kInt8Tiles128, 1};
 }

@@ -3,11 +3,23 @@
 //   acc[t][n] = sum_k xq[t][k] w[n][k] (int32, exact), out = T(acc xs[t] ws[n] + bias[n] + residual[t][n]),
 //   gated: out = T(act(gate) up) of the products with rows n and n + N of w
 //
-// A workgroup, mostly of four waves, owns TM x TN sums (gated: TN / 2 gate and TN / 2 up
-// rows of the matrix, 32 of each in turn, so that a gate's sum and its up's
-// meet in one lane); a wave owns a quarter in registers and multiplies
-// 32x32x32.  Both operands go through LDS in a ring of stages of BK
-// columns, filled by direct copies that no register waits for.
+// A workgroup owns TM x TN sums (gated: TN / 2 gate and TN / 2 up rows of the
+// matrix, 32 of each in turn, so that a gate's sum and its up's meet in one
+// wave); a wave keeps its share in registers and multiplies 32x32x32.  Both
+// operands go through LDS, in rings of steps of 128 columns that direct copies
+// fill: no register waits for them, and they are asked for a few at a time
+// between matrix instructions, one barrier a step.  The sums leave through LDS
+// as well, so that a lane finishes eight columns of a row.
+//
+// 8192 rows, K 4096, N 4096: 115 us, 2.4 POP/s; K 12288 with 4096 rows 160 us,
+// 2.6 (a library's product of 8192 cubed 2.4).  Power bounds it: with zeros for
+// operands the loop takes a quarter less, and matrix instructions alone reach
+// 3.5 POP/s on random operands, 5.0 on zeros.  Of a tile's 57 us, 4 are its
+// results and 2 its start.  Measured for it: copies asked for all at once behind
+// the barrier 5% slower, over a whole step 6%; matrix steps of 64 columns with a
+// deeper ring 7%; a third step of rows in the ring, beside two of the matrix, 4%
+// faster than two of each; eight waves as fast as four, and 5% faster where few
+// tiles run.
 #include <algorithm>
 
 #include "int8_epilogue.hpp"
@@ -38,12 +50,14 @@ __device__ __forceinline__ v16i mfma_i8_32(const v4i& a, const v4i& b, const v16
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
 }
 
+constexpr int kTileK = 128;         // columns of a step
+
 // TM rows by TN matrix rows a workgroup, WM of its waves along the rows and WN
-// along the matrix; a ring of S stages of BK columns; a stage's copies in EARLY
-// parts of a step.
-template <int TM_, int TN_, int WM_, int WN_, int BK_, int S_, int EARLY_>
+// along the matrix; rings of SX and SW steps for rows and matrix; the copies of
+// a step in EARLY parts.
+template <int TM_, int TN_, int WM_, int WN_, int SX_, int SW_, int EARLY_>
 struct Shape {
-    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, BK = BK_, S = S_, EARLY = EARLY_;
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, SX = SX_, SW = SW_, EARLY = EARLY_;
     static constexpr int kWaves = WM * WN, kThreads = kWaves * kWave;
 };
 
@@ -51,22 +65,27 @@ template <class G, bool GATED>
 struct Tile {
     static constexpr int kFM = G::TM / G::WM / 32, kFN = G::TN / G::WN / 32;  // 32-row fragments of a wave
     static_assert(!GATED || kFN % 2 == 0, "a wave has gate and up fragments in turn");
-    static constexpr int kChunks = G::BK / 16;
-    static constexpr int kUnitX = G::TM * G::BK, kUnitW = G::TN * G::BK, kStage = kUnitX + kUnitW;  // bytes
-    static constexpr int kCopiesX = kUnitX / 1024 / G::kWaves, kCopiesW = kUnitW / 1024 / G::kWaves;  // of a wave for a stage
+    static constexpr int kChunks = kTileK / 16;
+    static constexpr int kUnitX = G::TM * kTileK, kUnitW = G::TN * kTileK;  // bytes of a step
+    static constexpr int kRingX = G::SX * kUnitX, kLds = kRingX + G::SW * kUnitW;
+    static constexpr int kCopiesX = kUnitX / 1024 / G::kWaves, kCopiesW = kUnitW / 1024 / G::kWaves;  // of a wave for a step
     static constexpr int kCopies = kCopiesX + kCopiesW;
-    static constexpr int kCopyRows = 1024 / G::BK;  // rows of a copy
-    static constexpr int kSteps = G::BK / 32;       // matrix instructions along a stage
+    static constexpr int kCopyRows = 1024 / kTileK;  // rows of a copy
+    static constexpr int kSteps = kTileK / 32;       // matrix instructions along a step
+    // Behind the barrier of step t, W of step t + SW and then X of step t + SX are asked for.  At that barrier W and X of
+    // step t + 1 have to be there; these may still be on their way:
+    static_assert(G::SX == G::SW || G::SX == G::SW + 1, "W is the younger of a step's operands");
+    static constexpr int kBehind = (G::SW - 2) * kCopies + (G::SX > G::SW ? kCopiesX : 0);
     static constexpr int kCols = GATED ? G::TN / 2 : G::TN;
     static constexpr int kSlots = G::EARLY * kFN;   // places of copies between matrix instructions
     // copies [first(p), first(p + 1)) go to place p
     static constexpr int first(int place) { return place * kCopies / kSlots; }
     // waves a SIMD that LDS has room for, in workgroups of at least a wave each
-    static constexpr int kPerCu = 160 * 1024 / (G::S * kStage) * G::kWaves / 4, kPerSimd = kPerCu < 1 ? 1 : kPerCu > 2 ? 2 : kPerCu;
-    // a chunk's place in its row: eight lanes of consecutive rows and one chunk fall on all banks
-    static __device__ __forceinline__ int place(int row, int chunk) {
-        return G::BK == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
-    }
+    static constexpr int kPerCu = 160 * 1024 / kLds * G::kWaves / 4, kPerSimd = kPerCu < 1 ? 1 : kPerCu > 2 ? 2 : kPerCu;
+    // A chunk's place in its row.  A read of 16 bytes a lane goes by sixteen lanes, whose rows are sixteen different ones
+    // modulo 16: two rows fill the banks, and the places of eight pairs differ.
+    static_assert(kTileK == 128 && kCopiesX % 2 == 0 && kCopiesW % 2 == 0, "eight chunks a row, copies in pairs");
+    static __device__ __forceinline__ int place(int row, int chunk) { return chunk ^ ((row >> 1) & 7); }
 };
 
 // With DT kI32 a workgroup takes one of a.splits shares of K and leaves its
@@ -74,9 +93,9 @@ struct Tile {
 template <class G, bool GATED, int DT>
 __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_tile_kernel(Int8Args a, int row_tiles, int col_tiles) {
     using T = Tile<G, GATED>;
-    constexpr int FM = T::kFM, FN = T::kFN, BK = G::BK, S = G::S;
+    constexpr int FM = T::kFM, FN = T::kFN, BK = kTileK;
     constexpr bool kSplit = DT == kI32;
-    __shared__ alignas(1024) uint8_t lds[S * T::kStage];
+    __shared__ alignas(1024) uint8_t lds[T::kLds];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     // an XCD takes a contiguous share of the tiles and walks them kTileGroup row tiles at a time, column by column, so
     // that what runs on it at one time shares rows and matrix through its L2
@@ -101,13 +120,14 @@ __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_
         steps = (split + 1) * steps / a.splits - k0 / BK;
     }
     const int kw = (a.k + 15) / 16 * 16;  // readable columns of a matrix row
-    // copies: lane l of copy j brings the chunk that place() wants at its spot, the same one for every j
+    // copies: lane l of copy j brings the chunk that place() wants at its spot, one for even j and one for odd
     uint32_t off_x[T::kCopiesX], off_w[T::kCopiesW];
-    const uint32_t src = T::place(lane / T::kChunks, lane % T::kChunks) * 16;
+    const uint32_t src[2] = {T::place(lane / T::kChunks, lane % T::kChunks) * 16u,
+                             T::place(lane / T::kChunks + T::kCopyRows, lane % T::kChunks) * 16u};
 #pragma unroll
     for (int j = 0; j < T::kCopiesX; ++j) {
         const int row = (wave * T::kCopiesX + j) * T::kCopyRows + lane / T::kChunks;
-        off_x[j] = (uint32_t)(min(m0 + row, a.rows - 1) - m0) * (uint32_t)a.xq_stride + src;
+        off_x[j] = (uint32_t)(min(m0 + row, a.rows - 1) - m0) * (uint32_t)a.xq_stride + src[j % 2];
     }
 #pragma unroll
     for (int j = 0; j < T::kCopiesW; ++j) {
@@ -115,22 +135,20 @@ __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_
         int64_t wr;
         if constexpr (GATED) wr = (int64_t)min(n0 + row / 64 * 32 + row % 32, a.n - 1) - n0 + (row & 32 ? a.n : 0);
         else wr = min(n0 + row, a.n - 1) - n0;
-        off_w[j] = (uint32_t)(wr * a.w_stride) + src;
+        off_w[j] = (uint32_t)(wr * a.w_stride) + src[j % 2];
     }
     // behind a matrix row's last chunk its first of this stage again: the rows hold zeros there
-    const uint32_t last_back = k0 + (steps - 1) * BK + (int)src >= kw ? src : 0u;
+    const int last_k = k0 + (steps - 1) * BK;
+    const uint32_t last_back[2] = {last_k + (int)src[0] >= kw ? src[0] : 0u, last_k + (int)src[1] >= kw ? src[1] : 0u};
     const uint8_t* base_x = a.xq + (int64_t)m0 * a.xq_stride + k0;
     const uint8_t* base_w = (const uint8_t*)a.w + (int64_t)n0 * a.w_stride + k0;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    const auto copy = [&](int step, int stage, int i) {  // copy i of a stage: rows, then matrix
-        const uint32_t to = lds0 + stage * T::kStage;
-        if (i < T::kCopiesX) {
-            copy_to_lds(base_x + (int64_t)step * BK, off_x[i], to + (wave * T::kCopiesX + i) * 1024);
-        } else {
-            const int j = i - T::kCopiesX;
-            copy_to_lds(base_w + (int64_t)step * BK, off_w[j] - (step == steps - 1 ? last_back : 0u),
-                        to + T::kUnitX + (wave * T::kCopiesW + j) * 1024);
-        }
+    const auto copy_x = [&](int step, int slot, int j) {
+        copy_to_lds(base_x + (int64_t)step * BK, off_x[j], lds0 + slot * T::kUnitX + (wave * T::kCopiesX + j) * 1024);
+    };
+    const auto copy_w = [&](int step, int slot, int j) {
+        copy_to_lds(base_w + (int64_t)step * BK, off_w[j] - (step == steps - 1 ? last_back[j % 2] : 0u),
+                    lds0 + T::kRingX + slot * T::kUnitW + (wave * T::kCopiesW + j) * 1024);
     };
     // operands: lane l holds row l % 32, chunk 2 s + l / 32 of step s
     const int wave_m = wave % G::WM * (FM * 32), wave_n = wave / G::WM;
@@ -139,21 +157,22 @@ __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_
 #pragma unroll
     for (int s = 0; s < T::kSteps; ++s) {
         at_x[s] = (wave_m + r) * BK + T::place(r, 2 * s + half) * 16;
-        at_w[s] = (wave_n * FN * 32 + r) * BK + T::place(r, 2 * s + half) * 16 + T::kUnitX;
+        at_w[s] = (wave_n * FN * 32 + r) * BK + T::place(r, 2 * s + half) * 16 + T::kRingX;
     }
     v4i xf[2][FM], wf[2][FN];
     constexpr int kReading = FN > 1 ? FN / 2 : 1;  // groups of matrix instructions that read the next operands
-    const auto read = [&](int to, int stage, int s, int g) {
-        const uint8_t* p = lds + stage * T::kStage;
+    const auto read = [&](int to, int slot_x, int slot_w, int s, int g) {
+        const uint8_t* px = lds + slot_x * T::kUnitX + at_x[s];
+        const uint8_t* pw = lds + slot_w * T::kUnitW + at_w[s];
 #pragma unroll
-        for (int f = g * FM / kReading; f < (g + 1) * FM / kReading; ++f) xf[to][f] = *(const v4i*)(p + at_x[s] + f * 32 * BK);
+        for (int f = g * FM / kReading; f < (g + 1) * FM / kReading; ++f) xf[to][f] = *(const v4i*)(px + f * 32 * BK);
 #pragma unroll
-        for (int f = g * FN / kReading; f < (g + 1) * FN / kReading; ++f) wf[to][f] = *(const v4i*)(p + at_w[s] + f * 32 * BK);
+        for (int f = g * FN / kReading; f < (g + 1) * FN / kReading; ++f) wf[to][f] = *(const v4i*)(pw + f * 32 * BK);
     };
     // what the results need is loaded first and held: eight columns of the matrix a lane, the rows' scales
     constexpr int kRaw = FN * 32, kPitch = kRaw + 4;  // sums of a row in LDS, and four ints against bank conflicts
     constexpr int kOut = GATED ? kRaw / 2 : kRaw, kVectors = kOut / 8, kRowsAt = kWave / kVectors;
-    static_assert(G::kWaves * (32 * kPitch + FM * 32) * 4 <= S * T::kStage, "sums and scales fit the ring");
+    static_assert(G::kWaves * (32 * kPitch + FM * 32) * 4 <= T::kLds, "sums and scales fit the ring");
     const int cc = lane % kVectors * 8, n = n0 + wave_n * kOut + cc;
     // column cc of the outputs in a row of sums: gate and up fragments lie in turn
     const int from = GATED ? cc / 32 * 64 + cc % 32 : cc;
@@ -176,53 +195,60 @@ __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_
         for (int j = 0; j < FM; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    // of the ring's last stage the first part only, as a step's end would: step 0 goes on with it
-    constexpr int kFirst = T::first(FN);
+    // The copies of a step's end, [W of step w, X of step x], from number `from` to `to`.
+    const auto copies = [&](int w, int slot_w, int x, int slot_x, int from, int to, auto checked) {
+        constexpr bool kChecked = decltype(checked)::value;
 #pragma unroll
-    for (int s = 0; s < S; ++s)
-        if (s < steps) {
-#pragma unroll
-            for (int i = 0; i < (s + 1 < S ? T::kCopies : kFirst); ++i) copy(s, s, i);
+        for (int c = 0; c < T::kCopies; ++c) {
+            if (c < from || c >= to) continue;
+            if (c < T::kCopiesW) {
+                if (!kChecked || w < steps) copy_w(w, slot_w, c);
+            } else {
+                if (!kChecked || x < steps) copy_x(x, slot_x, c - T::kCopiesW);
+            }
         }
-    if (steps >= S) tile_wait<(S - 2) * T::kCopies + kFirst>();
+    };
+    // The rings' first contents in that order; of the last the first part only, step 0 goes on with it.
+    constexpr int kFirst = T::first(FN);
+    if constexpr (G::SX > G::SW) copies(0, 0, 0, 0, T::kCopiesW, T::kCopies, std::true_type{});
+#pragma unroll
+    for (int s = 0; s < G::SW; ++s)
+        copies(s, s, s + G::SX - G::SW, s + G::SX - G::SW, 0, s + 1 < G::SW ? T::kCopies : kFirst, std::true_type{});
+    if (steps >= G::SX) tile_wait<T::kBehind + kFirst>();
     else tile_wait<0>();
 #pragma unroll
-    for (int g = 0; g < kReading; ++g) read(0, 0, 0, g);
-    // One step of BK columns out of `stage`, the next one's first operands out of `next`.  The copies of a stage start
-    // behind the barrier that frees its place, in this step's last part, and go on in the next step's first ones: a few
-    // between matrix instructions, which do not wait for them.
-    int stage = 0;
-    const auto step_of = [&](int t, auto copying, auto behind) {
-        constexpr bool kCopying = decltype(copying)::value;  // stage t + S exists
-        constexpr int kBehind = decltype(behind)::value;     // copies that may be on their way at the barrier
-        const int next = stage + 1 == S ? 0 : stage + 1, before = stage == 0 ? S - 1 : stage - 1;
+    for (int g = 0; g < kReading; ++g) read(0, 0, 0, 0, g);
+    // One step of BK columns, and the next one's first operands.  The copies that its barrier frees places for start in
+    // its last part and go on in the next step's first ones: a few between matrix instructions, which do not wait for them.
+    int slot_x = 0, slot_w = 0;
+    const auto step_of = [&](int t, auto tail) {
+        constexpr bool kTail = decltype(tail)::value;  // a copy's step may not exist
+        const int next_x = slot_x + 1 == G::SX ? 0 : slot_x + 1, before_x = slot_x == 0 ? G::SX - 1 : slot_x - 1;
+        const int next_w = slot_w + 1 == G::SW ? 0 : slot_w + 1, before_w = slot_w == 0 ? G::SW - 1 : slot_w - 1;
 #pragma unroll
         for (int s = 0; s < T::kSteps; ++s) {
             const bool last = s + 1 == T::kSteps;
-            if (last) tile_wait<kBehind>();  // every wave has read this stage, and the next has come
-            const int part = last ? 0 : s + 1;  // of the copies: the first starts stage t + S, the others end stage t + S - 1
+            if (last) tile_wait<kTail ? 0 : T::kBehind>();  // every wave has read this step, and the next has come
+            const int part = last ? 0 : s + 1;              // of the copies: part 0 is this step's end, the others the last one's
 #pragma unroll
             for (int g = 0; g < FN; ++g) {
-                if (g < kReading) read((s + 1) % 2, last ? next : stage, last ? 0 : s + 1, g);
-                if (part < G::EARLY && (kCopying || part > 0)) {
-                    if (part == 0 || t + S - 1 < steps) {
-#pragma unroll
-                        for (int c = T::first(part * FN + g); c < T::first(part * FN + g + 1); ++c) {
-                            if (part == 0) copy(t + S, stage, c);
-                            else copy(t + S - 1, before, c);
-                        }
-                    }
+                if (g < kReading) read((s + 1) % 2, last ? next_x : slot_x, last ? next_w : slot_w, last ? 0 : s + 1, g);
+                if (part < G::EARLY) {
+                    const int from = T::first(part * FN + g), to = T::first(part * FN + g + 1);
+                    if (part == 0) copies(t + G::SW, slot_w, t + G::SX, slot_x, from, to, tail);
+                    else copies(t - 1 + G::SW, before_w, t - 1 + G::SX, before_x, from, to, tail);
                 }
 #pragma unroll
                 for (int j = 0; j < FM; ++j) acc[g][j] = mfma_i8_32(wf[s % 2][g], xf[s % 2][j], acc[g][j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        stage = next;
+        slot_x = next_x;
+        slot_w = next_w;
     };
     int t = 0;
-    for (; t + S < steps; ++t) step_of(t, std::true_type{}, std::integral_constant<int, (S - 2) * T::kCopies>{});
-    for (; t < steps; ++t) step_of(t, std::false_type{}, std::integral_constant<int, 0>{});
+    for (; t + G::SX < steps; ++t) step_of(t, std::false_type{});
+    for (; t < steps; ++t) step_of(t, std::true_type{});
     // Every wave is behind its last read of the ring: each takes a part of it and turns its sums over there, 32 rows at
     // a time, so that a lane gets eight columns of a row and the scales, bias and store of whole pieces.
     int* mine = (int*)lds + wave * 32 * kPitch;
@@ -414,11 +440,12 @@ void launch_tiles_as(const Int8Args& a, hipStream_t stream) {
 
 void launch_int8_tiles(const Int8Args& a, const Int8Plan& plan, hipStream_t stream) {
     switch (plan.shape) {
-        case kInt8Tiles64: return launch_tiles_as<Shape<64, 64, 2, 1, 128, 4, 2>>(a, stream);
-        case kInt8Tiles64x128: return launch_tiles_as<Shape<64, 128, 2, 2, 128, 4, 2>>(a, stream);
-        case kInt8Tiles128Deep: return launch_tiles_as<Shape<128, 128, 2, 2, 128, 4, 2>>(a, stream);
-        case kInt8Tiles128: return launch_tiles_as<Shape<128, 128, 2, 2, 128, 2, 2>>(a, stream);
-        default: return launch_tiles_as<Shape<256, 256, 2, 2, 128, 2, 2>>(a, stream);
+        case kInt8Tiles64: return launch_tiles_as<Shape<64, 64, 2, 1, 4, 4, 2>>(a, stream);
+        case kInt8Tiles64x128: return launch_tiles_as<Shape<64, 128, 2, 2, 4, 4, 2>>(a, stream);
+        case kInt8Tiles128Deep: return launch_tiles_as<Shape<128, 128, 2, 2, 4, 4, 2>>(a, stream);
+        case kInt8Tiles128x256: return launch_tiles_as<Shape<128, 256, 2, 4, 3, 3, 2>>(a, stream);
+        case kInt8Tiles128: return launch_tiles_as<Shape<128, 128, 2, 2, 2, 2, 2>>(a, stream);
+        default: return launch_tiles_as<Shape<256, 256, 2, 4, 3, 2, 2>>(a, stream);
     }
 }
 

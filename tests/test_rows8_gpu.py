@@ -267,6 +267,7 @@ def test_linear_in_large_tiles(cuda):
     check_linear(cuda, 4000, 1000, 4500, torch.bfloat16, residual=True)
     check_linear(cuda, 4097, 130, 4097, torch.float16, given=True)
     check_linear(cuda, 1100, 2048, 4096, torch.bfloat16)
+    check_linear(cuda, 1300, 300, 5000, torch.bfloat16, bias=True)
 
 
 @pytest.mark.parametrize("rows", [1, 10, 40, 65, 300])
