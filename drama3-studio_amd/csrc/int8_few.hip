@@ -228,7 +228,7 @@ bool int8_few_quantizes(int rows, int k) {
 // workgroup a CU (13 rows, K 4096, N 4096: 8.0 us against 6.6).
 void launch_int8_few(const Int8Args& a, hipStream_t stream) {
     if (a.gated) launch_few_of<2, 8, true>(a, stream);
-    else if (a.n <= 16 * 192) launch_few_of<1, 16, false>(a, stream);
+    else if (a.n <= 16 * 160) launch_few_of<1, 16, false>(a, stream);
     else launch_few_of<1, 8, false>(a, stream);
 }
 

@@ -68,8 +68,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
             int m = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                // squares of 16-bit types are exact in 32 bits
-                sum += DT == kF32 ? (double)u[v][j] * (double)u[v][j] : (double)(u[v][j] * u[v][j]);
+                sum = __builtin_fma((double)u[v][j], (double)u[v][j], sum);
                 u[v][j] *= a.offset + g[j];
                 m = max(m, magnitude(u[v][j]));
             }
@@ -102,11 +101,12 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
     if (NORM && a.y) {
         char* y = (char*)a.y + row * a.y_stride * kBytes;
         const float r = (float)by;
+        const bool plain = by > 0x1p-120 && by < 0x1p120;  // elsewhere r is no normal number or soon none
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float o[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = u[v][j] * r;
+            for (int j = 0; j < 8; ++j) o[j] = plain ? u[v][j] * r : (float)((double)u[v][j] * by);
             store_cols8<DT>(y, (v * T + t) * 8, a.cols, o);
         }
     }
@@ -145,12 +145,30 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
     }
 }
 
+// A launch holds fewer than 2^32 threads; more rows take several.
+constexpr int kRowsOfLaunch = 1 << 21;
+
 template <int DT, int T, int V>
-void launch_rows8_as(const NormArgs& a, hipStream_t stream) {
-    const int per = T < 256 ? 256 / T : 1;
-    const dim3 grid((unsigned)((a.rows + per - 1) / per)), block(T < 256 ? 256 : T);
-    if (a.weight) hipLaunchKernelGGL((rows8_kernel<DT, T, V, true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((rows8_kernel<DT, T, V, false>), grid, block, 0, stream, a);
+void launch_rows8_as(NormArgs a, hipStream_t stream) {
+    const int per = T < 256 ? 256 / T : 1, all = a.rows;
+    const dim3 block(T < 256 ? 256 : T);
+    const auto move = [](auto*& p, int64_t bytes) {
+        if (p) p = (std::remove_reference_t<decltype(p)>)((char*)p + bytes);
+    };
+    for (int at = 0;; at += kRowsOfLaunch) {
+        a.rows = std::min(all - at, kRowsOfLaunch);
+        const dim3 grid((unsigned)((a.rows + per - 1) / per));
+        if (a.weight) hipLaunchKernelGGL((rows8_kernel<DT, T, V, true>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((rows8_kernel<DT, T, V, false>), grid, block, 0, stream, a);
+        if (all - at <= kRowsOfLaunch) return;
+        constexpr int64_t kMoved = (int64_t)kRowsOfLaunch * elem_bytes<DT>();
+        move(a.x, a.x_stride * kMoved);
+        move(a.residual, a.residual_stride * kMoved);
+        move(a.hidden, a.hidden_stride * kMoved);
+        move(a.y, a.y_stride * kMoved);
+        move(a.q.q, a.q.stride * kRowsOfLaunch);
+        move(a.q.scales, (a.q.format == kRowsE4M3Group ? a.cols / 128 : 1) * (int64_t)kRowsOfLaunch * 4);
+    }
 }
 
 // Rows that do not fill the chip get more threads each: their time is a row's.
@@ -174,8 +192,8 @@ void launch_rows8_of(const NormArgs& a, hipStream_t stream) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void dequant8_kernel(Dequant8Args a, int per_row, int64_t total) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void dequant8_kernel(Dequant8Args a, int per_row, int64_t first, int64_t total) {
+    const int64_t i = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
     const int64_t row = i / per_row;
     const int col = (int)(i - row * per_row) * 8;
@@ -208,10 +226,14 @@ void launch_rows8(const NormArgs& a, hipStream_t stream) {
 void launch_dequant8(const Dequant8Args& a, hipStream_t stream) {
     const int per_row = (a.cols + 7) / 8;
     const int64_t total = (int64_t)a.rows * per_row;
-    const dim3 grid((unsigned)((total + 255) / 256)), block(256);
-    if (a.dtype == kBF16) hipLaunchKernelGGL(dequant8_kernel<kBF16>, grid, block, 0, stream, a, per_row, total);
-    else if (a.dtype == kF16) hipLaunchKernelGGL(dequant8_kernel<kF16>, grid, block, 0, stream, a, per_row, total);
-    else hipLaunchKernelGGL(dequant8_kernel<kF32>, grid, block, 0, stream, a, per_row, total);
+    constexpr int64_t kLaunch = (int64_t)1 << 31;  // threads: fewer than 2^32
+    for (int64_t first = 0; first < total; first += kLaunch) {
+        const dim3 grid((unsigned)((std::min(total - first, kLaunch) + 255) / 256)), block(256);
+        const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a, per_row, first, total); };
+        if (a.dtype == kBF16) go(dequant8_kernel<kBF16>);
+        else if (a.dtype == kF16) go(dequant8_kernel<kF16>);
+        else go(dequant8_kernel<kF32>);
+    }
 }
 
 }  // namespace dmoe

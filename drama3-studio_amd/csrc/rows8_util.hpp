@@ -16,7 +16,7 @@ struct __attribute__((packed, aligned(2))) Any16 {
 };
 
 template <int DT>
-__device__ __forceinline__ constexpr int elem_bytes() { return DT == kF32 ? 4 : 2; }
+__host__ __device__ __forceinline__ constexpr int elem_bytes() { return DT == kF32 ? 4 : 2; }
 
 // Eight columns of a row in its type.
 template <int DT>
@@ -238,7 +238,7 @@ __device__ __forceinline__ Units units_of(double by, float scale) { return {by, 
 __device__ __forceinline__ uint64_t int8_codes8(const float* u, const Units& by) {
     constexpr float kMagic = 12582912.0f;
     const float each = (float)by.each;
-    float t[8], close = 0.0f;
+    float t[8], close = __builtin_isinf(each) ? 0.5f : 0.0f;  // beyond 32 bits where all of a row lie below 2^-120
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         t[j] = __builtin_fmaf(u[j], each, kMagic);
@@ -283,7 +283,7 @@ __device__ __forceinline__ float round_to_odd(double d) {
 __device__ __forceinline__ uint64_t e4m3_codes8(const float* u, const Units& by) {
     const float each = (float)by.each;
     float f[8];
-    bool close = false;
+    bool close = __builtin_isinf(each);  // as above
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         f[j] = u[j] * each;

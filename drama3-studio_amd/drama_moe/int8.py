@@ -309,7 +309,7 @@ def int8_feed_forward(x: Tensor | QuantRows, gate_up: Int8Weight, down: Int8Weig
     (default as ``int8_linear``'s): ``gate_up`` [2 * I, K] holds the gate rows,
     then the up rows, ``down`` is [N, I].  The hidden rows are rounded to
     ``dtype`` and then to 8-bit integers with a scale a row; ``activation`` is
-    "silu" or "gelu_tanh"."""
+    "silu" or "gelu_tanh".  ``gate_up`` is smaller than 2 GiB."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")

@@ -42,8 +42,8 @@ def rms_norm(x: Tensor, weight: Tensor, *, residual: Tensor | None = None, eps: 
     x [..., columns] and residual have one type (bf16, fp16, fp32), weight
     [columns] any of them.  ``quant`` asks for y in 8 bits ("int8", "fp8",
     "fp8-128"), as rows of all leading dimensions; ``rows`` for y itself
-    (default: without ``quant``).  Sums are of 64 bits, y is rounded once, and
-    the codes are of y before that.  A row with an infinity or NaN gets codes
+    (default: without ``quant``).  Sums and roots are of 64 bits, products of 32,
+    and the codes are of y before its rounding to the rows' type.  A row with an infinity or NaN gets codes
     of 0 and a scale of NaN, and raises the device status bit."""
     fmt = None
     if quant is not None:

@@ -740,7 +740,7 @@ DMOE_API int dmoe_int8_linear(const DmoeRows* x, const DmoeQuantRows* quantized,
                               size_t workspace_bytes, int* status, void* stream);
 
 /* Gated feed-forward block: a = T(act(gate) * up) of the products with
- * gate_up [2 * inter, k] (gate rows first; act DMOE_ACT_SILU z / (1 + exp(-z)) or
+ * gate_up [2 * inter, k] (gate rows first, less than 2 GiB apart in all; act DMOE_ACT_SILU z / (1 + exp(-z)) or
  * DMOE_ACT_GELU_TANH), then out [rows, down->n] = T(product of a's 8-bit codes
  * with down [n, inter] + residual). */
 enum { DMOE_ACT_SILU = 0, DMOE_ACT_GELU_TANH = 1 };

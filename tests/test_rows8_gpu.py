@@ -8,6 +8,7 @@ import torch
 
 import rows8_reference as ref
 from conftest import print_case
+from drama_moe import _lib
 from drama_moe._lib import STATUS_NON_FINITE
 from drama_moe.int8 import (Int8FeedForward, Int8Linear, Int8Weight, QuantRows, int8_feed_forward, int8_linear,
                             quantize_rows)
@@ -420,3 +421,127 @@ def test_modules(cuda):
     made = norm(y, y)
     assert torch.equal(made.hidden, y + y) and made.rows is None
     assert torch.equal(block(made.quant, residual=made.hidden), block(made.quant, residual=made.hidden))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_norm_over_the_whole_range(cuda, dtype):
+    """Rows from the smallest to the largest numbers, whose squares and whose norms' factors pass 32 bits."""
+    print_case("norm range", dtype)
+    status(cuda)
+    g = torch.Generator().manual_seed(11)
+    sizes = (1e-44, 1e-39, 1e-37, 1e-30, 1e-25, 1e-10, 1.0, 1e15, 1e20, 1e30, 1e37)
+    x = torch.randn(len(sizes), 640, generator=g).clamp(-4, 4) * torch.tensor(sizes)[:, None]
+    x[0, 0] = x[1, 0] = 1e-38  # bf16 has no 1e-44
+    x = x.to(TYPES[dtype])
+    for gain in (1.0, 1e-6, 3.0):
+        weight = (torch.rand(640, generator=g) + 0.5) * gain
+        for eps in (0.0, 1e-60, 1e-6):
+            h, y = ref.norm(ref.wide(x), None, ref.wide(weight), TYPES[dtype], eps=eps)
+            for quant in ("int8", "fp8", "fp8-128"):
+                print_case("norm range", dtype, gain, eps, quant)
+                made = rms_norm(x.to(cuda), weight.to(cuda), eps=eps, quant=quant, rows=True)
+                near(made.rows, y, np.abs(y), TYPES[dtype])
+                same_rows8(made.quant, *(ref.int8(y) if quant == "int8" else ref.e4m3(y, 128 if quant == "fp8-128" else 640)))
+    assert status(cuda) == 0
+
+
+@pytest.mark.parametrize("cols", [8, 333, 1000, 2501, 9001])
+def test_outputs_in_their_inputs_places(cuda, cols):
+    """hidden in x's or residual's memory, a product's result in its residual's."""
+    print_case("in place", cols)
+    g = torch.Generator().manual_seed(cols)
+    lib, stream_of = _lib.library(), torch.cuda.current_stream(cuda).cuda_stream
+    desc = lambda t: _lib.Rows(t.data_ptr(), t.stride(0), _lib.dtype_code(t.dtype))  # noqa: E731
+    for dtype in TYPES.values():
+        for rows in (3, 700):
+            x, add = stream(rows, cols, dtype, g).to(cuda), stream(rows, cols, dtype, g).to(cuda)
+            weight = (torch.rand(cols, generator=g) + 0.5).to(cuda)
+            want = rms_norm(x, weight, residual=add)
+            for place in (0, 1):
+                both = [x.clone(), add.clone()]
+                out = torch.empty_like(x)
+                _lib.check(lib.dmoe_rms_norm(desc(both[0]), desc(both[1]), rows, cols, weight.data_ptr(), _lib.F32, 0.0, 1e-6,
+                                             desc(both[place]), desc(out), None, None, stream_of))
+                assert torch.equal(both[place], want.hidden) and torch.equal(out, want.rows)
+                assert torch.equal(both[1 - place], (x, add)[1 - place])
+    codes, scales = matrix(cols, 90, g)
+    weight = Int8Weight(codes.to(cuda), scales.to(cuda))
+    for rows in (2, 20, 70, 700):
+        x, add = quantize_rows(stream(rows, 90, torch.bfloat16, g).to(cuda)), stream(rows, cols, torch.bfloat16, g).to(cuda)
+        want = int8_linear(x, weight, residual=add)
+        need = lib.dmoe_int8_linear_workspace_bytes(rows, cols, 90, 1)
+        room = torch.empty(need + 256, dtype=torch.uint8, device=cuda)
+        _lib.check(lib.dmoe_int8_linear(None, x.desc, rows, weight.desc, None, desc(add), desc(add), room.data_ptr(), need, None,
+                                        stream_of))
+        assert torch.equal(add, want)
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """Rows, matrices, results and 8-bit rows of over 4 GiB: their ends are those of calls on the ends alone."""
+    print_case("linear with a matrix over 4 GiB")
+    n, k = 66000, 65536
+    codes = torch.randint(-128, 128, (n, k), dtype=torch.int8, device=cuda)
+    scales = torch.rand(n, device=cuda)
+    whole, end = Int8Weight(codes, scales), Int8Weight(codes[-300:], scales[-300:])
+    for rows in (1, 40, 70, 300):
+        x = torch.randn(rows, k, device=cuda)
+        assert torch.equal(int8_linear(x, whole)[:, -300:], int8_linear(x, end))
+    print_case("linear with rows over 4 GiB")
+    rows = codes[:, :k]  # in 8 bits
+    few = Int8Weight(codes[:130].clone(), scales[:130])
+    q = QuantRows(rows, scales)
+    assert q.values.data_ptr() == codes.data_ptr()
+    assert torch.equal(int8_linear(q, few)[-100:], int8_linear(QuantRows(rows[-100:], scales[-100:]), few))
+    assert torch.equal(q.dequantize(torch.float16)[-3:], QuantRows(rows[-3:], scales[-3:]).dequantize(torch.float16))
+    del codes, whole, end, rows, q
+    print_case("gate and up of almost 2 GiB apart")
+    held = torch.randint(-128, 128, (2 * 20000, 50000), dtype=torch.int8, device=cuda)
+    near_by = held[:, 1600:1700].contiguous()
+    down = Int8Weight(held[:50, :20000].contiguous(), scales[:50])
+    for rows in (1, 40, 100, 1100):
+        x = torch.randn(rows, 100, device=cuda) * 0.01
+        a = int8_feed_forward(x, Int8Weight(held[:, 1600:1700], scales[:40000] * 1e-3), down)
+        assert torch.equal(a, int8_feed_forward(x, Int8Weight(near_by, scales[:40000] * 1e-3), down)) and torch.isfinite(a).all()
+    del held, near_by, down
+    print_case("norm of rows over 4 GiB")
+    x = torch.randn(70000, 40000, device=cuda).bfloat16()
+    weight = torch.rand(40000, device=cuda)
+    made, alone = (rms_norm(t, weight, residual=t, quant="int8", rows=True) for t in (x, x[-9:]))
+    for a, b in ((made.hidden, alone.hidden), (made.rows, alone.rows), (made.quant.values, alone.quant.values),
+                 (made.quant.scales, alone.quant.scales)):
+        assert torch.equal(a[-9:], b)
+    del x, made, alone
+    print_case("results over 4 GiB")
+    q, w = (torch.randint(-128, 128, (n, 128), dtype=torch.int8, device=cuda) for n in (70000, 32000))
+    w = Int8Weight(w, scales[:32000])
+    ones = torch.rand(70000, device=cuda)
+    out = int8_linear(QuantRows(q, ones), w)
+    assert torch.equal(out[-300:], int8_linear(QuantRows(q[-300:], ones[-300:]), w))
+    del out
+    torch.cuda.empty_cache()
+
+
+def test_more_rows_than_a_launch_holds(cuda):
+    print_case("rows of several launches")
+    rows, tail = (1 << 21) + 5, (1 << 21) - 700
+    weight = torch.rand(128, device=cuda)
+    x, add = (torch.randn(rows, 128, device=cuda).half() for _ in range(2))
+    for quant in ("int8", "fp8-128"):
+        made, end = (rms_norm(x[at:], weight, residual=add[at:], quant=quant, rows=True) for at in (0, tail))
+        for a, b in ((made.hidden, end.hidden), (made.rows, end.rows), (made.quant.values.view(torch.int8), end.quant.values.view(torch.int8)),
+                     (made.quant.scales, end.quant.scales)):
+            assert torch.equal(a[tail:], b)
+        assert torch.equal(made.hidden[:tail], x[:tail] + add[:tail])
+    del made, end, x, add
+    print_case("the most rows of several waves each")
+    one = torch.randn(1, 1100, device=cuda).bfloat16()
+    q = quantize_rows(one.expand(1 << 24, 1100))
+    first = quantize_rows(one)
+    assert (q.scales == first.scales).all()
+    for part in q.values.split(1 << 21):
+        assert (part == first.values).all()
+    out, same = q.dequantize(), first.dequantize()
+    for part in out.split(1 << 21):
+        assert (part == same).all()
+    del q, out, part
+    torch.cuda.empty_cache()
