@@ -373,21 +373,23 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Int8Args a, int per_row)
     const int64_t row = at / per_row;
     const int n = (int)(at - row * per_row) * 8, cols = int8_part_cols(a.n, GATED);
     const int* p = a.part + row * cols + n;
+    // every share's loads first, also of those that are not
+    v4i part[GATED ? 2 : 1][kInt8MaxSplits][2];
+#pragma unroll
+    for (int s = 0; s < kInt8MaxSplits; ++s)
+#pragma unroll
+        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+            const int* q = p + (int64_t)min(s, a.splits - 1) * a.rows * cols + h * (cols / 2);
+            part[h][s][0] = *(const v4i*)q;
+            part[h][s][1] = *(const v4i*)(q + 4);
+        }
     int sum[GATED ? 2 : 1][8] = {};
 #pragma unroll
     for (int s = 0; s < kInt8MaxSplits; ++s)
-        if (s < a.splits) {
 #pragma unroll
-            for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-                const int* q = p + (int64_t)s * a.rows * cols + h * (cols / 2);
-                const v4i lo = *(const v4i*)q, hi = *(const v4i*)(q + 4);
+        for (int h = 0; h < (GATED ? 2 : 1); ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sum[h][e] += lo[e];
-                    sum[h][4 + e] += hi[e];
-                }
-            }
-        }
+            for (int e = 0; e < 8; ++e) sum[h][e] += s < a.splits ? part[h][s][e / 4][e % 4] : 0;
     const float by = a.xs[row];
     float v[8];
 #pragma unroll

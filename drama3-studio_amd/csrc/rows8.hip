@@ -13,6 +13,8 @@
 // stay in registers between the two halves.  The sum and r are of 64 bits, so
 // that scales and codes are those of the formula and do not depend on how a
 // row was cut; the codes are decided in 32 bits except next to a border.
+// Memory bounds many rows (8192 of 4096, bf16 with residual to integers: 45 us,
+// 5.2 TB/s), a row's latency few (one of 2048: 3.1 us with its launch).
 #include <algorithm>
 
 #include "rows8_util.hpp"
@@ -21,11 +23,13 @@ namespace dmoe {
 
 namespace {
 
-// T threads hold a row, V vectors of eight columns each; several rows a
-// workgroup where a wave holds one.
+// Rows of a workgroup of T threads a row: several where a wave holds one.
+constexpr int rows_per(int threads) { return threads == kWave ? 4 : 1; }
+
+// T threads hold a row, V vectors of eight columns each.
 template <int DT, int T, int V, bool NORM>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
-    constexpr int kRowsPer = T < 256 ? 256 / T : 1;
+__global__ __launch_bounds__(rows_per(T) * T) void rows8_kernel(NormArgs a) {
+    constexpr int kRowsPer = rows_per(T);
     constexpr int kWaves = T / kWave;
     constexpr int kBytes = elem_bytes<DT>();
     const int t = threadIdx.x % T;
@@ -116,10 +120,10 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows8_kernel(NormArgs a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int col = (v * T + t) * 8;
+            if (col >= a.cols) continue;
             const float top32 = (float)((double)__int_as_float(row_max_bits(group_top[v])) * by);
             const bool fine = finite_bits(top32);
             const float scale = e4m3_scale(top32);
-            if (col >= a.cols) continue;
             *(uint64_t*)(q + col) = fine ? e4m3_codes8(u[v], units_of(by, scale)) : 0;
             if (t % 16 == 0) {
                 a.q.scales[row * (a.cols / 128) + col / 128] = fine ? scale : __builtin_nanf("");
@@ -150,8 +154,8 @@ constexpr int kRowsOfLaunch = 1 << 21;
 
 template <int DT, int T, int V>
 void launch_rows8_as(NormArgs a, hipStream_t stream) {
-    const int per = T < 256 ? 256 / T : 1, all = a.rows;
-    const dim3 block(T < 256 ? 256 : T);
+    const int per = rows_per(T), all = a.rows;
+    const dim3 block(per * T);
     const auto move = [](auto*& p, int64_t bytes) {
         if (p) p = (std::remove_reference_t<decltype(p)>)((char*)p + bytes);
     };
@@ -171,24 +175,26 @@ void launch_rows8_as(NormArgs a, hipStream_t stream) {
     }
 }
 
-// Rows that do not fill the chip get more threads each: their time is a row's.
+// Two vectors a thread: its loads are on their way together, and a row's fixed part (sums of 64 bits, factors) is shared
+// by few threads.  Norms with residual, bf16, us: 8192 rows of 2048 by 128 threads 26.0, by 256 with one vector 36.2; 4000
+// rows of 1024 by 64 threads 9.1, with four vectors 10.3; 300 rows of 8192 by 512 threads 7.6, by 1024 with one 11.4, by
+// 256 with four 8.2; 2000 rows of 5120 by 256 threads with three 19.4, by 512 with two 20.5 (13.1 and 16.8 out of the
+// caches).  Rows that do not fill the chip get more threads each, or less code: their time is a row's (one row of 2048 to
+// E4M3 groups by 256 threads with one vector 3.4, with two 4.2; 250 rows of 2048 by 256 threads 4.2, by 128 4.6; 47 rows
+// of 14336 by 1024 threads 5.9, by 512 with four vectors 6.4, and 2000 such rows 43.4, 40.4).
 template <int DT>
 void launch_rows8_of(const NormArgs& a, hipStream_t stream) {
     const int end = padded_k(a.cols);
-    if (end <= 512) return launch_rows8_as<DT, 64, 1>(a, stream);
-    if (end <= 2048 && (end > 1024 || a.rows <= 1024)) return launch_rows8_as<DT, 256, 1>(a, stream);
+    const bool few = a.rows <= 256;
     if (end <= 1024) return launch_rows8_as<DT, 64, 2>(a, stream);
-    if (a.rows <= 512 || end > 16384) {
-        if (end <= 8192) return launch_rows8_as<DT, 1024, 1>(a, stream);
-        if (end <= 16384) return launch_rows8_as<DT, 1024, 2>(a, stream);
-        if (end <= 32768) return launch_rows8_as<DT, 1024, 4>(a, stream);
-        return launch_rows8_as<DT, 1024, 8>(a, stream);
-    }
+    if (end <= 2048) return few ? launch_rows8_as<DT, 256, 1>(a, stream) : launch_rows8_as<DT, 128, 2>(a, stream);
     if (end <= 4096) return launch_rows8_as<DT, 256, 2>(a, stream);
-    if (end <= 6144) return launch_rows8_as<DT, 256, 3>(a, stream);
-    if (end <= 8192) return launch_rows8_as<DT, 256, 4>(a, stream);
-    if (end <= 12288) return launch_rows8_as<DT, 256, 6>(a, stream);
-    return launch_rows8_as<DT, 256, 8>(a, stream);
+    if (end <= 6144 && !few) return launch_rows8_as<DT, 256, 3>(a, stream);
+    if (end <= 8192) return launch_rows8_as<DT, 512, 2>(a, stream);
+    if (end <= 12288 && !few) return launch_rows8_as<DT, 512, 3>(a, stream);
+    if (end <= 16384) return few ? launch_rows8_as<DT, 1024, 2>(a, stream) : launch_rows8_as<DT, 512, 4>(a, stream);
+    if (end <= 32768) return launch_rows8_as<DT, 1024, 4>(a, stream);
+    return launch_rows8_as<DT, 1024, 8>(a, stream);
 }
 
 template <int DT>
