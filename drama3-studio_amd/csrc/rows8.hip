@@ -181,13 +181,15 @@ void launch_rows8_as(NormArgs a, hipStream_t stream) {
 // 256 with four 8.2; 2000 rows of 5120 by 256 threads with three 19.4, by 512 with two 20.5 (13.1 and 16.8 out of the
 // caches).  Rows that do not fill the chip get more threads each, or less code: their time is a row's (one row of 2048 to
 // E4M3 groups by 256 threads with one vector 3.4, with two 4.2; 250 rows of 2048 by 256 threads 4.2, by 128 4.6; 47 rows
-// of 14336 by 1024 threads 5.9, by 512 with four vectors 6.4, and 2000 such rows 43.4, 40.4).
+// of 14336 by 1024 threads 5.9, by 512 with four vectors 6.4, and 2000 such rows 43.4, 40.4).  E4M3 groups have nothing
+// that two vectors share (400 rows of 2048 by 256 threads with one 4.4, by 128 5.5; 2000 8.9 and 8.5).
 template <int DT>
 void launch_rows8_of(const NormArgs& a, hipStream_t stream) {
     const int end = padded_k(a.cols);
     const bool few = a.rows <= 256;
     if (end <= 1024) return launch_rows8_as<DT, 64, 2>(a, stream);
-    if (end <= 2048) return few ? launch_rows8_as<DT, 256, 1>(a, stream) : launch_rows8_as<DT, 128, 2>(a, stream);
+    const bool groups = a.q.format == kRowsE4M3Group && a.rows <= 1024;
+    if (end <= 2048) return few || groups ? launch_rows8_as<DT, 256, 1>(a, stream) : launch_rows8_as<DT, 128, 2>(a, stream);
     if (end <= 4096) return launch_rows8_as<DT, 256, 2>(a, stream);
     if (end <= 6144 && !few) return launch_rows8_as<DT, 256, 3>(a, stream);
     if (end <= 8192) return launch_rows8_as<DT, 512, 2>(a, stream);

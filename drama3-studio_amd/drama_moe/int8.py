@@ -23,7 +23,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .attention import _no_gradients, _on, _stream
+from .attention import _on, _stream
 from .formats import FP8_DTYPE
 from .offload import _STATES, _device_of, device_state
 
@@ -33,6 +33,15 @@ _FLOATS = {t: _lib.dtype_code(t) for t in (torch.bfloat16, torch.float16, torch.
 INT8, E4M3, E4M3_GROUP = 1, 2, 3
 GROUP = 128  # columns of an E4M3 group
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
+
+
+def _no_gradients(names: str, *tensors) -> None:
+    """Refuses inputs whose gradients these calls, which have no backward, would lose."""
+    if torch.is_grad_enabled():
+        for i, t in enumerate(tensors):
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{names.split()[i]} needs gradients, which norms and products in 8 bits do not have: "
+                                 "call it under torch.no_grad()")
 
 
 def _padded(k: int) -> int:

@@ -19,9 +19,9 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .attention import _no_gradients, _on, _stream
+from .attention import _on, _stream
 from .int8 import (_FLOATS, E4M3, E4M3_GROUP, GROUP, INT8, QuantRows, _check_float, _check_sizes, _desc, _flat, _gpu,
-                   _same_device, _status)
+                   _no_gradients, _same_device, _status)
 
 QUANT_FORMATS = {"int8": INT8, "fp8": E4M3, "fp8-128": E4M3_GROUP}
 
