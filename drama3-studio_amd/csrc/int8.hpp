@@ -101,10 +101,10 @@ struct Int8Plan {
 
 constexpr int kInt8FewRows = 64;  // rows that the kernel of few rows takes
 
-// Every result is the same bits whichever is taken.  A CU brings at most 50 GB/s from memory, 35 where 64 of them do and
-// 18 (4.7 TB/s) where all do, whatever is on its way, and 140 GB/s from L2: a matrix is read fast only by all of them,
-// and tiles' rings deeper than three steps or operands read a whole step ahead gain nothing (47 rows, K 4096, gated N
-// 11008: 24.4 with three to six steps).  Measured on MI355X (256 CUs) with matrices that are in no cache, us:
+// Every result is the same bits whichever is taken.  A CU brings at most 50 GB/s from memory, 35 (2.2 TB/s) where 64 of
+// them do and 18 (4.7 TB/s) where all do, whatever is on its way, and 140 GB/s from L2: a matrix is read fast only by
+// most of them, and tiles' rings deeper than three steps or operands read a whole step ahead gain nothing (47 rows, K
+// 4096, gated N 11008: 24.4 with three to six steps).  Measured on MI355X (256 CUs) with matrices that are in no cache, us:
 // * Few rows: each workgroup of sixteen columns reads all rows, from L2.  Up to 72 MB of that it is as fast as tiles or
 //   faster (13 rows, K 4096, N 4096: 6.6 against 13.5; 64 rows, 67 MB: 13.0 against 13.6), above it slower (47 rows,
 //   132 MB: K 4096, gated N 11008 39 against 24; K 11008, N 4096 25 against 16.5).
