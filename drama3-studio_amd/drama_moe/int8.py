@@ -133,6 +133,7 @@ class QuantRows:
             raise ValueError("scales must be fp32 [rows] or, for E4M3, [rows, columns / 128]")
         if scales.device != values.device:
             raise ValueError("values and scales must share a device")
+        _no_gradients("scales", scales)
         stride = values.stride(0)
         if cols % GROUP or values.stride(1) != 1 or stride % 16 or not cols <= stride < 1 << 23 or values.data_ptr() % 16:
             held = torch.zeros((rows, _padded(cols)), dtype=torch.int8, device=values.device)
@@ -228,6 +229,8 @@ class Int8Weight:
         self.device = values.device
         if scales.device != self.device:
             raise ValueError("values and scales must share a device")
+        if scales.requires_grad:
+            _no_gradients("scales", scales)
         width = (k + 15) // 16 * 16
         stride, across = values.stride()
         if n == 1:

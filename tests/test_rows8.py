@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import rows8_reference as ref
-from drama_moe import _lib
+from drama_moe import _lib, int8
 from drama_moe.attention import KvCache4, PagedBatch
 from drama_moe.block import AttentionBlock, DenseBlock
 from drama_moe.int8 import (Int8FeedForward, Int8Linear, Int8Weight, QuantRows, int8_feed_forward, int8_linear,
@@ -326,3 +326,20 @@ def test_attention_block_takes_rows_in_8_bits_for_8_bit_projections_only():
     eight = [Int8Linear.from_linear(m) for m in linear]
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         AttentionBlock(*eight, cache, heads=4)(x, residual, batch)
+
+
+def test_a_capture_is_not_the_first_to_need_the_status_word(monkeypatch):
+    device = torch.device("cuda", 7)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="once eagerly"):
+        int8._status(device)
+    assert device not in int8._STATES
+
+
+def test_scales_that_need_gradients_are_refused():
+    scales = torch.ones(2, requires_grad=True)
+    for make in (QuantRows, Int8Weight):
+        with pytest.raises(ValueError, match="scales needs gradients"):
+            make(i8(2, 32), scales)
+        with torch.no_grad():
+            make(i8(2, 32), scales)
