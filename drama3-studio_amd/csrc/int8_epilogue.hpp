@@ -7,15 +7,20 @@ namespace dmoe {
 
 // A sum in units of its matrix row's scale and its activation row's: the
 // small one of the two first, so that neither product leaves fp32's range
-// where the result does not.
-__device__ __forceinline__ float int8_value(int sum, float channel, float row) { return (float)sum * channel * row; }
+// where the result does not.  The product is rounded before anything is added
+// to it, in every kernel: fused with an addition in one and not in another, a
+// row's bits would depend on the size of its call.
+__device__ __forceinline__ float int8_value(int sum, float channel, float row) {
+#pragma clang fp contract(off)
+    return (float)sum * channel * row;
+}
 
 // act(z): z / (1 + exp(-z)), or gelu in its tanh form, which is
 // z / (1 + exp(-2 sqrt(2 / pi) (z + 0.044715 z^3))).  The hardware's 2^x and
 // reciprocal, each within 2^-23; the argument's rounding costs |y| 2^-23 more.
 __device__ __forceinline__ float int8_gate(float z, int gelu) {
     constexpr float kLog2e = 1.4426950408889634f, kGelu = 1.5957691216057308f * kLog2e;
-    const float y = gelu ? kGelu * (z + 0.044715f * z * z * z) : kLog2e * z;
+    const float y = gelu ? kGelu * __builtin_fmaf(0.044715f * z * z, z, z) : kLog2e * z;
     // 2^-y beyond fp32's range is an infinity, and z by its reciprocal the right 0
     return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-y));
 }

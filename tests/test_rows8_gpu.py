@@ -545,3 +545,46 @@ def test_more_rows_than_a_launch_holds(cuda):
         assert (part == same).all()
     del q, out, part
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_row_with_bias_and_residual_does_not_depend_on_its_call(cuda, dtype):
+    """The steps behind a sum are the same in every kernel, whatever surrounds the row."""
+    print_case("rows with bias and residual across calls", dtype)
+    g = torch.Generator().manual_seed(21)
+    for k, n in ((1100, 500), (9000, 700), (4096, 4096)):
+        w, ws = matrix(n, k, g)
+        weight, bias = Int8Weight(w.to(cuda), ws.to(cuda)), torch.randn(n, generator=g).to(cuda)
+        x, add = stream(3000, k, TYPES[dtype], g).to(cuda), stream(3000, n, TYPES[dtype], g).to(cuda)
+        for b, r in ((bias, add), (bias, None), (None, add)):
+            whole = int8_linear(x, weight, bias=b, residual=r)
+            for at, rows in ((0, 1), (7, 3), (100, 5), (64, 30), (1, 64), (900, 65), (2000, 400), (100, 1100)):
+                got = int8_linear(x[at:at + rows], weight, bias=b, residual=r[at:at + rows] if r is not None else None)
+                assert torch.equal(got, whole[at:at + rows]), (k, n, rows, b is None, r is None)
+    for k, inter, n in ((500, 700, 300), (2048, 1500, 2048), (4096, 6000, 128)):
+        w, ws = matrix(2 * inter, k, g)
+        v, vs = matrix(n, inter, g)
+        up, down = Int8Weight(w.to(cuda), ws.to(cuda)), Int8Weight(v.to(cuda), vs.to(cuda))
+        x, add = stream(3000, k, TYPES[dtype], g, 0.4).to(cuda), stream(3000, n, TYPES[dtype], g).to(cuda)
+        for act in ("silu", "gelu_tanh"):
+            whole = int8_feed_forward(x, up, down, activation=act, residual=add)
+            for at, rows in ((0, 1), (7, 3), (100, 5), (64, 30), (1, 64), (900, 65), (2000, 400), (100, 1100)):
+                got = int8_feed_forward(x[at:at + rows], up, down, activation=act, residual=add[at:at + rows])
+                assert torch.equal(got, whole[at:at + rows]), (k, inter, n, act, rows)
+
+
+def test_a_norms_row_does_not_depend_on_its_call(cuda):
+    """Rows in calls of every size, held by other numbers of threads: the same bits.  (64-bit sums in another order move
+    the root by 2^-52, over a border of 24 bits in one row of 2^27.)"""
+    print_case("norm across calls")
+    g = torch.Generator().manual_seed(31)
+    for cols in (384, 1024, 2048, 2501, 5120, 8192, 11008, 14336):
+        x, add = (stream(1500, cols, torch.bfloat16, g).to(cuda) for _ in range(2))
+        weight = (torch.rand(cols, generator=g) + 0.5).to(cuda)
+        for quant in ("int8", "fp8", "fp8-128" if cols % 128 == 0 else "int8"):
+            whole = rms_norm(x, weight, residual=add, quant=quant, rows=True)
+            for at, rows in ((0, 1), (17, 30), (400, 256), (600, 257), (300, 1100)):
+                got = rms_norm(x[at:at + rows], weight, residual=add[at:at + rows], quant=quant, rows=True)
+                for a, b in ((got.hidden, whole.hidden), (got.rows, whole.rows), (got.quant.scales, whole.quant.scales),
+                             (got.quant.values.view(torch.int8), whole.quant.values.view(torch.int8))):
+                    assert torch.equal(a, b[at:at + rows]), (cols, quant, rows)
