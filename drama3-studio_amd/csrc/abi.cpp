@@ -1775,7 +1775,7 @@ dmoe::Rows read_rows(const DmoeRows* r, int rows, int64_t cols, const char* what
     return k;
 }
 
-dmoe::Rows8 to_kernel(const DmoeQuantRows* q, int rows, int cols) {
+dmoe::Rows8 to_kernel(const DmoeQuantRows* q, int cols) {
     require(q != nullptr && q->values != nullptr && q->scales != nullptr, "rows in 8 bits and their scales are required");
     require(q->format >= DMOE_ROWS_INT8 && q->format <= DMOE_ROWS_E4M3_GROUP, "unknown format of rows in 8 bits");
     require(q->format != DMOE_ROWS_E4M3_GROUP || cols % 128 == 0, "groups of 128 need a multiple of 128 columns");
@@ -1789,7 +1789,6 @@ dmoe::Rows8 to_kernel(const DmoeQuantRows* q, int rows, int cols) {
     k.stride = q->row_stride;
     k.scales = q->scales;
     k.format = q->format;
-    (void)rows;
     return k;
 }
 
@@ -1938,7 +1937,7 @@ int dmoe_rms_norm(const DmoeRows* x, const DmoeRows* residual, int rows, int col
             a.y = y.p;
             a.y_stride = y.stride;
         }
-        if (quantized) a.q = to_kernel(quantized, rows, cols);
+        if (quantized) a.q = to_kernel(quantized, cols);
         if (rows) dmoe::launch_rows8(a, as_stream(stream));
     });
 }
@@ -1947,7 +1946,7 @@ int dmoe_int8_quantize(const DmoeRows* x, int rows, int cols, const DmoeQuantRow
     return checked([&] {
         check_rows8_size(rows, cols);
         const dmoe::Rows in = read_rows(x, rows, cols, "x");
-        const dmoe::Rows8 q = to_kernel(quantized, rows, cols);
+        const dmoe::Rows8 q = to_kernel(quantized, cols);
         require(q.format == DMOE_ROWS_INT8, "rows are quantized to 8-bit integers");
         if (rows) quantize_into(in, rows, cols, q, status, as_stream(stream));
     });
@@ -1957,7 +1956,7 @@ int dmoe_rows8_read(const DmoeQuantRows* quantized, int rows, int cols, const Dm
     return checked([&] {
         check_rows8_size(rows, cols);
         dmoe::Dequant8Args a{};
-        a.q = to_kernel(quantized, rows, cols);
+        a.q = to_kernel(quantized, cols);
         const dmoe::Rows o = to_kernel(out, rows, cols, "out");
         a.rows = rows;
         a.cols = cols;
@@ -1997,7 +1996,7 @@ int dmoe_int8_linear(const DmoeRows* x, const DmoeQuantRows* quantized, int rows
         dmoe::Rows in;
         dmoe::Rows8 in8;
         if (quantized) {
-            in8 = to_kernel(quantized, rows, a.k);
+            in8 = to_kernel(quantized, a.k);
             require(in8.format == DMOE_ROWS_INT8, "products take rows of 8-bit integers");
         } else {
             in = read_rows(x, rows, a.k, "x");
@@ -2041,7 +2040,7 @@ int dmoe_int8_feed_forward(const DmoeRows* x, const DmoeQuantRows* quantized, in
         dmoe::Rows in;
         dmoe::Rows8 in8;
         if (quantized) {
-            in8 = to_kernel(quantized, rows, up.k);
+            in8 = to_kernel(quantized, up.k);
             require(in8.format == DMOE_ROWS_INT8, "products take rows of 8-bit integers");
         } else {
             in = read_rows(x, rows, up.k, "x");

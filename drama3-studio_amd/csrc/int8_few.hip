@@ -10,8 +10,6 @@
 // four rows that are not quantized yet are quantized by every workgroup for
 // itself while its first matrix pieces are on their way (one row, K 2048, N
 // 2560: 3.6 us against 3.3 and a launch of the quantizer, about 2.5).
-#include <algorithm>
-
 #include "rows8_util.hpp"
 #include "int8_epilogue.hpp"
 

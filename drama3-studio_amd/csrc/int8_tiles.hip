@@ -20,8 +20,6 @@
 // deeper ring 7%; a third step of rows in the ring, beside two of the matrix, 4%
 // faster than two of each; eight waves as fast as four, and 5% faster where few
 // tiles run.
-#include <algorithm>
-
 #include "int8_epilogue.hpp"
 #include "rows8_util.hpp"
 
