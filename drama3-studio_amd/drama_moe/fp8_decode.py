@@ -4,14 +4,14 @@
 ``forward(kernel, x, ids, weights, staged)`` -> [1, H] in x.dtype;
 ``quantized_pairs(kernel, q, scales, ids, weights, staged, dtype=)`` -> ordered
 fp32 partials from an activation the caller already quantized (a single
-shared row, or one row per pair).
+shared row, or one row per pair; a scale for every 128 columns, or one a row).
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib
-from .formats import StagedExperts, fp8_bank_struct
+from .formats import FP8_DTYPE, StagedExperts, fp8_bank_struct
 from .offload import DECODE_PAIRS, MAX_PAIRS, HipExpertBackend, device_state
 
 
@@ -22,25 +22,38 @@ def forward(kernel, x, ids, weights, staged: StagedExperts):
 
 def quantized_pairs(kernel, q, scales, ids, weights, staged: StagedExperts, *, dtype=torch.bfloat16):
     """Ordered fp32 partials of route pairs from FP8 rows q [R, H] + scales
-    [R, H/128]; R == 1 shares the row across all pairs."""
+    [R, H/128], or [R] (also [R, 1]) for a scale a row, as
+    ``norm.rms_norm(..., quant="fp8")`` gives; R == 1 shares the row across all
+    pairs."""
     ids = ids.reshape(-1).contiguous()
     weights = weights.reshape(-1).contiguous()
-    count, hidden = ids.numel(), q.shape[1]
+    count, hidden = ids.numel(), staged.hidden
     if count > MAX_PAIRS:
         raise ValueError(f"quantized_pairs takes at most {MAX_PAIRS} pairs per call")
-    if q.shape[0] not in (1, count):
+    if weights.numel() != count:
+        raise ValueError("there must be one weight per pair")
+    if q.ndim != 2 or q.shape[1] != hidden or q.dtype not in (FP8_DTYPE, torch.uint8) or q.stride(1) != 1:
+        raise ValueError(f"quantized rows must be FP8 [rows, {hidden}] with contiguous columns")
+    rows = q.shape[0]
+    if rows not in (1, count):
         raise ValueError("quantized rows must be one shared row or one per pair")
+    if scales.dtype is not torch.float32 or scales.shape not in ((rows,), (rows, 1), (rows, hidden // 128)):
+        raise ValueError(f"scales must be fp32 [rows] or [rows, {hidden // 128}]")
+    if any(t.device != staged.device for t in (q, scales, ids, weights)):
+        raise ValueError("rows, scales, ids, weights and experts must share a device")
+    groups = scales.shape[1] if scales.ndim == 2 else 1
+    scales = scales.reshape(rows, groups).contiguous()
     out = torch.empty((count, hidden), dtype=torch.float32, device=q.device)
     bank = fp8_bank_struct(staged)
     state = device_state(q.device)
     lib = _lib.library()
     ws = state.workspace_for(lib.dmoe_fp8_workspace_bytes(bank, count))
     qb = q.view(torch.uint8)
-    row_div = count if q.shape[0] == 1 else 1
+    row_div = count if rows == 1 else 1
     gu = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}[dtype]
     _lib.check(lib.dmoe_fp8_quantized_pairs(
-        bank, _lib.ptr(qb), _lib.ptr(scales), qb.stride(0), scales.stride(0), q.shape[0], row_div,
-        128 if scales.shape[1] == hidden // 128 else hidden, _lib.ptr(ids), _lib.dtype_code(ids.dtype),
+        bank, _lib.ptr(qb), _lib.ptr(scales), qb.stride(0), groups, rows, row_div,
+        128 if groups == hidden // 128 else hidden, _lib.ptr(ids), _lib.dtype_code(ids.dtype),
         _lib.ptr(weights), _lib.dtype_code(weights.dtype), count, gu, _lib.ptr(out), _lib.ptr(ws),
         ws.numel(), _lib.ptr(state.status), _lib.stream_handle(q.device)))
     return out
