@@ -4,7 +4,8 @@
 ``forward(kernel, x, ids, weights, staged)`` -> [1, H] in x.dtype;
 ``quantized_pairs(kernel, q, scales, ids, weights, staged, dtype=)`` -> ordered
 fp32 partials from an activation the caller already quantized (a single
-shared row, or one row per pair; a scale for every 128 columns, or one a row).
+shared row, one row per pair, or one row per token of ids [T, k]; a scale for
+every 128 columns, or one a row).
 """
 from __future__ import annotations
 
@@ -24,7 +25,11 @@ def quantized_pairs(kernel, q, scales, ids, weights, staged: StagedExperts, *, d
     """Ordered fp32 partials of route pairs from FP8 rows q [R, H] + scales
     [R, H/128], or [R] (also [R, 1]) for a scale a row, as
     ``norm.rms_norm(..., quant="fp8")`` gives; R == 1 shares the row across all
+    pairs.  ids and weights [R, k], a prompt's routes, take each row for its k
     pairs."""
+    rows = q.shape[0] if q.ndim else 0
+    routed = ids.ndim == 2 and ids.shape[0] == rows  # each row has its own k pairs
+    per_row = ids.shape[1] if routed else 1
     ids = ids.reshape(-1).contiguous()
     weights = weights.reshape(-1).contiguous()
     count, hidden = ids.numel(), staged.hidden
@@ -34,9 +39,8 @@ def quantized_pairs(kernel, q, scales, ids, weights, staged: StagedExperts, *, d
         raise ValueError("there must be one weight per pair")
     if q.ndim != 2 or q.shape[1] != hidden or q.dtype not in (FP8_DTYPE, torch.uint8) or q.stride(1) != 1:
         raise ValueError(f"quantized rows must be FP8 [rows, {hidden}] with contiguous columns")
-    rows = q.shape[0]
-    if rows not in (1, count):
-        raise ValueError("quantized rows must be one shared row or one per pair")
+    if rows not in (1, count) and not routed:
+        raise ValueError("quantized rows must be one shared row or one per pair, or one for each row of ids [R, k]")
     if scales.dtype is not torch.float32 or scales.shape not in ((rows,), (rows, 1), (rows, hidden // 128)):
         raise ValueError(f"scales must be fp32 [rows] or [rows, {hidden // 128}]")
     if any(t.device != staged.device for t in (q, scales, ids, weights)):
@@ -44,12 +48,14 @@ def quantized_pairs(kernel, q, scales, ids, weights, staged: StagedExperts, *, d
     groups = scales.shape[1] if scales.ndim == 2 else 1
     scales = scales.reshape(rows, groups).contiguous()
     out = torch.empty((count, hidden), dtype=torch.float32, device=q.device)
+    if count == 0:
+        return out
     bank = fp8_bank_struct(staged)
     state = device_state(q.device)
     lib = _lib.library()
     ws = state.workspace_for(lib.dmoe_fp8_workspace_bytes(bank, count))
     qb = q.view(torch.uint8)
-    row_div = count if rows == 1 else 1
+    row_div = count if rows == 1 else per_row
     gu = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}[dtype]
     _lib.check(lib.dmoe_fp8_quantized_pairs(
         bank, _lib.ptr(qb), _lib.ptr(scales), qb.stride(0), groups, rows, row_div,

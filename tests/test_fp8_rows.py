@@ -31,6 +31,8 @@ def call(bank, q=None, scales=None, ids=None, weights=None):
     (dict(scales=torch.ones(3, 2, 1)), "scales must be"),
     (dict(scales=torch.ones(3).double()), "scales must be"),
     (dict(q=rows(2), scales=torch.ones(2)), "one shared row or one per pair"),
+    (dict(q=rows(2), scales=torch.ones(2), ids=torch.zeros(3, 2, dtype=torch.int64), weights=torch.ones(3, 2)), "each row of ids"),
+    (dict(ids=torch.zeros(3, 2, dtype=torch.int64)), "one weight per pair"),
     (dict(q=rows(3, 128)), "rows must be FP8 \\[rows, 256\\]"),
     (dict(q=rows(3, 512)[:, ::2]), "contiguous columns"),
     (dict(q=rows(3).float()), "rows must be FP8"),
@@ -41,3 +43,10 @@ def call(bank, q=None, scales=None, ids=None, weights=None):
 def test_refusals(bank, inputs, message):
     with pytest.raises(ValueError, match=message):
         call(bank, **inputs)
+
+
+def test_no_pairs_are_no_launch(bank):
+    none = torch.zeros(0, 4, dtype=torch.int64)
+    assert call(bank, q=rows(0), scales=torch.ones(0), ids=none, weights=none.float()).shape == (0, HIDDEN)
+    assert call(bank, q=rows(1), scales=torch.ones(1), ids=none, weights=none.float()).shape == (0, HIDDEN)
+    assert call(bank, ids=none.reshape(3, 0), weights=none.reshape(3, 0).float()).shape == (0, HIDDEN)

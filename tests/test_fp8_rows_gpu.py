@@ -94,3 +94,21 @@ def test_a_norms_rows_with_a_scale_each_reach_the_experts(cuda, rows):
                                        weights[row].expand(4), staged, dtype=torch.float32)
         assert torch.equal(a, a[:1].expand(4, HIDDEN))
         assert (a[0] - got[row]).abs().max() <= 2e-2 * got[row].abs().max()
+
+
+@pytest.mark.parametrize("quant", ["fp8", "fp8-128"])
+@pytest.mark.parametrize("tokens,top_k", [(1, 8), (3, 1), (3, 8), (20, 4), (37, 8), (500, 4), (777, 6)])
+def test_a_prompts_rows_reach_their_experts_without_copies(cuda, tokens, top_k, quant):
+    """ids [T, k] take row t for its k pairs: the bits of a call on rows that were repeated k times."""
+    print_case("prompt's rows before experts", tokens, top_k, quant)
+    g = torch.Generator().manual_seed(tokens)
+    staged = bank(cuda)
+    x = torch.randn(tokens, HIDDEN, generator=g).half().to(cuda)
+    weight = (torch.rand(HIDDEN, generator=g) + 0.5).half().to(cuda)
+    made = rms_norm(x, weight, residual=x, quant=quant).quant
+    ids, weights = (t.reshape(tokens, top_k) for t in routes(tokens * top_k, g, cuda))
+    got = fp8_decode.quantized_pairs(fp8_moe, made.values, made.scales, ids, weights, staged)
+    assert got.shape == (tokens * top_k, HIDDEN)
+    repeat = made.values.view(torch.uint8).repeat_interleave(top_k, 0).view(FP8_DTYPE), made.scales.repeat_interleave(top_k, 0)
+    want = fp8_decode.quantized_pairs(fp8_moe, *repeat, ids.flatten(), weights.flatten(), staged)
+    assert torch.equal(got, want)
