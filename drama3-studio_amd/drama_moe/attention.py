@@ -13,12 +13,14 @@ The reference leaves attention to the model it drives, with a bf16 cache of
 No call synchronizes the host, every call can be captured in a hipGraph, and
 scratch is allocated for each call by torch, so calls on several streams and
 graphs captured apart share nothing but the cache and the status word.  There is
-no backward: with gradients enabled, inputs that need them are refused.
+no backward: with gradients enabled, inputs that need them are refused, and
+inputs with a forward-mode tangent always.
 """
 from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from .offload import _device_of, device_state
@@ -60,13 +62,20 @@ def _new(shape: tuple, dtype: torch.dtype, device):
     return t, _lib.HeadRows(t.data_ptr(), heads * dim if rows > 1 else 0, dim if heads > 1 else 0)
 
 
-def _no_gradients(names: str, *tensors: Tensor | None) -> None:
-    """Refuses inputs whose gradients the kernels, which have no backward, would lose."""
-    if torch.is_grad_enabled():
+def _no_gradients(names: str, *tensors: Tensor | None, what: str = "attention over the cache does not have") -> None:
+    """Refuses inputs whose gradients the calls, which have no backward and no
+    forward mode, would lose.  Tangents of forward mode do not show in
+    ``requires_grad``, and torch.no_grad() keeps them."""
+    backward = torch.is_grad_enabled()
+    forward = getattr(forward_ad, "_current_level", 0) >= 0  # outside of every level no tensor has a tangent
+    if backward or forward:
         for i, t in enumerate(tensors):
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{names.split()[i]} needs gradients, which attention over the cache does not have: "
-                                 "call it under torch.no_grad()")
+            if t is None:
+                continue
+            if backward and t.requires_grad:
+                raise ValueError(f"{names.split()[i]} needs gradients, which {what}: call it under torch.no_grad()")
+            if forward and isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{names.split()[i]} has a forward-mode tangent, which {what}: pass its primal")
 
 
 def _heads(q: Tensor) -> int:

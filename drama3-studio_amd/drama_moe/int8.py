@@ -15,15 +15,18 @@ The reference keeps its dense linears in bf16 or GPTQ
 (src/drama_low_vram/quantized_model.py:71-91).  No call synchronizes the host,
 every call can be captured in a hipGraph, and scratch is allocated for each
 call by torch.  Matrices are constants: there is no backward, and with
-gradients enabled inputs that need them are refused.
+gradients enabled inputs that need them are refused, and inputs with a
+forward-mode tangent always.
 """
 from __future__ import annotations
+
+from functools import partial
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from .attention import _on, _stream
+from .attention import _no_gradients, _on, _stream
 from .formats import FP8_DTYPE
 from .offload import _STATES, _device_of, device_state
 
@@ -35,13 +38,7 @@ GROUP = 128  # columns of an E4M3 group
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
 
 
-def _no_gradients(names: str, *tensors) -> None:
-    """Refuses inputs whose gradients these calls, which have no backward, would lose."""
-    if torch.is_grad_enabled():
-        for i, t in enumerate(tensors):
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{names.split()[i]} needs gradients, which norms and products in 8 bits do not have: "
-                                 "call it under torch.no_grad()")
+_no_gradients = partial(_no_gradients, what="norms and products in 8 bits do not have")
 
 
 def _padded(k: int) -> int:
@@ -229,8 +226,7 @@ class Int8Weight:
         self.device = values.device
         if scales.device != self.device:
             raise ValueError("values and scales must share a device")
-        if scales.requires_grad:
-            _no_gradients("scales", scales)
+        _no_gradients("scales", scales)
         width = (k + 15) // 16 * 16
         stride, across = values.stride()
         if n == 1:

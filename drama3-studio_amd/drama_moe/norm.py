@@ -9,7 +9,8 @@ E4M3 with a scale a row or for every 128 columns
 (``fp8_decode.quantized_pairs``) -- in one pass over the rows.  In the
 reference these are torch modules of the model it drives
 (src/drama_low_vram/backbone_graph.py:297-316).  Serving only: with gradients
-enabled, inputs that need them are refused.
+enabled, inputs that need them are refused, and inputs with a forward-mode
+tangent always.
 """
 from __future__ import annotations
 

@@ -1,0 +1,61 @@
+"""Norms and products in 8 bits on the CPU: inputs whose gradients or tangents
+the calls would lose, modules under casts, scales of quantized matrices."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from drama_moe.attention import KvCache4, PagedBatch
+from drama_moe.block import AttentionBlock
+from drama_moe.int8 import Int8Linear, Int8Weight, QuantRows, int8_feed_forward, int8_linear, quantize_rows
+from drama_moe.norm import rms_norm
+
+
+def i8(*shape):
+    return torch.zeros(shape, dtype=torch.int8)
+
+
+def weight(n=4, k=32):
+    return Int8Weight(i8(n, k) + 1, torch.ones(n))
+
+
+@pytest.mark.parametrize("name,call", [
+    ("x", lambda d: quantize_rows(d(2, 32))),
+    ("x", lambda d: int8_linear(d(2, 32), weight())),
+    ("bias", lambda d: int8_linear(torch.zeros(2, 32), weight(), bias=d(4))),
+    ("residual", lambda d: int8_linear(torch.zeros(2, 32), weight(), residual=d(2, 4))),
+    ("bias", lambda d: int8_linear(QuantRows(i8(2, 32), torch.ones(2)), weight(), bias=d(4))),
+    ("x", lambda d: int8_feed_forward(d(2, 32), weight(8), weight(5, 4))),
+    ("residual", lambda d: int8_feed_forward(torch.zeros(2, 32), weight(8), weight(5, 4), residual=d(2, 5))),
+    ("x", lambda d: rms_norm(d(2, 32), torch.ones(32))),
+    ("weight", lambda d: rms_norm(torch.zeros(2, 32), d(32))),
+    ("residual", lambda d: rms_norm(torch.zeros(2, 32), torch.ones(32), residual=d(2, 32))),
+    ("scales", lambda d: QuantRows(i8(2, 32), d(2))),
+    ("scales", lambda d: Int8Weight(i8(4, 32), d(4))),
+    ("x", lambda d: Int8Linear(i8(4, 32), torch.ones(4))(d(2, 32))),
+])
+def test_forward_mode_tangents_are_refused(name, call):
+    """A dual tensor has requires_grad false, and torch.no_grad() keeps its tangent."""
+    with forward_ad.dual_level():
+        dual = lambda *shape: forward_ad.make_dual(torch.zeros(shape), torch.ones(shape))  # noqa: E731
+        with pytest.raises(ValueError, match=f"{name} has a forward-mode tangent"):
+            call(dual)
+        with torch.no_grad(), pytest.raises(ValueError, match=f"{name} has a forward-mode tangent"):
+            call(dual)
+        with torch.inference_mode():  # drops tangents: so does the call
+            try:
+                call(dual)
+            except RuntimeError as e:
+                assert "ROCm GPU" in str(e)
+    with pytest.raises(ValueError, match="forward-mode tangent"):
+        torch.func.jvp(lambda x: quantize_rows(x), (torch.zeros(2, 32),), (torch.ones(2, 32),))
+
+
+def test_attention_block_refuses_forward_mode_tangents():
+    cache = KvCache4.allocate(4, 2, 64, page_size=16, device="cpu")
+    batch = PagedBatch(torch.ones(2, 2).int(), torch.ones(2).int())
+    linear = [torch.nn.Linear(32, 256), torch.nn.Linear(32, 128), torch.nn.Linear(32, 128), torch.nn.Linear(256, 32)]
+    block = AttentionBlock(*linear, cache, heads=4)
+    with torch.no_grad(), forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.zeros(2, 32), torch.ones(2, 32))
+        with pytest.raises(ValueError, match="attn_input has a forward-mode tangent"):
+            block(x, torch.zeros(2, 32), batch)
