@@ -130,7 +130,7 @@ class QuantRows:
             raise ValueError("scales must be fp32 [rows] or, for E4M3, [rows, columns / 128]")
         if scales.device != values.device:
             raise ValueError("values and scales must share a device")
-        _no_gradients("scales", scales)
+        _no_gradients("values scales", values, scales)
         stride = values.stride(0)
         if cols % GROUP or values.stride(1) != 1 or stride % 16 or not cols <= stride < 1 << 23 or values.data_ptr() % 16:
             held = torch.zeros((rows, _padded(cols)), dtype=torch.int8, device=values.device)

@@ -59,3 +59,12 @@ def test_attention_block_refuses_forward_mode_tangents():
         x = forward_ad.make_dual(torch.zeros(2, 32), torch.ones(2, 32))
         with pytest.raises(ValueError, match="attn_input has a forward-mode tangent"):
             block(x, torch.zeros(2, 32), batch)
+
+
+@pytest.mark.parametrize("cols", [32, 128])
+def test_e4m3_values_that_need_gradients_are_refused(cols):
+    values = torch.zeros(2, cols).to(torch.float8_e4m3fn).requires_grad_()
+    with pytest.raises(ValueError, match="values needs gradients"):
+        QuantRows(values, torch.ones(2))
+    with torch.no_grad():
+        QuantRows(values, torch.ones(2))
