@@ -349,7 +349,8 @@ class Int8Linear(torch.nn.Module):
     ``scales`` [N] and an optional ``bias`` [N]; ``forward`` takes rows
     [..., K] or ``QuantRows`` (so one norm's output serves several), and
     ``dtype`` is what ``QuantRows`` give where the call does not say.  The
-    buffer ``qweight`` has K rounded up to a multiple of 16."""
+    buffer ``qweight`` has K rounded up to a multiple of 16.  Casts of the
+    module (``half()``, ``to(dtype)``) move the buffers and leave their types."""
 
     def __init__(self, weight: Tensor, scales: Tensor, bias: Tensor | None = None, *, device=None,
                  dtype: torch.dtype = torch.bfloat16):
@@ -365,6 +366,14 @@ class Int8Linear(torch.nn.Module):
                                                                (held.desc.row_stride, 1)))
         self.register_buffer("scales", held.scales)
         self.register_buffer("bias", bias.detach().to(device, torch.float32) if bias is not None else None)
+
+    def _apply(self, fn, recurse=True):
+        held = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, t in held.items():
+            if t is not None and self._buffers[name].dtype is not t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
 
     def _weight(self) -> Int8Weight:
         return Int8Weight(self.qweight[:, :self.in_features], self.scales)

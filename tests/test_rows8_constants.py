@@ -6,7 +6,7 @@ from torch.autograd import forward_ad
 
 from drama_moe.attention import KvCache4, PagedBatch
 from drama_moe.block import AttentionBlock
-from drama_moe.int8 import Int8Linear, Int8Weight, QuantRows, int8_feed_forward, int8_linear, quantize_rows
+from drama_moe.int8 import Int8FeedForward, Int8Linear, Int8Weight, QuantRows, int8_feed_forward, int8_linear, quantize_rows
 from drama_moe.norm import rms_norm
 
 
@@ -68,3 +68,31 @@ def test_e4m3_values_that_need_gradients_are_refused(cols):
         QuantRows(values, torch.ones(2))
     with torch.no_grad():
         QuantRows(values, torch.ones(2))
+
+
+CASTS = {"bf16": lambda m: m.to(torch.bfloat16), "half": lambda m: m.half(), "double": lambda m: m.double(),
+         "type": lambda m: m.type(torch.float16), "both": lambda m: m.to("cpu", torch.float16)}
+
+
+@pytest.mark.parametrize("cast", CASTS)
+def test_casts_of_a_layer_leave_the_types_of_its_buffers(cast):
+    torch.manual_seed(0)
+    linear = Int8Linear.from_linear(torch.nn.Linear(40, 24))
+    bare = lambda k, n: torch.nn.Linear(k, n, bias=False)  # noqa: E731
+    ffn = Int8FeedForward.from_linears(bare(24, 40), bare(24, 40), bare(40, 24))
+    before = {n: t.clone() for m in (linear, ffn) for n, t in m.state_dict().items()}
+    layer = torch.nn.Sequential(linear, torch.nn.Linear(3, 3), ffn)
+    CASTS[cast](layer)
+    assert layer[1].weight.dtype is (torch.float64 if cast == "double" else torch.bfloat16 if cast == "bf16" else torch.float16)
+    after = {n: t for m in (linear, ffn) for n, t in m.state_dict().items()}
+    assert before.keys() == after.keys()
+    for n, t in before.items():
+        assert after[n].dtype is t.dtype and torch.equal(after[n], t), n
+    for m in (linear, ffn.gate_up, ffn.down):
+        assert torch.equal(m._weight().values, m.qweight[:, :m.in_features])
+
+
+def test_a_cast_of_a_layer_still_moves_its_buffers():
+    linear = Int8Linear.from_linear(torch.nn.Linear(40, 24)).to("meta", torch.bfloat16)
+    assert {t.device.type for t in linear.buffers()} == {"meta"}
+    assert linear.scales.dtype is linear.bias.dtype is torch.float32 and linear.qweight.dtype is torch.int8
