@@ -30,6 +30,21 @@ def select_fp8(weight: torch.Tensor, index) -> torch.Tensor:
     return weight.view(torch.uint8)[index].view(weight.dtype)
 
 
+class HeldTypes(torch.nn.Module):
+    """Module whose buffers ``_held`` a kernel reads in their own types: casts
+    of the module (``half()``, ``to(dtype)``, ``type()``) move them only."""
+
+    _held: tuple = ()
+
+    def _apply(self, fn, recurse=True):
+        held = {name: self._buffers[name] for name in self._held}
+        super()._apply(fn, recurse)
+        for name, t in held.items():
+            if t is not None and self._buffers[name].dtype is not t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
+
 # ------------------------------------------------------------- bank geometry
 
 @dataclass(frozen=True)

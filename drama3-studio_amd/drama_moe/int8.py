@@ -27,7 +27,7 @@ from torch import Tensor
 
 from . import _lib
 from .attention import _no_gradients, _on, _stream
-from .formats import FP8_DTYPE
+from .formats import FP8_DTYPE, HeldTypes
 from .offload import _STATES, _device_of, device_state
 
 MAX_K = 65536
@@ -344,13 +344,15 @@ def int8_feed_forward(x: Tensor | QuantRows, gate_up: Int8Weight, down: Int8Weig
     return out if len(lead) == 1 else out.reshape(*lead, n)
 
 
-class Int8Linear(torch.nn.Module):
+class Int8Linear(HeldTypes):
     """Dense linear on 8-bit integers: ``weight`` int8 [N, K] with fp32
     ``scales`` [N] and an optional ``bias`` [N]; ``forward`` takes rows
     [..., K] or ``QuantRows`` (so one norm's output serves several), and
     ``dtype`` is what ``QuantRows`` give where the call does not say.  The
     buffer ``qweight`` has K rounded up to a multiple of 16.  Casts of the
     module (``half()``, ``to(dtype)``) move the buffers and leave their types."""
+
+    _held = ("qweight", "scales", "bias")
 
     def __init__(self, weight: Tensor, scales: Tensor, bias: Tensor | None = None, *, device=None,
                  dtype: torch.dtype = torch.bfloat16):
@@ -366,14 +368,6 @@ class Int8Linear(torch.nn.Module):
                                                                (held.desc.row_stride, 1)))
         self.register_buffer("scales", held.scales)
         self.register_buffer("bias", bias.detach().to(device, torch.float32) if bias is not None else None)
-
-    def _apply(self, fn, recurse=True):
-        held = dict(self._buffers)
-        super()._apply(fn, recurse)
-        for name, t in held.items():
-            if t is not None and self._buffers[name].dtype is not t.dtype:
-                self._buffers[name] = t.to(self._buffers[name].device)
-        return self
 
     def _weight(self) -> Int8Weight:
         return Int8Weight(self.qweight[:, :self.in_features], self.scales)

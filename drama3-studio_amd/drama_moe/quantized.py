@@ -14,7 +14,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .formats import QuantizedStore
+from .formats import HeldTypes, QuantizedStore
 from .offload import DECODE_PAIRS, MAX_PAIRS, _device_of, device_state
 
 MODE_NAMES = ("W4A16-GPTQ", "INT8-ConvRot/BF16", "W6A8/BF16", "W4A8-Codebook/BF16", "W4A8-G128/FP8",
@@ -219,14 +219,17 @@ class QuantizedExpertBackend:
         return out, weights, ids
 
 
-class GPTQLinear(torch.nn.Module):
+class GPTQLinear(HeldTypes):
     """Dense W4A16 linear kept compressed on the GPU, the reference's
     GPTQLinear (src/drama_low_vram/quantized_model.py:71-91): GPTQ ``weight``
     [K/8, N] int32 and ``scales`` [K/128, N] fp16 are stored transposed
     (``qweight`` [N, K/8], ``scales`` [N, K/128]); ``forward`` multiplies rows
     of x (bf16 or fp16, any leading shape) by the dequantized matrix with the
     tiled W4A16 kernel (dmoe_w4a16_linear) and returns bf16 [..., N], as the
-    reference's projection(mode=0) over one expert does."""
+    reference's projection(mode=0) over one expert does.  Casts of the module
+    leave codes and scales in their types."""
+
+    _held = ("qweight", "scales")
 
     def __init__(self, weight: Tensor, scales: Tensor, *, device, dtype=torch.bfloat16):
         super().__init__()

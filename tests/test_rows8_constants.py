@@ -8,6 +8,7 @@ from drama_moe.attention import KvCache4, PagedBatch
 from drama_moe.block import AttentionBlock
 from drama_moe.int8 import Int8FeedForward, Int8Linear, Int8Weight, QuantRows, int8_feed_forward, int8_linear, quantize_rows
 from drama_moe.norm import rms_norm
+from drama_moe.quantized import GPTQLinear
 
 
 def i8(*shape):
@@ -96,3 +97,14 @@ def test_a_cast_of_a_layer_still_moves_its_buffers():
     linear = Int8Linear.from_linear(torch.nn.Linear(40, 24)).to("meta", torch.bfloat16)
     assert {t.device.type for t in linear.buffers()} == {"meta"}
     assert linear.scales.dtype is linear.bias.dtype is torch.float32 and linear.qweight.dtype is torch.int8
+
+
+@pytest.mark.parametrize("cast", CASTS)
+def test_casts_of_a_gptq_linear_leave_its_codes_and_scales(cast):
+    """Its kernel reads fp16 scales: bits of another type would be taken for them."""
+    linear = GPTQLinear(torch.arange(32 * 48, dtype=torch.int32).reshape(32, 48), torch.rand(2, 48).half(), device="cpu")
+    codes, scales = linear.qweight.clone(), linear.scales.clone()
+    CASTS[cast](torch.nn.Sequential(linear))
+    assert linear.scales.dtype is torch.float16 and torch.equal(linear.scales, scales)
+    assert linear.qweight.dtype is torch.int32 and torch.equal(linear.qweight, codes)
+    assert linear.weight.dtype is (torch.float64 if cast == "double" else torch.bfloat16 if cast == "bf16" else torch.float16)
