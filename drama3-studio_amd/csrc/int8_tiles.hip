@@ -34,10 +34,15 @@ constexpr int kTileGroup = 4;       // row tiles that are walked together
 
 // One copy of 64 x 16 bytes into LDS: lane l's bytes go to lds + 16 l.  Written
 // as an instruction of its own because the compiler waits for every copy
-// before the next LDS read; the waits here are tile_wait's.
+// before the next LDS read; the waits here are tile_wait's.  m0 is written and
+// not restored, and named as such; the compiler keeps nothing in it, which is
+// what its warning about reserved registers is about.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy_to_lds(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "m0");
 }
+#pragma clang diagnostic pop
 
 template <int N>
 __device__ __forceinline__ void tile_wait() {
