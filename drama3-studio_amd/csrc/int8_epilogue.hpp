@@ -5,14 +5,20 @@
 
 namespace dmoe {
 
-// A sum in units of its matrix row's scale and its activation row's: the
-// small one of the two first, so that neither product leaves fp32's range
-// where the result does not.  The product is rounded before anything is added
-// to it, in every kernel: fused with an addition in one and not in another, a
-// row's bits would depend on the size of its call.
+// A sum in units of its matrix row's scale and its activation row's, in that
+// order: only a scale from 2^98 up can take the first product out of fp32's
+// range where the result is in it, and then the row's comes first (a product
+// below 2^-126, of a scale that is itself, is exact).  The product is rounded
+// before anything is added to it, in every kernel: fused with an addition in
+// one and not in another, a row's bits would depend on the size of its call.
+// CHECKED false: for channels whose scale is known to be below kInt8Large.
+constexpr float kInt8Large = 0x1p97f;
+template <bool CHECKED = true>
 __device__ __forceinline__ float int8_value(int sum, float channel, float row) {
 #pragma clang fp contract(off)
-    return (float)sum * channel * row;
+    const float first = (float)sum * channel;
+    if (CHECKED && __builtin_expect(__builtin_isinf(first), 0)) return (float)sum * row * channel;
+    return first * row;
 }
 
 // act(z): z / (1 + exp(-z)), or gelu in its tanh form, which is

@@ -294,17 +294,26 @@ __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_
             }
         }
     } else {
-        const auto values = [&](int j, int rr, float* v) {
+        const auto values = [&](int j, int rr, float* v, auto checked) {
+            constexpr bool kChecked = decltype(checked)::value;
             int raw[GATED ? 2 : 1][8];
 #pragma unroll
             for (int h = 0; h < (GATED ? 2 : 1); ++h) sums(rr, h, raw[h]);
             const float by = mine_xs[j * 32 + rr];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[e] = int8_value(raw[0][e], ws[0][e], by);
-                if constexpr (GATED) v[e] = int8_gate(v[e], a.gelu) * int8_value(raw[GATED][e], ws[GATED][e], by);
+                v[e] = int8_value<kChecked>(raw[0][e], ws[0][e], by);
+                if constexpr (GATED) v[e] = int8_gate(v[e], a.gelu) * int8_value<kChecked>(raw[GATED][e], ws[GATED][e], by);
             }
         };
+        // The check is asked for a wave at a time: made for every value, it costs 2% of a large product (8192 rows, K 4096,
+        // N 4096: 114.0 us, 111.6) and 10% of a ragged one (509 rows, K 2048, N 5003: 18.6 us, 16.9).
+        float top = 0.0f;
+#pragma unroll
+        for (int h = 0; h < (GATED ? 2 : 1); ++h)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(ws[h][e]));
+        const bool large = __any(top >= kInt8Large);
         // whole pieces of eight columns: nothing waits for anything but the residual, which is asked for a strip ahead
         const auto whole = [&](auto more) {
             constexpr bool kMore = decltype(more)::value;  // bias or residual
@@ -324,7 +333,7 @@ __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_
                     const int rr = p * kRowsAt + lane / kVectors;
                     const int64_t row = m0 + wave_m + j * 32 + rr;
                     float v[8];
-                    values(j, rr, v);
+                    values(j, rr, v, std::false_type{});
                     if (kMore && a.bias) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) v[e] += bias[e];
@@ -337,7 +346,7 @@ __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_
                 }
             }
         };
-        if (n0 + T::kCols <= a.n) {
+        if (n0 + T::kCols <= a.n && !large) {
             if (a.bias || a.residual) whole(std::true_type{});
             else whole(std::false_type{});
             return;
@@ -351,7 +360,8 @@ __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_
                 const int64_t row = m0 + wave_m + j * 32 + rr;
                 if (row >= a.rows || n >= a.n) continue;
                 float v[8];
-                values(j, rr, v);
+                if (large) values(j, rr, v, std::true_type{});
+                else values(j, rr, v, std::false_type{});
                 if (a.bias) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] += bias[e];
@@ -376,7 +386,7 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Int8Args a, int per_row)
     const int64_t row = at / per_row;
     const int n = (int)(at - row * per_row) * 8, cols = int8_part_cols(a.n, GATED);
     const int* p = a.part + row * cols + n;
-    // every share's loads first, also of those that are not
+    // all loads first, also of shares that are not
     v4i part[GATED ? 2 : 1][kInt8MaxSplits][2];
 #pragma unroll
     for (int s = 0; s < kInt8MaxSplits; ++s)
@@ -386,6 +396,20 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Int8Args a, int per_row)
             part[h][s][0] = *(const v4i*)q;
             part[h][s][1] = *(const v4i*)(q + 4);
         }
+    const float by = a.xs[row];
+    float v[8], ws[GATED ? 2 : 1][8], bias[8], add[8], top = 0.0f;
+#pragma unroll
+    for (int h = 0; h < (GATED ? 2 : 1); ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            ws[h][e] = a.ws[min(n + e, a.n - 1) + h * a.n];
+            top = fmaxf(top, fabsf(ws[h][e]));
+        }
+    if (a.bias) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bias[e] = a.bias[min(n + e, a.n - 1)];
+    }
+    if (a.residual) load_cols8<DT>((const char*)a.residual + row * a.residual_stride * elem_bytes<DT>(), n, a.n, add);
     int sum[GATED ? 2 : 1][8] = {};
 #pragma unroll
     for (int s = 0; s < kInt8MaxSplits; ++s)
@@ -393,18 +417,21 @@ __global__ __launch_bounds__(256) void int8_join_kernel(Int8Args a, int per_row)
         for (int h = 0; h < (GATED ? 2 : 1); ++h)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[h][e] += s < a.splits ? part[h][s][e / 4][e % 4] : 0;
-    const float by = a.xs[row];
-    float v[8];
+    const auto values = [&](auto checked) {
+        constexpr bool kChecked = decltype(checked)::value;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int ne = min(n + e, a.n - 1);
-        v[e] = int8_value(sum[0][e], a.ws[ne], by);
-        if constexpr (GATED) v[e] = int8_gate(v[e], a.gelu) * int8_value(sum[GATED][e], a.ws[ne + a.n], by);
-        if (a.bias) v[e] += a.bias[ne];
+        for (int e = 0; e < 8; ++e) {
+            v[e] = int8_value<kChecked>(sum[0][e], ws[0][e], by);
+            if constexpr (GATED) v[e] = int8_gate(v[e], a.gelu) * int8_value<kChecked>(sum[GATED][e], ws[GATED][e], by);
+        }
+    };
+    if (__any(top >= kInt8Large)) values(std::true_type{});
+    else values(std::false_type{});
+    if (a.bias) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += bias[e];
     }
     if (a.residual) {
-        float add[8];
-        load_cols8<DT>((const char*)a.residual + row * a.residual_stride * elem_bytes<DT>(), n, a.n, add);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += add[e];
     }
