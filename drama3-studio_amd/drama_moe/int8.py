@@ -36,6 +36,7 @@ _FLOATS = {t: _lib.dtype_code(t) for t in (torch.bfloat16, torch.float16, torch.
 INT8, E4M3, E4M3_GROUP = 1, 2, 3
 GROUP = 128  # columns of an E4M3 group
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
+_STEP = torch.tensor(1 / 127, dtype=torch.float32).item()
 
 
 _no_gradients = partial(_no_gradients, what="norms and products in 8 bits do not have")
@@ -244,11 +245,12 @@ class Int8Weight:
 
     @classmethod
     def quantize(cls, weight: Tensor) -> Int8Weight:
-        """The nearest 8-bit integers of a float matrix [N, K], scales max |row| / 127."""
+        """The nearest 8-bit integers of a float matrix [N, K], with scales as rows have them:
+        max(max |row|, 1e-12) times 1/127 as fp32 has it, on every device."""
         if weight.ndim != 2 or not weight.is_floating_point():
             raise ValueError("weight must be a float matrix [N, K]")
         w = weight.detach().double()
-        scales = (w.abs().amax(1).float().clamp(min=1e-12) / 127)
+        scales = w.abs().amax(1).float().clamp(min=1e-12) * _STEP
         return cls((w / scales.double()[:, None]).round().clamp(-127, 127).to(torch.int8), scales)
 
 

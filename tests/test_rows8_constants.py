@@ -1,9 +1,11 @@
 """Norms and products in 8 bits on the CPU: inputs whose gradients or tangents
 the calls would lose, modules under casts, scales of quantized matrices."""
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+import rows8_reference as ref
 from drama_moe.attention import KvCache4, PagedBatch
 from drama_moe.block import AttentionBlock
 from drama_moe.int8 import Int8FeedForward, Int8Linear, Int8Weight, QuantRows, int8_feed_forward, int8_linear, quantize_rows
@@ -108,3 +110,13 @@ def test_casts_of_a_gptq_linear_leave_its_codes_and_scales(cast):
     assert linear.scales.dtype is torch.float16 and torch.equal(linear.scales, scales)
     assert linear.qweight.dtype is torch.int32 and torch.equal(linear.qweight, codes)
     assert linear.weight.dtype is (torch.float64 if cast == "double" else torch.bfloat16 if cast == "bf16" else torch.float16)
+
+
+def test_scales_of_a_matrix_are_those_of_rows():
+    """Largest magnitudes times fl32(1/127), which a division by 127 misses by a last bit in one row of twenty."""
+    w = torch.randn(4000, 40, generator=torch.Generator().manual_seed(3))
+    w[7] = 0
+    held = Int8Weight.quantize(w)
+    codes, scales = ref.int8(ref.wide(w))
+    assert np.array_equal(ref.wide(held.scales), scales) and np.array_equal(ref.wide(held.values), codes)
+    assert (held.scales != w.abs().amax(1).clamp(min=1e-12) / 127).float().mean() > 0.02
