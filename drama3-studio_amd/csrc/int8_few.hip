@@ -75,9 +75,9 @@ struct RowsToLds {
     }
 };
 
-// A wave's next U blocks are on their way while it multiplies U.
+// A wave's next block is on its way while it multiplies one.
 // DT is the type of rows that are not quantized yet, kI32 where they are.
-template <int NT, int MT, int U, int W, bool GATED, int DT>
+template <int NT, int MT, int W, bool GATED, int DT>
 __global__ __launch_bounds__(W * kWave, (W > 8 ? 4 : NT * MT <= 2 ? 6 : NT * MT <= 4 ? 4 : 2)) void int8_few_kernel(Int8Args a) {
     constexpr bool QUANT = DT != kI32;
     constexpr int kCols = GATED ? NT * 8 : NT * 16;
@@ -103,20 +103,17 @@ __global__ __launch_bounds__(W * kWave, (W > 8 ? 4 : NT * MT <= 2 ? 6 : NT * MT 
     const int pitch = padded_k(a.k) + 16;
     const uint8_t* xlds = xl + (QUANT ? min(r, a.rows - 1) * pitch : 0);
     struct Group {
-        v4i w[U][NT][2], x[QUANT ? 1 : U][QUANT ? 1 : MT][2];
+        v4i w[NT][2], x[QUANT ? 1 : MT][2];
     };
-    const auto fetch = [&](Group& g, int b0) {
+    const auto fetch = [&](Group& g, int b) {
+        const int at = min(b, blocks - 1) * kFewBlock + c * 16;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = min(b0 + u * W, blocks - 1) * kFewBlock + c * 16;
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int j = 0; j < NT; ++j) g.w[j][h] = *(const v4i*)(wrow[j] + min(at + h * 64, last));
+            if constexpr (!QUANT) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) g.w[u][j][h] = *(const v4i*)(wrow[j] + min(at + h * 64, last));
-                if constexpr (!QUANT) {
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) g.x[u][m][h] = *(const v4i*)(xrow[m] + at + h * 64);
-                }
+                for (int m = 0; m < MT; ++m) g.x[m][h] = *(const v4i*)(xrow[m] + at + h * 64);
             }
         }
     };
@@ -137,33 +134,29 @@ __global__ __launch_bounds__(W * kWave, (W > 8 ? 4 : NT * MT <= 2 ? 6 : NT * MT 
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[j][m] = v4i{0, 0, 0, 0};
-    const auto multiply = [&](const Group& g, int b0) {
+    const auto multiply = [&](const Group& g, int b) {
+        if (b >= blocks) return;  // the same for the wave
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int b = b0 + u * W;
-            if (b >= blocks) continue;  // the same for the wave
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int h = 0; h < 2; ++h) {
+                const v4i xf = QUANT ? *(const v4i*)(xlds + b * kFewBlock + c * 16 + h * 64) : g.x[QUANT ? 0 : m][h];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const v4i xf = QUANT ? *(const v4i*)(xlds + b * kFewBlock + c * 16 + h * 64) : g.x[QUANT ? 0 : u][QUANT ? 0 : m][h];
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[j][m] = mfma_i8(g.w[u][j][h], xf, acc[j][m]);
-                }
-        }
+                for (int j = 0; j < NT; ++j) acc[j][m] = mfma_i8(g.w[j][h], xf, acc[j][m]);
+            }
     };
-    int b0 = wave;
+    int b = wave;
     while (true) {
-        const bool more = b0 + U * W < blocks;
-        if (more) fetch(next, b0 + U * W);
-        multiply(now, b0);
+        const bool more = b + W < blocks;
+        if (more) fetch(next, b + W);
+        multiply(now, b);
         if (!more) break;
-        b0 += U * W;
-        const bool again = b0 + U * W < blocks;
-        if (again) fetch(now, b0 + U * W);
-        multiply(next, b0);
+        b += W;
+        const bool again = b + W < blocks;
+        if (again) fetch(now, b + W);
+        multiply(next, b);
         if (!again) break;
-        b0 += U * W;
+        b += W;
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -192,27 +185,27 @@ __global__ __launch_bounds__(W * kWave, (W > 8 ? 4 : NT * MT <= 2 ? 6 : NT * MT 
     }
 }
 
-template <int NT, int MT, int U, int W, bool GATED>
+template <int NT, int MT, int W, bool GATED>
 void launch_few_as(const Int8Args& a, hipStream_t stream) {
     constexpr int kCols = GATED ? NT * 8 : NT * 16;
     const dim3 grid((unsigned)((a.n + kCols - 1) / kCols)), block(W * kWave);
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
     if constexpr (MT == 1) {
         if (a.xq == nullptr) {
-            if (a.x_dtype == kBF16) go(int8_few_kernel<NT, MT, U, W, GATED, kBF16>);
-            else if (a.x_dtype == kF16) go(int8_few_kernel<NT, MT, U, W, GATED, kF16>);
-            else go(int8_few_kernel<NT, MT, U, W, GATED, kF32>);
+            if (a.x_dtype == kBF16) go(int8_few_kernel<NT, MT, W, GATED, kBF16>);
+            else if (a.x_dtype == kF16) go(int8_few_kernel<NT, MT, W, GATED, kF16>);
+            else go(int8_few_kernel<NT, MT, W, GATED, kF32>);
             return;
         }
     }
-    go(int8_few_kernel<NT, MT, U, W, GATED, kI32>);
+    go(int8_few_kernel<NT, MT, W, GATED, kI32>);
 }
 
 template <int NT, int W, bool GATED>
 void launch_few_of(const Int8Args& a, hipStream_t stream) {
-    if (a.rows <= 16) launch_few_as<NT, 1, 1, W, GATED>(a, stream);
-    else if (a.rows <= 32) launch_few_as<NT, 2, 1, W, GATED>(a, stream);
-    else launch_few_as<NT, 4, 1, W, GATED>(a, stream);
+    if (a.rows <= 16) launch_few_as<NT, 1, W, GATED>(a, stream);
+    else if (a.rows <= 32) launch_few_as<NT, 2, W, GATED>(a, stream);
+    else launch_few_as<NT, 4, W, GATED>(a, stream);
 }
 
 }  // namespace

@@ -54,13 +54,13 @@ __device__ __forceinline__ v16i mfma_i8_32(const v4i& a, const v4i& b, const v16
 }
 
 constexpr int kTileK = 128;         // columns of a step
+constexpr int kTileParts = 2;       // of a step's four, over which the copies behind its barrier go out
 
 // TM rows by TN matrix rows a workgroup, WM of its waves along the rows and WN
-// along the matrix; rings of SX and SW steps for rows and matrix; the copies of
-// a step in EARLY parts.
-template <int TM_, int TN_, int WM_, int WN_, int SX_, int SW_, int EARLY_>
+// along the matrix; rings of SX and SW steps for rows and matrix.
+template <int TM_, int TN_, int WM_, int WN_, int SX_, int SW_>
 struct Shape {
-    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, SX = SX_, SW = SW_, EARLY = EARLY_;
+    static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, SX = SX_, SW = SW_;
     static constexpr int kWaves = WM * WN, kThreads = kWaves * kWave;
 };
 
@@ -80,7 +80,7 @@ struct Tile {
     static_assert(G::SX == G::SW || G::SX == G::SW + 1, "W is the younger of a step's operands");
     static constexpr int kBehind = (G::SW - 2) * kCopies + (G::SX > G::SW ? kCopiesX : 0);
     static constexpr int kCols = GATED ? G::TN / 2 : G::TN;
-    static constexpr int kSlots = G::EARLY * kFN;   // places of copies between matrix instructions
+    static constexpr int kSlots = kTileParts * kFN;  // places of copies between matrix instructions
     // copies [first(p), first(p + 1)) go to place p
     static constexpr int first(int place) { return place * kCopies / kSlots; }
     // waves a SIMD that LDS has room for, in workgroups of at least a wave each
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(G::kThreads, (Tile<G, GATED>::kPerSimd)) void int8_
 #pragma unroll
             for (int g = 0; g < FN; ++g) {
                 if (g < kReading) read((s + 1) % 2, last ? next_x : slot_x, last ? next_w : slot_w, last ? 0 : s + 1, g);
-                if (part < G::EARLY) {
+                if (part < kTileParts) {
                     const int from = T::first(part * FN + g), to = T::first(part * FN + g + 1);
                     if (part == 0) copies(t + G::SW, slot_w, t + G::SX, slot_x, from, to, tail);
                     else copies(t - 1 + G::SW, before_w, t - 1 + G::SX, before_x, from, to, tail);
@@ -472,12 +472,12 @@ void launch_tiles_as(const Int8Args& a, hipStream_t stream) {
 
 void launch_int8_tiles(const Int8Args& a, const Int8Plan& plan, hipStream_t stream) {
     switch (plan.shape) {
-        case kInt8Tiles64: return launch_tiles_as<Shape<64, 64, 2, 1, 4, 4, 2>>(a, stream);
-        case kInt8Tiles64x128: return launch_tiles_as<Shape<64, 128, 2, 2, 4, 4, 2>>(a, stream);
-        case kInt8Tiles128Deep: return launch_tiles_as<Shape<128, 128, 2, 2, 4, 4, 2>>(a, stream);
-        case kInt8Tiles128x256: return launch_tiles_as<Shape<128, 256, 2, 4, 3, 3, 2>>(a, stream);
-        case kInt8Tiles128: return launch_tiles_as<Shape<128, 128, 2, 2, 2, 2, 2>>(a, stream);
-        default: return launch_tiles_as<Shape<256, 256, 2, 4, 3, 2, 2>>(a, stream);
+        case kInt8Tiles64: return launch_tiles_as<Shape<64, 64, 2, 1, 4, 4>>(a, stream);
+        case kInt8Tiles64x128: return launch_tiles_as<Shape<64, 128, 2, 2, 4, 4>>(a, stream);
+        case kInt8Tiles128Deep: return launch_tiles_as<Shape<128, 128, 2, 2, 4, 4>>(a, stream);
+        case kInt8Tiles128x256: return launch_tiles_as<Shape<128, 256, 2, 4, 3, 3>>(a, stream);
+        case kInt8Tiles128: return launch_tiles_as<Shape<128, 128, 2, 2, 2, 2>>(a, stream);
+        default: return launch_tiles_as<Shape<256, 256, 2, 4, 3, 2>>(a, stream);
     }
 }
 
