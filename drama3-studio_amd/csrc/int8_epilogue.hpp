@@ -27,7 +27,7 @@ __device__ __forceinline__ float int8_value(int sum, float channel, float row) {
 __device__ __forceinline__ float int8_gate(float z, int gelu) {
     constexpr float kLog2e = 1.4426950408889634f, kGelu = 1.5957691216057308f * kLog2e;
     const float y = gelu ? kGelu * __builtin_fmaf(0.044715f * z * z, z, z) : kLog2e * z;
-    // 2^-y beyond fp32's range is an infinity, and z by its reciprocal the right 0
+    // 2^-y above 2^126, or an infinity, has no normal reciprocal, and the result is 0: less than 2^-119 of it are lost
     return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-y));
 }
 
