@@ -185,27 +185,19 @@ __global__ __launch_bounds__(W * kWave, (W > 8 ? 4 : NT * MT <= 2 ? 6 : NT * MT 
     }
 }
 
-template <int NT, int MT, int W, bool GATED>
+template <int NT, int MT, int W, bool GATED, int DT>
 void launch_few_as(const Int8Args& a, hipStream_t stream) {
     constexpr int kCols = GATED ? NT * 8 : NT * 16;
-    const dim3 grid((unsigned)((a.n + kCols - 1) / kCols)), block(W * kWave);
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
-    if constexpr (MT == 1) {
-        if (a.xq == nullptr) {
-            if (a.x_dtype == kBF16) go(int8_few_kernel<NT, MT, W, GATED, kBF16>);
-            else if (a.x_dtype == kF16) go(int8_few_kernel<NT, MT, W, GATED, kF16>);
-            else go(int8_few_kernel<NT, MT, W, GATED, kF32>);
-            return;
-        }
-    }
-    go(int8_few_kernel<NT, MT, W, GATED, kI32>);
+    hipLaunchKernelGGL((int8_few_kernel<NT, MT, W, GATED, DT>), dim3((unsigned)((a.n + kCols - 1) / kCols)), dim3(W * kWave), 0,
+                       stream, a);
 }
 
+// Rows of a float type, which the workgroups quantize.
 template <int NT, int W, bool GATED>
-void launch_few_of(const Int8Args& a, hipStream_t stream) {
-    if (a.rows <= 16) launch_few_as<NT, 1, W, GATED>(a, stream);
-    else if (a.rows <= 32) launch_few_as<NT, 2, W, GATED>(a, stream);
-    else launch_few_as<NT, 4, W, GATED>(a, stream);
+void launch_few_floats(const Int8Args& a, hipStream_t stream) {
+    if (a.x_dtype == kBF16) launch_few_as<NT, 1, W, GATED, kBF16>(a, stream);
+    else if (a.x_dtype == kF16) launch_few_as<NT, 1, W, GATED, kF16>(a, stream);
+    else launch_few_as<NT, 1, W, GATED, kF32>(a, stream);
 }
 
 }  // namespace
@@ -214,13 +206,33 @@ bool int8_few_quantizes(int rows, int k) {
     return rows <= kFewQuantRows && rows * (padded_k(k) + 16) <= kFewQuantBytes;
 }
 
-// Sixteen waves a workgroup where those are few (one row, K 5632, N 2048, 128 workgroups: 5.6 us, with eight waves 6.2;
-// 16 rows, K 11008, N 4096, 256 workgroups: 15.2 against 14.1).  A second K block on its way costs the registers of a
-// workgroup a CU (13 rows, K 4096, N 4096: 8.0 us against 6.6).
+// Eight waves a workgroup, or sixteen: those have a K block each from K 2048 on and one round of workgroups to 256 (us,
+// eight in brackets; one row of floats, N 2048: K 1024 3.4 (3.1), 1280 3.6 (3.5), 1536 3.6 (3.6), 1792 3.7 (3.7), 2048 3.5
+// (3.8); K 5632: N 1280 5.6 (6.2), 4096 7.0 (8.3), 5120 11.1 (10.3)).  In between they are faster where the workgroups
+// quantize rows, which goes by threads (four rows, K 5632, N 2048: 8.1 (9.1)); where up to eight rows leave the call to the
+// matrix (four, K 5632: N 2048 6.1 (6.4), 4096 6.5 (7.1); eight, K 11008, N 2048 10.9 (10.9)); and where more than 32 rows
+// take the registers of all but two waves a SIMD (48 rows, K 4096: N 2048 9.7 (10.3), 4096 10.4 (11.1)).  Not for those
+// between (13 rows, K 11008, N 2048 12.2 (11.5); 32 rows, K 2048, N 2560 5.0 (4.9)).  A second K block on its way costs the
+// registers of a workgroup a CU (13 rows, K 4096, N 4096: 8.0 us against 6.6).
 void launch_int8_few(const Int8Args& a, hipStream_t stream) {
-    if (a.gated) launch_few_of<2, 8, true>(a, stream);
-    else if (a.n <= 16 * 160) launch_few_of<1, 16, false>(a, stream);
-    else launch_few_of<1, 8, false>(a, stream);
+    constexpr int kCus = 256, kWide = 1536;
+    const bool sixteen = a.k > kWide && a.n <= 16 * kCus;
+    if (a.xq == nullptr) {
+        if (a.gated) launch_few_floats<2, 8, true>(a, stream);
+        else if (sixteen) launch_few_floats<1, 16, false>(a, stream);
+        else launch_few_floats<1, 8, false>(a, stream);
+    } else if (a.rows <= 16) {
+        if (a.gated) launch_few_as<2, 1, 8, true, kI32>(a, stream);
+        else if (sixteen && a.rows <= 8) launch_few_as<1, 1, 16, false, kI32>(a, stream);
+        else launch_few_as<1, 1, 8, false, kI32>(a, stream);
+    } else if (a.rows <= 32) {
+        if (a.gated) launch_few_as<2, 2, 8, true, kI32>(a, stream);
+        else launch_few_as<1, 2, 8, false, kI32>(a, stream);
+    } else {
+        if (a.gated) launch_few_as<2, 4, 8, true, kI32>(a, stream);
+        else if (sixteen) launch_few_as<1, 4, 16, false, kI32>(a, stream);
+        else launch_few_as<1, 4, 8, false, kI32>(a, stream);
+    }
 }
 
 }  // namespace dmoe

@@ -27,3 +27,6 @@ GATED = [
     (1281, 130, 5632, 70, T128, 1), (1281, 200, 5601, 130, T128, 1),
     (2100, 100, 2176, 60, T256, 1), (2049, 257, 2201, 70, T256, 1),
 ]
+
+# few rows at both sides of the rule between eight and sixteen waves (rows, columns of a row, columns of the result)
+WAVES = [(rows, k, n) for rows in (1, 4, 5, 8, 9, 16, 17, 32, 33, 64) for k, n in ((1536, 100), (1537, 100), (2200, 4096), (1600, 4097))]

@@ -11,7 +11,7 @@ import rows8_reference as ref
 from conftest import print_case
 from drama_moe.int8 import Int8FeedForward, Int8Weight, QuantRows, int8_feed_forward, int8_linear, quantize_rows
 from drama_moe.norm import RmsNorm, rms_norm
-from int8_plan_cases import GATED, PRODUCTS, T64, T128
+from int8_plan_cases import GATED, PRODUCTS, T64, T128, WAVES
 from test_rows8_gpu import check_linear, matrix, same_rows8, stream
 
 pytestmark = pytest.mark.gpu
@@ -25,6 +25,13 @@ def test_products_in_every_kernel(cuda, case):
     check_linear(cuda, rows, k, n, torch.bfloat16)
     check_linear(cuda, rows, k, n, torch.float16, given=True, bias=True, residual=True)
     check_linear(cuda, rows, k, n, torch.float32, residual=True)
+
+
+@pytest.mark.parametrize("case", WAVES, ids=lambda c: "-".join(map(str, c)))
+def test_few_rows_in_workgroups_of_each_size(cuda, case):
+    rows, k, n = case
+    check_linear(cuda, rows, k, n, torch.bfloat16, given=True, bias=True)
+    check_linear(cuda, rows, k, n, torch.float16, residual=True)
 
 
 def check_gated(cuda, rows, k, inter, n, dtype, act, *, given, residual):
