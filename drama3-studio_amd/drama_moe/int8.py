@@ -378,7 +378,8 @@ class Int8Linear(HeldTypes):
     def from_linear(cls, linear: torch.nn.Linear, *, device=None, dtype: torch.dtype = torch.bfloat16) -> Int8Linear:
         """The nearest 8-bit integers of a float linear."""
         held = Int8Weight.quantize(linear.weight)
-        return cls(held.values, held.scales, linear.bias, device=device, dtype=dtype)
+        bias = linear.bias.detach().clone() if linear.bias is not None else None  # the linear keeps its own
+        return cls(held.values, held.scales, bias, device=device, dtype=dtype)
 
     def forward(self, x: Tensor | QuantRows, *, residual: Tensor | None = None, dtype: torch.dtype | None = None) -> Tensor:
         if dtype is None and residual is None and isinstance(x, QuantRows):

@@ -120,3 +120,13 @@ def test_scales_of_a_matrix_are_those_of_rows():
     codes, scales = ref.int8(ref.wide(w))
     assert np.array_equal(ref.wide(held.scales), scales) and np.array_equal(ref.wide(held.values), codes)
     assert (held.scales != w.abs().amax(1).clamp(min=1e-12) / 127).float().mean() > 0.02
+
+
+def test_a_linear_of_integers_leaves_the_float_one_alone():
+    """State loaded into the one made of a float linear does not reach that linear's bias."""
+    linear = torch.nn.Linear(40, 24)
+    before = linear.bias.detach().clone()
+    made = Int8Linear.from_linear(linear)
+    assert torch.equal(made.bias, before)
+    made.load_state_dict(Int8Linear.from_linear(torch.nn.Linear(40, 24)).state_dict())
+    assert torch.equal(linear.bias, before) and not torch.equal(made.bias, before)
