@@ -18,6 +18,8 @@ inputs with a forward-mode tangent always.
 """
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
@@ -62,20 +64,28 @@ def _new(shape: tuple, dtype: torch.dtype, device):
     return t, _lib.HeadRows(t.data_ptr(), heads * dim if rows > 1 else 0, dim if heads > 1 else 0)
 
 
-def _no_gradients(names: str, *tensors: Tensor | None, what: str = "attention over the cache does not have") -> None:
-    """Refuses inputs whose gradients the calls, which have no backward and no
-    forward mode, would lose.  Tangents of forward mode do not show in
+# outside of every level of torch.autograd.forward_ad (below 0) no tensor has a tangent
+_LEVEL = forward_ad if hasattr(forward_ad, "_current_level") else SimpleNamespace(_current_level=0)
+
+
+def _refusal(what: str):
+    """What refuses inputs whose gradients the calls, which have no backward and
+    no forward mode, would lose.  Tangents of forward mode do not show in
     ``requires_grad``, and torch.no_grad() keeps them."""
-    backward = torch.is_grad_enabled()
-    forward = getattr(forward_ad, "_current_level", 0) >= 0  # outside of every level no tensor has a tangent
-    if backward or forward:
-        for i, t in enumerate(tensors):
-            if t is None:
-                continue
-            if backward and t.requires_grad:
-                raise ValueError(f"{names.split()[i]} needs gradients, which {what}: call it under torch.no_grad()")
-            if forward and isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None:
-                raise ValueError(f"{names.split()[i]} has a forward-mode tangent, which {what}: pass its primal")
+    def no_gradients(names: str, *tensors: Tensor | None) -> None:
+        if torch.is_grad_enabled():
+            for t in tensors:
+                if t is not None and t.requires_grad:
+                    name = names.split()[next(i for i, other in enumerate(tensors) if other is t)]
+                    raise ValueError(f"{name} needs gradients, which {what} not have: call it under torch.no_grad()")
+        if _LEVEL._current_level >= 0:
+            for name, t in zip(names.split(), tensors):
+                if isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                    raise ValueError(f"{name} has a forward-mode tangent, which {what} not have: pass its primal")
+    return no_gradients
+
+
+_no_gradients = _refusal("attention over the cache does")
 
 
 def _heads(q: Tensor) -> int:

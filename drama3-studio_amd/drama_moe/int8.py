@@ -20,13 +20,11 @@ forward-mode tangent always.
 """
 from __future__ import annotations
 
-from functools import partial
-
 import torch
 from torch import Tensor
 
 from . import _lib
-from .attention import _no_gradients, _on, _stream
+from .attention import _LEVEL, _on, _refusal, _stream
 from .formats import FP8_DTYPE, HeldTypes
 from .offload import _STATES, _device_of, device_state
 
@@ -39,7 +37,7 @@ ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
 _STEP = torch.tensor(1 / 127, dtype=torch.float32).item()
 
 
-_no_gradients = partial(_no_gradients, what="norms and products in 8 bits do not have")
+_no_gradients = _refusal("norms and products in 8 bits do")
 
 
 def _padded(k: int) -> int:
@@ -131,7 +129,9 @@ class QuantRows:
             raise ValueError("scales must be fp32 [rows] or, for E4M3, [rows, columns / 128]")
         if scales.device != values.device:
             raise ValueError("values and scales must share a device")
-        _no_gradients("values scales", values, scales)
+        if values.dtype is not torch.int8:
+            _no_gradients("values", values)
+        _no_gradients("scales", scales)
         stride = values.stride(0)
         if cols % GROUP or values.stride(1) != 1 or stride % 16 or not cols <= stride < 1 << 23 or values.data_ptr() % 16:
             held = torch.zeros((rows, _padded(cols)), dtype=torch.int8, device=values.device)
@@ -227,7 +227,8 @@ class Int8Weight:
         self.device = values.device
         if scales.device != self.device:
             raise ValueError("values and scales must share a device")
-        _no_gradients("scales", scales)
+        if scales.requires_grad or _LEVEL._current_level >= 0:
+            _no_gradients("scales", scales)
         width = (k + 15) // 16 * 16
         stride, across = values.stride()
         if n == 1:
