@@ -106,7 +106,7 @@ constexpr int kInt8FewRows = 64;  // rows that the kernel of few rows takes
 // most of them, and tiles' rings deeper than three steps or operands read a whole step ahead gain nothing (47 rows, K
 // 4096, gated N 11008: 24.4 with three to six steps).  Measured on MI355X (256 CUs) with matrices that are in no cache, us:
 // * Few rows: each workgroup of sixteen columns reads all rows, from L2.  Up to 72 MB of that it is as fast as tiles or
-//   faster (13 rows, K 4096, N 4096: 6.6 against 13.5; 64 rows, 67 MB: 13.0 against 13.6), above it slower (47 rows,
+//   faster (13 rows, K 4096, N 4096: 6.6 against 13.5; 64 rows, 67 MB: 11.8 against 13.6), above it slower (47 rows,
 //   132 MB: K 4096, gated N 11008 39 against 24; K 11008, N 4096 25 against 16.5).
 // * 64 x 64 while they do not outnumber the CUs (256 rows, K 4096, N 4096, 256 tiles: 13.8, 64 x 128 17.4, 128 x 128
 //   22.5).  A step along K takes about 0.3, so where there are over twenty a share, up to four workgroups share a tile

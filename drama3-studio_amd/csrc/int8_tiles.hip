@@ -11,8 +11,9 @@
 // between matrix instructions, one barrier a step.  The sums leave through LDS
 // as well, so that a lane finishes eight columns of a row.
 //
-// 8192 rows, K 4096, N 4096: 115 us, 2.4 POP/s; K 12288 with 4096 rows 160 us,
-// 2.6 (a library's product of 8192 cubed 2.4).  Power bounds it: with zeros for
+// 8192 rows, K 4096, N 4096: 109 us a pass, 112 under a tracer, 2.5 POP/s; K
+// 12288 with 4096 rows 156 to 169 us, 2.4 to 2.6 (a library's product of 8192
+// cubed 2.4).  Power bounds it: with zeros for
 // operands the loop takes a quarter less, and matrix instructions alone reach
 // 3.5 POP/s on random operands, 5.0 on zeros.  Of a tile's 57 us, 4 are its
 // results and 2 its start.  Measured for it: copies asked for all at once behind

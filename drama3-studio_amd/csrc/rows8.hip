@@ -182,7 +182,9 @@ void launch_rows8_as(NormArgs a, hipStream_t stream) {
 // caches).  Rows that do not fill the chip get more threads each, or less code: their time is a row's (one row of 2048 to
 // E4M3 groups by 256 threads with one vector 3.4, with two 4.2; 250 rows of 2048 by 256 threads 4.2, by 128 4.6; 47 rows
 // of 14336 by 1024 threads 5.9, by 512 with four vectors 6.4, and 2000 such rows 43.4, 40.4).  E4M3 groups have nothing
-// that two vectors share (400 rows of 2048 by 256 threads with one 4.4, by 128 5.5; 2000 8.9 and 8.5).
+// that two vectors share (400 rows of 2048 by 256 threads with one 4.4, by 128 5.5; 2000 8.9 and 8.5).  Eight vectors a
+// thread, above 32768 columns, spill: 24 registers in norms of 16-bit types, 82 in the quantizer of fp16, 125 in the norm
+// of fp32 (2000 rows of 33024 and of 32768: 104 and 77, 52 and 46, 318 and 127).
 template <int DT>
 void launch_rows8_of(const NormArgs& a, hipStream_t stream) {
     const int end = padded_k(a.cols);

@@ -3,8 +3,8 @@ blocks of a decoder layer beside its routed experts.
 
 ``QuantRows`` are rows in 8 bits with their scales, as ``quantize_rows`` and
 ``norm.rms_norm`` make them: integers or E4M3 with a scale a row, or E4M3
-with a scale for every 128 columns (the rows ``fp8_decode.quantized_pairs``
-takes).  ``Int8Weight`` is a matrix of 8-bit integers with a scale for each
+with a scale for every 128 columns (``fp8_decode.quantized_pairs`` takes
+E4M3 rows of both kinds).  ``Int8Weight`` is a matrix of 8-bit integers with a scale for each
 output channel.  ``int8_linear`` multiplies the two, ``int8_feed_forward``
 runs a gated feed-forward block on two such matrices; ``Int8Linear`` and
 ``Int8FeedForward`` are the modules, ``Int8Linear`` next to

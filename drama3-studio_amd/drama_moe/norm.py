@@ -6,7 +6,7 @@ added to the residual stream, the sum is normalised, and what the next block
 reads leaves in its own form -- rows as they are (a router, ``MoeBlock``), 8-bit
 integers with a scale a row (``int8.Int8Linear``, ``int8.Int8FeedForward``), or
 E4M3 with a scale a row or for every 128 columns
-(``fp8_decode.quantized_pairs``) -- in one pass over the rows.  In the
+(``fp8_decode.quantized_pairs``, for single rows and prompts) -- in one pass over the rows.  In the
 reference these are torch modules of the model it drives
 (src/drama_low_vram/backbone_graph.py:297-316).  Serving only: with gradients
 enabled, inputs that need them are refused, and inputs with a forward-mode

@@ -728,7 +728,8 @@ DMOE_API int dmoe_int8_quantize(const DmoeRows* x, int rows, int cols, const Dmo
 DMOE_API int dmoe_rows8_read(const DmoeQuantRows* quantized, int rows, int cols, const DmoeRows* out, void* stream);
 
 /* out [rows, n] = T(sum(codes * codes) * row scale * channel scale + bias + residual):
- * sums exact in int32, the rest in fp32.  Rows come quantized (quantized,
+ * sums exact in int32, the rest in fp32, the channel's scale before the row's
+ * unless that product would pass fp32's range.  Rows come quantized (quantized,
  * DMOE_ROWS_INT8) or as x of a float type, never both; x is quantized on the
  * way.  The workspace (256-byte aligned, any contents; nothing is kept in it)
  * has dmoe_int8_linear_workspace_bytes, which may be none.

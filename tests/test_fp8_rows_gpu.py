@@ -112,3 +112,23 @@ def test_a_prompts_rows_reach_their_experts_without_copies(cuda, tokens, top_k, 
     repeat = made.values.view(torch.uint8).repeat_interleave(top_k, 0).view(FP8_DTYPE), made.scales.repeat_interleave(top_k, 0)
     want = fp8_decode.quantized_pairs(fp8_moe, *repeat, ids.flatten(), weights.flatten(), staged)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("quant", ["fp8", "fp8-128"])
+@pytest.mark.parametrize("tokens", [1, 40, 300])
+def test_a_layers_norm_router_and_experts(cuda, tokens, quant):
+    """One norm for router and experts: the sum of a prompt's partials is what the experts make of the held values."""
+    print_case("norm, router and experts", tokens, quant)
+    g = torch.Generator().manual_seed(tokens + 7)
+    staged = bank(cuda)
+    x, add = (torch.randn(tokens, HIDDEN, generator=g).bfloat16().to(cuda) for _ in range(2))
+    made = rms_norm(x, (torch.rand(HIDDEN, generator=g) + 0.5).bfloat16().to(cuda), residual=add, quant=quant, rows=True)
+    router = torch.randn(EXPERTS, HIDDEN, generator=g).bfloat16().to(cuda)
+    weights, ids = torch.softmax(made.rows.float() @ router.float().T, -1).topk(4)
+    partials = fp8_decode.quantized_pairs(fp8_moe, made.quant.values, made.quant.scales, ids, weights, staged,
+                                          dtype=torch.float32)
+    out = partials.view(*ids.shape, -1).sum(1)
+    backend = HipExpertBackend(x_group="token" if quant == "fp8" else 128, gu_dtype=torch.float32)
+    want = backend.forward(made.quant.dequantize(torch.float32), ids, weights, staged)
+    # the held values are quantized to themselves but for their scales' last bits; hidden codes may lie a step apart
+    assert (out - want).abs().max() <= 2e-2 * want.abs().max()
