@@ -27,41 +27,45 @@ def quantized_pairs(kernel, q, scales, ids, weights, staged: StagedExperts, *, d
     ``norm.rms_norm(..., quant="fp8")`` gives; R == 1 shares the row across all
     pairs.  ids and weights [R, k], a prompt's routes, take each row for its k
     pairs."""
-    rows = q.shape[0] if q.ndim else 0
-    routed = ids.ndim == 2 and ids.shape[0] == rows  # each row has its own k pairs
-    per_row = ids.shape[1] if routed else 1
-    ids = ids.reshape(-1).contiguous()
-    weights = weights.reshape(-1).contiguous()
-    count, hidden = ids.numel(), staged.hidden
+    shape, routes, hidden, device = q.shape, ids.shape, staged.hidden, staged.device
+    if len(shape) != 2 or shape[1] != hidden or q.dtype not in (FP8_DTYPE, torch.uint8) or q.stride(1) != 1:
+        raise ValueError(f"quantized rows must be FP8 [rows, {hidden}] with contiguous columns")
+    rows = shape[0]
+    routed = len(routes) == 2 and routes[0] == rows  # each row has its own k pairs
+    if len(routes) != 1 or not ids.is_contiguous():
+        ids = ids.reshape(-1).contiguous()
+    if weights.ndim != 1 or not weights.is_contiguous():
+        weights = weights.reshape(-1).contiguous()
+    count = ids.shape[0]
     if count > MAX_PAIRS:
         raise ValueError(f"quantized_pairs takes at most {MAX_PAIRS} pairs per call")
-    if weights.numel() != count:
+    if weights.shape[0] != count:
         raise ValueError("there must be one weight per pair")
-    if q.ndim != 2 or q.shape[1] != hidden or q.dtype not in (FP8_DTYPE, torch.uint8) or q.stride(1) != 1:
-        raise ValueError(f"quantized rows must be FP8 [rows, {hidden}] with contiguous columns")
-    if rows not in (1, count) and not routed:
+    if rows != 1 and rows != count and not routed:
         raise ValueError("quantized rows must be one shared row or one per pair, or one for each row of ids [R, k]")
-    if scales.dtype is not torch.float32 or scales.shape not in ((rows,), (rows, 1), (rows, hidden // 128)):
+    scaled = scales.shape
+    groups = scaled[1] if len(scaled) == 2 else 1
+    if scales.dtype is not torch.float32 or not 1 <= len(scaled) <= 2 or scaled[0] != rows or groups not in (1, hidden // 128):
         raise ValueError(f"scales must be fp32 [rows] or [rows, {hidden // 128}]")
-    if any(t.device != staged.device for t in (q, scales, ids, weights)):
+    if q.device != device or scales.device != device or ids.device != device or weights.device != device:
         raise ValueError("rows, scales, ids, weights and experts must share a device")
-    groups = scales.shape[1] if scales.ndim == 2 else 1
-    scales = scales.reshape(rows, groups).contiguous()
-    out = torch.empty((count, hidden), dtype=torch.float32, device=q.device)
+    if not scales.is_contiguous():
+        scales = scales.contiguous()
+    out = torch.empty((count, hidden), dtype=torch.float32, device=device)
     if count == 0:
         return out
     bank = fp8_bank_struct(staged)
-    state = device_state(q.device)
+    state = device_state(device)
     lib = _lib.library()
     ws = state.workspace_for(lib.dmoe_fp8_workspace_bytes(bank, count))
     qb = q.view(torch.uint8)
-    row_div = count if rows == 1 else per_row
+    row_div = count if rows == 1 else routes[1] if routed else 1
     gu = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}[dtype]
     _lib.check(lib.dmoe_fp8_quantized_pairs(
         bank, _lib.ptr(qb), _lib.ptr(scales), qb.stride(0), groups, rows, row_div,
         128 if groups == hidden // 128 else hidden, _lib.ptr(ids), _lib.dtype_code(ids.dtype),
         _lib.ptr(weights), _lib.dtype_code(weights.dtype), count, gu, _lib.ptr(out), _lib.ptr(ws),
-        ws.numel(), _lib.ptr(state.status), _lib.stream_handle(q.device)))
+        ws.numel(), _lib.ptr(state.status), _lib.stream_handle(device)))
     return out
 
 
